@@ -10,7 +10,9 @@ import sys
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
-SOURCES = ["clg_api.hip", "conv_binary.hip", "logic_fc.hip", "fc_tree.hip", "packbits.hip", "binarize.hip", "conv_generic.hip", "conv_forward.hip", "conv_small.hip", "conv_pair.hip", "conv_pair_grad.hip", "conv_block.hip", "net_step.hip"]
+SOURCES = ["clg_api.hip", "conv_binary.hip", "logic_fc.hip", "fc_tree.hip", "packbits.hip", "binarize.hip", "conv_generic.hip", "conv_forward.hip", "conv_small.hip", "conv_pair.hip", "conv_pair_grad.hip", "conv_block.hip", "net_step.hip",
+           "top_logits.hip", "distill.hip", "balance.hip"]
+NODE_SOURCES = ["nodes.cpp", "loss_nodes.cpp"]
 LIB = os.path.join(PKG, "libconvlogic_amd.so")
 NODES = os.path.join(PKG, "_nodes.so")
 
@@ -44,14 +46,14 @@ def build(verbose=False):
 
     with tempfile.TemporaryDirectory(prefix="clg_build_") as tmp:
         objs = [os.path.join(tmp, s.replace(".hip", ".o")) for s in SOURCES]
-        nodes = os.path.join(tmp, "nodes.o")
+        nodes = [os.path.join(tmp, s.replace(".cpp", ".o")) for s in NODE_SOURCES]
         with concurrent.futures.ThreadPoolExecutor(max_workers=8) as pool:
-            jobs = [pool.submit(run, [*_nodes_compiler(), "-c", os.path.join(PKG, "csrc", "nodes.cpp"), "-o", nodes])]
+            jobs = [pool.submit(run, [*_nodes_compiler(), "-c", os.path.join(PKG, "csrc", s), "-o", o]) for s, o in zip(NODE_SOURCES, nodes)]
             jobs += [pool.submit(run, [hipcc, *flags, "-c", os.path.join(PKG, "csrc", s), "-o", o]) for s, o in zip(SOURCES, objs)]
             for j in jobs:
                 j.result()
         run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", LIB])
-        run(["g++", "-shared", nodes, "-o", NODES, *_torch_libraries(), "-L" + PKG, "-l:libconvlogic_amd.so", "-Wl,-rpath,$ORIGIN"])
+        run(["g++", "-shared", *nodes, "-o", NODES, *_torch_libraries(), "-L" + PKG, "-l:libconvlogic_amd.so", "-Wl,-rpath,$ORIGIN"])
     return LIB
 
 

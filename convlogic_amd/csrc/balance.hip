@@ -1,0 +1,410 @@
+// How evenly rows choose among experts: with p = softmax(z) of a row's logits over E experts, the k highest of each row chosen (of equal ones the lowest),
+// c_e rows that chose expert e and n rows in all,
+//     loss = E / (k n^2) sum_e c_e sum_t p_te,        d loss / d z_ti = p_ti (w_i - sum_e w_e p_te),        w_e = E c_e / (k n^2)
+// (1 where the experts are chosen equally; the choice itself has no gradient).  The gates of a neuron are 16 experts of which it takes one: several tensors
+// of logits, a network's layers, go in one launch, each with a loss of its own, of which the mean is taken.
+#include <type_traits>
+
+#include "row_tile.h"
+
+namespace {
+
+constexpr int kSegments = 16, kThreads = 256, kMaxExperts = 1024;
+
+struct Segments {
+    const void *z[kSegments];
+    void *grad[kSegments];
+    int64_t rows[kSegments], stride[kSegments];
+    int first[kSegments + 1];                                         // workgroups first[i] .. first[i + 1] - 1 take segment i
+    int n;
+};
+
+struct BalanceArgs {
+    Segments seg;
+    int experts, k;
+    const uint8_t *mask;                                              // of the only segment, or NULL
+    float *sums;                                                      // [workgroups][experts] sums of probabilities
+    int *counts;                                                      // [workgroups][experts + 1] rows per expert, rows in all
+    const void *w;                                                    // [segments][experts] in A
+    const void *upstream;                                             // A
+};
+
+// reductions over groups of G lanes, in all of them
+template <int G, typename A, typename F>
+__device__ __forceinline__ A group_reduce(A v, F f)
+{
+#pragma unroll
+    for (int by = 1; by < G; by <<= 1) v = f(v, (A)__shfl_xor(v, by));
+    return v;
+}
+
+// the logits of a row that a lane holds: pieces lane, lane + G, ... of 16 bytes; -inf behind the row
+template <typename T, int G, int NV>
+struct RowPart {
+    typedef typename Wide<T>::type A;
+    static constexpr int VEC = Vec16<T>::N, N = NV * VEC;
+    A x[N];
+    __device__ __forceinline__ static int expert(int lane, int i) { return ((i / VEC) * G + lane) * VEC + i % VEC; }
+    __device__ __forceinline__ void load(const T *row, int lane, int experts)
+    {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int e = (j * G + lane) * VEC;
+            if (e + VEC <= experts) {
+                const auto v = *reinterpret_cast<const typename Vec16<T>::type *>(row + e);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) x[j * VEC + i] = (A)v[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) x[j * VEC + i] = e + i < experts ? (A)row[e + i] : lowest(A(0));
+            }
+        }
+    }
+    // x becomes the probabilities; false for a row of -inf alone, which has none
+    __device__ __forceinline__ bool softmax(A m)
+    {
+        const A safe = finite_or_zero(m), scale = exp_scale_of();
+        A s = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            x[i] = exp_scaled(x[i] - safe, scale);
+            s += x[i];
+        }
+        s = group_reduce<G>(s, [](A a, A b) { return a + b; });
+        const A inv = A(1) / s;
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] *= inv;
+        return !(s == 0);
+    }
+    __device__ __forceinline__ static A exp_scale_of() { return sizeof(A) == 4 ? A(1.4426950408889634074) : A(1); }
+    __device__ __forceinline__ A highest() const
+    {
+        A m = lowest(A(0));
+#pragma unroll
+        for (int i = 0; i < N; ++i) m = max_of(m, x[i]);
+        return group_reduce<G>(m, [](A a, A b) { return max_of(a, b); });
+    }
+};
+
+__device__ __forceinline__ int segment_of(const Segments &s)
+{
+    int at = 0;
+    for (int i = 1; i < s.n; ++i) at += (int)blockIdx.x >= s.first[i];
+    return at;
+}
+
+// sums and counts of a workgroup's rows
+template <typename T, int G, int NV>
+__global__ __launch_bounds__(kThreads) void balance_kernel(BalanceArgs a)
+{
+    typedef RowPart<T, G, NV> Part;
+    typedef typename Part::A A;
+    constexpr int N = Part::N, kGroups = kThreads / G;
+    __shared__ A room_p[kThreads / 64][G * N];
+    __shared__ int room_c[kThreads / 64][G * N + 1];
+    const int tid = threadIdx.x, lane = tid % G, seg = segment_of(a.seg);
+    const int64_t rows = a.seg.rows[seg], groups = (int64_t)(a.seg.first[seg + 1] - a.seg.first[seg]) * kGroups;
+    A p[N] = {};
+    int c[N] = {}, n = 0;
+    for (int64_t row = (int64_t)((int)blockIdx.x - a.seg.first[seg]) * kGroups + tid / G; row < rows; row += groups) {
+        if (a.mask && !a.mask[row]) continue;
+        Part part;
+        part.load(static_cast<const T *>(a.seg.z[seg]) + row * a.seg.stride[seg], lane, a.experts);
+        const A m = part.highest();
+        // the choice: k times the highest that is left, of equal ones the lowest; -inf is none, NaN is above everything
+        A left[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) left[i] = part.x[i] != part.x[i] ? -lowest(A(0)) : part.x[i];
+        A top = m;
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) nan |= part.x[i] != part.x[i];
+        nan = group_reduce<G>((int)nan, [](int x, int y) { return x | y; });
+        if (nan) top = -lowest(A(0));
+        const bool any = part.softmax(m);
+        if (!any) continue;                                           // (of the whole group)
+        n += 1;
+        for (int pick = 0; pick < a.k; ++pick) {
+            if (pick) {
+                top = lowest(A(0));
+#pragma unroll
+                for (int i = 0; i < N; ++i) top = max_of(top, left[i]);
+                top = group_reduce<G>(top, [](A x, A y) { return max_of(x, y); });
+            }
+            if (top == lowest(A(0))) break;
+            int chosen = kMaxExperts;
+#pragma unroll
+            for (int i = N - 1; i >= 0; --i) chosen = left[i] == top ? Part::expert(lane, i) : chosen;
+            chosen = group_reduce<G>(chosen, [](int x, int y) { return x < y ? x : y; });
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const bool it = Part::expert(lane, i) == chosen;
+                c[i] += it;
+                left[i] = it ? lowest(A(0)) : left[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] += part.x[i];
+    }
+    // groups of a wavefront, then its four wavefronts, in a fixed order
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int by = G; by < 64; by <<= 1) {
+            p[i] += __shfl_xor(p[i], by);
+            c[i] += __shfl_xor(c[i], by);
+        }
+#pragma unroll
+    for (int by = G; by < 64; by <<= 1) n += __shfl_xor(n, by);
+    if ((tid & 63) < G) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            room_p[tid >> 6][Part::expert(lane, i)] = p[i];
+            room_c[tid >> 6][Part::expert(lane, i)] = c[i];
+        }
+        if (lane == 0) room_c[tid >> 6][G * N] = n;
+    }
+    __syncthreads();
+    A *sums = reinterpret_cast<A *>(a.sums) + (int64_t)blockIdx.x * a.experts;
+    int *counts = a.counts + (int64_t)blockIdx.x * (a.experts + 1);
+    for (int e = tid; e <= a.experts; e += kThreads) {
+        const int s = e < a.experts ? e : G * N;
+        int cc = 0;
+        A pp = 0;
+        for (int w = 0; w < kThreads / 64; ++w) {
+            cc += room_c[w][s];
+            if (e < a.experts) pp += room_p[w][s];
+        }
+        counts[e] = cc;
+        if (e < a.experts) sums[e] = pp;
+    }
+}
+
+struct FinishArgs {
+    Segments seg;
+    int experts, k;
+    const void *sums;
+    const int *counts;
+    double weight;
+    void *loss, *w;                                                   // A, [segments][experts] in A
+    int64_t *count_out;                                               // [segments][experts]
+    double *seg_loss;                                                 // [segments]
+};
+
+// One workgroup per segment: rows per expert and in all, the coefficients of the gradient and the segment's share of the loss.
+template <typename A>
+__global__ __launch_bounds__(1024) void balance_finish_kernel(FinishArgs a)
+{
+    __shared__ double room[16], sum_p[1024];
+    __shared__ int64_t sum_c[1024];
+    const int seg = blockIdx.x, tid = threadIdx.x, first = a.seg.first[seg], end = a.seg.first[seg + 1];
+    double n[1] = {0};
+    for (int w = first + tid; w < end; w += 1024) n[0] += a.counts[(int64_t)w * (a.experts + 1) + a.experts];
+    block_reduce<true, 1024>(n, room);
+    // threads in `slices` rows of `experts`: each adds the workgroups slice, slice + slices, ...
+    const int slices = 1024 / a.experts, slice = tid / a.experts, e = tid % a.experts;
+    double p = 0;
+    int64_t c = 0;
+    if (slice < slices)
+        for (int w = first + slice; w < end; w += slices) {
+            p += (double)static_cast<const A *>(a.sums)[(int64_t)w * a.experts + e];
+            c += a.counts[(int64_t)w * (a.experts + 1) + e];
+        }
+    sum_p[tid] = p;
+    sum_c[tid] = c;
+    __syncthreads();
+    double term[1] = {0};
+    if (tid < a.experts) {
+        for (int s = 1; s < slices; ++s) {
+            p += sum_p[s * a.experts + tid];
+            c += sum_c[s * a.experts + tid];
+        }
+        const double w = n[0] == 0 ? 0 : a.weight * a.experts * (double)c / ((double)a.k * n[0] * n[0]);
+        a.count_out[(int64_t)seg * a.experts + tid] = c;
+        static_cast<A *>(a.w)[(int64_t)seg * a.experts + tid] = (A)w;
+        term[0] = w * p;
+    }
+    block_reduce<true, 1024>(term, room);
+    if (tid == 0) {
+        if (a.seg.n == 1) *static_cast<A *>(a.loss) = (A)term[0];
+        else a.seg_loss[seg] = term[0];
+    }
+}
+
+template <typename A>
+__global__ void balance_sum_kernel(const double *seg_loss, int n, A *loss)
+{
+    double s = 0;
+    for (int i = 0; i < n; ++i) s += seg_loss[i];
+    *loss = (A)s;
+}
+
+// the gradient
+template <typename T, int G, int NV>
+__global__ __launch_bounds__(kThreads) void balance_grad_kernel(BalanceArgs a)
+{
+    typedef RowPart<T, G, NV> Part;
+    typedef typename Part::A A;
+    constexpr int N = Part::N, VEC = Part::VEC, kGroups = kThreads / G;
+    const int tid = threadIdx.x, lane = tid % G, seg = segment_of(a.seg);
+    const int64_t rows = a.seg.rows[seg], groups = (int64_t)(a.seg.first[seg + 1] - a.seg.first[seg]) * kGroups;
+    const A up = *static_cast<const A *>(a.upstream);
+    A w[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int e = Part::expert(lane, i);
+        w[i] = e < a.experts ? static_cast<const A *>(a.w)[(int64_t)seg * a.experts + e] : A(0);
+    }
+    for (int64_t row = (int64_t)((int)blockIdx.x - a.seg.first[seg]) * kGroups + tid / G; row < rows; row += groups) {
+        T *out = static_cast<T *>(a.seg.grad[seg]) + row * a.experts;
+        Part part;
+        bool any = !a.mask || a.mask[row];
+        if (any) {
+            part.load(static_cast<const T *>(a.seg.z[seg]) + row * a.seg.stride[seg], lane, a.experts);
+            any = part.softmax(part.highest());
+        }
+        A mean = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) mean += any ? w[i] * part.x[i] : A(0);
+        mean = group_reduce<G>(mean, [](A x, A y) { return x + y; });
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int e = (j * G + lane) * VEC;
+            typename Vec16<T>::type v;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = any ? (T)(part.x[j * VEC + i] * (w[j * VEC + i] - mean) * up) : (T)0.f;
+            if (e + VEC <= a.experts) {
+                *reinterpret_cast<typename Vec16<T>::type *>(out + e) = v;
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i)
+                    if (e + i < a.experts) out[e + i] = v[i];
+            }
+        }
+    }
+}
+
+// call(T(), lanes per row, pieces per lane) for a number of experts
+template <typename T, typename F>
+void with_part(int experts, F call)
+{
+    const int pieces = (experts + Vec16<T>::N - 1) / Vec16<T>::N;
+    if (pieces <= 1) return call(std::integral_constant<int, 1>(), std::integral_constant<int, 1>());
+    if (pieces <= 2) return call(std::integral_constant<int, 2>(), std::integral_constant<int, 1>());
+    if (pieces <= 4) return call(std::integral_constant<int, 4>(), std::integral_constant<int, 1>());
+    if (pieces <= 8) return call(std::integral_constant<int, 8>(), std::integral_constant<int, 1>());
+    if (pieces <= 16) return call(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
+    if (pieces <= 64) return call(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+    if (pieces <= 256) return call(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+    call(std::integral_constant<int, 64>(), std::integral_constant<int, 8>());
+}
+
+template <typename T>
+int lanes_of(int experts)
+{
+    int g = 0;
+    with_part<T>(experts, [&](auto lanes, auto) { g = decltype(lanes)::value; });
+    return g;
+}
+
+constexpr int kMostGroups = 1024;                                     // workgroups of the sums
+
+// workgroups per segment, `most` in all or a few more: by rows, one at least
+int64_t share_out(Segments &s, int64_t per_group, int64_t most)
+{
+    int64_t total = 0;
+    for (int i = 0; i < s.n; ++i) total += s.rows[i];
+    int64_t at = 0;
+    for (int i = 0; i < s.n; ++i) {
+        s.first[i] = (int)at;
+        const int64_t need = clg_ceil_div(s.rows[i], per_group), fair = total ? (int64_t)((double)most * s.rows[i] / total) : 0;
+        at += need < fair ? need : fair < 1 ? 1 : fair;
+        if (at == s.first[i]) ++at;
+    }
+    s.first[s.n] = (int)at;
+    return at;
+}
+
+int check_segments(const char *name, int dtype, int n, const void *const *logits, const int64_t *rows, const int64_t *strides, int64_t experts, int64_t k,
+                   const uint8_t *mask, Segments &s)
+{
+    CLG_REQUIRE(clg_score_type(dtype), "%s: unsupported dtype %d", name, dtype);
+    CLG_REQUIRE(n >= 1 && n <= kSegments && logits && rows && strides, "%s: 1 to %d tensors, got %d", name, kSegments, n);
+    CLG_REQUIRE(experts >= 1 && experts <= kMaxExperts, "%s: 1 to %d experts, got %lld", name, kMaxExperts, (long long)experts);
+    CLG_REQUIRE(k >= 1 && k <= experts, "%s: a row chooses 1 to %lld experts, got %lld", name, (long long)experts, (long long)k);
+    CLG_REQUIRE(!mask || n == 1, "%s: a mask is of one tensor", name);
+    s.n = n;
+    for (int i = 0; i < n; ++i) {
+        CLG_REQUIRE(rows[i] >= 0 && rows[i] < (int64_t)1 << 31, "%s: %lld rows", name, (long long)rows[i]);
+        CLG_REQUIRE(logits[i] || !rows[i], "%s: null pointer", name);
+        CLG_REQUIRE(strides[i] >= 0, "%s: negative row stride", name);
+        s.z[i] = logits[i], s.rows[i] = rows[i], s.stride[i] = strides[i], s.grad[i] = nullptr;
+    }
+    return CLG_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t clg_balance_scratch_bytes(int dtype, int64_t experts)
+{
+    if (!clg_score_type(dtype) || experts < 1 || experts > kMaxExperts) return 0;
+    const int64_t groups = kMostGroups + kSegments;
+    return groups * experts * (dtype == CLG_F64 ? 8 : 4) + groups * (experts + 1) * 4 + kSegments * 8 + 8;
+}
+
+extern "C" int clg_balance_forward(int dtype, int n, const void *const *logits, const int64_t *rows, const int64_t *row_strides, int64_t experts, int64_t k,
+                                   const uint8_t *mask, double weight, void *loss, int64_t *counts, void *coefs, void *scratch, void *stream)
+{
+    BalanceArgs a{};
+    if (const int rc = check_segments("clg_balance_forward", dtype, n, logits, rows, row_strides, experts, k, mask, a.seg)) return rc;
+    CLG_REQUIRE(loss && counts && coefs && scratch, "clg_balance_forward: null pointer");
+    const bool f64 = dtype == CLG_F64;
+    double *seg_loss = static_cast<double *>(scratch);
+    a.experts = (int)experts, a.k = (int)k, a.mask = mask;
+    a.sums = reinterpret_cast<float *>(seg_loss + kSegments);
+    a.counts = reinterpret_cast<int *>(reinterpret_cast<char *>(a.sums) + (kMostGroups + kSegments) * experts * (f64 ? 8 : 4));
+    const int rc = clg_with_type(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        const int64_t grid = share_out(a.seg, kThreads / lanes_of<T>(a.experts) * 4, kMostGroups);
+        with_part<T>(a.experts, [&](auto g, auto nv) {
+            balance_kernel<T, decltype(g)::value, decltype(nv)::value><<<dim3((unsigned)grid), dim3(kThreads), 0, clg_stream(stream)>>>(a);
+        });
+        return CLG_OK;
+    });
+    if (rc) return rc;
+    CLG_CHECK_LAUNCH("clg_balance_forward");
+    const FinishArgs f{a.seg, a.experts, a.k, a.sums, a.counts, weight / n, loss, coefs, counts, seg_loss};
+    if (f64) balance_finish_kernel<double><<<dim3(n), dim3(1024), 0, clg_stream(stream)>>>(f);
+    else balance_finish_kernel<float><<<dim3(n), dim3(1024), 0, clg_stream(stream)>>>(f);
+    CLG_CHECK_LAUNCH("clg_balance_forward");
+    if (n > 1) {
+        if (f64) balance_sum_kernel<double><<<dim3(1), dim3(1), 0, clg_stream(stream)>>>(seg_loss, n, static_cast<double *>(loss));
+        else balance_sum_kernel<float><<<dim3(1), dim3(1), 0, clg_stream(stream)>>>(seg_loss, n, static_cast<float *>(loss));
+        CLG_CHECK_LAUNCH("clg_balance_forward");
+    }
+    return CLG_OK;
+}
+
+extern "C" int clg_balance_backward(int dtype, int n, const void *const *logits, const int64_t *rows, const int64_t *row_strides, int64_t experts,
+                                    const uint8_t *mask, const void *coefs, const void *upstream, void *const *grads, void *stream)
+{
+    BalanceArgs a{};
+    if (const int rc = check_segments("clg_balance_backward", dtype, n, logits, rows, row_strides, experts, 1, mask, a.seg)) return rc;
+    CLG_REQUIRE(coefs && upstream && grads, "clg_balance_backward: null pointer");
+    for (int i = 0; i < n; ++i) {
+        CLG_REQUIRE(grads[i] || !rows[i], "clg_balance_backward: null pointer");
+        a.seg.grad[i] = grads[i];
+    }
+    a.experts = (int)experts, a.mask = mask, a.w = coefs, a.upstream = upstream;
+    const int rc = clg_with_type(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        const int64_t grid = share_out(a.seg, kThreads / lanes_of<T>(a.experts), 8192);
+        with_part<T>(a.experts, [&](auto g, auto nv) {
+            balance_grad_kernel<T, decltype(g)::value, decltype(nv)::value><<<dim3((unsigned)grid), dim3(kThreads), 0, clg_stream(stream)>>>(a);
+        });
+        return CLG_OK;
+    });
+    if (rc) return rc;
+    CLG_CHECK_LAUNCH("clg_balance_backward");
+    return CLG_OK;
+}

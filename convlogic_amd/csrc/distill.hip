@@ -1,0 +1,330 @@
+// Distillation from a teacher's top logits: the loss of each row and, in the same pass, its gradient w.r.t. the student's logits.
+//
+// With u = z / tau, q = softmax(u), entries (t_j, c_j) of the teacher and p_j their probabilities (over the entries alone, or with the teacher's
+// logsumexp L over all columns, p_j = exp(t_j / tau - L), and p_r = 1 - sum p_j for everything else):
+//     loss = tau^2 [ sum_j p_j (log p_j - log q_{c_j}) + p_r (log p_r - log q_r) ],        q_r = sum of q over the columns that are not listed
+//     d loss / d z_v = tau [ M q_v - sum_{j: c_j = v} p_j ]  listed,    tau q_v [ M - p_r / q_r ]  not listed,        M = sum_j p_j + p_r
+// q_r is small where the student agrees with its teacher, so it is no difference of sums: listed columns leave the row first (a bit per column in
+// LDS), their few exponentials are added to the sum of the others afterwards.
+#include "row_tile.h"
+
+namespace {
+
+struct DistillArgs {
+    const void *z;                                                    // [rows][cols] with a stride between rows
+    int64_t rows, cols, row_stride;
+    const void *values, *columns, *lse;                               // [rows][k], [rows][k], [rows] or NULL
+    int values_type, lse_type, columns64, k;
+    const uint8_t *mask;                                              // [rows] or NULL
+    double temperature, loss_scale, grad_scale;
+    const double *per_count;                                          // factor of both that is known on the device only, or NULL
+    double *row_loss;                                                 // [rows] or NULL
+    void *out;                                                        // [rows] losses in A, or NULL
+    void *grad;                                                       // [rows][cols] or NULL
+    void *applied;                                                    // [rows] in A: the factor that `grad` was written with, or NULL
+    const void *upstream;                                             // A, [rows] with upstream_rows, or NULL for 1
+    int upstream_rows, only_changed;
+};
+
+constexpr int kFlagTwice = 1, kFlagListed = 2, kFlagBad = 4;
+
+// LDS of a workgroup: reduction room (16 wavefronts of 5 doubles), entries (probability, logit, column), bits of a tile
+template <typename A>
+size_t distill_lds(int k, int cols_of_tile /* whole words of bits */)
+{
+    return 16 * 5 * 8 + 16 + (size_t)k * (8 + sizeof(A) + 4) + (size_t)(cols_of_tile / 32) * 4;
+}
+
+// One workgroup per row.  A row that fits its registers (COLS columns) is read from memory once, for the sum and for the gradient; longer ones (MULTI)
+// tile by tile, twice.
+template <typename T, int THREADS, int NV, bool MULTI>
+__global__ __launch_bounds__(THREADS) void distill_kernel(DistillArgs a)
+{
+    typedef typename Wide<T>::type A;
+    typedef RowTile<T, THREADS, NV> Tile;
+    extern __shared__ char lds[];
+    double *room = reinterpret_cast<double *>(lds), *prob = room + 16 * 5 + 2;
+    int *flags = reinterpret_cast<int *>(room + 16 * 5);
+    A *logit = reinterpret_cast<A *>(prob + a.k);
+    int *column = reinterpret_cast<int *>(logit + a.k);
+    uint32_t *bits = reinterpret_cast<uint32_t *>(column + a.k);
+    const int tid = threadIdx.x, k = a.k;
+    const A scale = exp_scale<A>(a.temperature);
+    const double inv_tau = 1.0 / a.temperature;
+
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const A up = a.upstream ? static_cast<const A *>(a.upstream)[a.upstream_rows ? row : 0] : A(1);
+        if (a.only_changed && static_cast<const A *>(a.applied)[row] == up) continue;
+        T *grad = a.grad ? static_cast<T *>(a.grad) + row * a.cols : nullptr;
+        const bool kept = !a.mask || a.mask[row];
+        const T *z = static_cast<const T *>(a.z) + row * a.row_stride;
+        Tile tile;
+        if (kept) tile.load(z, 0, a.cols);
+
+        // the teacher's entries
+        __syncthreads();
+        if (tid == 0) *flags = 0;
+        __syncthreads();
+        double top_t[3] = {lowest(0.0), lowest(0.0), 0};              // highest of the teacher, of the student's listed logits
+        if (kept) {
+            int seen = 0;
+            for (int j = tid; j < k; j += THREADS) {
+                const int64_t at = row * k + j, c = a.columns64 ? static_cast<const int64_t *>(a.columns)[at] : static_cast<const int32_t *>(a.columns)[at];
+                const bool there = c >= 0 && c < a.cols;
+                seen |= there ? kFlagListed : c >= a.cols ? kFlagBad : 0;
+                column[j] = there ? (int)c : -1;
+                if (!there) continue;
+                prob[j] = load_any(a.values, a.values_type, at) * inv_tau;
+                logit[j] = (A)z[c];
+                top_t[0] = max_of(top_t[0], prob[j]);
+                top_t[1] = max_of(top_t[1], (double)logit[j]);
+            }
+            if (seen) atomicOr(flags, seen);
+        }
+        // the sum over what is not listed
+        A m_t = lowest(A(0)), s_t = 0;
+        for (int64_t base = 0; kept && base < a.cols; base += Tile::COLS) {
+            if (MULTI && base) tile.load(z, base, a.cols);
+            const int n = (int)(a.cols - base < Tile::COLS ? a.cols - base : Tile::COLS);
+            for (int w = tid; w < (n + 31) / 32; w += THREADS) bits[w] = 0;
+            __syncthreads();
+            for (int j = tid; j < k; j += THREADS) {
+                const int64_t c = (int64_t)column[j] - base;
+                if (column[j] < 0 || c < 0 || c >= n) continue;
+                if (atomicOr(&bits[c >> 5], 1u << (c & 31)) >> (c & 31) & 1) atomicOr(flags, kFlagTwice);
+            }
+            __syncthreads();
+            A m = m_t;
+            tile.each([&](T &x, int c) {
+                if (bits[c >> 5] >> (c & 31) & 1) x = (T)lowest(0.f);
+                m = max_of(m, (A)x);
+            });
+            const A safe = finite_or_zero(m);
+            if (MULTI) s_t = rescaled(s_t, m_t, m, scale);
+            tile.each([&](T &x, int) { s_t += exp_scaled((A)x - safe, scale); });
+            m_t = m;
+            if (MULTI) __syncthreads();
+        }
+        __syncthreads();
+        const int flag = *flags;
+        if (!kept || !(flag & (kFlagListed | kFlagBad))) {            // a row that says nothing
+            if (tid == 0) {
+                if (a.row_loss) a.row_loss[row] = 0;
+                if (a.out) static_cast<A *>(a.out)[row] = 0;
+                if (a.applied) static_cast<A *>(a.applied)[row] = up;
+            }
+            if (grad)
+                for (int64_t c = tid; c < a.cols; c += THREADS) grad[c] = (T)0.f;
+            continue;
+        }
+        top_t[2] = m_t;
+        block_reduce<false, THREADS>(top_t, room);
+        const A m_u = (A)top_t[2], safe_u = finite_or_zero(m_u);
+        const double m = max_of(top_t[1], top_t[2]), base_t = a.lse ? load_any(a.lse, a.lse_type, row) : finite_or_zero(top_t[0]);
+        __syncthreads();
+
+        // sums: the rest of the row; listed exponentials, the teacher's, its share times the difference of the logarithms; distinct columns
+        double sums[5] = {(double)rescaled(s_t, m_t, m_u, scale), 0, 0, 0, 0};
+        for (int j = tid; j < k; j += THREADS) {
+            if (column[j] < 0) continue;
+            bool first = true;
+            if (flag & kFlagTwice)
+                for (int i = 0; i < j && first; ++i) first = column[i] != column[j];
+            const double u = ((double)logit[j] - m) * inv_tau, t = prob[j] - base_t, e = exp(t);
+            if (first) {
+                sums[1] += exp(u);
+                sums[4] += 1;
+            }
+            sums[2] += e;
+            if (e != 0) sums[3] += e * (t - u);
+            prob[j] = e;
+        }
+        block_reduce<true, THREADS>(sums, room);
+        const double shift = exp((m_u - m) * inv_tau), s_u = sums[0], total = s_u * shift + sums[1], log_total = log(total);
+        double mass, rest = 0, loss, per = 1;                         // per: of an entry's exponential
+        if (a.lse) {
+            rest = sums[4] == (double)a.cols ? 0 : max_of(0.0, 1 - sums[2]);
+            if (sums[2] != sums[2]) rest = sums[2];
+            mass = sums[2] + rest;
+            loss = sums[3] + sums[2] * log_total;
+            if (rest != 0) loss += rest * (log(rest) - ((m_u - m) * inv_tau + log(s_u) - log_total));
+        } else {
+            per = sums[2] == 0 ? 0 : 1 / sums[2];
+            mass = sums[2] * per;
+            loss = sums[2] == 0 ? 0 : sums[3] * per + log_total - log(sums[2]);
+        }
+        if (flag & kFlagBad) loss = mass = __builtin_nan("");
+        const double factor = a.per_count ? *a.per_count : 1;
+        if (tid == 0) {
+            if (a.row_loss) a.row_loss[row] = loss * a.loss_scale;
+            if (a.out) static_cast<A *>(a.out)[row] = (A)(loss * a.loss_scale * factor);
+            if (a.applied) static_cast<A *>(a.applied)[row] = up;
+        }
+        if (!grad) continue;
+        const double g = a.grad_scale * factor * (double)up;
+        const double of_listed = mass / total;
+        const A of_rest = s_u == 0 && total > 0 && mass == mass ? A(0) : (A)(g * (of_listed * shift - rest / s_u));
+        for (int64_t base = 0; base < a.cols; base += Tile::COLS) {
+            if (MULTI) tile.load(z, base, a.cols);
+            tile.store(grad, base, [&](T x) { return exp_scaled((A)x - safe_u, scale) * of_rest; });
+        }
+        __syncthreads();                                              // the listed columns' own values go over those
+        for (int j = tid; j < k; j += THREADS) {
+            if (column[j] < 0) continue;
+            double p = prob[j];
+            if (flag & kFlagTwice) {
+                bool first = true;
+                for (int i = 0; i < j && first; ++i) first = column[i] != column[j];
+                if (!first) continue;
+                for (int i = j + 1; i < k; ++i) p += column[i] == column[j] ? prob[i] : 0;
+            }
+            grad[column[j]] = (T)(A)(g * (of_listed * exp(((double)logit[j] - m) * inv_tau) - p * per));
+        }
+    }
+}
+
+// 1 / number of kept rows, 0 where there are none
+__global__ __launch_bounds__(1024) void count_kept_kernel(const uint8_t *mask, int64_t rows, double *per_count)
+{
+    __shared__ double room[16];
+    double n[1] = {0};
+    for (int64_t i = threadIdx.x; i < rows; i += 1024) n[0] += mask[i] != 0;
+    block_reduce<true, 1024>(n, room);
+    if (threadIdx.x == 0) *per_count = n[0] == 0 ? 0 : 1 / n[0];
+}
+
+// the sum of the rows' losses, in a fixed order
+template <typename A>
+__global__ __launch_bounds__(1024) void sum_rows_kernel(const double *row_loss, int64_t rows, const double *per_count, A *out)
+{
+    __shared__ double room[16];
+    double s[1] = {0};
+    for (int64_t i = threadIdx.x; i < rows; i += 1024) s[0] += row_loss[i];
+    block_reduce<true, 1024>(s, room);
+    if (threadIdx.x == 0) *out = (A)(s[0] * (per_count ? *per_count : 1));
+}
+
+template <typename T, int THREADS, int NV, bool MULTI>
+void launch_as(const DistillArgs &a, int64_t grid, hipStream_t stream)
+{
+    typedef RowTile<T, THREADS, NV> Tile;
+    static_assert(Tile::COLS % 32 == 0, "bits of a tile fill whole words");
+    const size_t lds = distill_lds<typename Wide<T>::type>(a.k, Tile::COLS);
+    distill_kernel<T, THREADS, NV, MULTI><<<dim3((unsigned)grid), dim3(THREADS), lds, stream>>>(a);
+}
+
+template <typename T>
+void launch(const DistillArgs &a, int64_t grid, hipStream_t stream)
+{
+    const int64_t pieces = (a.cols + Vec16<T>::N - 1) / Vec16<T>::N;
+    if (pieces <= 64) return launch_as<T, 64, 1, false>(a, grid, stream);
+    if (pieces <= 64 * 4) return launch_as<T, 64, 4, false>(a, grid, stream);
+    if (pieces <= 256 * 4) return launch_as<T, 256, 4, false>(a, grid, stream);
+    if (pieces <= 256 * 16) return launch_as<T, 256, 16, false>(a, grid, stream);
+    if (pieces <= 1024 * 8) return launch_as<T, 1024, 8, false>(a, grid, stream);
+    if (pieces <= 1024 * 16) return launch_as<T, 1024, 16, false>(a, grid, stream);
+    launch_as<T, 1024, 8, true>(a, grid, stream);
+}
+
+}  // namespace
+
+constexpr int kMaxEntries = 1024;
+
+// what both entry points require of a call
+static int check_call(const char *name, int dtype, const void *logits, int64_t row_stride, const void *values, int values_dtype, const void *columns,
+                      int columns_bits, const void *lse, int lse_dtype, int64_t rows, int64_t cols, int64_t k, double temperature)
+{
+    CLG_REQUIRE(clg_score_type(dtype), "%s: unsupported dtype %d", name, dtype);
+    CLG_REQUIRE(clg_score_type(values_dtype) && (!lse || clg_score_type(lse_dtype)), "%s: unsupported dtype of the teacher's values", name);
+    CLG_REQUIRE(columns_bits == 32 || columns_bits == 64, "%s: columns must have 32 or 64 bits, got %d", name, columns_bits);
+    CLG_REQUIRE(rows >= 0 && cols >= 1 && cols < (int64_t)1 << 31, "%s: bad shape [%lld, %lld]", name, (long long)rows, (long long)cols);
+    CLG_REQUIRE(k >= 1 && k <= kMaxEntries, "%s: 1 to %d entries per row, got %lld", name, kMaxEntries, (long long)k);
+    CLG_REQUIRE(rows < (int64_t)1 << 31, "%s: %lld rows are more than a launch holds", name, (long long)rows);
+    CLG_REQUIRE(row_stride >= 0, "%s: negative row stride", name);
+    CLG_REQUIRE(temperature > 0 && temperature < 1e30, "%s: the temperature must be positive and finite", name);
+    CLG_REQUIRE(!rows || (logits && values && columns), "%s: null pointer", name);
+    return CLG_OK;
+}
+
+extern "C" int64_t clg_distill_scratch_bytes(int64_t rows) { return rows < 0 ? 0 : (rows + 2) * 8; }
+
+extern "C" int clg_distill_forward(int dtype, const void *logits, int64_t row_stride, const void *values, int values_dtype, const void *columns,
+                                   int columns_bits, const void *lse, int lse_dtype, const uint8_t *mask, int64_t rows, int64_t cols, int64_t k,
+                                   double temperature, double weight, int reduction, void *loss, void *grad, void *applied, void *scratch, void *stream)
+{
+    if (const int rc = check_call("clg_distill_forward", dtype, logits, row_stride, values, values_dtype, columns, columns_bits, lse, lse_dtype, rows, cols, k,
+                                  temperature))
+        return rc;
+    CLG_REQUIRE(reduction == CLG_REDUCE_NONE || reduction == CLG_REDUCE_SUM || reduction == CLG_REDUCE_MEAN, "clg_distill_forward: bad reduction %d", reduction);
+    CLG_REQUIRE(loss || (reduction == CLG_REDUCE_NONE && !rows), "clg_distill_forward: null pointer");
+    CLG_REQUIRE(reduction == CLG_REDUCE_NONE || scratch, "clg_distill_forward: null scratch");
+    CLG_REQUIRE(!grad == !applied, "clg_distill_forward: grad and applied come together");
+    CLG_REQUIRE(!grad || reduction != CLG_REDUCE_NONE, "clg_distill_forward: the gradient of a loss per row is clg_distill_backward's");
+    double *row_loss = static_cast<double *>(scratch), *per_count = row_loss ? row_loss + rows : nullptr;
+    DistillArgs a{};
+    a.z = logits, a.rows = rows, a.cols = cols, a.row_stride = row_stride;
+    a.values = values, a.columns = columns, a.lse = lse, a.values_type = values_dtype, a.lse_type = lse_dtype, a.columns64 = columns_bits == 64, a.k = (int)k;
+    a.mask = mask, a.temperature = temperature, a.loss_scale = temperature * temperature * weight, a.grad_scale = temperature * weight;
+    a.grad = grad, a.applied = applied;
+    if (reduction == CLG_REDUCE_NONE) a.out = loss;
+    else a.row_loss = row_loss;
+    if (reduction == CLG_REDUCE_MEAN && mask && rows) {
+        count_kept_kernel<<<dim3(1), dim3(1024), 0, clg_stream(stream)>>>(mask, rows, per_count);
+        CLG_CHECK_LAUNCH("clg_distill_forward");
+        a.per_count = per_count;
+    } else if (reduction == CLG_REDUCE_MEAN && rows) {
+        a.loss_scale /= rows, a.grad_scale /= rows;
+    }
+    if (rows) {
+        const int rc = clg_with_type(dtype, [&](auto t) {
+            launch<decltype(t)>(a, rows, clg_stream(stream));
+            return CLG_OK;
+        });
+        if (rc) return rc;
+        CLG_CHECK_LAUNCH("clg_distill_forward");
+    }
+    if (reduction == CLG_REDUCE_NONE) return CLG_OK;
+    if (dtype == CLG_F64)
+        sum_rows_kernel<double><<<dim3(1), dim3(1024), 0, clg_stream(stream)>>>(row_loss, rows, a.per_count, static_cast<double *>(loss));
+    else
+        sum_rows_kernel<float><<<dim3(1), dim3(1024), 0, clg_stream(stream)>>>(row_loss, rows, a.per_count, static_cast<float *>(loss));
+    CLG_CHECK_LAUNCH("clg_distill_forward");
+    return CLG_OK;
+}
+
+extern "C" int clg_distill_backward(int dtype, const void *logits, int64_t row_stride, const void *values, int values_dtype, const void *columns,
+                                    int columns_bits, const void *lse, int lse_dtype, const uint8_t *mask, int64_t rows, int64_t cols, int64_t k,
+                                    double temperature, double weight, int reduction, const void *upstream, void *grad, void *applied, void *scratch,
+                                    void *stream)
+{
+    if (const int rc = check_call("clg_distill_backward", dtype, logits, row_stride, values, values_dtype, columns, columns_bits, lse, lse_dtype, rows, cols,
+                                  k, temperature))
+        return rc;
+    CLG_REQUIRE(reduction == CLG_REDUCE_NONE || reduction == CLG_REDUCE_SUM || reduction == CLG_REDUCE_MEAN, "clg_distill_backward: bad reduction %d", reduction);
+    if (!rows) return CLG_OK;
+    CLG_REQUIRE(upstream && grad, "clg_distill_backward: null pointer");
+    DistillArgs a{};
+    a.z = logits, a.rows = rows, a.cols = cols, a.row_stride = row_stride;
+    a.values = values, a.columns = columns, a.lse = lse, a.values_type = values_dtype, a.lse_type = lse_dtype, a.columns64 = columns_bits == 64, a.k = (int)k;
+    a.mask = mask, a.temperature = temperature, a.grad_scale = temperature * weight;
+    a.grad = grad, a.applied = applied, a.only_changed = applied != nullptr, a.upstream = upstream, a.upstream_rows = reduction == CLG_REDUCE_NONE;
+    if (reduction == CLG_REDUCE_MEAN && mask) {
+        CLG_REQUIRE(scratch, "clg_distill_backward: null scratch");
+        a.per_count = static_cast<const double *>(scratch) + rows;
+        if (!applied) {
+            count_kept_kernel<<<dim3(1), dim3(1024), 0, clg_stream(stream)>>>(mask, rows, static_cast<double *>(scratch) + rows);
+            CLG_CHECK_LAUNCH("clg_distill_backward");
+        }
+    } else if (reduction == CLG_REDUCE_MEAN) {
+        a.grad_scale /= rows;
+    }
+    // (rows whose gradient is there already are passed over: few workgroups look at many of them)
+    const int64_t grid = applied && rows > 2048 ? 2048 : rows;
+    const int rc = clg_with_type(dtype, [&](auto t) {
+        launch<decltype(t)>(a, grid, clg_stream(stream));
+        return CLG_OK;
+    });
+    if (rc) return rc;
+    CLG_CHECK_LAUNCH("clg_distill_backward");
+    return CLG_OK;
+}

@@ -11,6 +11,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include "convlogic_amd.h"
+#include "loss_nodes.h"
 
 namespace {
 
@@ -650,4 +651,5 @@ PYBIND11_MODULE(_nodes, m)
     m.def("binary_block", &binary_block, no_gil);
     m.def("trees", &trees, no_gil);
     m.def("network", &network, no_gil);
+    add_loss_nodes(m);
 }

@@ -36,6 +36,7 @@ extern "C" {
 #define CLG_F32 0
 #define CLG_F64 1
 #define CLG_F16 2 /* IEEE half as a storage format of clg_fc_forward / _backward_w / _backward_x (arithmetic in float32) */
+#define CLG_BF16 3 /* bfloat16: scores and logits of clg_top_logits / clg_distill_* / clg_balance_*, which take all four types */
 
 #define CLG_OK 0
 #define CLG_EINVAL (-1)  /* rejected argument (shape, dtype, null pointer, limit) */
@@ -663,6 +664,54 @@ int clg_pack_binary_images(const float *x, uint64_t *words, int64_t n, int64_t c
  * travel in the launch itself. */
 int clg_threshold_pack_images_host(const float *x, const float *thresholds, uint64_t *words, int64_t n, int64_t c0,
                                    int64_t hw, int64_t levels, void *stream);
+
+/* ---------------------------------------------------------------------------------
+ * losses on scores and on gate logits (no counterpart in the reference)
+ * ------------------------------------------------------------------------------- */
+
+/* The k highest logits of each row, highest first, and the columns they are in; of equal values the lowest column comes first, a NaN counts
+ * as the maximum, as in clg_gate_argmax.  lse, if not NULL: log sum_v exp(logits[v] / temperature) of the whole row, float32 (float64 for CLG_F64).
+ * dtype: CLG_F32, CLG_F64, CLG_F16 or CLG_BF16; row_stride: elements from one row to the next, the columns of a row are dense.  1 <= k <= 1024. */
+int clg_top_logits(int dtype, const void *logits /*[rows,cols]*/, int64_t row_stride, int64_t rows, int64_t cols, int64_t k, double temperature,
+                   void *values /*[rows,k]*/, int64_t *columns /*[rows,k]*/, void *lse /*[rows] or NULL*/, void *stream);
+
+/* Distillation from a teacher's top logits.  Per row, with u = logits / temperature, q = softmax(u) and the teacher's probabilities p_j of its entries
+ * (values[j], columns[j]) -- their softmax, or with lse (as clg_top_logits gives it) exp(values[j] / temperature - lse) and one more answer, "none of
+ * these", for what is left of 1 --
+ *     loss = weight temperature^2 [sum_j p_j (log p_j - log q_columns[j]) + p_r (log p_r - log q_r)],    q_r = sum of q over the columns that are not listed.
+ * An entry with a negative column is none; a row without entries or with mask[row] == 0 has loss 0 and gradient 0 whatever its logits; a column of cols or
+ * more makes its row NaN.  The terms of a column that is listed twice add up.  CLG_REDUCE_MEAN divides by the number of rows whose mask is set (0 rows: 0).
+ *   loss      one value, or [rows] for CLG_REDUCE_NONE; float32, float64 for CLG_F64
+ *   grad      NULL, or [rows,cols] dense: the gradient for an upstream gradient of 1, from the same pass over the logits (not for CLG_REDUCE_NONE)
+ *   applied   NULL, or [rows] of loss's type, with grad: the upstream gradient that each row of it holds
+ *   scratch   clg_distill_scratch_bytes(rows) bytes (not for CLG_REDUCE_NONE); clg_distill_backward takes it as the forward call left it
+ * clg_distill_backward: upstream is one value, or [rows] for CLG_REDUCE_NONE.  With applied, rows of grad that hold it already are left
+ * as they are and the others are computed again; without, all are. */
+#define CLG_REDUCE_NONE 0
+#define CLG_REDUCE_SUM 1
+#define CLG_REDUCE_MEAN 2
+int64_t clg_distill_scratch_bytes(int64_t rows);
+int clg_distill_forward(int dtype, const void *logits /*[rows,cols]*/, int64_t row_stride, const void *values /*[rows,k]*/, int values_dtype,
+                        const void *columns /*[rows,k]*/, int columns_bits /*32 or 64*/, const void *lse /*[rows] or NULL*/, int lse_dtype,
+                        const uint8_t *mask /*[rows] or NULL*/, int64_t rows, int64_t cols, int64_t k, double temperature, double weight, int reduction,
+                        void *loss, void *grad, void *applied, void *scratch, void *stream);
+int clg_distill_backward(int dtype, const void *logits, int64_t row_stride, const void *values, int values_dtype, const void *columns, int columns_bits,
+                         const void *lse, int lse_dtype, const uint8_t *mask, int64_t rows, int64_t cols, int64_t k, double temperature, double weight,
+                         int reduction, const void *upstream, void *grad, void *applied, void *scratch, void *stream);
+
+/* How evenly rows choose among experts, for up to 16 tensors of logits [rows[i], experts] at once (the gates of a network's layers are 16 experts
+ * of which each neuron takes one).  Per tensor, with p = softmax of a row, the k highest logits chosen (of equal ones the lowest; -inf never), counts[e] rows
+ * that chose expert e and n rows in all: experts / (k n^2) sum_e counts[e] sum_t p[t][e]; loss is weight times the mean over the tensors.  Rows with mask == 0
+ * (one tensor only) and rows of -inf alone do not count and have gradient 0.
+ *   logits, rows, row_strides, grads   host arrays of n entries; grads dense
+ *   loss      float32, float64 for CLG_F64; coefs [n,experts] of the same type: what clg_balance_backward needs of the forward call
+ *   scratch   clg_balance_scratch_bytes(dtype, experts) bytes
+ * 1 <= experts <= 1024. */
+int64_t clg_balance_scratch_bytes(int dtype, int64_t experts);
+int clg_balance_forward(int dtype, int n, const void *const *logits, const int64_t *rows, const int64_t *row_strides, int64_t experts, int64_t k,
+                        const uint8_t *mask, double weight, void *loss, int64_t *counts /*[n,experts]*/, void *coefs, void *scratch, void *stream);
+int clg_balance_backward(int dtype, int n, const void *const *logits, const int64_t *rows, const int64_t *row_strides, int64_t experts,
+                         const uint8_t *mask, const void *coefs, const void *upstream, void *const *grads, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,501 @@
+"""The kernels of the losses on scores and gate logits against their definitions in 64 bits (oracle/losses_oracle.py).
+
+Bounds.  An exponential of a float32 argument x = (z - max) / temperature * log2(e) is off by the two roundings of x, 2 |x| 2^-24 relative, and by its
+own 2 steps; the terms that matter have |x| <= X = log2(e) (max - min) / temperature, and what is further down than 2^-126 may vanish.  A sum of n such
+terms in at most 160 additions in a row (128 elements of a thread, a tree over the workgroup, tiles) is off by 160 steps more.  So values are within
+(2 X + 170) 2^-24 of the sum of the magnitudes they are made of, and half a step of the type they are rounded to; 2^-53 in place of 2^-24 for float64."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import convlogic_amd as C
+from oracle import losses_oracle as L
+from tests.gpu_util import DEV
+
+pytestmark = pytest.mark.gpu
+
+NAN, INF = math.nan, math.inf
+TYPES = [torch.float32, torch.bfloat16, torch.float16, torch.float64]
+
+
+def scores(rows, cols, dtype=torch.float32, seed=0, scale=3.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(rows, cols, generator=g) * scale).to(dtype).to(DEV)
+
+
+def spread(z, temperature=1.0):
+    finite = z.detach()[torch.isfinite(z)].double()
+    return min(1.4427 * float(finite.max() - finite.min()) / temperature if finite.numel() else 0.0, 150.0)
+
+
+def close(got, want, size, z, name, temperature=1.0, steps=170):
+    unit = 2.0 ** -53 if z.dtype == torch.float64 else 2.0 ** -24
+    half = torch.finfo(got.dtype).eps / 2
+    least = torch.finfo(got.dtype).smallest_normal * (1 if got.dtype == torch.float32 else torch.finfo(got.dtype).eps)
+    g = got.detach().double().cpu().numpy()
+    bound = (2 * spread(z, temperature) + steps) * unit * np.asarray(size) + half * np.abs(want) * (1 + 2.0 ** -10) + least
+    assert g.shape == np.shape(want), name
+    assert np.array_equal(np.isnan(g), np.isnan(want)), name
+    with np.errstate(invalid="ignore"):
+        bad = ~(np.isnan(want) | (np.abs(g - want) <= bound) | (g == want))
+    assert not bad.any(), (name, int(bad.sum()), np.abs(g - want)[bad].max(), np.broadcast_to(bound, g.shape)[bad].min())
+
+
+def host(t):
+    return None if t is None else t.detach().double().cpu().numpy()
+
+
+# ---- top logits ----------------------------------------------------------------------------------
+def check_top(z, k, temperature=1.0):
+    got = C.top_logits(z, k, temperature=temperature)
+    flat = z.detach().double().cpu().reshape(-1, z.shape[-1])
+    values, columns, lse = [], [], []
+    for row in flat:                                                  # (as the oracle, with a sort that takes long rows)
+        order = np.lexsort((np.arange(len(row)), -row.nan_to_num(nan=INF, posinf=INF, neginf=-INF).numpy(), ~row.isnan().numpy()))[:k]
+        columns.append(order)
+        values.append(row.numpy()[order])
+        lse.append(float(torch.logsumexp(row / temperature, 0)) if not row.isnan().any() else NAN)
+    indices = got.indices.cpu().reshape(-1, k).numpy()
+    assert np.array_equal(indices, np.array(columns)), (indices, columns)
+    assert np.array_equal(got.values.double().cpu().reshape(-1, k).numpy(), np.array(values), equal_nan=True)
+    assert got.values.dtype == z.dtype and got.values.shape == (*z.shape[:-1], k) and got.logsumexp.shape == z.shape[:-1]
+    want = np.array(lse).reshape(got.logsumexp.shape)
+    close(got.logsumexp, want, 1 + np.where(np.isfinite(want), np.abs(want), 0) * 0, z, "logsumexp", temperature)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [1, 2, 7, 8, 9, 10, 63, 64, 65, 128, 129, 255, 257, 511, 512, 513, 1000, 1025, 2047, 2049, 4097, 8191, 8193])
+def test_top_logits(dtype, cols):
+    for k in sorted({1, min(3, cols), min(cols, 40), min(cols, 300)}):
+        check_top(scores(3, cols, dtype, cols + k), k, 1.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [16385, 32767, 32768, 32769, 65535, 65537, 131071, 131072, 131073, 200003])
+def test_top_logits_of_long_rows(dtype, cols):
+    for k in (1, 64, 257):
+        check_top(scores(2, cols, dtype, cols + k), k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols,k", [(10, 10), (700, 700), (700, 5), (5000, 64), (5000, 1024), (40000, 20), (140000, 100), (300000, 1024)])
+def test_top_logits_of_rows_that_are_hard_to_sort(dtype, cols, k):
+    up = torch.linspace(-50, 50, cols, dtype=torch.float64)
+    few = torch.randint(0, 3, (cols,), generator=torch.Generator().manual_seed(1)).double()
+    rows = [up, up.flip(0), torch.zeros(cols, dtype=torch.float64), few, torch.full((cols,), -INF, dtype=torch.float64)]
+    block = torch.randn(cols, generator=torch.Generator().manual_seed(2)).double()
+    start = cols // 3
+    block[start:start + 2 * k] += 100                                 # the highest next to one another
+    rows.append(block)
+    low = torch.full((cols,), float(torch.finfo(dtype).min), dtype=torch.float64)
+    low[-1] = 0
+    rows.append(low)
+    check_top(torch.stack(rows).to(dtype).to(DEV), k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [9, 600, 70000, 150000])
+def test_top_logits_orders_nan_infinities_and_zeros(dtype, cols):
+    z = scores(4, cols, dtype, cols)
+    z[0, 1], z[0, cols - 1], z[0, 4], z[0, cols // 2] = NAN, NAN, INF, -INF
+    z[1] = -z[1].abs()
+    z[1, cols - 2], z[1, 3] = -0.0, 0.0
+    z[2] = -INF
+    z[2, cols - 3] = -7.0
+    z[3, 2], z[3, 6] = INF, INF
+    check_top(z, 9)
+
+
+def test_top_logits_of_views_streams_and_graphs():
+    z = scores(40, 333, torch.float32, 1)
+    for view in (z[:, 5:300], z[::3, ::2], z.t(), z.view(4, 10, 333), z.view(4, 10, 333).transpose(0, 1), z[0], z[:1].expand(5, -1)):
+        check_top(view, 7)
+    assert C.top_logits(z[:0], 4).values.shape == (0, 4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = C.top_logits(z, 7)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        recorded = C.top_logits(z, 7)
+    for i in range(3):
+        want = C.top_logits(z, 7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(recorded, want)) and (i or all(torch.equal(a, b) for a, b in zip(other, want)))
+        z.copy_(scores(40, 333, torch.float32, 7 + i))
+
+
+# ---- distillation --------------------------------------------------------------------------------
+def teacher(rows, cols, k, rest, seed, temperature):
+    t = C.top_logits(scores(rows, cols, torch.float32, seed + 1000), k, temperature=temperature)
+    return t.values, t.indices, t.logsumexp if rest else None
+
+
+def check_distill(z, values, columns, lse, temperature=1.0, mask=None, weight=1.0, reduction="mean", upstream=None):
+    leaf = z.detach().requires_grad_(True)
+    kw = dict(temperature=temperature, mask=mask, weight=weight, reduction=reduction)
+    loss = C.distillation_loss(leaf, values, columns, lse, **kw)
+    alone = C.distillation_loss(z.detach(), values, columns, lse, **kw)
+    assert torch.equal(loss, alone) or bool(loss.isnan().any())
+    grad, = torch.autograd.grad(loss, leaf, upstream)
+    flat = (lambda t: None if t is None else t.reshape(-1, t.shape[-1]))
+    want = L.distillation(host(flat(z)), host(flat(values)), flat(columns).cpu().numpy(), None if lse is None else host(lse.reshape(-1)), temperature,
+                          None if mask is None else mask.reshape(-1).cpu().numpy(), weight, reduction,
+                          None if upstream is None else host(upstream.reshape(-1)) if reduction == "none" else host(upstream))
+    close(loss, np.reshape(want[0], loss.shape), np.reshape(want[2], loss.shape), z, "loss", temperature)
+    close(grad, np.reshape(want[1], grad.shape), np.reshape(want[3], grad.shape), z, "grad", temperature)
+    assert grad.dtype == z.dtype
+    return loss, grad
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("cols", [1, 2, 7, 8, 9, 10, 33, 64, 127, 255, 256, 257, 511, 513, 1000, 2047, 2049, 4100, 8191, 8193])
+def test_distillation(dtype, rest, cols):
+    for k in sorted({1, min(4, cols), min(33, cols), min(300, cols)}):
+        z = scores(3, cols, dtype, cols)
+        check_distill(z, *teacher(3, cols, k, rest, k, 2.0), temperature=2.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("cols", [16385, 32768, 32769, 65535, 65536, 65537, 131071, 131072, 131073, 200003])
+def test_distillation_over_long_rows(dtype, rest, cols):
+    z = scores(2, cols, dtype, cols)
+    check_distill(z, *teacher(2, cols, 64, rest, 3, 1.0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("cols", [10, 301, 9000])
+def test_distillation_of_padded_rows(dtype, reduction, cols):
+    z = scores(7, cols, dtype, 5)
+    values, columns, _ = teacher(7, cols, 6, False, 5, 1.5)
+    columns[0, 3:], columns[1], columns[2, 0] = -1, -5, -1            # short rows, one without entries
+    mask = torch.tensor([True, True, True, False, True, False, True], device=DEV)
+    z[3], z[5, 0], z[1, 2] = NAN, INF, NAN                            # rows that do not count
+    up = torch.rand(7, device=DEV).to(torch.float64 if dtype == torch.float64 else torch.float32)
+    up = up if reduction == "none" else up[0]
+    _, grad = check_distill(z, values, columns, None, 1.5, mask, 0.3, reduction, up)
+    assert (grad[[1, 3, 5]] == 0).all()
+    none = C.distillation_loss(z, values, columns, mask=torch.zeros_like(mask), reduction=reduction)
+    assert (none == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [12, 700, 70000, 140000])
+def test_distillation_of_special_values(dtype, cols):
+    # columns that the student masks, by -inf and by the type's lowest value; a row that is lowest everywhere; all scores far below zero
+    z = scores(5, cols, dtype, 6)
+    values, columns, lse = teacher(5, cols, 5, True, 6, 1.0)
+    for r in range(5):
+        free = [c for c in range(8) if c not in columns[r].tolist()]
+        z[r, free[0]] = -INF
+        z[r, free[1]] = torch.finfo(dtype).min
+    z[3] = torch.finfo(dtype).min
+    z[4] -= 500.0
+    for r in (slice(0, 3), slice(3, 4), slice(4, 5)):
+        for l in (None, lse[r]):
+            check_distill(z[r], values[r], columns[r], l)
+    # the teacher has mass where the student has none
+    x = scores(2, cols, dtype, 7)
+    x[1, columns[1, 0]] = -INF
+    loss = C.distillation_loss(x, values[:2], columns[:2], reduction="none")
+    assert loss[0].isfinite() and loss[1] == INF
+    # a student that has nothing but the listed columns
+    y = torch.full((1, cols), -INF, dtype=dtype, device=DEV)
+    y[0, columns[0]] = 1.0
+    assert C.distillation_loss(y, values[:1], columns[:1]).isfinite() and C.distillation_loss(y, values[:1], columns[:1], lse[:1]) == INF
+    # NaN and +inf of the student, NaN of the teacher, a column behind the last: their own rows
+    x = scores(5, cols, dtype, 8).requires_grad_(True)
+    v, c = values.clone(), columns.clone()
+    with torch.no_grad():
+        x[0, [i for i in range(8) if i not in c[0].tolist()][0]] = NAN
+        x[1, 3] = INF
+    v[2, 1] = NAN
+    c[3, 4] = cols
+    for l in (None, lse):
+        loss = C.distillation_loss(x, v, c, l, reduction="none")
+        grad, = torch.autograd.grad(loss.sum(), x)
+        assert loss.isnan().tolist() == [True, True, True, True, False]
+        assert grad.isnan().any(1).tolist() == [True, True, True, True, False]
+    # teacher's values of -inf are no mass
+    v = values.clone()
+    v[0, 2], v[1] = -INF, -INF
+    check_distill(scores(5, cols, dtype, 9), v, columns, None)
+    check_distill(scores(5, cols, dtype, 9), v, columns, lse)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols,k", [(3, 3), (40, 7), (40, 100), (3000, 700), (70000, 1024), (140000, 50)])
+def test_distillation_of_columns_listed_twice(dtype, cols, k):
+    g = torch.Generator().manual_seed(k)
+    columns = torch.randint(0, cols, (4, k), generator=g).to(DEV)
+    columns[:, k // 2] = columns[:, 0]
+    columns[1] = columns[1, 0]
+    values = torch.randn(4, k, generator=g).to(DEV)
+    check_distill(scores(4, cols, dtype, 3), values, columns, None)
+    check_distill(scores(4, cols, dtype, 3), values, columns, torch.logsumexp(values, 1) + 1.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distillation_of_every_type_shape_and_layout_of_its_arguments(dtype):
+    z = scores(6, 50, dtype, 1)
+    values, columns, lse = teacher(6, 50, 4, True, 1, 1.0)
+    want = check_distill(z, values, columns, lse)
+    for c in (columns.int(), columns.t().contiguous().t()):
+        got = check_distill(z, values, c, lse)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for t in TYPES:
+        check_distill(z, values.to(t), columns, None)
+        check_distill(z, values.to(t), columns, lse.to(t))
+    wide = scores(12, 60, dtype, 2)
+    for view in (wide[::2, 3:53], wide[:6, :50], wide[:6, ::1][:, 10:], wide[6:, 5:55], wide[:1, :50].expand(6, -1)):
+        check_distill(view, values, columns, lse)
+    strided = scores(50, 6, dtype, 3).t()
+    check_distill(strided, values, columns, lse)
+    three = (z.view(2, 3, 50), values.view(2, 3, 4), columns.view(2, 3, 4), lse.view(2, 3))
+    for reduction in ("mean", "none"):
+        check_distill(*three, reduction=reduction, upstream=torch.ones(2, 3, device=DEV, dtype=lse.dtype if dtype != torch.float64 else dtype) if reduction == "none" else None)
+    check_distill(three[0].transpose(0, 1), three[1].transpose(0, 1), three[2].transpose(0, 1), three[3].transpose(0, 1))
+    check_distill(z[0], values[0], columns[0], lse[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [10, 3000])
+@pytest.mark.parametrize("masked", [False, True])
+def test_distillation_under_other_upstream_gradients_and_retained_graphs(dtype, cols, masked):
+    z = scores(5, cols, dtype, 2).requires_grad_(True)
+    values, columns, lse = teacher(5, cols, 4, True, 2, 1.0)
+    mask = torch.tensor([True, False, True, True, True], device=DEV) if masked else None
+    call = lambda: C.distillation_loss(z, values, columns, lse, mask=mask)
+    one, = torch.autograd.grad(call(), z)
+    half, = torch.autograd.grad(0.5 * call(), z)
+    assert torch.equal(half.double() * 2, one.double()) or dtype == torch.float16      # (powers of two are exact but for subnormal halves)
+    loss = call()
+    first, = torch.autograd.grad(loss, z, retain_graph=True)
+    keep = first.clone()
+    first.mul_(7)                                                     # the receiver's to change
+    second, = torch.autograd.grad(loss, z, torch.full_like(loss, 0.5), retain_graph=True)
+    third, = torch.autograd.grad(loss, z)
+    assert torch.equal(keep, one) and torch.equal(second, half) and torch.equal(third, one) and torch.equal(first, keep * 7)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(loss, z)
+    z.grad = None
+    call().backward()
+    call().backward()
+    assert torch.equal(z.grad, one + one)
+    zero, = torch.autograd.grad(call() * 0.0, z)
+    assert (zero == 0).all()
+    with torch.no_grad():
+        assert not call().requires_grad
+    # a second differentiation is refused, not answered with zero
+    g, = torch.autograd.grad(call(), z, create_graph=True)
+    assert torch.equal(g, one)
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        g.double().sum().backward()
+    # logits that change between the passes
+    x = z.detach().clone().requires_grad_(True)
+    y = x * 1
+    loss = C.distillation_loss(y, values, columns, lse)
+    y.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    again = torch.utils.checkpoint.checkpoint(lambda t: C.distillation_loss(t, values, columns, lse, mask=mask), z, use_reentrant=False)
+    assert torch.equal(torch.autograd.grad(again, z)[0], one)
+
+
+def test_distillation_of_many_rows():
+    # more rows than workgroups of the pass that looks at another upstream gradient
+    z = scores(5000, 17, torch.float32, 4)
+    t = teacher(5000, 17, 3, True, 4, 1.0)
+    check_distill(z, *t)
+    check_distill(z, *t, mask=torch.arange(5000, device=DEV) % 3 > 0, upstream=torch.tensor(0.3, device=DEV))
+
+
+# ---- balance -------------------------------------------------------------------------------------
+def check_balance(z, k, mask=None, weight=1.0):
+    leaf = z.detach().requires_grad_(True)
+    loss, counts = C.balance_loss(leaf, k, mask=mask, weight=weight)
+    grad, = torch.autograd.grad(loss, leaf)
+    flat = z.reshape(-1, z.shape[-1])
+    want = L.balance(host(flat), k, None if mask is None else mask.reshape(-1).cpu().numpy(), weight)
+    assert counts.cpu().tolist() == want[1].tolist() and counts.dtype == torch.int64
+    close(loss, want[0], abs(want[0]), z, "loss")
+    close(grad, np.reshape(want[2], grad.shape), np.reshape(want[3], grad.shape), z, "grad")
+    return loss, counts, grad
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("experts", [1, 2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 31, 60, 64, 65, 128, 130, 200, 256, 257, 512, 600, 1023, 1024])
+def test_balance(dtype, experts):
+    for rows, k in ((1, 1), (37, min(3, experts)), (130, min(8, experts))):
+        check_balance(scores(rows, experts, dtype, experts), k, None, 0.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("experts,k", [(4, 4), (16, 1), (16, 16), (60, 33), (300, 5)])
+def test_balance_of_padded_and_masked_rows(dtype, experts, k):
+    z = scores(200, experts, dtype, 3)
+    z[5], z[6] = -INF, NAN                                            # no row at all; one that the mask leaves out
+    z[7, 1:] = -INF                                                   # one expert left
+    z[8] = torch.finfo(dtype).min
+    z[9, 0] = torch.finfo(dtype).min
+    z[10] = 0.0                                                       # ties
+    z[11] = scores(1, experts, dtype, 4).round()
+    mask = torch.arange(200, device=DEV) % 5 != 1
+    _, _, grad = check_balance(z, k, mask)
+    assert (grad[5] == 0).all() and (grad[6] == 0).all()
+    nothing = C.balance_loss(z.requires_grad_(True), k, mask=torch.zeros_like(mask))
+    assert nothing.loss == 0 and (nothing.counts == 0).all() and (torch.autograd.grad(nothing.loss, z)[0] == 0).all()
+    assert C.balance_loss(z, k).loss.isnan()
+
+
+@pytest.mark.parametrize("rows,experts,k,dtype", [(40000, 16, 1, torch.float32), (9000, 64, 8, torch.bfloat16), (20011, 5, 2, torch.float32)])
+def test_balance_of_many_rows(rows, experts, k, dtype):
+    z = scores(rows, experts, dtype, 8)
+    p = torch.softmax(z.double(), 1)
+    chosen = torch.zeros_like(p).scatter_(1, torch.sort(z.double(), dim=1, descending=True, stable=True).indices[:, :k], 1.0)
+    w = chosen.sum(0) * experts / (k * float(rows) ** 2)
+    leaf = z.requires_grad_(True)
+    loss, counts = C.balance_loss(leaf, k)
+    grad, = torch.autograd.grad(loss, leaf)
+    mean = (p * w).sum(1, keepdim=True)
+    assert torch.equal(counts, chosen.sum(0).long())
+    close(loss, float((w * p.sum(0)).sum()), float((w * p.sum(0)).sum()), z, "loss", steps=600)      # (rows / 1024 workgroups * lanes: 160 in a row at most)
+    close(grad, (p * (w - mean)).cpu().numpy(), (p * (w + mean)).cpu().numpy(), z, "grad")
+    again = C.balance_loss(leaf, k)
+    assert torch.equal(again.loss, loss) and torch.equal(torch.autograd.grad(again.loss * 2, leaf)[0].double(), 2 * grad.double())
+
+
+def test_balance_of_views_and_shapes():
+    z = scores(60, 48, torch.float32, 1)
+    for view in (z[:, 4:36], z[::2, ::3], z.t(), z.view(3, 20, 48), z.view(3, 20, 48).transpose(0, 1), z[0], z[:1].expand(7, -1)):
+        check_balance(view, 2)
+    check_balance(z.view(3, 20, 48), 2, torch.rand(3, 20, device=DEV) < 0.7)
+    empty = C.balance_loss(z[:0])
+    assert empty.loss == 0 and (empty.counts == 0).all()
+    leaf = z.clone().requires_grad_(True)
+    loss = C.balance_loss(leaf, 2).loss
+    one, = torch.autograd.grad(loss, leaf, retain_graph=True)
+    assert torch.equal(torch.autograd.grad(loss, leaf)[0], one)
+    g, = torch.autograd.grad(C.balance_loss(leaf, 2).loss, leaf, create_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gate_balance(dtype):
+    sizes = [7, 1, 300, 0, 64, 5000, 16, 33, 2, 90, 11, 5, 8, 70, 129, 31, 40, 3]    # more than one launch takes
+    tensors = [scores(n, 16, dtype, n).requires_grad_(n != 64) for n in sizes]
+    loss, counts = C.gate_balance(tensors, weight=3.0)
+    wanted = [t for t in tensors if t.requires_grad]
+    grads = iter(torch.autograd.grad(loss, wanted))
+    total = 0.0
+    for t, c in zip(tensors, counts):
+        want = L.balance(host(t), 1, None, 3.0 / len(tensors))
+        total += want[0]
+        assert c.cpu().tolist() == want[1].tolist()
+        if t.requires_grad:
+            close(next(grads), want[2], want[3], t, "grad")
+    close(loss, np.array(total), np.array(total), tensors[5], "loss", steps=300)
+
+
+# ---- together ------------------------------------------------------------------------------------
+def networks():
+    torch.manual_seed(11)
+    big, small = C.ConvLogicMnistModel(k_param=6).to(DEV).eval(), C.ConvLogicMnistModel(k_param=2).to(DEV)
+    with torch.no_grad():
+        for p in [*big.parameters(), *small.parameters()]:
+            p.add_(torch.randn(p.shape, device=DEV))
+    x = (torch.rand(40, 1, 28, 28, device=DEV) < 0.5).float()
+    return big, small, x
+
+
+def test_a_student_learns_from_a_teachers_answers():
+    # answers of a larger network, the student's loss against them, the balance of its gates: gradients of the whole against the plain forms' in float64
+    big, small, x = networks()
+    with torch.no_grad():
+        answers = C.top_logits(big(x), 4, temperature=2.0)
+    params = list(small.parameters())
+    scores_ = small(x)
+    loss = C.distillation_loss(scores_, *answers, temperature=2.0) + C.gate_balance(small, weight=0.1).loss
+    got = torch.autograd.grad(loss, [scores_, *params])
+    again = small(x)
+    plain = scores_.detach().cpu().double().requires_grad_(True)
+    cpu = [p.detach().cpu().double().requires_grad_(True) for p in params]
+    host_loss = C.distillation_loss(plain, *(t.cpu() for t in answers), temperature=2.0)
+    host_balance = C.gate_balance(cpu, weight=0.1).loss
+    assert abs(float(host_loss + host_balance) - float(loss)) <= 1e-5 * abs(float(loss))
+    of_scores, = torch.autograd.grad(host_loss, plain)
+    assert (got[0].cpu().double() - of_scores).abs().max() <= 1e-5 * of_scores.abs().max()
+    through = torch.autograd.grad(again, params, of_scores.float().to(DEV))
+    for g, a, b in zip(got[1:], through, torch.autograd.grad(host_balance, cpu)):
+        want = a.double().cpu() + b
+        assert (g.double().cpu() - want).abs().max() <= 1e-4 * want.abs().max() + 1e-9
+
+
+def test_the_step_replays_from_a_graph():
+    big, small, x = networks()
+    with torch.no_grad():
+        answers = C.top_logits(big(x), 4, temperature=2.0)
+    mask = torch.arange(40, device=DEV) % 4 != 3
+
+    def loss_of(x, values, columns, lse, mask):
+        return 0.5 * C.distillation_loss(small(x), values, columns, lse, temperature=2.0, mask=mask) + C.gate_balance(small, weight=0.1).loss
+
+    step = C.GraphedStep(loss_of, (x, *answers, mask), small.parameters())
+    params = list(small.parameters())
+    for i in range(4):
+        x = (torch.rand(40, 1, 28, 28, device=DEV) < 0.4 + 0.05 * i).float()
+        with torch.no_grad():
+            answers = C.top_logits(big(x), 4, temperature=2.0)
+        mask = mask.roll(1)
+        loss = step(x, *answers, mask).clone()
+        got = [p.grad.clone() for p in params]
+        torch.cuda.synchronize()
+        with torch.enable_grad():
+            eager = loss_of(x, *answers, mask)
+            want = torch.autograd.grad(eager, params)
+        assert torch.equal(loss, eager.detach())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_two_recorded_steps_share_nothing():
+    z, w = scores(64, 700, torch.bfloat16, 1), scores(64, 700, torch.bfloat16, 2)
+    t = teacher(64, 700, 8, True, 1, 1.0)
+    steps = [C.GraphedStep(lambda x, m: C.distillation_loss(x, *t, mask=m, weight=c), (s, torch.ones(64, dtype=torch.bool, device=DEV)), [], input_grads=True)
+             for s, c in ((z, 1.0), (w, 0.5))]
+    for i in range(3):
+        m = torch.arange(64, device=DEV) % (i + 2) > 0
+        for s in steps:
+            s(s.inputs[0].detach().clone(), m)
+        torch.cuda.synchronize()
+        for s, c in zip(steps, (1.0, 0.5)):
+            leaf = s.inputs[0].detach().clone().requires_grad_(True)
+            loss = C.distillation_loss(leaf, *t, mask=m, weight=c)
+            assert torch.equal(loss, s.loss) and torch.equal(torch.autograd.grad(loss, leaf)[0], s.input_grads[0])
+
+
+def test_calls_on_another_stream_and_refusals_on_the_gpu():
+    z = scores(300, 2000, torch.bfloat16, 1).requires_grad_(True)
+    t = teacher(300, 2000, 8, True, 1, 1.0)
+    want = torch.autograd.grad(C.distillation_loss(z, *t), z)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = torch.autograd.grad(C.distillation_loss(z, *t), z)[0]
+        balanced = C.balance_loss(z, 3) if z.shape[1] <= 1024 else None
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and balanced is None
+    for call in (lambda: C.distillation_loss(z, t[0].cpu(), t[1], t[2]), lambda: C.distillation_loss(z, *t, mask=torch.ones(300, dtype=torch.bool)),
+                 lambda: C.gate_balance([torch.zeros(2, 16, device=DEV), torch.zeros(2, 16)]), lambda: C.balance_loss(z[:, :9], mask=torch.ones(300, dtype=torch.bool))):
+        with pytest.raises(RuntimeError):
+            call()
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda a: C.top_logits(a, 2).values, z.detach()[:3, :5])
