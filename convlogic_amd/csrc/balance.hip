@@ -29,14 +29,41 @@ struct BalanceArgs {
     const void *upstream;                                             // A
 };
 
-// reductions over groups of G lanes, in all of them
+// Reductions over groups of G lanes, in all of them: up to 16 lanes by DPP, beyond by LDS permutation.
+template <int CTRL>
+__device__ __forceinline__ int dpp_keep(int v)
+{
+    return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xF, 0xF, false);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp_keep(float v)
+{
+    return __builtin_bit_cast(float, dpp_keep<CTRL>(__builtin_bit_cast(int, v)));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_keep(double v)
+{
+    return ::dpp_keep<CTRL, 0xF>(v);
+}
 template <int G, typename A, typename F>
 __device__ __forceinline__ A group_reduce(A v, F f)
 {
-#pragma unroll
-    for (int by = 1; by < G; by <<= 1) v = f(v, (A)__shfl_xor(v, by));
+    if constexpr (G > 1) v = f(v, dpp_keep<0xB1>(v));                 // quad_perm [1,0,3,2]
+    if constexpr (G > 2) v = f(v, dpp_keep<0x4E>(v));                 // quad_perm [2,3,0,1]
+    if constexpr (G > 4) v = f(v, dpp_keep<0x141>(v));                // row_half_mirror
+    if constexpr (G > 8) v = f(v, dpp_keep<0x140>(v));                // row_mirror
+    if constexpr (G > 16) v = f(v, (A)__shfl_xor(v, 16));
+    if constexpr (G > 32) v = f(v, (A)__shfl_xor(v, 32));
     return v;
 }
+struct Max {
+    template <typename A>
+    __device__ __forceinline__ A operator()(A a, A b) const { return max_of(a, b); }
+};
+struct Sum {
+    template <typename A>
+    __device__ __forceinline__ A operator()(A a, A b) const { return a + b; }
+};
 
 // the logits of a row that a lane holds: pieces lane, lane + G, ... of 16 bytes; -inf behind the row
 template <typename T, int G, int NV>
@@ -60,29 +87,24 @@ struct RowPart {
             }
         }
     }
-    // x becomes the probabilities; false for a row of -inf alone, which has none
-    __device__ __forceinline__ bool softmax(A m)
+    __device__ __forceinline__ A highest() const
     {
-        const A safe = finite_or_zero(m), scale = exp_scale_of();
+        A m = x[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) m = max_of(m, x[i]);
+        return group_reduce<G>(m, Max());
+    }
+    // e = exponentials relative to the row's highest, m -> their sum: 0 for a row of -inf alone, NaN for one with a NaN
+    __device__ __forceinline__ A exponentials(A m, A (&e)[N]) const
+    {
+        const Exps<A> f(m, (A)Exps<A>::unit(1.0));
         A s = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            x[i] = exp_scaled(x[i] - safe, scale);
-            s += x[i];
+            e[i] = f(x[i]);
+            s += e[i];
         }
-        s = group_reduce<G>(s, [](A a, A b) { return a + b; });
-        const A inv = A(1) / s;
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] *= inv;
-        return !(s == 0);
-    }
-    __device__ __forceinline__ static A exp_scale_of() { return sizeof(A) == 4 ? A(1.4426950408889634074) : A(1); }
-    __device__ __forceinline__ A highest() const
-    {
-        A m = lowest(A(0));
-#pragma unroll
-        for (int i = 0; i < N; ++i) m = max_of(m, x[i]);
-        return group_reduce<G>(m, [](A a, A b) { return max_of(a, b); });
+        return group_reduce<G>(s, Sum());
     }
 };
 
@@ -93,58 +115,85 @@ __device__ __forceinline__ int segment_of(const Segments &s)
     return at;
 }
 
+// rows that a group of lanes has in flight
+template <int N>
+constexpr int kAhead = N <= 4 ? 4 : N <= 8 ? 2 : 1;
+
 // sums and counts of a workgroup's rows
 template <typename T, int G, int NV>
 __global__ __launch_bounds__(kThreads) void balance_kernel(BalanceArgs a)
 {
     typedef RowPart<T, G, NV> Part;
     typedef typename Part::A A;
-    constexpr int N = Part::N, kGroups = kThreads / G;
+    constexpr int N = Part::N, kGroups = kThreads / G, R = kAhead<N>;
     __shared__ A room_p[kThreads / 64][G * N];
     __shared__ int room_c[kThreads / 64][G * N + 1];
     const int tid = threadIdx.x, lane = tid % G, seg = segment_of(a.seg);
     const int64_t rows = a.seg.rows[seg], groups = (int64_t)(a.seg.first[seg + 1] - a.seg.first[seg]) * kGroups;
+    const T *z = static_cast<const T *>(a.seg.z[seg]);
     A p[N] = {};
     int c[N] = {}, n = 0;
-    for (int64_t row = (int64_t)((int)blockIdx.x - a.seg.first[seg]) * kGroups + tid / G; row < rows; row += groups) {
-        if (a.mask && !a.mask[row]) continue;
-        Part part;
-        part.load(static_cast<const T *>(a.seg.z[seg]) + row * a.seg.stride[seg], lane, a.experts);
-        const A m = part.highest();
-        // the choice: k times the highest that is left, of equal ones the lowest; -inf is none, NaN is above everything
-        A left[N];
+    for (int64_t row0 = (int64_t)((int)blockIdx.x - a.seg.first[seg]) * kGroups + tid / G; row0 < rows; row0 += R * groups) {
+        Part part[R];
+        bool kept[R];
 #pragma unroll
-        for (int i = 0; i < N; ++i) left[i] = part.x[i] != part.x[i] ? -lowest(A(0)) : part.x[i];
-        A top = m;
-        bool nan = false;
-#pragma unroll
-        for (int i = 0; i < N; ++i) nan |= part.x[i] != part.x[i];
-        nan = group_reduce<G>((int)nan, [](int x, int y) { return x | y; });
-        if (nan) top = -lowest(A(0));
-        const bool any = part.softmax(m);
-        if (!any) continue;                                           // (of the whole group)
-        n += 1;
-        for (int pick = 0; pick < a.k; ++pick) {
-            if (pick) {
-                top = lowest(A(0));
-#pragma unroll
-                for (int i = 0; i < N; ++i) top = max_of(top, left[i]);
-                top = group_reduce<G>(top, [](A x, A y) { return max_of(x, y); });
-            }
-            if (top == lowest(A(0))) break;
-            int chosen = kMaxExperts;
-#pragma unroll
-            for (int i = N - 1; i >= 0; --i) chosen = left[i] == top ? Part::expert(lane, i) : chosen;
-            chosen = group_reduce<G>(chosen, [](int x, int y) { return x < y ? x : y; });
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const bool it = Part::expert(lane, i) == chosen;
-                c[i] += it;
-                left[i] = it ? lowest(A(0)) : left[i];
-            }
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = row0 + r * groups;
+            kept[r] = row < rows && !(a.mask && !a.mask[row]);
+            if (kept[r]) part[r].load(z + row * a.seg.stride[seg], lane, a.experts);
         }
 #pragma unroll
-        for (int i = 0; i < N; ++i) p[i] += part.x[i];
+        for (int r = 0; r < R; ++r) {
+            if (!kept[r]) continue;
+            Part &x = part[r];
+            const A m = x.highest();
+            A e[N];
+            const A s = x.exponentials(m, e), inv = A(1) / s;
+            if (s == 0) continue;                                     // (of the whole group)
+            n += 1;
+            // The choice: k times the highest below the last one.  Where values are equal these are too few or too many experts, and the slow way
+            // takes one at a time, the lowest of the highest.  -inf is none, NaN is above everything.
+            A least = m;
+            if (s != s) {
+                least = -lowest(A(0));
+#pragma unroll
+                for (int i = 0; i < N; ++i) x.x[i] = x.x[i] != x.x[i] ? least : x.x[i];
+            }
+#pragma unroll 1
+            for (int pick = 1; pick < a.k; ++pick) {
+                A next = lowest(A(0));
+#pragma unroll
+                for (int i = 0; i < N; ++i) next = max_of(next, x.x[i] < least ? x.x[i] : lowest(A(0)));
+                least = group_reduce<G>(next, Max());
+            }
+            int chosen = 0;
+            const A floor = lowest(A(0));
+#pragma unroll
+            for (int i = 0; i < N; ++i) chosen += x.x[i] >= least && x.x[i] > floor;
+            chosen = group_reduce<G>(chosen, Sum());
+            if (chosen <= a.k) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) c[i] += x.x[i] >= least && x.x[i] > floor;
+            } else {
+#pragma unroll 1
+                for (int pick = 0; pick < a.k; ++pick) {
+                    const A top = x.highest();
+                    if (top == floor) break;
+                    int which = kMaxExperts;
+#pragma unroll
+                    for (int i = N - 1; i >= 0; --i) which = x.x[i] == top ? Part::expert(lane, i) : which;
+                    which = group_reduce<G>(which, [](int u, int v) { return u < v ? u : v; });
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const bool it = Part::expert(lane, i) == which;
+                        c[i] += it;
+                        x.x[i] = it ? floor : x.x[i];
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) p[i] += e[i] * inv;
+        }
     }
     // groups of a wavefront, then its four wavefronts, in a fixed order
 #pragma unroll
@@ -188,55 +237,64 @@ struct FinishArgs {
     double weight;
     void *loss, *w;                                                   // A, [segments][experts] in A
     int64_t *count_out;                                               // [segments][experts]
-    double *seg_loss;                                                 // [segments]
+    double *terms;                                                    // [segments][blocks of 16 experts]
 };
 
-// One workgroup per segment: rows per expert and in all, the coefficients of the gradient and the segment's share of the loss.
+// One workgroup per 16 experts of a segment, 64 slices of its workgroups' sums at once: rows per expert and in all, the coefficients of the gradient and
+// these experts' part of the loss.
 template <typename A>
 __global__ __launch_bounds__(1024) void balance_finish_kernel(FinishArgs a)
 {
     __shared__ double room[16], sum_p[1024];
     __shared__ int64_t sum_c[1024];
-    const int seg = blockIdx.x, tid = threadIdx.x, first = a.seg.first[seg], end = a.seg.first[seg + 1];
+    const int seg = blockIdx.y, tid = threadIdx.x, first = a.seg.first[seg], end = a.seg.first[seg + 1];
+    const int e = (int)blockIdx.x * 16 + tid % 16;
     double n[1] = {0};
     for (int w = first + tid; w < end; w += 1024) n[0] += a.counts[(int64_t)w * (a.experts + 1) + a.experts];
-    block_reduce<true, 1024>(n, room);
-    // threads in `slices` rows of `experts`: each adds the workgroups slice, slice + slices, ...
-    const int slices = 1024 / a.experts, slice = tid / a.experts, e = tid % a.experts;
     double p = 0;
     int64_t c = 0;
-    if (slice < slices)
-        for (int w = first + slice; w < end; w += slices) {
+    if (e < a.experts) {
+#pragma unroll 4
+        for (int w = first + tid / 16; w < end; w += 64) {
             p += (double)static_cast<const A *>(a.sums)[(int64_t)w * a.experts + e];
             c += a.counts[(int64_t)w * (a.experts + 1) + e];
         }
+    }
     sum_p[tid] = p;
     sum_c[tid] = c;
-    __syncthreads();
-    double term[1] = {0};
-    if (tid < a.experts) {
-        for (int s = 1; s < slices; ++s) {
-            p += sum_p[s * a.experts + tid];
-            c += sum_c[s * a.experts + tid];
-        }
+    block_reduce<true, 1024>(n, room);
+    if (tid >= kWave) return;
+    // the first wavefront: its lanes take every fourth slice, then the four are added
+    p = 0, c = 0;
+    for (int s = tid / 16; s < 64; s += 4) {
+        p += sum_p[s * 16 + tid % 16];
+        c += sum_c[s * 16 + tid % 16];
+    }
+#pragma unroll
+    for (int by = 16; by < 64; by <<= 1) {
+        p += __shfl_xor(p, by);
+        c += __shfl_xor(c, by);
+    }
+    double term = 0;
+    if (tid < 16 && e < a.experts) {
         const double w = n[0] == 0 ? 0 : a.weight * a.experts * (double)c / ((double)a.k * n[0] * n[0]);
-        a.count_out[(int64_t)seg * a.experts + tid] = c;
-        static_cast<A *>(a.w)[(int64_t)seg * a.experts + tid] = (A)w;
-        term[0] = w * p;
+        a.count_out[(int64_t)seg * a.experts + e] = c;
+        static_cast<A *>(a.w)[(int64_t)seg * a.experts + e] = (A)w;
+        term = w * p;
     }
-    block_reduce<true, 1024>(term, room);
-    if (tid == 0) {
-        if (a.seg.n == 1) *static_cast<A *>(a.loss) = (A)term[0];
-        else a.seg_loss[seg] = term[0];
-    }
+    term = wave_sum(term);
+    if (tid != 0) return;
+    if (gridDim.x * gridDim.y == 1) *static_cast<A *>(a.loss) = (A)term;
+    else a.terms[(int64_t)seg * gridDim.x + blockIdx.x] = term;
 }
 
 template <typename A>
-__global__ void balance_sum_kernel(const double *seg_loss, int n, A *loss)
+__global__ __launch_bounds__(64) void balance_sum_kernel(const double *terms, int n, A *loss)
 {
     double s = 0;
-    for (int i = 0; i < n; ++i) s += seg_loss[i];
-    *loss = (A)s;
+    for (int i = threadIdx.x; i < n; i += 64) s += terms[i];
+    s = wave_sum(s);
+    if (threadIdx.x == 0) *loss = (A)s;
 }
 
 // the gradient
@@ -245,9 +303,12 @@ __global__ __launch_bounds__(kThreads) void balance_grad_kernel(BalanceArgs a)
 {
     typedef RowPart<T, G, NV> Part;
     typedef typename Part::A A;
-    constexpr int N = Part::N, VEC = Part::VEC, kGroups = kThreads / G;
+    typedef typename Vec16<T>::type V;
+    constexpr int N = Part::N, VEC = Part::VEC, kGroups = kThreads / G, R = kAhead<N>;
     const int tid = threadIdx.x, lane = tid % G, seg = segment_of(a.seg);
     const int64_t rows = a.seg.rows[seg], groups = (int64_t)(a.seg.first[seg + 1] - a.seg.first[seg]) * kGroups;
+    const T *z = static_cast<const T *>(a.seg.z[seg]);
+    T *grad = static_cast<T *>(a.seg.grad[seg]);
     const A up = *static_cast<const A *>(a.upstream);
     A w[N];
 #pragma unroll
@@ -255,36 +316,51 @@ __global__ __launch_bounds__(kThreads) void balance_grad_kernel(BalanceArgs a)
         const int e = Part::expert(lane, i);
         w[i] = e < a.experts ? static_cast<const A *>(a.w)[(int64_t)seg * a.experts + e] : A(0);
     }
-    for (int64_t row = (int64_t)((int)blockIdx.x - a.seg.first[seg]) * kGroups + tid / G; row < rows; row += groups) {
-        T *out = static_cast<T *>(a.seg.grad[seg]) + row * a.experts;
-        Part part;
-        bool any = !a.mask || a.mask[row];
-        if (any) {
-            part.load(static_cast<const T *>(a.seg.z[seg]) + row * a.seg.stride[seg], lane, a.experts);
-            any = part.softmax(part.highest());
+    for (int64_t row0 = (int64_t)((int)blockIdx.x - a.seg.first[seg]) * kGroups + tid / G; row0 < rows; row0 += R * groups) {
+        Part part[R];
+        bool kept[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = row0 + r * groups;
+            kept[r] = row < rows && !(a.mask && !a.mask[row]);
+            if (kept[r]) part[r].load(z + row * a.seg.stride[seg], lane, a.experts);
         }
-        A mean = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) mean += any ? w[i] * part.x[i] : A(0);
-        mean = group_reduce<G>(mean, [](A x, A y) { return x + y; });
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = row0 + r * groups;
+            if (row >= rows) break;
+            A e[N], inv = 0, mean = 0;
+            if (kept[r]) {
+                const A s = part[r].exponentials(part[r].highest(), e);
+                kept[r] = !(s == 0);
+                inv = A(1) / s;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int e = (j * G + lane) * VEC;
-            typename Vec16<T>::type v;
+                for (int i = 0; i < N; ++i) {
+                    e[i] *= inv;
+                    mean += w[i] * e[i];
+                }
+                mean = group_reduce<G>(mean, Sum());
+            }
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) v[i] = any ? (T)(part.x[j * VEC + i] * (w[j * VEC + i] - mean) * up) : (T)0.f;
-            if (e + VEC <= a.experts) {
-                *reinterpret_cast<typename Vec16<T>::type *>(out + e) = v;
-            } else {
+            for (int j = 0; j < NV; ++j) {
+                const int at = (j * G + lane) * VEC;
+                V v;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i)
-                    if (e + i < a.experts) out[e + i] = v[i];
+                for (int i = 0; i < VEC; ++i) v[i] = kept[r] ? (T)(e[j * VEC + i] * (w[j * VEC + i] - mean) * up) : (T)0.f;
+                T *out = grad + row * a.experts + at;
+                if (at + VEC <= a.experts) {
+                    *reinterpret_cast<V *>(out) = v;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i)
+                        if (at + i < a.experts) out[i] = v[i];
+                }
             }
         }
     }
 }
 
-// call(T(), lanes per row, pieces per lane) for a number of experts
+// call(lanes per row, pieces per lane) for a number of experts
 template <typename T, typename F>
 void with_part(int experts, F call)
 {
@@ -294,9 +370,9 @@ void with_part(int experts, F call)
     if (pieces <= 4) return call(std::integral_constant<int, 4>(), std::integral_constant<int, 1>());
     if (pieces <= 8) return call(std::integral_constant<int, 8>(), std::integral_constant<int, 1>());
     if (pieces <= 16) return call(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
-    if (pieces <= 64) return call(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
-    if (pieces <= 256) return call(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
-    call(std::integral_constant<int, 64>(), std::integral_constant<int, 8>());
+    if (pieces <= 32) return call(std::integral_constant<int, 16>(), std::integral_constant<int, 2>());
+    if (pieces <= 64) return call(std::integral_constant<int, 16>(), std::integral_constant<int, 4>());
+    return call(std::integral_constant<int, 64>(), std::integral_constant<int, kMaxExperts / 64 / Vec16<T>::N>());
 }
 
 template <typename T>
@@ -307,6 +383,7 @@ int lanes_of(int experts)
     return g;
 }
 
+constexpr int kTerms = kSegments * (kMaxExperts / 16);                // of the loss
 constexpr int kMostGroups = 1024;                                     // workgroups of the sums
 
 // workgroups per segment, `most` in all or a few more: by rows, one at least
@@ -349,7 +426,7 @@ extern "C" int64_t clg_balance_scratch_bytes(int dtype, int64_t experts)
 {
     if (!clg_score_type(dtype) || experts < 1 || experts > kMaxExperts) return 0;
     const int64_t groups = kMostGroups + kSegments;
-    return groups * experts * (dtype == CLG_F64 ? 8 : 4) + groups * (experts + 1) * 4 + kSegments * 8 + 8;
+    return groups * experts * (dtype == CLG_F64 ? 8 : 4) + groups * (experts + 1) * 4 + kTerms * 8 + 8;
 }
 
 extern "C" int clg_balance_forward(int dtype, int n, const void *const *logits, const int64_t *rows, const int64_t *row_strides, int64_t experts, int64_t k,
@@ -359,9 +436,9 @@ extern "C" int clg_balance_forward(int dtype, int n, const void *const *logits, 
     if (const int rc = check_segments("clg_balance_forward", dtype, n, logits, rows, row_strides, experts, k, mask, a.seg)) return rc;
     CLG_REQUIRE(loss && counts && coefs && scratch, "clg_balance_forward: null pointer");
     const bool f64 = dtype == CLG_F64;
-    double *seg_loss = static_cast<double *>(scratch);
+    double *terms = static_cast<double *>(scratch);
     a.experts = (int)experts, a.k = (int)k, a.mask = mask;
-    a.sums = reinterpret_cast<float *>(seg_loss + kSegments);
+    a.sums = reinterpret_cast<float *>(terms + kTerms);
     a.counts = reinterpret_cast<int *>(reinterpret_cast<char *>(a.sums) + (kMostGroups + kSegments) * experts * (f64 ? 8 : 4));
     const int rc = clg_with_type(dtype, [&](auto t) {
         typedef decltype(t) T;
@@ -373,13 +450,14 @@ extern "C" int clg_balance_forward(int dtype, int n, const void *const *logits, 
     });
     if (rc) return rc;
     CLG_CHECK_LAUNCH("clg_balance_forward");
-    const FinishArgs f{a.seg, a.experts, a.k, a.sums, a.counts, weight / n, loss, coefs, counts, seg_loss};
-    if (f64) balance_finish_kernel<double><<<dim3(n), dim3(1024), 0, clg_stream(stream)>>>(f);
-    else balance_finish_kernel<float><<<dim3(n), dim3(1024), 0, clg_stream(stream)>>>(f);
+    const FinishArgs f{a.seg, a.experts, a.k, a.sums, a.counts, weight / n, loss, coefs, counts, terms};
+    const int blocks = (int)clg_ceil_div(experts, 16);
+    if (f64) balance_finish_kernel<double><<<dim3(blocks, n), dim3(1024), 0, clg_stream(stream)>>>(f);
+    else balance_finish_kernel<float><<<dim3(blocks, n), dim3(1024), 0, clg_stream(stream)>>>(f);
     CLG_CHECK_LAUNCH("clg_balance_forward");
-    if (n > 1) {
-        if (f64) balance_sum_kernel<double><<<dim3(1), dim3(1), 0, clg_stream(stream)>>>(seg_loss, n, static_cast<double *>(loss));
-        else balance_sum_kernel<float><<<dim3(1), dim3(1), 0, clg_stream(stream)>>>(seg_loss, n, static_cast<float *>(loss));
+    if (n * blocks > 1) {
+        if (f64) balance_sum_kernel<double><<<dim3(1), dim3(64), 0, clg_stream(stream)>>>(terms, n * blocks, static_cast<double *>(loss));
+        else balance_sum_kernel<float><<<dim3(1), dim3(64), 0, clg_stream(stream)>>>(terms, n * blocks, static_cast<float *>(loss));
         CLG_CHECK_LAUNCH("clg_balance_forward");
     }
     return CLG_OK;

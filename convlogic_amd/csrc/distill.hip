@@ -28,158 +28,186 @@ struct DistillArgs {
 
 constexpr int kFlagTwice = 1, kFlagListed = 2, kFlagBad = 4;
 
-// LDS of a workgroup: reduction room (16 wavefronts of 5 doubles), entries (probability, logit, column), bits of a tile
+// LDS of a workgroup: reduction room (16 wavefronts of 4 doubles), flags, entries (probability, logit, column), bits of a tile
 template <typename A>
 size_t distill_lds(int k, int cols_of_tile /* whole words of bits */)
 {
-    return 16 * 5 * 8 + 16 + (size_t)k * (8 + sizeof(A) + 4) + (size_t)(cols_of_tile / 32) * 4;
+    return 16 * 4 * 8 + 16 + (size_t)k * (8 + sizeof(A) + 4) + (size_t)(cols_of_tile / 32) * 4;
+}
+
+// whether entry j is the first of its column, and with all the others' probabilities on it
+__device__ __forceinline__ bool first_of(const int *column, int j)
+{
+    bool first = true;
+    for (int i = 0; i < j && first; ++i) first = column[i] != column[j];
+    return first;
+}
+__device__ __forceinline__ double all_of(const int *column, const double *prob, int j, int k)
+{
+    double p = prob[j];
+    for (int i = j + 1; i < k; ++i) p += column[i] == column[j] ? prob[i] : 0;
+    return p;
 }
 
 // One workgroup per row.  A row that fits its registers (COLS columns) is read from memory once, for the sum and for the gradient; longer ones (MULTI)
 // tile by tile, twice.
 template <typename T, int THREADS, int NV, bool MULTI>
-__global__ __launch_bounds__(THREADS) void distill_kernel(DistillArgs a)
+__global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
 {
     typedef typename Wide<T>::type A;
     typedef RowTile<T, THREADS, NV> Tile;
     extern __shared__ char lds[];
-    double *room = reinterpret_cast<double *>(lds), *prob = room + 16 * 5 + 2;
-    int *flags = reinterpret_cast<int *>(room + 16 * 5);
+    double *room = reinterpret_cast<double *>(lds), *prob = room + 16 * 4 + 2;
+    int *flags = reinterpret_cast<int *>(room + 16 * 4);
     A *logit = reinterpret_cast<A *>(prob + a.k);
     int *column = reinterpret_cast<int *>(logit + a.k);
     uint32_t *bits = reinterpret_cast<uint32_t *>(column + a.k);
     const int tid = threadIdx.x, k = a.k;
-    const A scale = exp_scale<A>(a.temperature);
+    const A unit = (A)Exps<A>::unit(a.temperature);
     const double inv_tau = 1.0 / a.temperature;
 
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const A up = a.upstream ? static_cast<const A *>(a.upstream)[a.upstream_rows ? row : 0] : A(1);
-        if (a.only_changed && static_cast<const A *>(a.applied)[row] == up) continue;
-        T *grad = a.grad ? static_cast<T *>(a.grad) + row * a.cols : nullptr;
-        const bool kept = !a.mask || a.mask[row];
-        const T *z = static_cast<const T *>(a.z) + row * a.row_stride;
-        Tile tile;
-        if (kept) tile.load(z, 0, a.cols);
+    const int64_t row = blockIdx.x;
+    const A up = a.upstream ? static_cast<const A *>(a.upstream)[a.upstream_rows ? row : 0] : A(1);
+    if (a.only_changed && static_cast<const A *>(a.applied)[row] == up) return;
+    T *grad = a.grad ? static_cast<T *>(a.grad) + row * a.cols : nullptr;
+    const bool kept = !a.mask || a.mask[row];
+    const T *z = static_cast<const T *>(a.z) + row * a.row_stride;
+    Tile tile;
+    if (kept) tile.load(z, 0, a.cols);
 
-        // the teacher's entries
-        __syncthreads();
-        if (tid == 0) *flags = 0;
-        __syncthreads();
-        double top_t[3] = {lowest(0.0), lowest(0.0), 0};              // highest of the teacher, of the student's listed logits
-        if (kept) {
-            int seen = 0;
-            for (int j = tid; j < k; j += THREADS) {
-                const int64_t at = row * k + j, c = a.columns64 ? static_cast<const int64_t *>(a.columns)[at] : static_cast<const int32_t *>(a.columns)[at];
-                const bool there = c >= 0 && c < a.cols;
-                seen |= there ? kFlagListed : c >= a.cols ? kFlagBad : 0;
-                column[j] = there ? (int)c : -1;
-                if (!there) continue;
-                prob[j] = load_any(a.values, a.values_type, at) * inv_tau;
-                logit[j] = (A)z[c];
-                top_t[0] = max_of(top_t[0], prob[j]);
-                top_t[1] = max_of(top_t[1], (double)logit[j]);
-            }
-            if (seen) atomicOr(flags, seen);
+    // the teacher's entries
+    if (tid == 0) *flags = 0;
+    __syncthreads();
+    A tops[3] = {lowest(A(0)), lowest(A(0)), lowest(A(0))};       // highest of the teacher, of the student's listed logits, of the others
+    if (kept) {
+        int seen = 0;
+#pragma unroll 1
+    for (int j = tid; j < k; j += THREADS) {
+            const int64_t at = row * k + j, c = a.columns64 ? static_cast<const int64_t *>(a.columns)[at] : static_cast<const int32_t *>(a.columns)[at];
+            const bool there = c >= 0 && c < a.cols;
+            seen |= there ? kFlagListed : c >= a.cols ? kFlagBad : 0;
+            column[j] = there ? (int)c : -1;
+            if (!there) continue;
+            const double t = load_any(a.values, a.values_type, at) * inv_tau;
+            const A l = (A)z[c];
+            prob[j] = t;
+            logit[j] = l;
+            tops[0] = max_of(tops[0], (A)t);
+            tops[1] = max_of(tops[1], l);
         }
-        // the sum over what is not listed
-        A m_t = lowest(A(0)), s_t = 0;
-        for (int64_t base = 0; kept && base < a.cols; base += Tile::COLS) {
-            if (MULTI && base) tile.load(z, base, a.cols);
-            const int n = (int)(a.cols - base < Tile::COLS ? a.cols - base : Tile::COLS);
-            for (int w = tid; w < (n + 31) / 32; w += THREADS) bits[w] = 0;
-            __syncthreads();
-            for (int j = tid; j < k; j += THREADS) {
-                const int64_t c = (int64_t)column[j] - base;
-                if (column[j] < 0 || c < 0 || c >= n) continue;
-                if (atomicOr(&bits[c >> 5], 1u << (c & 31)) >> (c & 31) & 1) atomicOr(flags, kFlagTwice);
-            }
-            __syncthreads();
-            A m = m_t;
-            tile.each([&](T &x, int c) {
-                if (bits[c >> 5] >> (c & 31) & 1) x = (T)lowest(0.f);
-                m = max_of(m, (A)x);
-            });
-            const A safe = finite_or_zero(m);
-            if (MULTI) s_t = rescaled(s_t, m_t, m, scale);
-            tile.each([&](T &x, int) { s_t += exp_scaled((A)x - safe, scale); });
-            m_t = m;
-            if (MULTI) __syncthreads();
+        if (seen) atomicOr(flags, seen);
+    }
+    // the sum over what is not listed
+    A m_t = lowest(A(0)), s_t = 0;
+    for (int64_t base = 0; kept && base < a.cols; base += Tile::COLS) {
+        if (MULTI && base) tile.load(z, base, a.cols);
+        const int n = (int)(a.cols - base < Tile::COLS ? a.cols - base : Tile::COLS);
+        for (int w = tid; w < (n + 31) / 32; w += THREADS) bits[w] = 0;
+        __syncthreads();
+#pragma unroll 1
+    for (int j = tid; j < k; j += THREADS) {
+            const int64_t c = (int64_t)column[j] - base;
+            if (column[j] < 0 || c < 0 || c >= n) continue;
+            if (atomicOr(&bits[c >> 5], 1u << (c & 31)) >> (c & 31) & 1) atomicOr(flags, kFlagTwice);
         }
         __syncthreads();
-        const int flag = *flags;
-        if (!kept || !(flag & (kFlagListed | kFlagBad))) {            // a row that says nothing
-            if (tid == 0) {
-                if (a.row_loss) a.row_loss[row] = 0;
-                if (a.out) static_cast<A *>(a.out)[row] = 0;
-                if (a.applied) static_cast<A *>(a.applied)[row] = up;
-            }
-            if (grad)
-                for (int64_t c = tid; c < a.cols; c += THREADS) grad[c] = (T)0.f;
-            continue;
-        }
-        top_t[2] = m_t;
-        block_reduce<false, THREADS>(top_t, room);
-        const A m_u = (A)top_t[2], safe_u = finite_or_zero(m_u);
-        const double m = max_of(top_t[1], top_t[2]), base_t = a.lse ? load_any(a.lse, a.lse_type, row) : finite_or_zero(top_t[0]);
-        __syncthreads();
-
-        // sums: the rest of the row; listed exponentials, the teacher's, its share times the difference of the logarithms; distinct columns
-        double sums[5] = {(double)rescaled(s_t, m_t, m_u, scale), 0, 0, 0, 0};
-        for (int j = tid; j < k; j += THREADS) {
-            if (column[j] < 0) continue;
-            bool first = true;
-            if (flag & kFlagTwice)
-                for (int i = 0; i < j && first; ++i) first = column[i] != column[j];
-            const double u = ((double)logit[j] - m) * inv_tau, t = prob[j] - base_t, e = exp(t);
-            if (first) {
-                sums[1] += exp(u);
-                sums[4] += 1;
-            }
-            sums[2] += e;
-            if (e != 0) sums[3] += e * (t - u);
-            prob[j] = e;
-        }
-        block_reduce<true, THREADS>(sums, room);
-        const double shift = exp((m_u - m) * inv_tau), s_u = sums[0], total = s_u * shift + sums[1], log_total = log(total);
-        double mass, rest = 0, loss, per = 1;                         // per: of an entry's exponential
-        if (a.lse) {
-            rest = sums[4] == (double)a.cols ? 0 : max_of(0.0, 1 - sums[2]);
-            if (sums[2] != sums[2]) rest = sums[2];
-            mass = sums[2] + rest;
-            loss = sums[3] + sums[2] * log_total;
-            if (rest != 0) loss += rest * (log(rest) - ((m_u - m) * inv_tau + log(s_u) - log_total));
-        } else {
-            per = sums[2] == 0 ? 0 : 1 / sums[2];
-            mass = sums[2] * per;
-            loss = sums[2] == 0 ? 0 : sums[3] * per + log_total - log(sums[2]);
-        }
-        if (flag & kFlagBad) loss = mass = __builtin_nan("");
-        const double factor = a.per_count ? *a.per_count : 1;
+        tile.drop(bits);
+        tile.fence();
+        const A m = max_of(m_t, tile.highest());
+        const Exps<A> e(m, unit);
+        if (MULTI) s_t = rescaled(s_t, m_t, Exps<A>(m_t, unit), e);
+        tile.fence();
+        s_t += tile.sum(e);
+        m_t = m;
+        tile.fence();
+        if (MULTI) __syncthreads();
+    }
+    __syncthreads();
+    const int flag = *flags;
+    if (!kept || !(flag & (kFlagListed | kFlagBad))) {            // a row that says nothing
         if (tid == 0) {
-            if (a.row_loss) a.row_loss[row] = loss * a.loss_scale;
-            if (a.out) static_cast<A *>(a.out)[row] = (A)(loss * a.loss_scale * factor);
+            if (a.row_loss) a.row_loss[row] = 0;
+            if (a.out) static_cast<A *>(a.out)[row] = 0;
             if (a.applied) static_cast<A *>(a.applied)[row] = up;
         }
-        if (!grad) continue;
-        const double g = a.grad_scale * factor * (double)up;
-        const double of_listed = mass / total;
-        const A of_rest = s_u == 0 && total > 0 && mass == mass ? A(0) : (A)(g * (of_listed * shift - rest / s_u));
-        for (int64_t base = 0; base < a.cols; base += Tile::COLS) {
-            if (MULTI) tile.load(z, base, a.cols);
-            tile.store(grad, base, [&](T x) { return exp_scaled((A)x - safe_u, scale) * of_rest; });
+        if (grad) {
+            for (int64_t c = (int64_t)tid * Tile::VEC; c + Tile::VEC <= a.cols; c += THREADS * Tile::VEC)
+                *reinterpret_cast<typename Tile::V *>(grad + c) = (typename Tile::V)(T)0.f;
+            if (tid < a.cols % Tile::VEC) grad[a.cols - 1 - tid] = (T)0.f;
         }
-        __syncthreads();                                              // the listed columns' own values go over those
-        for (int j = tid; j < k; j += THREADS) {
-            if (column[j] < 0) continue;
-            double p = prob[j];
-            if (flag & kFlagTwice) {
-                bool first = true;
-                for (int i = 0; i < j && first; ++i) first = column[i] != column[j];
-                if (!first) continue;
-                for (int i = j + 1; i < k; ++i) p += column[i] == column[j] ? prob[i] : 0;
-            }
-            grad[column[j]] = (T)(A)(g * (of_listed * exp(((double)logit[j] - m) * inv_tau) - p * per));
+        return;
+    }
+    tops[2] = m_t;
+    block_reduce<false, THREADS>(tops, reinterpret_cast<A *>(room));
+    const A m_u = tops[2], m = max_of(tops[1], m_u);
+    const Exps<A> of_rest(m_u, unit), of_all(m, unit);
+    __syncthreads();
+
+    // sums: the others' exponentials relative to m_u, the listed ones' relative to m, the teacher's, the teacher's share times the difference of the
+    // logarithms
+    double sums[4] = {(double)rescaled(s_t, m_t, Exps<A>(m_t, unit), of_rest), 0, 0, 0};
+    const double base_t = a.lse ? load_any(a.lse, a.lse_type, row) : (double)finite_or_zero(tops[0]);
+#pragma unroll 1
+    for (int j = tid; j < k; j += THREADS) {
+        if (column[j] < 0) continue;
+        const A l = logit[j];
+        if (!(flag & kFlagTwice) || first_of(column, j)) sums[1] += (double)of_all(l);
+        const double u = ((double)l - (double)m) * inv_tau, t = prob[j] - base_t, e = exp(t);
+        sums[2] += e;
+        if (e != 0) sums[3] += e * (t - u);
+        prob[j] = e;
+    }
+    block_reduce<true, THREADS>(sums, room);
+    const double s_u = sums[0], total = (m_u == lowest(A(0)) ? s_u : s_u * (double)of_rest.factor(of_all)) + sums[1];
+    bool all_listed = false;                                      // (then there is nothing else)
+    if (a.lse && k >= a.cols) {
+        double n[1] = {0};
+#pragma unroll 1
+    for (int j = tid; j < k; j += THREADS) n[0] += column[j] >= 0 && first_of(column, j);
+        __syncthreads();
+        block_reduce<true, THREADS>(n, room);
+        all_listed = n[0] == (double)a.cols;
+    }
+    double rest = 0;
+    if (a.lse && !all_listed) rest = sums[2] != sums[2] ? sums[2] : max_of(0.0, 1 - sums[2]);
+    // four logarithms at once, one in a lane
+    const int lane = tid & 63;
+    const double logs = log(lane == 0 ? total : lane == 1 ? s_u : lane == 2 ? rest : sums[2]);
+    const double log_total = of_lane(logs, 0) + of_all.residue(m), log_p = of_lane(logs, 3);
+    double mass, loss, per = 1;                                   // per: of an entry's exponential
+    if (a.lse) {
+        mass = sums[2] + rest;
+        loss = sums[3] + sums[2] * log_total;
+        if (rest != 0) loss += rest * (of_lane(logs, 2) - (((double)m_u - (double)m) * inv_tau + of_lane(logs, 1) + of_rest.residue(m_u) - log_total));
+    } else {
+        per = sums[2] == 0 ? 0 : 1 / sums[2];
+        mass = sums[2] * per;
+        loss = sums[2] == 0 ? 0 : sums[3] * per + log_total - log_p;
+    }
+    if ((flag & kFlagBad) || total > 1.7e308) loss = mass = __builtin_nan("");           // (a logit of +inf)
+    const double factor = a.per_count ? *a.per_count : 1;
+    if (tid == 0) {
+        if (a.row_loss) a.row_loss[row] = loss * a.loss_scale;
+        if (a.out) static_cast<A *>(a.out)[row] = (A)(loss * a.loss_scale * factor);
+        if (a.applied) static_cast<A *>(a.applied)[row] = up;
+    }
+    if (!grad) return;
+    const double g = a.grad_scale * factor * (double)up, of_listed = mass / total;
+    const A others = s_u == 0 && total > 0 && mass == mass ? A(0) : (A)(g * (of_listed * (double)of_rest.factor(of_all) - rest / s_u));
+    for (int64_t base = 0; base < a.cols; base += Tile::COLS) {
+        if (MULTI) tile.load(z, base, a.cols);
+        tile.store(grad, base, [&](A x) { return of_rest(x) * others; });
+    }
+    __syncthreads();                                              // the listed columns' own values go over those
+#pragma unroll 1
+    for (int j = tid; j < k; j += THREADS) {
+        if (column[j] < 0) continue;
+        double p = prob[j];
+        if (flag & kFlagTwice) {
+            if (!first_of(column, j)) continue;
+            p = all_of(column, prob, j, k);
         }
+        grad[column[j]] = (T)(A)(g * (of_listed * (double)of_all(logit[j]) - p * per));
     }
 }
 
@@ -205,25 +233,25 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const double *row_loss, 
 }
 
 template <typename T, int THREADS, int NV, bool MULTI>
-void launch_as(const DistillArgs &a, int64_t grid, hipStream_t stream)
+void launch_as(const DistillArgs &a, hipStream_t stream)
 {
     typedef RowTile<T, THREADS, NV> Tile;
     static_assert(Tile::COLS % 32 == 0, "bits of a tile fill whole words");
     const size_t lds = distill_lds<typename Wide<T>::type>(a.k, Tile::COLS);
-    distill_kernel<T, THREADS, NV, MULTI><<<dim3((unsigned)grid), dim3(THREADS), lds, stream>>>(a);
+    distill_kernel<T, THREADS, NV, MULTI><<<dim3((unsigned)a.rows), dim3(THREADS), lds, stream>>>(a);
 }
 
 template <typename T>
-void launch(const DistillArgs &a, int64_t grid, hipStream_t stream)
+void launch(const DistillArgs &a, hipStream_t stream)
 {
     const int64_t pieces = (a.cols + Vec16<T>::N - 1) / Vec16<T>::N;
-    if (pieces <= 64) return launch_as<T, 64, 1, false>(a, grid, stream);
-    if (pieces <= 64 * 4) return launch_as<T, 64, 4, false>(a, grid, stream);
-    if (pieces <= 256 * 4) return launch_as<T, 256, 4, false>(a, grid, stream);
-    if (pieces <= 256 * 16) return launch_as<T, 256, 16, false>(a, grid, stream);
-    if (pieces <= 1024 * 8) return launch_as<T, 1024, 8, false>(a, grid, stream);
-    if (pieces <= 1024 * 16) return launch_as<T, 1024, 16, false>(a, grid, stream);
-    launch_as<T, 1024, 8, true>(a, grid, stream);
+    if (pieces <= 64) return launch_as<T, 64, 1, false>(a, stream);
+    if (pieces <= 64 * 4) return launch_as<T, 64, 4, false>(a, stream);
+    if (pieces <= 64 * 16) return launch_as<T, 64, 16, false>(a, stream);
+    if (pieces <= 256 * 16) return launch_as<T, 256, 16, false>(a, stream);
+    if (pieces <= 512 * 16) return launch_as<T, 512, 16, false>(a, stream);
+    if (pieces <= 1024 * 16) return launch_as<T, 1024, 16, false>(a, stream);
+    launch_as<T, 512, 8, true>(a, stream);
 }
 
 }  // namespace
@@ -277,7 +305,7 @@ extern "C" int clg_distill_forward(int dtype, const void *logits, int64_t row_st
     }
     if (rows) {
         const int rc = clg_with_type(dtype, [&](auto t) {
-            launch<decltype(t)>(a, rows, clg_stream(stream));
+            launch<decltype(t)>(a, clg_stream(stream));
             return CLG_OK;
         });
         if (rc) return rc;
@@ -318,10 +346,8 @@ extern "C" int clg_distill_backward(int dtype, const void *logits, int64_t row_s
     } else if (reduction == CLG_REDUCE_MEAN) {
         a.grad_scale /= rows;
     }
-    // (rows whose gradient is there already are passed over: few workgroups look at many of them)
-    const int64_t grid = applied && rows > 2048 ? 2048 : rows;
     const int rc = clg_with_type(dtype, [&](auto t) {
-        launch<decltype(t)>(a, grid, clg_stream(stream));
+        launch<decltype(t)>(a, clg_stream(stream));
         return CLG_OK;
     });
     if (rc) return rc;

@@ -201,6 +201,7 @@ struct Balance : torch::autograd::Function<Balance> {
         keep.insert(keep.end(), {c->mask, coefs});
         ctx->save_for_backward(std::move(keep));
         ctx->mark_non_differentiable({counts});
+        ctx->set_materialize_grads(false);
         return {loss, counts};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)

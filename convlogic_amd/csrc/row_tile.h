@@ -26,15 +26,6 @@ __device__ __forceinline__ double lowest(double) { return -__builtin_inf(); }
 __device__ __forceinline__ float max_of(float a, float b) { return __builtin_fmaxf(a, b); }
 __device__ __forceinline__ double max_of(double a, double b) { return __builtin_fmax(a, b); }
 
-// e^(x / temperature) for x <= 0 up to the sign of rounding: scale is log2(e) / temperature for floats, 1 / temperature for doubles
-__device__ __forceinline__ float exp_scaled(float x, float scale) { return __builtin_amdgcn_exp2f(x * scale); }
-__device__ __forceinline__ double exp_scaled(double x, double scale) { return exp(x * scale); }
-template <typename A>
-__host__ __device__ inline A exp_scale(double temperature)
-{
-    return (A)((sizeof(A) == 4 ? 1.4426950408889634074 : 1.0) / temperature);
-}
-
 // a maximum as the sums subtract it: an infinite one is left out, so that rows of -inf sum to 0, rows with +inf to inf and NaN stays NaN
 template <typename A>
 __device__ __forceinline__ A finite_or_zero(A m)
@@ -42,11 +33,42 @@ __device__ __forceinline__ A finite_or_zero(A m)
     return __builtin_isinf(m) ? A(0) : m;
 }
 
-// the sum s of exponentials relative to the maximum `from` as one relative to `to`, which is no lower (a sum over -inf alone is 0, or NaN)
+// Exponentials of z / temperature relative to that of a value m.  Floats: 2^(scale z - at) in one multiply-add and the instruction for 2^x, with
+// scale = log2(e) / temperature and at = scale m as it is rounded; residue() is what that rounding moved, in 64 bits, for the few values that are not such
+// sums.  Beyond +-1e30 scale z would overflow, and two values that differ do so by more than any temperature reaches: there scale is 1.
 template <typename A>
-__device__ __forceinline__ A rescaled(A s, A from, A to, A scale)
+struct Exps;
+template <>
+struct Exps<float> {
+    float scale, at;
+    __host__ __device__ static double unit(double temperature) { return 1.4426950408889634074 / temperature; }
+    __device__ __forceinline__ Exps(float m, float unit_)
+    {
+#pragma clang fp contract(off)                                        // (`at` is the rounded product in all that is computed of it)
+        m = finite_or_zero(m);
+        scale = __builtin_fabsf(m) > 1e30f ? 1.f : unit_;
+        at = m * scale;
+    }
+    __device__ __forceinline__ float operator()(float z) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(z, scale, -at)); }
+    // the factor that makes a sum relative to this one of one relative to `to`, which is of a value no lower
+    __device__ __forceinline__ float factor(const Exps &to) const { return __builtin_amdgcn_exp2f(at - to.at); }
+    // natural logarithm of the sum 1 relative to m
+    __device__ __forceinline__ double residue(float m) const { return scale == 1.f ? 0.0 : ((double)at - (double)finite_or_zero(m) * (double)scale) * 0.69314718055994530942; }
+};
+template <>
+struct Exps<double> {
+    double scale, at;
+    __host__ __device__ static double unit(double temperature) { return 1.0 / temperature; }
+    __device__ __forceinline__ Exps(double m, double unit_) : scale(unit_), at(finite_or_zero(m)) {}
+    __device__ __forceinline__ double operator()(double z) const { return exp((z - at) * scale); }
+    __device__ __forceinline__ double factor(const Exps &to) const { return exp((at - to.at) * scale); }
+    __device__ __forceinline__ double residue(double) const { return 0.0; }
+};
+// the sum s of exponentials relative to `from` as one relative to `to` (a sum over -inf alone is 0, or NaN)
+template <typename A>
+__device__ __forceinline__ A rescaled(A s, A m_from, const Exps<A> &from, const Exps<A> &to)
 {
-    return from == lowest(A(0)) ? s : s * exp_scaled(finite_or_zero(from) - finite_or_zero(to), scale);
+    return m_from == lowest(A(0)) ? s : s * from.factor(to);
 }
 
 // Maximum over the 64 lanes (NaN is passed over), valid in all of them.
@@ -64,11 +86,11 @@ __device__ __forceinline__ double dpp_keep(double v)
     const uint32_t lo = __builtin_amdgcn_update_dpp(l, l, CTRL, ROW_MASK, 0xF, false), hi = __builtin_amdgcn_update_dpp(h, h, CTRL, ROW_MASK, 0xF, false);
     return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
-__device__ __forceinline__ float last_lane(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63)); }
-__device__ __forceinline__ double last_lane(double v)
+__device__ __forceinline__ float of_lane(float v, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); }
+__device__ __forceinline__ double of_lane(double v, int lane)
 {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, 63), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 63);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
     return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 template <typename A>
@@ -80,7 +102,14 @@ __device__ __forceinline__ A wave_max(A v)
     v = max_of(v, dpp_keep<0x140, 0xF>(v));
     v = max_of(v, dpp_keep<0x142, 0xA>(v));
     v = max_of(v, dpp_keep<0x143, 0xC>(v));
-    return last_lane(v);
+    return of_lane(v, 63);
+}
+
+// the value, computed where it stands: of a loop around a pass over a tile the compiler would keep every element's column in a register
+__device__ __forceinline__ int opaque(int v)
+{
+    asm volatile("" : "+v"(v));
+    return v;
 }
 
 // Columns base .. of one row in the registers of a workgroup: thread t holds the 16-byte pieces t, t + THREADS, ... and, of what is left of a row
@@ -89,6 +118,7 @@ template <typename T, int THREADS, int NV>
 struct RowTile {
     static constexpr int VEC = Vec16<T>::N, COLS = THREADS * NV * VEC;
     typedef typename Vec16<T>::type V;
+    typedef typename Wide<T>::type A;
     V v[NV];
     T last;
     int whole, tail;                                                  // whole pieces in the tile, elements behind them
@@ -99,51 +129,117 @@ struct RowTile {
         whole = n / VEC;
         tail = n % VEC;
         const T none = (T)lowest(0.f);
+        const T *at = row + base;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int p = j * THREADS + tid;
             if (j * THREADS < whole) {                                // (of the workgroup; lanes behind the row read its last piece again)
-                v[j] = *reinterpret_cast<const V *>(row + base + (int64_t)(p < whole ? p : whole - 1) * VEC);
-                if (p >= whole) v[j] = (V)none;
+                v[j] = *reinterpret_cast<const V *>(at + (uint32_t)((p < whole ? p : whole - 1) * VEC));
+                if ((j + 1) * THREADS > whole && p >= whole) v[j] = (V)none;
             } else {
                 v[j] = (V)none;
             }
         }
-        last = tid < tail ? row[base + (int64_t)whole * VEC + tid] : none;
+        last = tid < tail ? at[whole * VEC + tid] : none;
+    }
+    // keeps the values of the next pass apart from those of the last: both in registers at once would be twice the row
+    __device__ __forceinline__ void fence()
+    {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            u32x4 r = __builtin_bit_cast(u32x4, v[j]);
+            asm volatile("" : "+v"(r));
+            v[j] = __builtin_bit_cast(V, r);
+        }
     }
     // f(element, column in the tile) for the row's elements that this thread holds
     template <typename F>
     __device__ __forceinline__ void each(F f)
     {
-        const int tid = threadIdx.x;
+        const int tid = opaque(threadIdx.x);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             if (j * THREADS >= whole) break;
             if (j * THREADS + tid >= whole) break;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                T x = v[j][i];
-                f(x, (j * THREADS + tid) * VEC + i);
-                v[j][i] = x;
-            }
+            for (int i = 0; i < VEC; ++i) f(v[j][i], (j * THREADS + tid) * VEC + i);
         }
         if (tid < tail) f(last, whole * VEC + tid);
+    }
+    // f(highest of a piece, its elements as f2 takes them with their columns) for the pieces of this thread, and for its last element
+    template <typename F>
+    __device__ __forceinline__ void pieces(F f)
+    {
+        const int tid = opaque(threadIdx.x);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            if (j * THREADS >= whole) break;
+            if (j * THREADS + tid >= whole) break;
+            A high = (A)v[j][0];
+#pragma unroll
+            for (int i = 1; i < VEC; ++i) high = max_of(high, (A)v[j][i]);
+            f(high, [&](auto f2) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) f2((A)v[j][i], (j * THREADS + tid) * VEC + i);
+            });
+        }
+        if (tid < tail) f((A)last, [&](auto f2) { f2((A)last, whole * VEC + tid); });
+    }
+    // the columns with a bit become -inf
+    __device__ __forceinline__ void drop(const uint32_t *bits)
+    {
+        const int tid = threadIdx.x;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            if (j * THREADS >= whole) break;
+            const int c = (j * THREADS + tid) * VEC;
+            const uint32_t b = bits[c >> 5] >> (c & 31) & ((1u << VEC) - 1);
+            if (b)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i)
+                    if (b >> i & 1) v[j][i] = (T)lowest(0.f);
+        }
+        const int c = whole * VEC + tid;
+        if (tid < tail && (bits[c >> 5] >> (c & 31) & 1)) last = (T)lowest(0.f);
+    }
+    __device__ __forceinline__ A highest() const
+    {
+        A m = (A)last;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            if (j * THREADS >= whole) break;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) m = max_of(m, (A)v[j][i]);
+        }
+        return m;
+    }
+    __device__ __forceinline__ A sum(const Exps<A> &e) const
+    {
+        A s = e((A)last);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            if (j * THREADS >= whole) break;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) s += e((A)v[j][i]);
+        }
+        return s;
     }
     // the same columns of `row` = f(element); f's result is A
     template <typename F>
     __device__ __forceinline__ void store(T *__restrict__ row, int64_t base, F f) const
     {
         const int tid = threadIdx.x;
+        T *at = row + base;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int p = j * THREADS + tid;
             if (j * THREADS >= whole) break;
             V out;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) out[i] = (T)f(v[j][i]);
-            if (p < whole) *reinterpret_cast<V *>(row + base + (int64_t)p * VEC) = out;
+            for (int i = 0; i < VEC; ++i) out[i] = (T)f((A)v[j][i]);
+            if (p < whole) *reinterpret_cast<V *>(at + (uint32_t)(p * VEC)) = out;
         }
-        if (tid < tail) row[base + (int64_t)whole * VEC + tid] = (T)f(last);
+        if (tid < tail) at[whole * VEC + tid] = (T)f((A)last);
     }
 };
 
@@ -160,11 +256,12 @@ __device__ __forceinline__ void block_reduce(A (&x)[COUNT], A *room)
 #pragma unroll
             for (int c = 0; c < COUNT; ++c) room[(threadIdx.x >> 6) * COUNT + c] = x[c];
         __syncthreads();
+        static_assert(WAVES <= 16, "one row of lanes");
+        const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int c = 0; c < COUNT; ++c) {
-            A r = room[c];
-            for (int w = 1; w < WAVES; ++w) r = SUM ? r + room[w * COUNT + c] : max_of(r, room[w * COUNT + c]);
-            x[c] = r;
+            const A r = lane < WAVES ? room[lane * COUNT + c] : SUM ? A(0) : lowest(A(0));
+            x[c] = of_lane(SUM ? row16_sum(r) : row16_max(r), 0);
         }
     }
 }

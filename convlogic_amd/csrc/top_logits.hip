@@ -2,7 +2,7 @@
 // whole row, in one pass over the logits.
 //
 // No row is sorted.  The k-th highest of the threads' own maxima is a value that at least k elements reach, and hardly more do: they alone are written
-// to LDS, where each counts the candidates before it.  Rows with more candidates than room (equal values, ascending order) find the
+// to LDS, where each counts the candidates before it.  Rows with more candidates than room (equal values, the highest next to one another) find the
 // threshold bit by bit instead.
 #include "row_tile.h"
 
@@ -19,13 +19,30 @@ __device__ __forceinline__ uint64_t ordered(double v)
     const uint64_t u = __builtin_bit_cast(uint64_t, v + 0.0);
     return v != v ? ~0ull : (u ^ ((u >> 63) ? ~0ull : 1ull << 63));
 }
+__device__ __forceinline__ float value_of(uint32_t o) { return __builtin_bit_cast(float, (o >> 31) ? o ^ 0x80000000u : ~o); }
+__device__ __forceinline__ double value_of(uint64_t o) { return __builtin_bit_cast(double, (o >> 63) ? o ^ (1ull << 63) : ~o); }
+
+// candidates in the order of the answer: by value, of equal ones by column
 template <typename A>
-struct Key {
-    typedef uint32_t type;
+struct Cand;
+template <>
+struct Cand<float> {
+    typedef uint32_t K;
+    uint64_t v;
+    __device__ __forceinline__ Cand(K key, uint32_t column) : v((uint64_t)key << 32 | ~column) {}
+    __device__ __forceinline__ uint32_t column() const { return ~(uint32_t)v; }
+    __device__ __forceinline__ K key() const { return (K)(v >> 32); }
+    __device__ __forceinline__ bool before(const Cand &o) const { return v > o.v; }
 };
 template <>
-struct Key<double> {
-    typedef uint64_t type;
+struct Cand<double> {
+    typedef uint64_t K;
+    K k;
+    uint64_t c;
+    __device__ __forceinline__ Cand(K key, uint32_t column) : k(key), c(column) {}
+    __device__ __forceinline__ uint32_t column() const { return (uint32_t)c; }
+    __device__ __forceinline__ K key() const { return k; }
+    __device__ __forceinline__ bool before(const Cand &o) const { return k > o.k || (k == o.k && c < o.c); }
 };
 
 struct TopArgs {
@@ -38,135 +55,172 @@ struct TopArgs {
     void *lse;                                                        // [rows] in A
 };
 
-// Greatest t that at least `want` of the workgroup's values reach, or any such t that no more than `enough` reach: count(t) values of this thread
-// are t or more.
-template <int THREADS, typename K, typename F>
-__device__ __forceinline__ K search(int want, int enough, double *sums, F count)
+// A value that at least `want` of the keys of a wavefront reach, the greatest or one that no more than `enough` reach.
+template <int PER, typename K>
+__device__ __forceinline__ K wave_threshold(const K (&x)[PER], int want, int enough)
 {
     K t = 0;
+#pragma unroll 1
+    for (int b = 8 * sizeof(K) - 1; b >= 0; --b) {
+        const K next = t | (K)1 << b;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) n += __popcll(__ballot(x[i] >= next));
+        if (n < want) continue;
+        t = next;
+        if (n <= enough) break;
+    }
+    return t;
+}
+
+// The same of all values of a workgroup: count(t) of this thread's are t or more.
+template <int THREADS, typename K, typename F>
+__device__ __forceinline__ K threshold(int want, int enough, double *sums, F count)
+{
+    K t = 0;
+#pragma unroll 1
     for (int b = 8 * sizeof(K) - 1; b >= 0; --b) {
         const K next = t | (K)1 << b;
         double n[1] = {(double)count(next)};
         __syncthreads();
         block_reduce<true, THREADS>(n, sums);
-        if (n[0] >= want) t = next;
-        if (n[0] >= want && n[0] <= enough) break;
+        if (n[0] < want) continue;
+        t = next;
+        if (n[0] <= enough) break;
     }
     return t;
 }
 
-// One workgroup per row.  MULTI: rows that its registers do not hold go tile by tile, the k best so far before each tile's candidates.
+template <typename C>
+size_t top_lds(int threads, int room, int best)
+{
+    return 16 * 8 + 16 + (size_t)(room + best) * sizeof(C) + (size_t)threads * sizeof(typename C::K);
+}
+
+// One workgroup per row.  MULTI: rows that its registers do not hold go tile by tile, the k best so far in front of each tile's candidates.
 template <typename T, int THREADS, int NV, bool MULTI>
-__global__ __launch_bounds__(THREADS) void top_kernel(TopArgs a)
+__global__ __launch_bounds__(THREADS, 4) void top_kernel(TopArgs a)
 {
     typedef typename Wide<T>::type A;
-    typedef typename Key<A>::type K;
+    typedef Cand<A> C;
+    typedef typename C::K K;
     typedef RowTile<T, THREADS, NV> Tile;
     extern __shared__ char lds[];
     double *sums = reinterpret_cast<double *>(lds);                   // 16
-    int *count = reinterpret_cast<int *>(sums + 16);                  // (2 words)
-    K *cand = reinterpret_cast<K *>(sums + 17), *best = cand + a.room;                // candidates; the best so far, twice (MULTI)
-    uint32_t *at = reinterpret_cast<uint32_t *>(best + (MULTI ? 2 * a.k : 0)), *best_at = at + a.room;
+    K *shared = reinterpret_cast<K *>(sums + 16);                     // the threshold
+    int *count = reinterpret_cast<int *>(sums + 17);
+    C *cand = reinterpret_cast<C *>(sums + 18), *best = cand + a.room, *next = best + a.k;            // (best, next: MULTI)
+    K *maxima = reinterpret_cast<K *>(best + (MULTI ? 2 * a.k : 0));
     const int tid = threadIdx.x, k = a.k;
-    K *next = best + k;
-    uint32_t *next_at = best_at + k;
-    const A scale = exp_scale<A>(a.temperature);
+    const A unit = (A)Exps<A>::unit(a.temperature);
     const int64_t row = blockIdx.x;
     const T *z = static_cast<const T *>(a.z) + row * a.row_stride;
 
     A m_t = lowest(A(0)), s_t = 0;
     int have = 0;                                                     // in best
+#pragma unroll 1
     for (int64_t base = 0; base < a.cols; base += Tile::COLS) {
         Tile tile;
         tile.load(z, base, a.cols);
         const int n = (int)(a.cols - base < Tile::COLS ? a.cols - base : Tile::COLS);
-        // logsumexp, and the thread's highest
-        A m = lowest(A(0));
-        tile.each([&](T &x, int) { m = max_of(m, (A)x); });
-        const A both = max_of(m_t, m), safe = finite_or_zero(both);
-        if (MULTI) s_t = rescaled(s_t, m_t, both, scale);
-        tile.each([&](T &x, int) { s_t += exp_scaled((A)x - safe, scale); });
-        m_t = both;
-        const bool nan = s_t != s_t;                                  // (NaN of this thread, now or in an earlier tile)
-        // the threshold
-        K from;
-        if (have == k) from = best[k - 1];                            // (later columns have to be higher than the k-th, not equal)
-        else {
-            const K mine = nan ? ~(K)0 : ordered(m);
-            from = search<THREADS, K>(k, k + k / 4, sums, [&](K t) { return mine >= t; });
-            from -= from != 0;
-        }
-        // what is above it
-        __syncthreads();
+        const A mine = tile.highest();
+        if (have == 0) maxima[tid] = ordered(mine);
         if (tid == 0) *count = 0;
+        tile.fence();
+        const A m = max_of(m_t, mine);
+        const Exps<A> e(m, unit);
+        if (MULTI) s_t = rescaled(s_t, m_t, Exps<A>(m_t, unit), e);
+        s_t += tile.sum(e);
+        m_t = m;
+        const bool nan = s_t != s_t;                                  // (of this thread, now or in an earlier tile; it is in no maximum)
+        tile.fence();
         __syncthreads();
-        tile.each([&](T &x, int c) {
-            const K o = ordered((A)x);
-            if (o > from && c < n) {
-                const int i = atomicAdd(count, 1);
-                if (i < a.room) cand[i] = o, at[i] = (uint32_t)(base + c);
+        // what has to be exceeded
+        K from;
+        if (have) from = best[k - 1].key();                           // (a later column has to be higher than the k-th, not equal)
+        else {
+            if (tid < kWave) {
+                constexpr int PER = THREADS / kWave;
+                K x[PER];
+#pragma unroll
+                for (int i = 0; i < PER; ++i) x[i] = maxima[i * kWave + tid];
+                const K t = wave_threshold(x, k, k + k / 4);
+                if (tid == 0) *shared = t - (t != 0);
             }
-        });
+            __syncthreads();
+            from = *shared;
+        }
+        const A least = value_of((K)(from + (from != ~(K)0)));
+        const bool all = from < ordered(lowest(A(0))) || nan;
+        const auto collect = [&](auto wanted) {
+            tile.pieces([&](A high, auto each) {
+                if (high >= least || all)
+                    each([&](A x, int c) {
+                        const K o = ordered(x);
+                        if (wanted(o, c)) {
+                            const int i = atomicAdd(count, 1);
+                            if (i < a.room) cand[i] = C(o, (uint32_t)(base + c));
+                        }
+                    });
+            });
+        };
+        collect([&](K o, int) { return o > from; });
         __syncthreads();
         int found = *count;
         if (found > a.room) {
             // more than there is room for: the value that at least k reach, then the last column of those that equal it
-            const K value = search<THREADS, K>(k, a.room, sums, [&](K t) {
+            const K value = threshold<THREADS, K>(k, a.room, sums, [&](K t) {
                 int c_t = 0;
-                tile.each([&](T &x, int c) { c_t += c < n && ordered((A)x) >= t; });
+                tile.each([&](T x, int) { c_t += ordered((A)x) >= t; });
+                tile.fence();
                 return c_t;
             });
             double reach[2] = {0, 0};
-            tile.each([&](T &x, int c) {
+            tile.each([&](T x, int) {
                 const K o = ordered((A)x);
-                reach[0] += c < n && o > value;
-                reach[1] += c < n && o == value;
+                reach[0] += o > value;
+                reach[1] += o == value;
             });
+            tile.fence();
             __syncthreads();
             block_reduce<true, THREADS>(reach, sums);
             uint32_t last = ~0u;                                      // equal ones up to this column of the tile
             if (reach[0] + reach[1] > a.room) {
-                const uint32_t less = search<THREADS, uint32_t>(k - (int)reach[0], k - (int)reach[0], sums, [&](uint32_t t) {
-                    int c_t = 0;                                      // (columns counted from the end, so that t or more are the lowest columns)
-                    tile.each([&](T &x, int c) { c_t += c < n && ordered((A)x) == value && ~(uint32_t)c >= t; });
+                // (columns counted from the end, so that those that reach a threshold are the lowest)
+                last = ~threshold<THREADS, uint32_t>(k - (int)reach[0], k - (int)reach[0], sums, [&](uint32_t t) {
+                    int c_t = 0;
+                    tile.each([&](T x, int c) { c_t += ordered((A)x) == value && ~(uint32_t)c >= t; });
+                    tile.fence();
                     return c_t;
                 });
-                last = ~less;
             }
             __syncthreads();
             if (tid == 0) *count = 0;
             __syncthreads();
-            tile.each([&](T &x, int c) {
-                const K o = ordered((A)x);
-                if (c < n && (o > value || (o == value && (uint32_t)c <= last))) {
-                    const int i = atomicAdd(count, 1);
-                    if (i < a.room) cand[i] = o, at[i] = (uint32_t)(base + c);
-                }
-            });
+            collect([&](K o, int c) { return o > value || (o == value && (uint32_t)c <= last); });
             __syncthreads();
             found = *count;
         }
         // ranks: earlier tiles' best, then the candidates
         const bool end = !MULTI || base + Tile::COLS >= a.cols;
+#pragma unroll 1
         for (int i = tid; i < have + found; i += THREADS) {
-            const K mine = i < have ? best[i] : cand[i - have];
-            const uint32_t c = i < have ? best_at[i] : at[i - have];
+            const C mine = i < have ? best[i] : cand[i - have];
             int rank = 0;
-            for (int j = 0; j < have; ++j) rank += best[j] > mine || (best[j] == mine && best_at[j] < c);
-            for (int j = 0; j < found; ++j) rank += cand[j] > mine || (cand[j] == mine && at[j] < c);
+            for (int j = 0; j < have; ++j) rank += best[j].before(mine);
+            for (int j = 0; j < found; ++j) rank += cand[j].before(mine);
             if (rank >= k) continue;
             if (end) {
-                static_cast<T *>(a.values)[row * k + rank] = z[c];
-                a.columns[row * k + rank] = c;
+                static_cast<T *>(a.values)[row * k + rank] = z[mine.column()];
+                a.columns[row * k + rank] = mine.column();
             } else if (MULTI) {
-                next[rank] = mine, next_at[rank] = c;
+                next[rank] = mine;
             }
         }
         if (MULTI) {
             __syncthreads();
-            K *const spare = best;
-            uint32_t *const spare_at = best_at;
-            best = next, best_at = next_at, next = spare, next_at = spare_at;
+            C *const spare = best;
+            best = next, next = spare;
             have = k;
         }
     }
@@ -174,18 +228,20 @@ __global__ __launch_bounds__(THREADS) void top_kernel(TopArgs a)
     A top[1] = {m_t};
     __syncthreads();
     block_reduce<false, THREADS>(top, reinterpret_cast<A *>(sums));
-    double s[1] = {(double)rescaled(s_t, m_t, top[0], scale)};
+    const Exps<A> e(top[0], unit);
+    double s[1] = {(double)rescaled(s_t, m_t, Exps<A>(m_t, unit), e)};
     __syncthreads();
     block_reduce<true, THREADS>(s, sums);
-    if (tid == 0) static_cast<A *>(a.lse)[row] = (A)((double)finite_or_zero(top[0]) / a.temperature + log(s[0]));
+    if (tid == 0) static_cast<A *>(a.lse)[row] = (A)((double)finite_or_zero(top[0]) / a.temperature + log(s[0]) + e.residue(top[0]));
 }
 
 template <typename T, int THREADS, int NV, bool MULTI>
 void launch_as(TopArgs a, hipStream_t stream)
 {
-    typedef typename Key<typename Wide<T>::type>::type K;
-    a.room = a.k <= 128 ? 256 : 2 * a.k;
-    const size_t lds = 17 * 8 + (size_t)(a.room + (MULTI ? 2 * a.k : 0)) * (sizeof(K) + 4);
+    // (up to 64 KB of LDS: 1024 entries of a long row are 48 KB, in float64 60)
+    if (sizeof(T) == 8) a.room = a.k <= 128 ? 256 : a.k <= 512 ? 2 * a.k : a.k + a.k / 2;
+    else a.room = a.k <= 64 ? 256 : 4 * a.k;
+    const size_t lds = top_lds<Cand<typename Wide<T>::type>>(THREADS, a.room, MULTI ? 2 * a.k : 0);
     top_kernel<T, THREADS, NV, MULTI><<<dim3((unsigned)a.rows), dim3(THREADS), lds, stream>>>(a);
 }
 
@@ -197,9 +253,9 @@ void launch(const TopArgs &a, hipStream_t stream)
     if (pieces <= 64 * 4) return launch_as<T, 64, 4, false>(a, stream);
     if (pieces <= 256 * 4) return launch_as<T, 256, 4, false>(a, stream);
     if (pieces <= 256 * 16) return launch_as<T, 256, 16, false>(a, stream);
-    if (pieces <= 1024 * 8) return launch_as<T, 1024, 8, false>(a, stream);
+    if (pieces <= 512 * 16) return launch_as<T, 512, 16, false>(a, stream);
     if (pieces <= 1024 * 16) return launch_as<T, 1024, 16, false>(a, stream);
-    launch_as<T, 1024, 8, true>(a, stream);
+    launch_as<T, 512, 8, true>(a, stream);
 }
 
 constexpr int kMaxTop = 1024;
