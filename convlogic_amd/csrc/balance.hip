@@ -69,7 +69,7 @@ struct Sum {
 template <typename T, int G, int NV>
 struct RowPart {
     typedef typename Wide<T>::type A;
-    static constexpr int VEC = Vec16<T>::N, N = NV * VEC;
+    static constexpr int VEC = Vec16<T>::N, N = NV * VEC, kLanes = G;
     A x[N];
     __device__ __forceinline__ static int expert(int lane, int i) { return ((i / VEC) * G + lane) * VEC + i % VEC; }
     __device__ __forceinline__ void load(const T *row, int lane, int experts)
@@ -119,6 +119,35 @@ __device__ __forceinline__ int segment_of(const Segments &s)
 template <int N>
 constexpr int kAhead = N <= 4 ? 4 : N <= 8 ? 2 : 1;
 
+// (off by one step of its type at most, as the exponentials are)
+__device__ __forceinline__ float reciprocal(float v) { return __builtin_amdgcn_rcpf(v); }
+__device__ __forceinline__ double reciprocal(double v) { return 1.0 / v; }
+
+// the choice of one row, one expert at a time: the lowest of the highest that are left
+template <typename Part, int N>
+__device__ __forceinline__ void choose(Part &part, int lane, int k, int (&c)[N])
+{
+    typedef typename Part::A A;
+    const A none = lowest(A(0));
+#pragma unroll
+    for (int i = 0; i < N; ++i) part.x[i] = part.x[i] != part.x[i] ? -none : part.x[i];
+#pragma unroll 1
+    for (int pick = 0; pick < k; ++pick) {
+        const A top = part.highest();
+        if (top == none) break;
+        int which = kMaxExperts;
+#pragma unroll
+        for (int i = N - 1; i >= 0; --i) which = part.x[i] == top ? Part::expert(lane, i) : which;
+        which = group_reduce<Part::kLanes>(which, [](int u, int v) { return u < v ? u : v; });
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool it = Part::expert(lane, i) == which;
+            c[i] += it;
+            part.x[i] = it ? none : part.x[i];
+        }
+    }
+}
+
 // sums and counts of a workgroup's rows
 template <typename T, int G, int NV>
 __global__ __launch_bounds__(kThreads) void balance_kernel(BalanceArgs a)
@@ -140,59 +169,64 @@ __global__ __launch_bounds__(kThreads) void balance_kernel(BalanceArgs a)
         for (int r = 0; r < R; ++r) {
             const int64_t row = row0 + r * groups;
             kept[r] = row < rows && !(a.mask && !a.mask[row]);
-            if (kept[r]) part[r].load(z + row * a.seg.stride[seg], lane, a.experts);
+            part[r].load(z + (kept[r] ? row : row0) * a.seg.stride[seg], lane, a.experts);
+        }
+        // (rows that do not count go the same way with a weight of 0: the steps of R rows fill one another's waits)
+        A m[R], e[R][N], s[R];
+        bool odd = false;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) part[r].x[i] = kept[r] ? part[r].x[i] : A(0);
+            m[r] = part[r].highest();
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r] = part[r].exponentials(m[r], e[r]);
+        // The choice: k times the highest below the last one.  -inf is none, NaN is above everything.  Where values are equal, or too few are there,
+        // these are too many or too few experts, and the slow way takes one at a time, the lowest of the highest.
+        A least[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            kept[r] = kept[r] && !(s[r] == 0);
+            n += kept[r];
+            least[r] = m[r];
+            odd |= s[r] != s[r];
+        }
+#pragma unroll 1
+        for (int pick = 1; pick < a.k; ++pick) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                A next = lowest(A(0));
+#pragma unroll
+                for (int i = 0; i < N; ++i) next = max_of(next, part[r].x[i] < least[r] ? part[r].x[i] : lowest(A(0)));
+                least[r] = group_reduce<G>(next, Max());
+            }
+        }
+        int want = 0, have = 0;                                       // of the wavefront
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            odd |= kept[r] && least[r] == lowest(A(0));
+            want += __popcll(__ballot(kept[r]));
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const bool it = kept[r] && part[r].x[i] >= least[r];
+                have += __popcll(__ballot(it));
+                c[i] += it;
+            }
+        }
+        if (__any(odd) || have * G != want * a.k) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) c[i] -= kept[r] && part[r].x[i] >= least[r];
+                if (kept[r]) choose(part[r], lane, a.k, c);
+            }
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (!kept[r]) continue;
-            Part &x = part[r];
-            const A m = x.highest();
-            A e[N];
-            const A s = x.exponentials(m, e), inv = A(1) / s;
-            if (s == 0) continue;                                     // (of the whole group)
-            n += 1;
-            // The choice: k times the highest below the last one.  Where values are equal these are too few or too many experts, and the slow way
-            // takes one at a time, the lowest of the highest.  -inf is none, NaN is above everything.
-            A least = m;
-            if (s != s) {
-                least = -lowest(A(0));
+            const A inv = kept[r] ? reciprocal(s[r]) : A(0);
 #pragma unroll
-                for (int i = 0; i < N; ++i) x.x[i] = x.x[i] != x.x[i] ? least : x.x[i];
-            }
-#pragma unroll 1
-            for (int pick = 1; pick < a.k; ++pick) {
-                A next = lowest(A(0));
-#pragma unroll
-                for (int i = 0; i < N; ++i) next = max_of(next, x.x[i] < least ? x.x[i] : lowest(A(0)));
-                least = group_reduce<G>(next, Max());
-            }
-            int chosen = 0;
-            const A floor = lowest(A(0));
-#pragma unroll
-            for (int i = 0; i < N; ++i) chosen += x.x[i] >= least && x.x[i] > floor;
-            chosen = group_reduce<G>(chosen, Sum());
-            if (chosen <= a.k) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) c[i] += x.x[i] >= least && x.x[i] > floor;
-            } else {
-#pragma unroll 1
-                for (int pick = 0; pick < a.k; ++pick) {
-                    const A top = x.highest();
-                    if (top == floor) break;
-                    int which = kMaxExperts;
-#pragma unroll
-                    for (int i = N - 1; i >= 0; --i) which = x.x[i] == top ? Part::expert(lane, i) : which;
-                    which = group_reduce<G>(which, [](int u, int v) { return u < v ? u : v; });
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        const bool it = Part::expert(lane, i) == which;
-                        c[i] += it;
-                        x.x[i] = it ? floor : x.x[i];
-                    }
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < N; ++i) p[i] += e[i] * inv;
+            for (int i = 0; i < N; ++i) p[i] += e[r][i] * inv;
         }
     }
     // groups of a wavefront, then its four wavefronts, in a fixed order
@@ -333,7 +367,7 @@ __global__ __launch_bounds__(kThreads) void balance_grad_kernel(BalanceArgs a)
             if (kept[r]) {
                 const A s = part[r].exponentials(part[r].highest(), e);
                 kept[r] = !(s == 0);
-                inv = A(1) / s;
+                inv = reciprocal(s);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     e[i] *= inv;

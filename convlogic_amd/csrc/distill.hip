@@ -72,24 +72,36 @@ __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
     T *grad = a.grad ? static_cast<T *>(a.grad) + row * a.cols : nullptr;
     const bool kept = !a.mask || a.mask[row];
     const T *z = static_cast<const T *>(a.z) + row * a.row_stride;
+    // the teacher's entries, of which the first come with the row, in front of it: the logits in their columns are a load more
+    const auto column_of = [&](int j) -> int64_t {
+        const int64_t at = row * k + j;
+        return a.columns64 ? static_cast<const int64_t *>(a.columns)[at] : static_cast<const int32_t *>(a.columns)[at];
+    };
+    int64_t first_column = -1;
+    uint64_t first_value = 0, lse_bits = 0;
+    if (kept) {
+        if (tid < k) {
+            first_column = column_of(tid);
+            first_value = load_bits(a.values, a.values_type, row * k + tid);
+        }
+        if (a.lse) lse_bits = load_bits(a.lse, a.lse_type, row);
+    }
     Tile tile;
     if (kept) tile.load(z, 0, a.cols);
-
-    // the teacher's entries
     if (tid == 0) *flags = 0;
     __syncthreads();
-    A tops[3] = {lowest(A(0)), lowest(A(0)), lowest(A(0))};       // highest of the teacher, of the student's listed logits, of the others
+    A tops[3] = {lowest(A(0)), lowest(A(0)), lowest(A(0))};           // highest of the teacher, of the student's listed logits, of the others
     if (kept) {
         int seen = 0;
 #pragma unroll 1
-    for (int j = tid; j < k; j += THREADS) {
-            const int64_t at = row * k + j, c = a.columns64 ? static_cast<const int64_t *>(a.columns)[at] : static_cast<const int32_t *>(a.columns)[at];
+        for (int j = tid; j < k; j += THREADS) {
+            const int64_t c = j == tid ? first_column : column_of(j);
             const bool there = c >= 0 && c < a.cols;
             seen |= there ? kFlagListed : c >= a.cols ? kFlagBad : 0;
             column[j] = there ? (int)c : -1;
             if (!there) continue;
-            const double t = load_any(a.values, a.values_type, at) * inv_tau;
             const A l = (A)z[c];
+            const double t = value_of_bits(j == tid ? first_value : load_bits(a.values, a.values_type, row * k + j), a.values_type) * inv_tau;
             prob[j] = t;
             logit[j] = l;
             tops[0] = max_of(tops[0], (A)t);
@@ -146,7 +158,7 @@ __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
     // sums: the others' exponentials relative to m_u, the listed ones' relative to m, the teacher's, the teacher's share times the difference of the
     // logarithms
     double sums[4] = {(double)rescaled(s_t, m_t, Exps<A>(m_t, unit), of_rest), 0, 0, 0};
-    const double base_t = a.lse ? load_any(a.lse, a.lse_type, row) : (double)finite_or_zero(tops[0]);
+    const double base_t = a.lse ? value_of_bits(lse_bits, a.lse_type) : (double)finite_or_zero(tops[0]);
 #pragma unroll 1
     for (int j = tid; j < k; j += THREADS) {
         if (column[j] < 0) continue;

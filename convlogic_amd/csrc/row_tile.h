@@ -130,17 +130,18 @@ struct RowTile {
         tail = n % VEC;
         const T none = (T)lowest(0.f);
         const T *at = row + base;
+        // (all loads before anything waits for one: lanes behind the row read its last piece again, and drop it afterwards)
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int p = j * THREADS + tid;
-            if (j * THREADS < whole) {                                // (of the workgroup; lanes behind the row read its last piece again)
-                v[j] = *reinterpret_cast<const V *>(at + (uint32_t)((p < whole ? p : whole - 1) * VEC));
-                if ((j + 1) * THREADS > whole && p >= whole) v[j] = (V)none;
-            } else {
-                v[j] = (V)none;
-            }
+            if (j * THREADS < whole) v[j] = *reinterpret_cast<const V *>(at + (uint32_t)((p < whole ? p : whole - 1) * VEC));
+            else v[j] = (V)none;
         }
-        last = tid < tail ? at[whole * VEC + tid] : none;
+        last = none;
+        if (tid < tail) last = at[whole * VEC + tid];
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS < whole && (j + 1) * THREADS > whole && j * THREADS + tid >= whole) v[j] = (V)none;
     }
     // keeps the values of the next pass apart from those of the last: both in registers at once would be twice the row
     __device__ __forceinline__ void fence()
@@ -266,14 +267,22 @@ __device__ __forceinline__ void block_reduce(A (&x)[COUNT], A *room)
     }
 }
 
-// element i of an array of one of the C ABI's types, as a double
-__device__ __forceinline__ double load_any(const void *p, int dtype, int64_t i)
+// element i of an array of one of the C ABI's types: its bits, which may still be on their way, and its value
+__device__ __forceinline__ uint64_t load_bits(const void *p, int dtype, int64_t i)
 {
     switch (dtype) {
-    case CLG_F64: return static_cast<const double *>(p)[i];
-    case CLG_F16: return (double)(float)static_cast<const _Float16 *>(p)[i];
-    case CLG_BF16: return (double)(float)static_cast<const __bf16 *>(p)[i];
-    default: return (double)static_cast<const float *>(p)[i];
+    case CLG_F64: return static_cast<const uint64_t *>(p)[i];
+    case CLG_F32: return static_cast<const uint32_t *>(p)[i];
+    default: return static_cast<const uint16_t *>(p)[i];
+    }
+}
+__device__ __forceinline__ double value_of_bits(uint64_t u, int dtype)
+{
+    switch (dtype) {
+    case CLG_F64: return __builtin_bit_cast(double, u);
+    case CLG_F16: return (double)(float)__builtin_bit_cast(_Float16, (uint16_t)u);
+    case CLG_BF16: return (double)__builtin_bit_cast(float, (uint32_t)u << 16);
+    default: return (double)__builtin_bit_cast(float, (uint32_t)u);
     }
 }
 
