@@ -105,13 +105,6 @@ __device__ __forceinline__ A wave_max(A v)
     return of_lane(v, 63);
 }
 
-// the value, computed where it stands: of a loop around a pass over a tile the compiler would keep every element's column in a register
-__device__ __forceinline__ int opaque(int v)
-{
-    asm volatile("" : "+v"(v));
-    return v;
-}
-
 // Columns base .. of one row in the registers of a workgroup: thread t holds the 16-byte pieces t, t + THREADS, ... and, of what is left of a row
 // behind its last whole piece, one element.  What is behind the row is -inf.
 template <typename T, int THREADS, int NV>
@@ -153,38 +146,16 @@ struct RowTile {
             v[j] = __builtin_bit_cast(V, r);
         }
     }
-    // f(element, column in the tile) for the row's elements that this thread holds
-    template <typename F>
-    __device__ __forceinline__ void each(F f)
+    // the highest of each piece
+    __device__ __forceinline__ void peaks(A (&high)[NV]) const
     {
-        const int tid = opaque(threadIdx.x);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            if (j * THREADS >= whole) break;
-            if (j * THREADS + tid >= whole) break;
+            high[j] = lowest(A(0));
+            if (j * THREADS >= whole) continue;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) f(v[j][i], (j * THREADS + tid) * VEC + i);
+            for (int i = 0; i < VEC; ++i) high[j] = max_of(high[j], (A)v[j][i]);
         }
-        if (tid < tail) f(last, whole * VEC + tid);
-    }
-    // f(highest of a piece, its elements as f2 takes them with their columns) for the pieces of this thread, and for its last element
-    template <typename F>
-    __device__ __forceinline__ void pieces(F f)
-    {
-        const int tid = opaque(threadIdx.x);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            if (j * THREADS >= whole) break;
-            if (j * THREADS + tid >= whole) break;
-            A high = (A)v[j][0];
-#pragma unroll
-            for (int i = 1; i < VEC; ++i) high = max_of(high, (A)v[j][i]);
-            f(high, [&](auto f2) {
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) f2((A)v[j][i], (j * THREADS + tid) * VEC + i);
-            });
-        }
-        if (tid < tail) f((A)last, [&](auto f2) { f2((A)last, whole * VEC + tid); });
     }
     // the columns with a bit become -inf
     __device__ __forceinline__ void drop(const uint32_t *bits)
