@@ -74,9 +74,10 @@ std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor &logits_in, int64_t k
     shape.back() = k;
     Tensor values = at::empty(shape, logits.options()), columns = at::empty(shape, logits.options().dtype(at::kLong));
     shape.pop_back();
-    Tensor lse = at::empty(shape, wide(logits));
+    Tensor lse = at::empty(shape, wide(logits)), scratch;
+    if (const int64_t n = clg_top_logits_scratch_bytes(code_of(logits), r.rows, r.cols, k)) scratch = at::empty({n}, logits.options().dtype(at::kByte));
     check(clg_top_logits(code_of(logits), r.at, r.stride, r.rows, r.cols, k, temperature, values.data_ptr(), static_cast<int64_t *>(columns.data_ptr()),
-                         lse.data_ptr(), stream_of(logits)));
+                         lse.data_ptr(), scratch.defined() ? scratch.data_ptr() : nullptr, stream_of(logits)));
     return {values, columns, lse};
 }
 

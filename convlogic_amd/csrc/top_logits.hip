@@ -55,6 +55,10 @@ struct TopArgs {
     void *values;                                                     // [rows][k]
     int64_t *columns;                                                 // [rows][k]
     void *lse;                                                        // [rows] in A
+    int parts;                                                        // of a row, each with a workgroup of its own
+    int64_t width;                                                    // columns of a part
+    void *part_best;                                                  // [rows][parts][k] candidates in order
+    double *part_lse;                                                 // [rows][parts]
 };
 
 // A value that at least `want` of the keys of a wavefront reach, the greatest or one that no more than `enough` reach.
@@ -75,24 +79,27 @@ __device__ __forceinline__ K wave_threshold(const K (&x)[PER], int want, int eno
     return t;
 }
 
-// Maxima that the first threshold is made of: the threads' own, or of each piece where k is more than a third of the threads.
+// Maxima that the threshold is made of: the threads' own, or where k is more than a third of the threads up to four of each.
 template <int THREADS, int NV>
-__host__ __device__ __forceinline__ bool of_pieces(int k)
+constexpr int kSeen = THREADS >= 1024 ? 1 : NV < 4 ? NV : 4;
+template <int THREADS, int NV>
+__host__ __device__ __forceinline__ bool by_pieces(int k)
 {
-    return NV > 1 && 3 * k > THREADS;
+    return kSeen<THREADS, NV> > 1 && 3 * k > THREADS;
 }
 
 constexpr int kSpare = 512;                                           // candidates that there is room for beside the k best
-constexpr int kNoted = 512;                                           // pieces that may be noted when a tile begins
+constexpr int kAllRanked = 128;                                       // columns of rows without a threshold
+constexpr int kNoted = 1024;                                          // pieces that may be noted when a tile begins
 
 // LDS of a workgroup: reduction room, counters, candidates, the best k, maxima, noted pieces
-template <typename T, int THREADS, int NV>
+template <typename T, int THREADS, int NV, bool MULTI>
 struct TopRoom {
     typedef Cand<typename Wide<T>::type> C;
     int room, maxima, notes;
     size_t bytes;
     __host__ __device__ explicit TopRoom(int k)
-        : room(k + (k > kSpare ? k : kSpare)), maxima(THREADS * (of_pieces<THREADS, NV>(k) ? NV : 1)), notes(THREADS * NV + Vec16<T>::N + kNoted),
+        : room(k + (k > kSpare ? k : kSpare)), maxima(THREADS * (by_pieces<THREADS, NV>(k) ? kSeen<THREADS, NV> : 1)), notes(THREADS * NV + Vec16<T>::N + (MULTI ? kNoted : 0)),
           bytes(18 * 8 + (size_t)(room + k) * sizeof(C) + (size_t)maxima * sizeof(typename C::K) + (size_t)notes * 4)
     {
     }
@@ -100,25 +107,25 @@ struct TopRoom {
 
 // One workgroup per row; MULTI: of more than one tile.
 template <typename T, int THREADS, int NV, bool MULTI>
-__global__ __launch_bounds__(THREADS) void top_kernel(TopArgs a)
+__global__ __launch_bounds__(THREADS, sizeof(T) == 8 ? 2 : 6) void top_kernel(TopArgs a)
 {
     typedef typename Wide<T>::type A;
     typedef Cand<A> C;
     typedef typename C::K K;
     typedef RowTile<T, THREADS, NV> Tile;
     extern __shared__ char lds[];
-    const TopRoom<T, THREADS, NV> size(a.k);
+    const TopRoom<T, THREADS, NV, MULTI> size(a.k);
     double *sums = reinterpret_cast<double *>(lds);                   // of 16 wavefronts
     K *shared = reinterpret_cast<K *>(sums + 16);                     // the threshold
     int *noted = reinterpret_cast<int *>(sums + 17), *count = noted + 1;
     C *cand = reinterpret_cast<C *>(sums + 18), *best = cand + size.room;
     K *maxima = reinterpret_cast<K *>(best + a.k);
     uint32_t *note = reinterpret_cast<uint32_t *>(maxima + size.maxima);             // first columns
-    const int tid = threadIdx.x, k = a.k;
+    const int tid = threadIdx.x, part = blockIdx.y;
     const A unit = (A)Exps<A>::unit(a.temperature);
-    const int64_t row = blockIdx.x;
-    const T *z = static_cast<const T *>(a.z) + row * a.row_stride;
-    const int64_t whole = a.cols / Tile::VEC * Tile::VEC;
+    const int64_t row = blockIdx.x, start = part * a.width, cols = a.cols - start < a.width ? a.cols - start : a.width, whole = cols / Tile::VEC * Tile::VEC;
+    const int k = a.k < cols ? a.k : (int)cols;
+    const T *z = static_cast<const T *>(a.z) + row * a.row_stride + start;
 
     int found = 0;                                                    // candidates
     C from(0, 0);                                                     // what a candidate has to be before
@@ -185,15 +192,16 @@ __global__ __launch_bounds__(THREADS) void top_kernel(TopArgs a)
         }
     };
 
-    A m_t = lowest(A(0)), s_t = 0, seen[NV];                          // seen: highest by piece, of the tiles so far
+    A m_t = lowest(A(0)), s_t = 0, seen[kSeen<THREADS, NV>];          // seen: highest of the tiles so far, in parts
+    constexpr int SEEN = kSeen<THREADS, NV>;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) seen[j] = lowest(A(0));
-    const bool pieces = of_pieces<THREADS, NV>(k);
+    for (int j = 0; j < SEEN; ++j) seen[j] = lowest(A(0));
+    const bool pieces = by_pieces<THREADS, NV>(k);
     // the k-th highest of the maxima, by the first wavefront, between two barriers
     const auto show = [&]() {
         if (pieces) {
 #pragma unroll
-            for (int j = 0; j < NV; ++j) maxima[j * THREADS + tid] = ordered(seen[j]);
+            for (int j = 0; j < SEEN; ++j) maxima[j * THREADS + tid] = ordered(seen[j]);
         } else {
             maxima[tid] = ordered(m_t);
         }
@@ -203,15 +211,15 @@ __global__ __launch_bounds__(THREADS) void top_kernel(TopArgs a)
         constexpr int PER = THREADS / kWave;
         K t;
         if (pieces) {
-            K x[PER * NV];
+            K x[PER * SEEN];
 #pragma unroll
-            for (int i = 0; i < PER * NV; ++i) x[i] = maxima[i * kWave + tid];
-            t = wave_threshold(x, k, k + k / 4);
+            for (int i = 0; i < PER * SEEN; ++i) x[i] = maxima[i * kWave + tid];
+            t = wave_threshold(x, k, k + k / 4 + 8);
         } else {
             K x[PER];
 #pragma unroll
             for (int i = 0; i < PER; ++i) x[i] = maxima[i * kWave + tid];
-            t = wave_threshold(x, k, k + k / 4);
+            t = wave_threshold(x, k, k + k / 4 + 8);
         }
         if (tid == 0) *shared = t - (t != 0);
     };
@@ -221,19 +229,17 @@ __global__ __launch_bounds__(THREADS) void top_kernel(TopArgs a)
         if (now.key() > from.key()) from = now;
     };
 
-    Tile tile, coming;
-    coming.load(z, 0, a.cols);
+    Tile tile;
     if (tid == 0) *noted = 0;
 #pragma unroll 1
-    for (int64_t base = 0, tiles = 1; base < a.cols; base += Tile::COLS, ++tiles) {
-        tile = coming;
-        if (MULTI && base + Tile::COLS < a.cols) coming.load(z, base + Tile::COLS, a.cols);
+    for (int64_t base = 0, tiles = 1; base < cols; base += Tile::COLS, ++tiles) {
+        tile.load(z, base, cols);
         A high[NV], m = max_of(m_t, (A)tile.last);
         tile.peaks(high);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             m = max_of(m, high[j]);
-            seen[j] = max_of(seen[j], high[j]);
+            seen[j % SEEN] = max_of(seen[j % SEEN], high[j]);
         }
         seen[0] = max_of(seen[0], (A)tile.last);
         tile.fence();
@@ -242,6 +248,19 @@ __global__ __launch_bounds__(THREADS) void top_kernel(TopArgs a)
         s_t += tile.sum(e);
         m_t = m;
         const bool nan = s_t != s_t;                                  // (of this thread, now or in an earlier tile; it is in no maximum)
+        if (!MULTI && NV == 1 && cols <= kAllRanked) {                // (a short row: every element is a candidate)
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = (j * THREADS + tid) * Tile::VEC;
+#pragma unroll
+                for (int i = 0; i < Tile::VEC; ++i)
+                    if (c + i < tile.whole * Tile::VEC) cand[c + i] = C(ordered((A)tile.v[j][i]), c + i);
+            }
+            const int c = tile.whole * Tile::VEC + tid;
+            if (tid < tile.tail) cand[c] = C(ordered((A)tile.last), c);
+            found = (int)cols;
+            break;
+        }
         if (base == 0) {
             show();
             __syncthreads();
@@ -260,7 +279,7 @@ __global__ __launch_bounds__(THREADS) void top_kernel(TopArgs a)
         }
         if (tid < tile.tail && ((A)tile.last >= least || all)) note[atomicAdd(noted, 1)] = (uint32_t)(base + tile.whole * Tile::VEC + tid);
         if (MULTI) {
-            const bool last = base + Tile::COLS >= a.cols, anew = base && (last || (tiles & (tiles - 1)) == 0);
+            const bool last = base + Tile::COLS >= cols, anew = base && (last || (tiles & (tiles - 1)) == 0);
             if (anew) show();
             __syncthreads();
             if (anew) search();
@@ -276,10 +295,17 @@ __global__ __launch_bounds__(THREADS) void top_kernel(TopArgs a)
     }
     if (!MULTI) __syncthreads();
     take_all(*noted);
+    C *const mine = static_cast<C *>(a.part_best) + (row * a.parts + part) * a.k;
     rank([&](C c, int i) {
-        static_cast<T *>(a.values)[row * k + i] = z[c.column()];
-        a.columns[row * k + i] = c.column();
+        if (a.parts > 1) {
+            mine[i] = C(c.key(), (uint32_t)start + c.column());
+        } else {
+            static_cast<T *>(a.values)[row * k + i] = z[c.column()];
+            a.columns[row * k + i] = c.column();
+        }
     });
+    if (a.parts > 1)
+        for (int i = k + tid; i < a.k; i += THREADS) mine[i] = C(0, ~0u);
     if (!a.lse) return;
     A top[1] = {m_t};
     block_reduce<false, THREADS>(top, reinterpret_cast<A *>(sums));
@@ -287,32 +313,105 @@ __global__ __launch_bounds__(THREADS) void top_kernel(TopArgs a)
     double s[1] = {(double)rescaled(s_t, m_t, Exps<A>(m_t, unit), e)};
     __syncthreads();
     block_reduce<true, THREADS>(s, sums);
-    if (tid == 0) static_cast<A *>(a.lse)[row] = (A)((double)finite_or_zero(top[0]) / a.temperature + log(s[0]) + e.residue(top[0]));
+    if (tid != 0) return;
+    const double lse = (double)finite_or_zero(top[0]) / a.temperature + log(s[0]) + e.residue(top[0]);
+    if (a.parts > 1) a.part_lse[row * a.parts + part] = lse;
+    else static_cast<A *>(a.lse)[row] = (A)lse;
+}
+
+constexpr int kMostParts = 64, kMerged = 1024;                        // parts of a row, and their candidates
+
+// The parts of a row together: the candidates that reach a value which k of them reach, by rank.
+template <typename T>
+__global__ __launch_bounds__(256) void top_merge_kernel(TopArgs a)
+{
+    typedef typename Wide<T>::type A;
+    typedef Cand<A> C;
+    typedef typename C::K K;
+    extern __shared__ char lds[];
+    const int64_t row = blockIdx.x;
+    const int n = a.parts * a.k, tid = threadIdx.x;
+    K *shared = reinterpret_cast<K *>(lds);
+    int *count = reinterpret_cast<int *>(lds + 8);
+    C *all = reinterpret_cast<C *>(lds + 16), *some = all + n;
+    const C *mine = static_cast<const C *>(a.part_best) + row * n;
+    const T *z = static_cast<const T *>(a.z) + row * a.row_stride;
+    for (int i = tid; i < n; i += 256) all[i] = mine[i];
+    if (tid == 0) *count = 0;
+    __syncthreads();
+    if (tid < kWave) {
+        K x[kMerged / kWave];
+#pragma unroll
+        for (int i = 0; i < kMerged / kWave; ++i) x[i] = i * kWave + tid < n ? all[i * kWave + tid].key() : K(0);
+        const K t = wave_threshold(x, a.k, a.k + a.k / 4 + 8);
+        if (tid == 0) *shared = t;
+    }
+    __syncthreads();
+    const K least = *shared;
+    for (int i = tid; i < n; i += 256) {
+        const C c = all[i];
+        if (c.key() >= least && c.key() != 0) some[atomicAdd(count, 1)] = c;
+    }
+    __syncthreads();
+    const int m = *count;
+    for (int i = tid; i < m; i += 256) {
+        const C c = some[i];
+        int before = 0;
+#pragma unroll 8
+        for (int j = 0; j < m; ++j) before += some[j].before(c);
+        if (before >= a.k) continue;
+        static_cast<T *>(a.values)[row * a.k + before] = z[c.column()];
+        a.columns[row * a.k + before] = c.column();
+    }
+    if (!a.lse || tid >= kWave) return;
+    const double l = tid < a.parts ? a.part_lse[row * a.parts + tid] : lowest(0.0), top = finite_or_zero(wave_max(l)), s = wave_sum(exp(l - top));
+    if (tid == 0) static_cast<A *>(a.lse)[row] = (A)(top + log(s));
 }
 
 template <typename T, int THREADS, int NV, bool MULTI>
 void launch_as(const TopArgs &a, hipStream_t stream)
 {
-    top_kernel<T, THREADS, NV, MULTI><<<dim3((unsigned)a.rows), dim3(THREADS), TopRoom<T, THREADS, NV>(a.k).bytes, stream>>>(a);
+    top_kernel<T, THREADS, NV, MULTI><<<dim3((unsigned)a.rows, a.parts), dim3(THREADS), TopRoom<T, THREADS, NV, MULTI>(a.k).bytes, stream>>>(a);
 }
 
 template <typename T>
 void launch(const TopArgs &a, hipStream_t stream)
 {
-    const int64_t pieces = (a.cols + Vec16<T>::N - 1) / Vec16<T>::N;
-    if (pieces <= 64) return launch_as<T, 64, 1, false>(a, stream);
-    if (pieces <= 64 * 4) return launch_as<T, 64, 4, false>(a, stream);
-    if (pieces <= 256 * 4) return launch_as<T, 256, 4, false>(a, stream);
-    if (a.rows > 512) return launch_as<T, 256, 4, true>(a, stream);
-    launch_as<T, sizeof(T) == 8 ? 256 : 1024, 4, true>(a, stream);
+    const int64_t pieces = (a.width + Vec16<T>::N - 1) / Vec16<T>::N;
+    if (pieces <= 64) launch_as<T, 64, 1, false>(a, stream);
+    else if (pieces <= 64 * 4) launch_as<T, 64, 4, false>(a, stream);
+    else if (pieces <= 256 * 4) launch_as<T, 256, 4, false>(a, stream);
+    else if (a.rows * a.parts > 512) launch_as<T, 256, 8, true>(a, stream);
+    else launch_as<T, sizeof(T) == 8 ? 256 : 1024, 8, true>(a, stream);
+    if (a.parts > 1)
+        top_merge_kernel<T><<<dim3((unsigned)a.rows), dim3(256), 16 + (size_t)a.parts * a.k * 2 * sizeof(Cand<typename Wide<T>::type>), stream>>>(a);
+}
+
+// Few long rows are shared out among workgroups, whose best are merged by a second launch.
+int parts_of(int64_t rows, int64_t cols, int64_t k)
+{
+    if (rows > 64 || rows == 0) return 1;
+    if (cols <= 65536) return 1;
+    int64_t parts = cols / 4096;
+    if (parts > kMostParts) parts = kMostParts;
+    if (parts * k > kMerged) parts = kMerged / k;
+    if (parts * rows > 1024) parts = 1024 / rows;
+    return parts < 4 ? 1 : (int)parts;
 }
 
 constexpr int kMaxTop = 1024;
 
 }  // namespace
 
+extern "C" int64_t clg_top_logits_scratch_bytes(int dtype, int64_t rows, int64_t cols, int64_t k)
+{
+    if (!clg_score_type(dtype) || rows < 0 || cols < 1 || k < 1 || k > kMaxTop) return 0;
+    const int parts = parts_of(rows, cols, k);
+    return parts == 1 ? 0 : rows * parts * (k * (dtype == CLG_F64 ? 16 : 8) + 8);
+}
+
 extern "C" int clg_top_logits(int dtype, const void *logits, int64_t row_stride, int64_t rows, int64_t cols, int64_t k, double temperature, void *values,
-                              int64_t *columns, void *lse, void *stream)
+                              int64_t *columns, void *lse, void *scratch, void *stream)
 {
     CLG_REQUIRE(clg_score_type(dtype), "clg_top_logits: unsupported dtype %d", dtype);
     CLG_REQUIRE(rows >= 0 && rows < (int64_t)1 << 31 && cols >= 1 && cols < (int64_t)1 << 31, "clg_top_logits: bad shape [%lld, %lld]", (long long)rows,
@@ -322,7 +421,14 @@ extern "C" int clg_top_logits(int dtype, const void *logits, int64_t row_stride,
     CLG_REQUIRE(temperature > 0 && temperature < 1e30, "clg_top_logits: the temperature must be positive and finite");
     if (!rows) return CLG_OK;
     CLG_REQUIRE(logits && values && columns, "clg_top_logits: null pointer");
-    TopArgs a{logits, rows, cols, row_stride, (int)k, temperature, values, columns, lse};
+    TopArgs a{logits, rows, cols, row_stride, (int)k, temperature, values, columns, lse, parts_of(rows, cols, k), cols, nullptr, nullptr};
+    if (a.parts > 1) {
+        CLG_REQUIRE(scratch, "clg_top_logits: null scratch");
+        a.width = clg_ceil_div(clg_ceil_div(cols, a.parts), 64) * 64;
+        a.parts = (int)clg_ceil_div(cols, a.width);
+        a.part_lse = static_cast<double *>(scratch);
+        a.part_best = a.part_lse + rows * a.parts;
+    }
     const int rc = clg_with_type(dtype, [&](auto t) {
         launch<decltype(t)>(a, clg_stream(stream));
         return CLG_OK;

@@ -137,7 +137,8 @@ SIGNATURES = {
     "clg_late_sums_run": (_i, [_p, _i, _p]),
     "clg_fc_tree_fold_slots": (_i, [_p] * 6 + [_i64, _p]),
     "clg_net_packed_scratch_bytes": (_i64, [_p, _i, _i64, _i64, _i64, _i64]),
-    "clg_top_logits": (_i, [_i, _p, _i64, _i64, _i64, _i64, _f64, _p, _p, _p, _p]),
+    "clg_top_logits_scratch_bytes": (_i64, [_i, _i64, _i64, _i64]),
+    "clg_top_logits": (_i, [_i, _p, _i64, _i64, _i64, _i64, _f64, _p, _p, _p, _p, _p]),
     "clg_distill_scratch_bytes": (_i64, [_i64]),
     "clg_distill_forward": (_i, [_i, _p, _i64, _p, _i, _p, _i, _p, _i, _p, _i64, _i64, _i64, _f64, _f64, _i] + [_p] * 5),
     "clg_distill_backward": (_i, [_i, _p, _i64, _p, _i, _p, _i, _p, _i, _p, _i64, _i64, _i64, _f64, _f64, _i] + [_p] * 5),

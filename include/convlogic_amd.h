@@ -671,9 +671,11 @@ int clg_threshold_pack_images_host(const float *x, const float *thresholds, uint
 
 /* The k highest logits of each row, highest first, and the columns they are in; of equal values the lowest column comes first, a NaN counts
  * as the maximum, as in clg_gate_argmax.  lse, if not NULL: log sum_v exp(logits[v] / temperature) of the whole row, float32 (float64 for CLG_F64).
- * dtype: CLG_F32, CLG_F64, CLG_F16 or CLG_BF16; row_stride: elements from one row to the next, the columns of a row are dense.  1 <= k <= 1024. */
+ * dtype: CLG_F32, CLG_F64, CLG_F16 or CLG_BF16; row_stride: elements from one row to the next, the columns of a row are dense.  1 <= k <= 1024.
+ * scratch: clg_top_logits_scratch_bytes() bytes, NULL where that is 0 (few long rows are shared out among workgroups, whose results it holds). */
+int64_t clg_top_logits_scratch_bytes(int dtype, int64_t rows, int64_t cols, int64_t k);
 int clg_top_logits(int dtype, const void *logits /*[rows,cols]*/, int64_t row_stride, int64_t rows, int64_t cols, int64_t k, double temperature,
-                   void *values /*[rows,k]*/, int64_t *columns /*[rows,k]*/, void *lse /*[rows] or NULL*/, void *stream);
+                   void *values /*[rows,k]*/, int64_t *columns /*[rows,k]*/, void *lse /*[rows] or NULL*/, void *scratch, void *stream);
 
 /* Distillation from a teacher's top logits.  Per row, with u = logits / temperature, q = softmax(u) and the teacher's probabilities p_j of its entries
  * (values[j], columns[j]) -- their softmax, or with lse (as clg_top_logits gives it) exp(values[j] / temperature - lse) and one more answer, "none of

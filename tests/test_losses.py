@@ -194,12 +194,14 @@ def test_the_c_entry_points_refuse_before_they_launch():
 def refused_by_the_c_entry_points():
     lib = _lib.load()
     p = 4096                                                          # never read: every call is refused on the host
-    top = [0, p, 8, 2, 8, 3, 1.0, p, p, p, None]
+    top = [0, p, 8, 2, 8, 3, 1.0, p, p, p, None, None]
     for at, value in [(0, 7), (2, -1), (3, -1), (3, 1 << 31), (4, 0), (4, 1 << 31), (5, 0), (5, 9), (5, 1025), (6, 0.0), (6, NAN), (1, None), (7, None), (8, None)]:
         args = list(top)
         args[at] = value
         assert lib.clg_top_logits(*args) == -1 and b"clg_top_logits" in lib.clg_last_error(), (at, value)
-    assert lib.clg_top_logits(0, None, 8, 0, 8, 3, 1.0, None, None, None, None) == 0
+    assert lib.clg_top_logits(0, None, 8, 0, 8, 3, 1.0, None, None, None, None, None) == 0
+    assert lib.clg_top_logits_scratch_bytes(0, 2, 8, 3) == 0 and lib.clg_top_logits_scratch_bytes(0, 2, 1 << 20, 3) > 0
+    assert lib.clg_top_logits(0, p, 1 << 20, 2, 1 << 20, 3, 1.0, p, p, p, None, None) == -1 and b"scratch" in lib.clg_last_error()
     forward = [0, p, 8, p, 0, p, 64, p, 0, p, 2, 8, 3, 1.0, 1.0, 2, p, p, p, p, None]
     for at, value in [(0, 9), (1, None), (2, -8), (3, None), (4, 9), (5, None), (6, 16), (8, 9), (10, -1), (10, 1 << 31), (11, 0), (11, 1 << 31), (12, 0), (12, 1025),
                       (13, 0.0), (13, INF), (15, 3), (15, 0), (16, None), (17, None), (18, None), (19, None)]:
