@@ -9,7 +9,11 @@
 
 namespace {
 
-constexpr int kSegments = 16, kThreads = 256, kMaxExperts = 1024;
+constexpr int kSegments = 16, kThreads = 256, kMaxExperts = 1024, kEach = 16;
+
+// Logits from so many MB on are read past the caches, gradients written so: smaller ones are still in the last-level cache when the backward pass
+// reads them again (131072 rows of 256 experts, 134 MB: 81 us a step through the caches, 87 past them; the gates of 79 M logits, 316 MB: 201 and 179).
+constexpr int kPastMb = 192;
 
 struct Segments {
     const void *z[kSegments];
@@ -25,33 +29,36 @@ struct BalanceArgs {
     const uint8_t *mask;                                              // of the only segment, or NULL
     float *sums;                                                      // [workgroups][experts] sums of probabilities
     int *counts;                                                      // [workgroups][experts + 1] rows per expert, rows in all
+    int *ticket;                                                      // 0 for the launch behind
     const void *w;                                                    // [segments][experts] in A
     const void *upstream;                                             // A
 };
 
 // Reductions over groups of G lanes, in all of them: up to 16 lanes by DPP, beyond by LDS permutation.
 template <int CTRL>
-__device__ __forceinline__ int dpp_keep(int v)
+__device__ __forceinline__ int of_lanes(int v)                        // (every lane has a source: one instruction with what takes the value)
 {
-    return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xF, 0xF, false);
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, true);
 }
 template <int CTRL>
-__device__ __forceinline__ float dpp_keep(float v)
+__device__ __forceinline__ float of_lanes(float v)
 {
-    return __builtin_bit_cast(float, dpp_keep<CTRL>(__builtin_bit_cast(int, v)));
+    return __builtin_bit_cast(float, of_lanes<CTRL>(__builtin_bit_cast(int, v)));
 }
 template <int CTRL>
-__device__ __forceinline__ double dpp_keep(double v)
+__device__ __forceinline__ double of_lanes(double v)
 {
-    return ::dpp_keep<CTRL, 0xF>(v);
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)of_lanes<CTRL>((int)(uint32_t)u), hi = (uint32_t)of_lanes<CTRL>((int)(uint32_t)(u >> 32));
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 template <int G, typename A, typename F>
 __device__ __forceinline__ A group_reduce(A v, F f)
 {
-    if constexpr (G > 1) v = f(v, dpp_keep<0xB1>(v));                 // quad_perm [1,0,3,2]
-    if constexpr (G > 2) v = f(v, dpp_keep<0x4E>(v));                 // quad_perm [2,3,0,1]
-    if constexpr (G > 4) v = f(v, dpp_keep<0x141>(v));                // row_half_mirror
-    if constexpr (G > 8) v = f(v, dpp_keep<0x140>(v));                // row_mirror
+    if constexpr (G > 1) v = f(v, of_lanes<0xB1>(v));                 // quad_perm [1,0,3,2]
+    if constexpr (G > 2) v = f(v, of_lanes<0x4E>(v));                 // quad_perm [2,3,0,1]
+    if constexpr (G > 4) v = f(v, of_lanes<0x141>(v));                // row_half_mirror
+    if constexpr (G > 8) v = f(v, of_lanes<0x140>(v));                // row_mirror
     if constexpr (G > 16) v = f(v, (A)__shfl_xor(v, 16));
     if constexpr (G > 32) v = f(v, (A)__shfl_xor(v, 32));
     return v;
@@ -66,7 +73,7 @@ struct Sum {
 };
 
 // the logits of a row that a lane holds: pieces lane, lane + G, ... of 16 bytes; -inf behind the row
-template <typename T, int G, int NV>
+template <typename T, int G, int NV, bool STREAM>
 struct RowPart {
     typedef typename Wide<T>::type A;
     static constexpr int VEC = Vec16<T>::N, N = NV * VEC, kLanes = G;
@@ -78,7 +85,7 @@ struct RowPart {
         for (int j = 0; j < NV; ++j) {
             const int e = (j * G + lane) * VEC;
             if (e + VEC <= experts) {
-                const auto v = *reinterpret_cast<const typename Vec16<T>::type *>(row + e);
+                const auto v = load_vec<STREAM>(reinterpret_cast<const typename Vec16<T>::type *>(row + e));
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) x[j * VEC + i] = (A)v[i];
             } else {
@@ -149,10 +156,10 @@ __device__ __forceinline__ void choose(Part &part, int lane, int k, int (&c)[N])
 }
 
 // sums and counts of a workgroup's rows
-template <typename T, int G, int NV>
+template <typename T, int G, int NV, bool STREAM>
 __global__ __launch_bounds__(kThreads) void balance_kernel(BalanceArgs a)
 {
-    typedef RowPart<T, G, NV> Part;
+    typedef RowPart<T, G, NV, STREAM> Part;
     typedef typename Part::A A;
     constexpr int N = Part::N, kGroups = kThreads / G, R = kAhead<N>;
     __shared__ A room_p[kThreads / 64][G * N];
@@ -248,6 +255,7 @@ __global__ __launch_bounds__(kThreads) void balance_kernel(BalanceArgs a)
         if (lane == 0) room_c[tid >> 6][G * N] = n;
     }
     __syncthreads();
+    if (blockIdx.x == 0 && tid == 0) *a.ticket = 0;
     A *sums = reinterpret_cast<A *>(a.sums) + (int64_t)blockIdx.x * a.experts;
     int *counts = a.counts + (int64_t)blockIdx.x * (a.experts + 1);
     for (int e = tid; e <= a.experts; e += kThreads) {
@@ -271,25 +279,28 @@ struct FinishArgs {
     double weight;
     void *loss, *w;                                                   // A, [segments][experts] in A
     int64_t *count_out;                                               // [segments][experts]
-    double *terms;                                                    // [segments][blocks of 16 experts]
+    double *terms;                                                    // [segments][blocks of experts]
+    int *ticket;
 };
 
 // One workgroup per 16 experts of a segment, 64 slices of its workgroups' sums at once: rows per expert and in all, the coefficients of the gradient and
-// these experts' part of the loss.
+// these experts' part of the loss.  The workgroup that is done last adds the parts up, in their order.  (64 experts to a workgroup: 10 us in place of 5 for
+// the 512 KB of sums of 64 experts.)
 template <typename A>
 __global__ __launch_bounds__(1024) void balance_finish_kernel(FinishArgs a)
 {
+    constexpr int EACH = kEach, SLICES = 1024 / EACH;
     __shared__ double room[16], sum_p[1024];
     __shared__ int64_t sum_c[1024];
     const int seg = blockIdx.y, tid = threadIdx.x, first = a.seg.first[seg], end = a.seg.first[seg + 1];
-    const int e = (int)blockIdx.x * 16 + tid % 16;
+    const int e = (int)blockIdx.x * EACH + tid % EACH;
     double n[1] = {0};
     for (int w = first + tid; w < end; w += 1024) n[0] += a.counts[(int64_t)w * (a.experts + 1) + a.experts];
     double p = 0;
     int64_t c = 0;
     if (e < a.experts) {
 #pragma unroll 4
-        for (int w = first + tid / 16; w < end; w += 64) {
+        for (int w = first + tid / EACH; w < end; w += SLICES) {
             p += (double)static_cast<const A *>(a.sums)[(int64_t)w * a.experts + e];
             c += a.counts[(int64_t)w * (a.experts + 1) + e];
         }
@@ -298,44 +309,45 @@ __global__ __launch_bounds__(1024) void balance_finish_kernel(FinishArgs a)
     sum_c[tid] = c;
     block_reduce<true, 1024>(n, room);
     if (tid >= kWave) return;
-    // the first wavefront: its lanes take every fourth slice, then the four are added
+    // the first wavefront: 64 / EACH parts of the slices, then these
     p = 0, c = 0;
-    for (int s = tid / 16; s < 64; s += 4) {
-        p += sum_p[s * 16 + tid % 16];
-        c += sum_c[s * 16 + tid % 16];
+    for (int s = tid / EACH; s < SLICES; s += kWave / EACH) {
+        p += sum_p[s * EACH + tid % EACH];
+        c += sum_c[s * EACH + tid % EACH];
     }
 #pragma unroll
-    for (int by = 16; by < 64; by <<= 1) {
+    for (int by = EACH; by < kWave; by <<= 1) {
         p += __shfl_xor(p, by);
         c += __shfl_xor(c, by);
     }
     double term = 0;
-    if (tid < 16 && e < a.experts) {
+    if (tid < EACH && e < a.experts) {
         const double w = n[0] == 0 ? 0 : a.weight * a.experts * (double)c / ((double)a.k * n[0] * n[0]);
         a.count_out[(int64_t)seg * a.experts + e] = c;
         static_cast<A *>(a.w)[(int64_t)seg * a.experts + e] = (A)w;
         term = w * p;
     }
     term = wave_sum(term);
-    if (tid != 0) return;
-    if (gridDim.x * gridDim.y == 1) *static_cast<A *>(a.loss) = (A)term;
-    else a.terms[(int64_t)seg * gridDim.x + blockIdx.x] = term;
-}
-
-template <typename A>
-__global__ __launch_bounds__(64) void balance_sum_kernel(const double *terms, int n, A *loss)
-{
-    double s = 0;
-    for (int i = threadIdx.x; i < n; i += 64) s += terms[i];
-    s = wave_sum(s);
-    if (threadIdx.x == 0) *loss = (A)s;
+    const int blocks = gridDim.x * gridDim.y;
+    if (blocks > 1) {
+        int mine = 0;
+        if (tid == 0) {
+            __hip_atomic_store(a.terms + seg * gridDim.x + blockIdx.x, term, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            mine = __hip_atomic_fetch_add(a.ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        if (__builtin_amdgcn_readfirstlane(mine) != blocks - 1) return;
+        term = 0;
+        for (int i = tid; i < blocks; i += kWave) term += __hip_atomic_load(a.terms + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        term = wave_sum(term);
+    }
+    if (tid == 0) *static_cast<A *>(a.loss) = (A)term;
 }
 
 // the gradient
-template <typename T, int G, int NV>
+template <typename T, int G, int NV, bool STREAM>
 __global__ __launch_bounds__(kThreads) void balance_grad_kernel(BalanceArgs a)
 {
-    typedef RowPart<T, G, NV> Part;
+    typedef RowPart<T, G, NV, STREAM> Part;
     typedef typename Part::A A;
     typedef typename Vec16<T>::type V;
     constexpr int N = Part::N, VEC = Part::VEC, kGroups = kThreads / G, R = kAhead<N>;
@@ -383,7 +395,7 @@ __global__ __launch_bounds__(kThreads) void balance_grad_kernel(BalanceArgs a)
                 for (int i = 0; i < VEC; ++i) v[i] = kept[r] ? (T)(e[j * VEC + i] * (w[j * VEC + i] - mean) * up) : (T)0.f;
                 T *out = grad + row * a.experts + at;
                 if (at + VEC <= a.experts) {
-                    *reinterpret_cast<V *>(out) = v;
+                    store_vec<STREAM>(reinterpret_cast<V *>(out), v);
                 } else {
 #pragma unroll
                     for (int i = 0; i < VEC; ++i)
@@ -417,7 +429,7 @@ int lanes_of(int experts)
     return g;
 }
 
-constexpr int kTerms = kSegments * (kMaxExperts / 16);                // of the loss
+constexpr int kTerms = kSegments * (kMaxExperts / kEach);               // of the loss
 constexpr int kMostGroups = 1024;                                     // workgroups of the sums
 
 // workgroups per segment, `most` in all or a few more: by rows, one at least
@@ -460,7 +472,7 @@ extern "C" int64_t clg_balance_scratch_bytes(int dtype, int64_t experts)
 {
     if (!clg_score_type(dtype) || experts < 1 || experts > kMaxExperts) return 0;
     const int64_t groups = kMostGroups + kSegments;
-    return groups * experts * (dtype == CLG_F64 ? 8 : 4) + groups * (experts + 1) * 4 + kTerms * 8 + 8;
+    return groups * experts * (dtype == CLG_F64 ? 8 : 4) + groups * (experts + 1) * 4 + kTerms * 8 + 8 + 8;
 }
 
 extern "C" int clg_balance_forward(int dtype, int n, const void *const *logits, const int64_t *rows, const int64_t *row_strides, int64_t experts, int64_t k,
@@ -472,28 +484,30 @@ extern "C" int clg_balance_forward(int dtype, int n, const void *const *logits, 
     const bool f64 = dtype == CLG_F64;
     double *terms = static_cast<double *>(scratch);
     a.experts = (int)experts, a.k = (int)k, a.mask = mask;
-    a.sums = reinterpret_cast<float *>(terms + kTerms);
+    a.ticket = reinterpret_cast<int *>(terms + kTerms);
+    a.sums = reinterpret_cast<float *>(terms + kTerms + 1);
     a.counts = reinterpret_cast<int *>(reinterpret_cast<char *>(a.sums) + (kMostGroups + kSegments) * experts * (f64 ? 8 : 4));
+    int64_t elements = 0;
+    for (int i = 0; i < n; ++i) elements += rows[i] * experts;
     const int rc = clg_with_type(dtype, [&](auto t) {
         typedef decltype(t) T;
-        const int64_t grid = share_out(a.seg, kThreads / lanes_of<T>(a.experts) * 4, kMostGroups);
+        const int64_t grid = share_out(a.seg, kThreads / lanes_of<T>(a.experts), kMostGroups);
         with_part<T>(a.experts, [&](auto g, auto nv) {
-            balance_kernel<T, decltype(g)::value, decltype(nv)::value><<<dim3((unsigned)grid), dim3(kThreads), 0, clg_stream(stream)>>>(a);
+            const auto run = [&](auto past) {
+                balance_kernel<T, decltype(g)::value, decltype(nv)::value, decltype(past)::value><<<dim3((unsigned)grid), dim3(kThreads), 0, clg_stream(stream)>>>(a);
+            };
+            if (clg_past_caches(elements * sizeof(T), kPastMb)) run(std::true_type());
+            else run(std::false_type());
         });
         return CLG_OK;
     });
     if (rc) return rc;
     CLG_CHECK_LAUNCH("clg_balance_forward");
-    const FinishArgs f{a.seg, a.experts, a.k, a.sums, a.counts, weight / n, loss, coefs, counts, terms};
-    const int blocks = (int)clg_ceil_div(experts, 16);
-    if (f64) balance_finish_kernel<double><<<dim3(blocks, n), dim3(1024), 0, clg_stream(stream)>>>(f);
-    else balance_finish_kernel<float><<<dim3(blocks, n), dim3(1024), 0, clg_stream(stream)>>>(f);
+    const FinishArgs f{a.seg, a.experts, a.k, a.sums, a.counts, weight / n, loss, coefs, counts, terms, a.ticket};
+    const dim3 blocks((unsigned)clg_ceil_div(experts, kEach), n);
+    if (f64) balance_finish_kernel<double><<<blocks, dim3(1024), 0, clg_stream(stream)>>>(f);
+    else balance_finish_kernel<float><<<blocks, dim3(1024), 0, clg_stream(stream)>>>(f);
     CLG_CHECK_LAUNCH("clg_balance_forward");
-    if (n * blocks > 1) {
-        if (f64) balance_sum_kernel<double><<<dim3(1), dim3(64), 0, clg_stream(stream)>>>(terms, n * blocks, static_cast<double *>(loss));
-        else balance_sum_kernel<float><<<dim3(1), dim3(64), 0, clg_stream(stream)>>>(terms, n * blocks, static_cast<float *>(loss));
-        CLG_CHECK_LAUNCH("clg_balance_forward");
-    }
     return CLG_OK;
 }
 
@@ -508,11 +522,17 @@ extern "C" int clg_balance_backward(int dtype, int n, const void *const *logits,
         a.seg.grad[i] = grads[i];
     }
     a.experts = (int)experts, a.mask = mask, a.w = coefs, a.upstream = upstream;
+    int64_t elements = 0;
+    for (int i = 0; i < n; ++i) elements += rows[i] * experts;
     const int rc = clg_with_type(dtype, [&](auto t) {
         typedef decltype(t) T;
         const int64_t grid = share_out(a.seg, kThreads / lanes_of<T>(a.experts), 8192);
         with_part<T>(a.experts, [&](auto g, auto nv) {
-            balance_grad_kernel<T, decltype(g)::value, decltype(nv)::value><<<dim3((unsigned)grid), dim3(kThreads), 0, clg_stream(stream)>>>(a);
+            const auto run = [&](auto past) {
+                balance_grad_kernel<T, decltype(g)::value, decltype(nv)::value, decltype(past)::value><<<dim3((unsigned)grid), dim3(kThreads), 0, clg_stream(stream)>>>(a);
+            };
+            if (clg_past_caches(elements * sizeof(T), kPastMb)) run(std::true_type());
+            else run(std::false_type());
         });
         return CLG_OK;
     });

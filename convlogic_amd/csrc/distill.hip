@@ -51,11 +51,11 @@ __device__ __forceinline__ double all_of(const int *column, const double *prob, 
 
 // One workgroup per row.  A row that fits its registers (COLS columns) is read from memory once, for the sum and for the gradient; longer ones (MULTI)
 // tile by tile, twice.
-template <typename T, int THREADS, int NV, bool MULTI>
+template <typename T, int THREADS, int NV, bool MULTI, int STREAM>
 __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
 {
     typedef typename Wide<T>::type A;
-    typedef RowTile<T, THREADS, NV> Tile;
+    typedef RowTile<T, THREADS, NV, STREAM> Tile;
     extern __shared__ char lds[];
     double *room = reinterpret_cast<double *>(lds), *prob = room + 16 * 4 + 2;
     int *flags = reinterpret_cast<int *>(room + 16 * 4);
@@ -244,26 +244,37 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const double *row_loss, 
     if (threadIdx.x == 0) *out = (A)(s[0] * (per_count ? *per_count : 1));
 }
 
-template <typename T, int THREADS, int NV, bool MULTI>
+template <typename T, int THREADS, int NV, bool MULTI, int STREAM>
 void launch_as(const DistillArgs &a, hipStream_t stream)
 {
-    typedef RowTile<T, THREADS, NV> Tile;
+    typedef RowTile<T, THREADS, NV, STREAM> Tile;
     static_assert(Tile::COLS % 32 == 0, "bits of a tile fill whole words");
     const size_t lds = distill_lds<typename Wide<T>::type>(a.k, Tile::COLS);
-    distill_kernel<T, THREADS, NV, MULTI><<<dim3((unsigned)a.rows), dim3(THREADS), lds, stream>>>(a);
+    distill_kernel<T, THREADS, NV, MULTI, STREAM><<<dim3((unsigned)a.rows), dim3(THREADS), lds, stream>>>(a);
+}
+
+template <typename T, int STREAM>
+void launch_rows(const DistillArgs &a, hipStream_t stream)
+{
+    const int64_t pieces = (a.cols + Vec16<T>::N - 1) / Vec16<T>::N;
+    if (pieces <= 64) return launch_as<T, 64, 1, false, STREAM>(a, stream);
+    if (pieces <= 64 * 4) return launch_as<T, 64, 4, false, STREAM>(a, stream);
+    if (pieces <= 64 * 16) return launch_as<T, 64, 16, false, STREAM>(a, stream);
+    if (pieces <= 256 * 16) return launch_as<T, 256, 16, false, STREAM>(a, stream);
+    if (pieces <= 512 * 16) return launch_as<T, 512, 16, false, STREAM>(a, stream);
+    if (pieces <= 1024 * 16) return launch_as<T, 1024, 16, false, STREAM>(a, stream);
+    launch_as<T, 512, 8, true, STREAM>(a, stream);
 }
 
 template <typename T>
 void launch(const DistillArgs &a, hipStream_t stream)
 {
-    const int64_t pieces = (a.cols + Vec16<T>::N - 1) / Vec16<T>::N;
-    if (pieces <= 64) return launch_as<T, 64, 1, false>(a, stream);
-    if (pieces <= 64 * 4) return launch_as<T, 64, 4, false>(a, stream);
-    if (pieces <= 64 * 16) return launch_as<T, 64, 16, false>(a, stream);
-    if (pieces <= 256 * 16) return launch_as<T, 256, 16, false>(a, stream);
-    if (pieces <= 512 * 16) return launch_as<T, 512, 16, false>(a, stream);
-    if (pieces <= 1024 * 16) return launch_as<T, 1024, 16, false>(a, stream);
-    launch_as<T, 512, 8, true>(a, stream);
+    // Past the caches from 16 MB on: the lines that other kernels left there modified have to be written out first to take rows that are read once (32768
+    // columns behind a pass over 512 MB of other memory: 256 MB of logits 138 us through the caches, 118 past them, 32 MB 36 and 29; where the logits
+    // were in the caches, the same either way).  Gradient rows that are no whole cache lines are written through the caches, which put the lines together.
+    if (!clg_past_caches(a.rows * a.cols * sizeof(T), 16)) launch_rows<T, 0>(a, stream);
+    else if (a.cols * sizeof(T) % 128 != 0) launch_rows<T, 1>(a, stream);
+    else launch_rows<T, 3>(a, stream);
 }
 
 }  // namespace

@@ -106,8 +106,8 @@ __device__ __forceinline__ A wave_max(A v)
 }
 
 // Columns base .. of one row in the registers of a workgroup: thread t holds the 16-byte pieces t, t + THREADS, ... and, of what is left of a row
-// behind its last whole piece, one element.  What is behind the row is -inf.
-template <typename T, int THREADS, int NV>
+// behind its last whole piece, one element.  What is behind the row is -inf.  STREAM: loads (1) and stores (2) past the caches.
+template <typename T, int THREADS, int NV, int STREAM>
 struct RowTile {
     static constexpr int VEC = Vec16<T>::N, COLS = THREADS * NV * VEC;
     typedef typename Vec16<T>::type V;
@@ -127,7 +127,7 @@ struct RowTile {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int p = j * THREADS + tid;
-            if (j * THREADS < whole) v[j] = *reinterpret_cast<const V *>(at + (uint32_t)((p < whole ? p : whole - 1) * VEC));
+            if (j * THREADS < whole) v[j] = load_vec<(STREAM & 1) != 0>(reinterpret_cast<const V *>(at + (uint32_t)((p < whole ? p : whole - 1) * VEC)));
             else v[j] = (V)none;
         }
         last = none;
@@ -209,7 +209,7 @@ struct RowTile {
             V out;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) out[i] = (T)f((A)v[j][i]);
-            if (p < whole) *reinterpret_cast<V *>(at + (uint32_t)(p * VEC)) = out;
+            if (p < whole) store_vec<(STREAM & 2) != 0>(reinterpret_cast<V *>(at + (uint32_t)(p * VEC)), out);
         }
         if (tid < tail) at[whole * VEC + tid] = (T)f((A)last);
     }
