@@ -16,7 +16,7 @@ struct DistillArgs {
     const void *values, *columns, *lse;                               // [rows][k], [rows][k], [rows] or NULL
     int values_type, lse_type, columns64, k;
     const uint8_t *mask;                                              // [rows] or NULL
-    double temperature, loss_scale, grad_scale;
+    double temperature, inv_tau, loss_scale, grad_scale;
     const double *per_count;                                          // factor of both that is known on the device only, or NULL
     double *row_loss;                                                 // [rows] or NULL
     void *out;                                                        // [rows] losses in A, or NULL
@@ -26,13 +26,14 @@ struct DistillArgs {
     int upstream_rows, only_changed;
 };
 
+constexpr int kFewEntries = 32, kManyRows = 2048;
 constexpr int kFlagTwice = 1, kFlagListed = 2, kFlagBad = 4;
 
-// LDS of a workgroup: reduction room (16 wavefronts of 4 doubles), flags, entries (probability, logit, column), bits of a tile
+// LDS of a team: reduction room (16 wavefronts of 4 doubles, for a workgroup), flags, entries (probability, logit, column), bits of a tile
 template <typename A>
-size_t distill_lds(int k, int cols_of_tile /* whole words of bits */)
+__host__ __device__ inline int distill_lds(bool workgroup, int k, int cols_of_tile /* whole words of bits */)
 {
-    return 16 * 4 * 8 + 16 + (size_t)k * (8 + sizeof(A) + 4) + (size_t)(cols_of_tile / 32) * 4;
+    return ((workgroup ? 16 * 4 * 8 : 0) + 16 + k * (8 + (int)sizeof(A) + 4) + cols_of_tile / 32 * 4 + 15) & ~15;
 }
 
 // whether entry j is the first of its column, and with all the others' probabilities on it
@@ -49,80 +50,86 @@ __device__ __forceinline__ double all_of(const int *column, const double *prob, 
     return p;
 }
 
-// One workgroup per row.  A row that fits its registers (COLS columns) is read from memory once, for the sum and for the gradient; longer ones (MULTI)
-// tile by tile, twice.
-template <typename T, int THREADS, int NV, bool MULTI, int STREAM>
+// A team of LANES threads per row: a workgroup, or 16 lanes where there are many short rows.  A row that fits its registers (COLS columns) is read from memory
+// once, for the sum and for the gradient; longer ones (MULTI) tile by tile, twice.
+template <typename T, int THREADS, int LANES, int NV, bool MULTI, int STREAM>
 __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
 {
     typedef typename Wide<T>::type A;
-    typedef RowTile<T, THREADS, NV, STREAM> Tile;
+    typedef RowTile<T, LANES, NV, STREAM> Tile;
+    typedef Team<THREADS, LANES> Mine;
+    constexpr int TEAMS = THREADS / LANES, ROOM = Mine::kWhole ? 16 * 4 : 0;
+    static_assert(TEAMS == 1 || THREADS == kWave, "teams share a wavefront, where LDS is in order");
     extern __shared__ char lds[];
-    double *room = reinterpret_cast<double *>(lds), *prob = room + 16 * 4 + 2;
-    int *flags = reinterpret_cast<int *>(room + 16 * 4);
-    A *logit = reinterpret_cast<A *>(prob + a.k);
-    int *column = reinterpret_cast<int *>(logit + a.k);
-    uint32_t *bits = reinterpret_cast<uint32_t *>(column + a.k);
-    const int tid = threadIdx.x, k = a.k;
+    const int tid = Mine::kWhole ? threadIdx.x : threadIdx.x % LANES, team = Mine::kWhole ? 0 : threadIdx.x / LANES, k = a.k;
+    double *room = reinterpret_cast<double *>(lds + team * distill_lds<A>(Mine::kWhole, k, Tile::COLS)), *prob = room + ROOM + 2;
+    int *flags = reinterpret_cast<int *>(room + ROOM);
+    A *logit = reinterpret_cast<A *>(prob + k);
+    int *column = reinterpret_cast<int *>(logit + k);
+    uint32_t *bits = reinterpret_cast<uint32_t *>(column + k);
     const A unit = (A)Exps<A>::unit(a.temperature);
-    const double inv_tau = 1.0 / a.temperature;
 
-    const int64_t row = blockIdx.x;
+    const int64_t row = Mine::kWhole ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * TEAMS + team;
+    if (TEAMS > 1 && row >= a.rows) return;
     const A up = a.upstream ? static_cast<const A *>(a.upstream)[a.upstream_rows ? row : 0] : A(1);
     if (a.only_changed && static_cast<const A *>(a.applied)[row] == up) return;
     T *grad = a.grad ? static_cast<T *>(a.grad) + row * a.cols : nullptr;
     const bool kept = !a.mask || a.mask[row];
     const T *z = static_cast<const T *>(a.z) + row * a.row_stride;
-    // the teacher's entries, of which the first come with the row, in front of it: the logits in their columns are a load more
-    const auto column_of = [&](int j) -> int64_t {
-        const int64_t at = row * k + j;
-        return a.columns64 ? static_cast<const int64_t *>(a.columns)[at] : static_cast<const int32_t *>(a.columns)[at];
-    };
-    int64_t first_column = -1;
-    uint64_t first_value = 0, lse_bits = 0;
-    if (kept) {
-        if (tid < k) {
-            first_column = column_of(tid);
-            first_value = load_bits(a.values, a.values_type, row * k + tid);
-        }
-        if (a.lse) lse_bits = load_bits(a.lse, a.lse_type, row);
-    }
-    Tile tile;
-    if (kept) tile.load(z, 0, a.cols);
+    // The teacher's entries in front of the row: the logits in their columns are a load behind theirs, and of a workgroup most wavefronts have none and go
+    // on to the row.  What this thread's first entry loads is taken up after the row is on its way.
     if (tid == 0) *flags = 0;
     __syncthreads();
     A tops[3] = {lowest(A(0)), lowest(A(0)), lowest(A(0))};           // highest of the teacher, of the student's listed logits, of the others
+    T first_logit = (T)0.f;
+    uint64_t first_value = 0, lse_bits = 0;
+    bool first_there = false;
+    const auto enter = [&](int j, T logit_j, uint64_t value) {
+        const double t = value_of_bits(value, a.values_type) * a.inv_tau;
+        const A l = (A)logit_j;
+        prob[j] = t;
+        logit[j] = l;
+        tops[0] = max_of(tops[0], (A)t);
+        tops[1] = max_of(tops[1], l);
+    };
     if (kept) {
         int seen = 0;
 #pragma unroll 1
-        for (int j = tid; j < k; j += THREADS) {
-            const int64_t c = j == tid ? first_column : column_of(j);
+        for (int j = tid; j < k; j += LANES) {
+            const int64_t at = row * k + j, c = a.columns64 ? static_cast<const int64_t *>(a.columns)[at] : static_cast<const int32_t *>(a.columns)[at];
+            const uint64_t value = load_bits(a.values, a.values_type, at);
             const bool there = c >= 0 && c < a.cols;
             seen |= there ? kFlagListed : c >= a.cols ? kFlagBad : 0;
             column[j] = there ? (int)c : -1;
             if (!there) continue;
-            const A l = (A)z[c];
-            const double t = value_of_bits(j == tid ? first_value : load_bits(a.values, a.values_type, row * k + j), a.values_type) * inv_tau;
-            prob[j] = t;
-            logit[j] = l;
-            tops[0] = max_of(tops[0], (A)t);
-            tops[1] = max_of(tops[1], l);
+            if (j == tid) {
+                first_there = true;
+                first_value = value;
+                first_logit = z[c];
+            } else {
+                enter(j, z[c], value);
+            }
         }
         if (seen) atomicOr(flags, seen);
+        if (a.lse) lse_bits = load_bits(a.lse, a.lse_type, row);
     }
+    Tile tile(tid);
+    if (kept) tile.load(z, 0, a.cols);
     // the sum over what is not listed
     A m_t = lowest(A(0)), s_t = 0;
-    for (int64_t base = 0; kept && base < a.cols; base += Tile::COLS) {
-        if (MULTI && base) tile.load(z, base, a.cols);
+    const auto look = [&](int64_t base) {
         const int n = (int)(a.cols - base < Tile::COLS ? a.cols - base : Tile::COLS);
-        for (int w = tid; w < (n + 31) / 32; w += THREADS) bits[w] = 0;
+        for (int w = tid; w < (n + 31) / 32; w += LANES) bits[w] = 0;
         __syncthreads();
 #pragma unroll 1
-    for (int j = tid; j < k; j += THREADS) {
+        for (int j = tid; j < k; j += LANES) {
             const int64_t c = (int64_t)column[j] - base;
             if (column[j] < 0 || c < 0 || c >= n) continue;
             if (atomicOr(&bits[c >> 5], 1u << (c & 31)) >> (c & 31) & 1) atomicOr(flags, kFlagTwice);
         }
         __syncthreads();
+        if (base == 0 && first_there) enter(tid, first_logit, first_value);
+        tile.trim();
         tile.drop(bits);
         tile.fence();
         const A m = max_of(m_t, tile.highest());
@@ -132,71 +139,80 @@ __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
         s_t += tile.sum(e);
         m_t = m;
         tile.fence();
-        if (MULTI) __syncthreads();
+    };
+    if (kept) {
+        look(0);
+        if (MULTI)
+            for (int64_t base = Tile::COLS; base < a.cols; base += Tile::COLS) {
+                __syncthreads();
+                tile.load(z, base, a.cols);
+                look(base);
+            }
     }
     __syncthreads();
     const int flag = *flags;
-    if (!kept || !(flag & (kFlagListed | kFlagBad))) {            // a row that says nothing
+    if (!kept || !(flag & (kFlagListed | kFlagBad))) {                // a row that says nothing
         if (tid == 0) {
             if (a.row_loss) a.row_loss[row] = 0;
             if (a.out) static_cast<A *>(a.out)[row] = 0;
             if (a.applied) static_cast<A *>(a.applied)[row] = up;
         }
         if (grad) {
-            for (int64_t c = (int64_t)tid * Tile::VEC; c + Tile::VEC <= a.cols; c += THREADS * Tile::VEC)
+            for (int64_t c = (int64_t)tid * Tile::VEC; c + Tile::VEC <= a.cols; c += LANES * Tile::VEC)
                 *reinterpret_cast<typename Tile::V *>(grad + c) = (typename Tile::V)(T)0.f;
             if (tid < a.cols % Tile::VEC) grad[a.cols - 1 - tid] = (T)0.f;
         }
         return;
     }
     tops[2] = m_t;
-    block_reduce<false, THREADS>(tops, reinterpret_cast<A *>(room));
+    Mine::template reduce<false>(tops, reinterpret_cast<A *>(room));
     const A m_u = tops[2], m = max_of(tops[1], m_u);
     const Exps<A> of_rest(m_u, unit), of_all(m, unit);
     __syncthreads();
 
-    // sums: the others' exponentials relative to m_u, the listed ones' relative to m, the teacher's, the teacher's share times the difference of the
-    // logarithms
-    double sums[4] = {(double)rescaled(s_t, m_t, Exps<A>(m_t, unit), of_rest), 0, 0, 0};
+    // sums: the others' exponentials relative to m_u, the listed ones' relative to m; in 64 bits the teacher's, of which small differences are taken, and
+    // its share times the difference of the logarithms
+    A sums[2] = {rescaled(s_t, m_t, Exps<A>(m_t, unit), of_rest), 0};
+    double parts[2] = {0, 0};
     const double base_t = a.lse ? value_of_bits(lse_bits, a.lse_type) : (double)finite_or_zero(tops[0]);
 #pragma unroll 1
-    for (int j = tid; j < k; j += THREADS) {
+    for (int j = tid; j < k; j += LANES) {
         if (column[j] < 0) continue;
         const A l = logit[j];
-        if (!(flag & kFlagTwice) || first_of(column, j)) sums[1] += (double)of_all(l);
-        const double u = ((double)l - (double)m) * inv_tau, t = prob[j] - base_t, e = exp(t);
-        sums[2] += e;
-        if (e != 0) sums[3] += e * (t - u);
+        if (!(flag & kFlagTwice) || first_of(column, j)) sums[1] += of_all(l);
+        const double u = ((double)l - (double)m) * a.inv_tau, t = prob[j] - base_t, e = exp(t);
+        parts[0] += e;
+        if (e != 0) parts[1] += e * (t - u);
         prob[j] = e;
     }
-    block_reduce<true, THREADS>(sums, room);
-    const double s_u = sums[0], total = (m_u == lowest(A(0)) ? s_u : s_u * (double)of_rest.factor(of_all)) + sums[1];
-    bool all_listed = false;                                      // (then there is nothing else)
+    Mine::sums(sums, parts, reinterpret_cast<A *>(room), room + 32);
+    const double s_u = sums[0], mass_p = parts[0], total = (m_u == lowest(A(0)) ? s_u : s_u * (double)of_rest.factor(of_all)) + (double)sums[1];
+    bool all_listed = false;                                          // (then there is nothing else)
     if (a.lse && k >= a.cols) {
-        double n[1] = {0};
+        A n[1] = {0};
 #pragma unroll 1
-    for (int j = tid; j < k; j += THREADS) n[0] += column[j] >= 0 && first_of(column, j);
+        for (int j = tid; j < k; j += LANES) n[0] += column[j] >= 0 && first_of(column, j);
         __syncthreads();
-        block_reduce<true, THREADS>(n, room);
-        all_listed = n[0] == (double)a.cols;
+        Mine::template reduce<true>(n, reinterpret_cast<A *>(room));
+        all_listed = n[0] == (A)a.cols;
     }
     double rest = 0;
-    if (a.lse && !all_listed) rest = sums[2] != sums[2] ? sums[2] : max_of(0.0, 1 - sums[2]);
-    // four logarithms at once, one in a lane
+    if (a.lse && !all_listed) rest = mass_p != mass_p ? mass_p : max_of(0.0, 1 - mass_p);
+    // four logarithms and three inverses at once, one in a lane
     const int lane = tid & 63;
-    const double logs = log(lane == 0 ? total : lane == 1 ? s_u : lane == 2 ? rest : sums[2]);
-    const double log_total = of_lane(logs, 0) + of_all.residue(m), log_p = of_lane(logs, 3);
-    double mass, loss, per = 1;                                   // per: of an entry's exponential
+    const double value = lane == 0 ? total : lane == 1 ? s_u : lane == 2 ? rest : mass_p, logs = log(value), inverses = quick_inverse(value);
+    const double log_total = Mine::from(logs, 0) + of_all.residue(m);
+    double mass, loss, per = 1;                                       // per: of an entry's exponential
     if (a.lse) {
-        mass = sums[2] + rest;
-        loss = sums[3] + sums[2] * log_total;
-        if (rest != 0) loss += rest * (of_lane(logs, 2) - (((double)m_u - (double)m) * inv_tau + of_lane(logs, 1) + of_rest.residue(m_u) - log_total));
+        mass = mass_p + rest;
+        loss = parts[1] + mass_p * log_total;
+        if (rest != 0) loss += rest * (Mine::from(logs, 2) - (((double)m_u - (double)m) * a.inv_tau + Mine::from(logs, 1) + of_rest.residue(m_u) - log_total));
     } else {
-        per = sums[2] == 0 ? 0 : 1 / sums[2];
-        mass = sums[2] * per;
-        loss = sums[2] == 0 ? 0 : sums[3] * per + log_total - log_p;
+        per = mass_p == 0 ? 0 : Mine::from(inverses, 3);
+        mass = mass_p * per;
+        loss = mass_p == 0 ? 0 : parts[1] * per + log_total - Mine::from(logs, 3);
     }
-    if ((flag & kFlagBad) || total > 1.7e308) loss = mass = __builtin_nan("");           // (a logit of +inf)
+    if ((flag & kFlagBad) || total > 1e300) loss = mass = __builtin_nan("");             // (a logit of +inf)
     const double factor = a.per_count ? *a.per_count : 1;
     if (tid == 0) {
         if (a.row_loss) a.row_loss[row] = loss * a.loss_scale;
@@ -204,15 +220,22 @@ __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
         if (a.applied) static_cast<A *>(a.applied)[row] = up;
     }
     if (!grad) return;
-    const double g = a.grad_scale * factor * (double)up, of_listed = mass / total;
-    const A others = s_u == 0 && total > 0 && mass == mass ? A(0) : (A)(g * (of_listed * (double)of_rest.factor(of_all) - rest / s_u));
-    for (int64_t base = 0; base < a.cols; base += Tile::COLS) {
-        if (MULTI) tile.load(z, base, a.cols);
-        tile.store(grad, base, [&](A x) { return of_rest(x) * others; });
+    const double g = a.grad_scale * factor * (double)up, of_listed = mass * Mine::from(inverses, 0);
+    const A others = s_u == 0 && total > 0 && mass == mass
+                         ? A(0)
+                         : (A)(g * (of_listed * (double)of_rest.factor(of_all) - (rest == 0 ? 0 : rest * Mine::from(inverses, 1))));
+    const auto of = [&](A x) { return of_rest(x) * others; };
+    if (MULTI) {
+        for (int64_t base = 0; base < a.cols; base += Tile::COLS) {
+            tile.load(z, base, a.cols);
+            tile.store(grad, base, of);
+        }
+    } else {
+        tile.store(grad, 0, of);                                      // (no loop: in one, all values come before the first store)
     }
-    __syncthreads();                                              // the listed columns' own values go over those
+    __syncthreads();                                                  // the listed columns' own values go over those
 #pragma unroll 1
-    for (int j = tid; j < k; j += THREADS) {
+    for (int j = tid; j < k; j += LANES) {
         if (column[j] < 0) continue;
         double p = prob[j];
         if (flag & kFlagTwice) {
@@ -244,26 +267,34 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const double *row_loss, 
     if (threadIdx.x == 0) *out = (A)(s[0] * (per_count ? *per_count : 1));
 }
 
-template <typename T, int THREADS, int NV, bool MULTI, int STREAM>
+template <typename T, int THREADS, int LANES, int NV, bool MULTI, int STREAM>
 void launch_as(const DistillArgs &a, hipStream_t stream)
 {
-    typedef RowTile<T, THREADS, NV, STREAM> Tile;
+    typedef RowTile<T, LANES, NV, STREAM> Tile;
     static_assert(Tile::COLS % 32 == 0, "bits of a tile fill whole words");
-    const size_t lds = distill_lds<typename Wide<T>::type>(a.k, Tile::COLS);
-    distill_kernel<T, THREADS, NV, MULTI, STREAM><<<dim3((unsigned)a.rows), dim3(THREADS), lds, stream>>>(a);
+    constexpr int TEAMS = THREADS / LANES;
+    const size_t lds = (size_t)TEAMS * distill_lds<typename Wide<T>::type>(TEAMS == 1, a.k, Tile::COLS);
+    distill_kernel<T, THREADS, LANES, NV, MULTI, STREAM><<<dim3((unsigned)clg_ceil_div(a.rows, TEAMS)), dim3(THREADS), lds, stream>>>(a);
 }
 
 template <typename T, int STREAM>
 void launch_rows(const DistillArgs &a, hipStream_t stream)
 {
     const int64_t pieces = (a.cols + Vec16<T>::N - 1) / Vec16<T>::N;
-    if (pieces <= 64) return launch_as<T, 64, 1, false, STREAM>(a, stream);
-    if (pieces <= 64 * 4) return launch_as<T, 64, 4, false, STREAM>(a, stream);
-    if (pieces <= 64 * 16) return launch_as<T, 64, 16, false, STREAM>(a, stream);
-    if (pieces <= 256 * 16) return launch_as<T, 256, 16, false, STREAM>(a, stream);
-    if (pieces <= 512 * 16) return launch_as<T, 512, 16, false, STREAM>(a, stream);
-    if (pieces <= 1024 * 16) return launch_as<T, 1024, 16, false, STREAM>(a, stream);
-    launch_as<T, 512, 8, true, STREAM>(a, stream);
+    // 16 lanes to a row: what is done once for a row is done for four at a time, which is most of the work of short rows
+    if (a.k <= kFewEntries) {
+        if (pieces <= 16) return launch_as<T, 64, 16, 1, false, STREAM>(a, stream);
+        if (a.rows >= kManyRows) {
+            if (pieces <= 16 * 4) return launch_as<T, 64, 16, 4, false, STREAM>(a, stream);
+            if (pieces <= 16 * 16) return launch_as<T, 64, 16, 16, false, STREAM>(a, stream);
+        }
+    }
+    if (pieces <= 64 * 4) return launch_as<T, 64, 64, 4, false, STREAM>(a, stream);
+    if (pieces <= 64 * 16) return launch_as<T, 64, 64, 16, false, STREAM>(a, stream);
+    if (pieces <= 256 * 16) return launch_as<T, 256, 256, 16, false, STREAM>(a, stream);
+    if (pieces <= 512 * 16) return launch_as<T, 512, 512, 16, false, STREAM>(a, stream);
+    if (pieces <= 1024 * 16) return launch_as<T, 1024, 1024, 16, false, STREAM>(a, stream);
+    launch_as<T, 512, 512, 8, true, STREAM>(a, stream);
 }
 
 template <typename T>
@@ -315,7 +346,7 @@ extern "C" int clg_distill_forward(int dtype, const void *logits, int64_t row_st
     DistillArgs a{};
     a.z = logits, a.rows = rows, a.cols = cols, a.row_stride = row_stride;
     a.values = values, a.columns = columns, a.lse = lse, a.values_type = values_dtype, a.lse_type = lse_dtype, a.columns64 = columns_bits == 64, a.k = (int)k;
-    a.mask = mask, a.temperature = temperature, a.loss_scale = temperature * temperature * weight, a.grad_scale = temperature * weight;
+    a.mask = mask, a.temperature = temperature, a.inv_tau = 1 / temperature, a.loss_scale = temperature * temperature * weight, a.grad_scale = temperature * weight;
     a.grad = grad, a.applied = applied;
     if (reduction == CLG_REDUCE_NONE) a.out = loss;
     else a.row_loss = row_loss;
@@ -357,7 +388,7 @@ extern "C" int clg_distill_backward(int dtype, const void *logits, int64_t row_s
     DistillArgs a{};
     a.z = logits, a.rows = rows, a.cols = cols, a.row_stride = row_stride;
     a.values = values, a.columns = columns, a.lse = lse, a.values_type = values_dtype, a.lse_type = lse_dtype, a.columns64 = columns_bits == 64, a.k = (int)k;
-    a.mask = mask, a.temperature = temperature, a.grad_scale = temperature * weight;
+    a.mask = mask, a.temperature = temperature, a.inv_tau = 1 / temperature, a.grad_scale = temperature * weight;
     a.grad = grad, a.applied = applied, a.only_changed = applied != nullptr, a.upstream = upstream, a.upstream_rows = reduction == CLG_REDUCE_NONE;
     if (reduction == CLG_REDUCE_MEAN && mask) {
         CLG_REQUIRE(scratch, "clg_distill_backward: null scratch");

@@ -105,36 +105,42 @@ __device__ __forceinline__ A wave_max(A v)
     return of_lane(v, 63);
 }
 
-// Columns base .. of one row in the registers of a workgroup: thread t holds the 16-byte pieces t, t + THREADS, ... and, of what is left of a row
-// behind its last whole piece, one element.  What is behind the row is -inf.  STREAM: loads (1) and stores (2) past the caches.
-template <typename T, int THREADS, int NV, int STREAM>
+// Columns base .. of one row in the registers of a team of LANES threads (a workgroup, or a part of a wavefront): thread t holds the 16-byte pieces t, t +
+// LANES, ... and, of what is left of a row behind its last whole piece, one element.  What is behind the row is -inf.  STREAM: loads (1) and stores (2) past the caches.
+template <typename T, int LANES, int NV, int STREAM>
 struct RowTile {
-    static constexpr int VEC = Vec16<T>::N, COLS = THREADS * NV * VEC;
+    static constexpr int VEC = Vec16<T>::N, COLS = LANES * NV * VEC;
     typedef typename Vec16<T>::type V;
     typedef typename Wide<T>::type A;
     V v[NV];
     T last;
-    int whole, tail;                                                  // whole pieces in the tile, elements behind them
+    int tid, whole, tail;                                             // of the team; whole pieces in the tile, elements behind them
+
+    __device__ __forceinline__ explicit RowTile(int tid_) : tid(tid_) {}
 
     __device__ __forceinline__ void load(const T *__restrict__ row, int64_t base, int64_t cols)
     {
-        const int n = (int)(cols - base < COLS ? cols - base : COLS), tid = threadIdx.x;
+        const int n = (int)(cols - base < COLS ? cols - base : COLS);
         whole = n / VEC;
         tail = n % VEC;
         const T none = (T)lowest(0.f);
         const T *at = row + base;
-        // (all loads before anything waits for one: lanes behind the row read its last piece again, and drop it afterwards)
+        // (all loads before anything waits for one: lanes behind the row read its last piece again, which trim() drops)
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int p = j * THREADS + tid;
-            if (j * THREADS < whole) v[j] = load_vec<(STREAM & 1) != 0>(reinterpret_cast<const V *>(at + (uint32_t)((p < whole ? p : whole - 1) * VEC)));
+            const int p = j * LANES + tid;
+            if (j * LANES < whole) v[j] = load_vec<(STREAM & 1) != 0>(reinterpret_cast<const V *>(reinterpret_cast<const char *>(at) + (uint32_t)(p < whole ? p : whole - 1) * 16u));
             else v[j] = (V)none;
         }
         last = none;
         if (tid < tail) last = at[whole * VEC + tid];
+    }
+    // the second half of load, which waits for the row
+    __device__ __forceinline__ void trim()
+    {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-            if (j * THREADS < whole && (j + 1) * THREADS > whole && j * THREADS + tid >= whole) v[j] = (V)none;
+            if (j * LANES < whole && (j + 1) * LANES > whole && j * LANES + tid >= whole) v[j] = (V)(T)lowest(0.f);
     }
     // keeps the values of the next pass apart from those of the last: both in registers at once would be twice the row
     __device__ __forceinline__ void fence()
@@ -145,6 +151,7 @@ struct RowTile {
             asm volatile("" : "+v"(r));
             v[j] = __builtin_bit_cast(V, r);
         }
+        asm volatile("" : "+s"(whole));                               // (compared again rather than kept as a condition per piece)
     }
     // the highest of each piece
     __device__ __forceinline__ void peaks(A (&high)[NV]) const
@@ -152,7 +159,7 @@ struct RowTile {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             high[j] = lowest(A(0));
-            if (j * THREADS >= whole) continue;
+            if (j * LANES >= whole) continue;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) high[j] = max_of(high[j], (A)v[j][i]);
         }
@@ -160,11 +167,10 @@ struct RowTile {
     // the columns with a bit become -inf
     __device__ __forceinline__ void drop(const uint32_t *bits)
     {
-        const int tid = threadIdx.x;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            if (j * THREADS >= whole) break;
-            const int c = (j * THREADS + tid) * VEC;
+            if (j * LANES >= whole) break;
+            const int c = (j * LANES + tid) * VEC;
             const uint32_t b = bits[c >> 5] >> (c & 31) & ((1u << VEC) - 1);
             if (b)
 #pragma unroll
@@ -179,7 +185,7 @@ struct RowTile {
         A m = (A)last;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            if (j * THREADS >= whole) break;
+            if (j * LANES >= whole) break;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) m = max_of(m, (A)v[j][i]);
         }
@@ -190,7 +196,7 @@ struct RowTile {
         A s = e((A)last);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            if (j * THREADS >= whole) break;
+            if (j * LANES >= whole) break;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) s += e((A)v[j][i]);
         }
@@ -200,16 +206,15 @@ struct RowTile {
     template <typename F>
     __device__ __forceinline__ void store(T *__restrict__ row, int64_t base, F f) const
     {
-        const int tid = threadIdx.x;
         T *at = row + base;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int p = j * THREADS + tid;
-            if (j * THREADS >= whole) break;
+            const int p = j * LANES + tid;
+            if (j * LANES >= whole) break;
             V out;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) out[i] = (T)f((A)v[j][i]);
-            if (p < whole) store_vec<(STREAM & 2) != 0>(reinterpret_cast<V *>(at + (uint32_t)(p * VEC)), out);
+            if (p < whole) store_vec<(STREAM & 2) != 0>(reinterpret_cast<V *>(reinterpret_cast<char *>(at) + (uint32_t)p * 16u), out);
         }
         if (tid < tail) at[whole * VEC + tid] = (T)f((A)last);
     }
@@ -236,6 +241,72 @@ __device__ __forceinline__ void block_reduce(A (&x)[COUNT], A *room)
             x[c] = of_lane(SUM ? row16_sum(r) : row16_max(r), 0);
         }
     }
+}
+
+// The same for sums of two types at once.
+template <int THREADS, int CA, int CB, typename A, typename B>
+__device__ __forceinline__ void block_sums(A (&x)[CA], B (&y)[CB], A *room_x, B *room_y)
+{
+#pragma unroll
+    for (int c = 0; c < CA; ++c) x[c] = wave_sum(x[c]);
+#pragma unroll
+    for (int c = 0; c < CB; ++c) y[c] = wave_sum(y[c]);
+    if constexpr (THREADS > kWave) {
+        constexpr int WAVES = THREADS / kWave;
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int c = 0; c < CA; ++c) room_x[(threadIdx.x >> 6) * CA + c] = x[c];
+#pragma unroll
+            for (int c = 0; c < CB; ++c) room_y[(threadIdx.x >> 6) * CB + c] = y[c];
+        }
+        __syncthreads();
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int c = 0; c < CA; ++c) x[c] = of_lane(row16_sum(lane < WAVES ? room_x[lane * CA + c] : A(0)), 0);
+#pragma unroll
+        for (int c = 0; c < CB; ++c) y[c] = of_lane(row16_sum(lane < WAVES ? room_y[lane * CB + c] : B(0)), 0);
+    }
+}
+
+// The team that has a row: a workgroup of THREADS, or LANES = 16 of them, one row of DPP.
+template <int THREADS, int LANES>
+struct Team {
+    static constexpr bool kWhole = THREADS == LANES;
+    static_assert(kWhole || LANES == 16, "a workgroup or a row of lanes");
+    template <bool SUM, int COUNT, typename A>
+    __device__ __forceinline__ static void reduce(A (&x)[COUNT], A *room)
+    {
+        if constexpr (kWhole) {
+            block_reduce<SUM, THREADS>(x, room);
+        } else {
+#pragma unroll
+            for (int c = 0; c < COUNT; ++c) x[c] = SUM ? row16_sum(x[c]) : row16_max(x[c]);
+        }
+    }
+    template <int CA, int CB, typename A>
+    __device__ __forceinline__ static void sums(A (&x)[CA], double (&y)[CB], A *room_x, double *room_y)
+    {
+        if constexpr (kWhole) {
+            block_sums<THREADS>(x, y, room_x, room_y);
+        } else {
+            reduce<true>(x, room_x);
+            reduce<true>(y, room_y);
+        }
+    }
+    template <typename A>
+    __device__ __forceinline__ static A from(A v, int lane)             // of the team's first wavefront
+    {
+        if constexpr (kWhole) return of_lane(v, lane);
+        else return __shfl(v, lane, 16);
+    }
+};
+
+// 1 / v, to the last few bits
+__device__ __forceinline__ double quick_inverse(double v)
+{
+    double r = __builtin_amdgcn_rcp(v);
+    r = __builtin_fma(__builtin_fma(-v, r, 1.0), r, r);
+    return __builtin_fma(__builtin_fma(-v, r, 1.0), r, r);
 }
 
 // element i of an array of one of the C ABI's types: its bits, which may still be on their way, and its value

@@ -229,11 +229,12 @@ __global__ __launch_bounds__(THREADS, sizeof(T) == 8 ? 2 : 6) void top_kernel(To
         if (now.key() > from.key()) from = now;
     };
 
-    Tile tile;
+    Tile tile(tid);
     if (tid == 0) *noted = 0;
 #pragma unroll 1
     for (int64_t base = 0, tiles = 1; base < cols; base += Tile::COLS, ++tiles) {
         tile.load(z, base, cols);
+        tile.trim();
         A high[NV], m = max_of(m_t, (A)tile.last);
         tile.peaks(high);
 #pragma unroll

@@ -12,7 +12,7 @@ import torch
 
 import convlogic_amd as C
 from oracle import losses_oracle as L
-from tests.gpu_util import DEV
+from tests.gpu_util import DEV, set_knobs
 
 pytestmark = pytest.mark.gpu
 
@@ -315,6 +315,44 @@ def test_distillation_of_many_rows():
     t = teacher(5000, 17, 3, True, 4, 1.0)
     check_distill(z, *t)
     check_distill(z, *t, mask=torch.arange(5000, device=DEV) % 3 > 0, upstream=torch.tensor(0.3, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("cols,k", [(9, 3), (100, 20), (250, 64), (251, 65), (900, 5), (2047, 7)])
+def test_distillation_of_many_short_rows(dtype, rest, cols, k):
+    # enough rows that several share a wavefront, the last one not full; some without entries, masked, with other rows' special values beside them
+    rows = 2050
+    z = scores(rows, cols, dtype, cols)
+    values, columns, lse = teacher(rows, cols, k, rest, k, 1.5)
+    mask = torch.arange(rows, device=DEV) % 5 != 2
+    z[2] = NAN
+    z[9] -= 300.0
+    if not rest:
+        columns[4] = -1
+        columns[5, 1:] = -1
+    columns[13, 0] = columns[13, -1]
+    check_distill(z, values, columns, lse, 1.5, mask, 0.5, "mean", torch.tensor(3.0, device=DEV, dtype=torch.float64 if dtype == torch.float64 else torch.float32))
+    x = z[:2049].clone().requires_grad_(True)
+    columns[8, 0] = cols
+    loss = C.distillation_loss(x, values[:2049], columns[:2049], None if lse is None else lse[:2049], mask=mask[:2049], reduction="none")
+    grad, = torch.autograd.grad(loss.sum(), x)
+    assert loss.isnan().nonzero().tolist() == [[8]] and grad.isnan().any(1).nonzero().tolist() == [[8]]
+
+
+@pytest.mark.parametrize("past", [0, 1 << 20])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_through_and_past_the_caches(monkeypatch, dtype, past):
+    # the accesses that large tensors get, on small ones
+    set_knobs(monkeypatch, CLG_STREAM_MB=past)
+    for cols in (64, 100, 1024, 1027, 20000, 40000, 66000, 140000):
+        z = scores(3, cols, dtype, cols)
+        check_top(z, 20)
+        check_distill(z, *teacher(3, cols, 20, True, 1, 1.0))
+    z = scores(2100, 128, dtype, 1)
+    check_distill(z, *teacher(2100, 128, 9, True, 1, 1.0))
+    for experts in (16, 60, 256):
+        check_balance(scores(70, experts, dtype, experts), 2)
 
 
 # ---- balance -------------------------------------------------------------------------------------
