@@ -12,7 +12,7 @@ namespace {
 
 struct DistillArgs {
     const void *z;                                                    // [rows][cols] with a stride between rows
-    int64_t rows, cols, row_stride;
+    int64_t rows, cols, row_stride, first_row;                        // (first_row: of this launch)
     const void *values, *columns, *lse;                               // [rows][k], [rows][k], [rows] or NULL
     int values_type, lse_type, columns64, k;
     const uint8_t *mask;                                              // [rows] or NULL
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
     uint32_t *bits = reinterpret_cast<uint32_t *>(column + k);
     const A unit = (A)Exps<A>::unit(a.temperature);
 
-    const int64_t row = Mine::kWhole ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * TEAMS + team;
+    const int64_t row = a.first_row + (Mine::kWhole ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * TEAMS + team);
     if (TEAMS > 1 && row >= a.rows) return;
     const A up = a.upstream ? static_cast<const A *>(a.upstream)[a.upstream_rows ? row : 0] : A(1);
     if (a.only_changed && static_cast<const A *>(a.applied)[row] == up) return;
@@ -249,22 +249,45 @@ __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
 // 1 / number of kept rows, 0 where there are none
 __global__ __launch_bounds__(1024) void count_kept_kernel(const uint8_t *mask, int64_t rows, double *per_count)
 {
+    typedef uint32_t Four __attribute__((ext_vector_type(4), aligned(1)));
     __shared__ double room[16];
-    double n[1] = {0};
-    for (int64_t i = threadIdx.x; i < rows; i += 1024) n[0] += mask[i] != 0;
+    int64_t count = 0;
+    const int64_t whole = rows / 16;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < whole; i += 1024) {
+        const Four x = reinterpret_cast<const Four *>(mask)[i];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) count += __popc(((x[w] & 0x7F7F7F7Fu) + 0x7F7F7F7Fu | x[w]) & 0x80808080u);     // bytes that are not 0
+    }
+    if (threadIdx.x < rows % 16) count += mask[rows - 1 - threadIdx.x] != 0;
+    double n[1] = {(double)count};
     block_reduce<true, 1024>(n, room);
     if (threadIdx.x == 0) *per_count = n[0] == 0 ? 0 : 1 / n[0];
 }
 
-// the sum of the rows' losses, in a fixed order
+// The sum of the rows' losses, in a fixed order: of all rows, or of kSlice to a workgroup first.
+constexpr int kSlice = 16384;
+__device__ __forceinline__ double sum_of(const double *v, int64_t n, double *room)
+{
+    double s[1] = {0};
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < n; i += 1024) s[0] += v[i];
+    block_reduce<true, 1024>(s, room);
+    return s[0];
+}
+__global__ __launch_bounds__(1024) void sum_slices_kernel(const double *row_loss, int64_t rows, double *slices)
+{
+    __shared__ double room[16];
+    const int64_t first = (int64_t)blockIdx.x * kSlice;
+    const double s = sum_of(row_loss + first, rows - first < kSlice ? rows - first : kSlice, room);
+    if (threadIdx.x == 0) slices[blockIdx.x] = s;
+}
 template <typename A>
 __global__ __launch_bounds__(1024) void sum_rows_kernel(const double *row_loss, int64_t rows, const double *per_count, A *out)
 {
     __shared__ double room[16];
-    double s[1] = {0};
-    for (int64_t i = threadIdx.x; i < rows; i += 1024) s[0] += row_loss[i];
-    block_reduce<true, 1024>(s, room);
-    if (threadIdx.x == 0) *out = (A)(s[0] * (per_count ? *per_count : 1));
+    const double s = sum_of(row_loss, rows, room);
+    if (threadIdx.x == 0) *out = (A)(s * (per_count ? *per_count : 1));
 }
 
 template <typename T, int THREADS, int LANES, int NV, bool MULTI, int STREAM>
@@ -274,7 +297,12 @@ void launch_as(const DistillArgs &a, hipStream_t stream)
     static_assert(Tile::COLS % 32 == 0, "bits of a tile fill whole words");
     constexpr int TEAMS = THREADS / LANES;
     const size_t lds = (size_t)TEAMS * distill_lds<typename Wide<T>::type>(TEAMS == 1, a.k, Tile::COLS);
-    distill_kernel<T, THREADS, LANES, NV, MULTI, STREAM><<<dim3((unsigned)clg_ceil_div(a.rows, TEAMS)), dim3(THREADS), lds, stream>>>(a);
+    DistillArgs part = a;
+    constexpr int64_t kMost = (int64_t)1 << 31;                       // threads of a launch
+    for (; part.first_row < a.rows; part.first_row += kMost / LANES) {
+        const int64_t rows = a.rows - part.first_row < kMost / LANES ? a.rows - part.first_row : kMost / LANES;
+        distill_kernel<T, THREADS, LANES, NV, MULTI, STREAM><<<dim3((unsigned)clg_ceil_div(rows, TEAMS)), dim3(THREADS), lds, stream>>>(part);
+    }
 }
 
 template <typename T, int STREAM>
@@ -328,7 +356,7 @@ static int check_call(const char *name, int dtype, const void *logits, int64_t r
     return CLG_OK;
 }
 
-extern "C" int64_t clg_distill_scratch_bytes(int64_t rows) { return rows < 0 ? 0 : (rows + 2) * 8; }
+extern "C" int64_t clg_distill_scratch_bytes(int64_t rows) { return rows < 0 ? 0 : (rows + 2 + clg_ceil_div(rows, kSlice)) * 8; }
 
 extern "C" int clg_distill_forward(int dtype, const void *logits, int64_t row_stride, const void *values, int values_dtype, const void *columns,
                                    int columns_bits, const void *lse, int lse_dtype, const uint8_t *mask, int64_t rows, int64_t cols, int64_t k,
@@ -366,10 +394,16 @@ extern "C" int clg_distill_forward(int dtype, const void *logits, int64_t row_st
         CLG_CHECK_LAUNCH("clg_distill_forward");
     }
     if (reduction == CLG_REDUCE_NONE) return CLG_OK;
-    if (dtype == CLG_F64)
-        sum_rows_kernel<double><<<dim3(1), dim3(1024), 0, clg_stream(stream)>>>(row_loss, rows, a.per_count, static_cast<double *>(loss));
-    else
-        sum_rows_kernel<float><<<dim3(1), dim3(1024), 0, clg_stream(stream)>>>(row_loss, rows, a.per_count, static_cast<float *>(loss));
+    const double *terms = row_loss;
+    int64_t n = rows;
+    if (rows > 4 * kSlice) {
+        n = clg_ceil_div(rows, kSlice);
+        sum_slices_kernel<<<dim3((unsigned)n), dim3(1024), 0, clg_stream(stream)>>>(row_loss, rows, per_count + 1);
+        CLG_CHECK_LAUNCH("clg_distill_forward");
+        terms = per_count + 1;
+    }
+    if (dtype == CLG_F64) sum_rows_kernel<double><<<dim3(1), dim3(1024), 0, clg_stream(stream)>>>(terms, n, a.per_count, static_cast<double *>(loss));
+    else sum_rows_kernel<float><<<dim3(1), dim3(1024), 0, clg_stream(stream)>>>(terms, n, a.per_count, static_cast<float *>(loss));
     CLG_CHECK_LAUNCH("clg_distill_forward");
     return CLG_OK;
 }

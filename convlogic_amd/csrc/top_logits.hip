@@ -49,7 +49,7 @@ struct Cand<double> {
 
 struct TopArgs {
     const void *z;
-    int64_t rows, cols, row_stride;
+    int64_t rows, cols, row_stride, first_row;                        // (first_row: of this launch)
     int k;
     double temperature;
     void *values;                                                     // [rows][k]
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(THREADS, sizeof(T) == 8 ? 2 : 6) void top_kernel(To
     uint32_t *note = reinterpret_cast<uint32_t *>(maxima + size.maxima);             // first columns
     const int tid = threadIdx.x, part = blockIdx.y;
     const A unit = (A)Exps<A>::unit(a.temperature);
-    const int64_t row = blockIdx.x, start = part * a.width, cols = a.cols - start < a.width ? a.cols - start : a.width, whole = cols / Tile::VEC * Tile::VEC;
+    const int64_t row = a.first_row + blockIdx.x, start = part * a.width, cols = a.cols - start < a.width ? a.cols - start : a.width, whole = cols / Tile::VEC * Tile::VEC;
     const int k = a.k < cols ? a.k : (int)cols;
     const T *z = static_cast<const T *>(a.z) + row * a.row_stride + start;
 
@@ -372,7 +372,12 @@ __global__ __launch_bounds__(256) void top_merge_kernel(TopArgs a)
 template <typename T, int THREADS, int NV, bool MULTI, bool STREAM>
 void launch_as(const TopArgs &a, hipStream_t stream)
 {
-    top_kernel<T, THREADS, NV, MULTI, STREAM><<<dim3((unsigned)a.rows, a.parts), dim3(THREADS), TopRoom<T, THREADS, NV, MULTI>(a.k).bytes, stream>>>(a);
+    TopArgs some = a;
+    constexpr int64_t kMost = ((int64_t)1 << 31) / THREADS;           // rows of a launch: 2^31 threads
+    for (; some.first_row < a.rows; some.first_row += kMost) {
+        const int64_t rows = a.rows - some.first_row < kMost ? a.rows - some.first_row : kMost;
+        top_kernel<T, THREADS, NV, MULTI, STREAM><<<dim3((unsigned)rows, a.parts), dim3(THREADS), TopRoom<T, THREADS, NV, MULTI>(a.k).bytes, stream>>>(some);
+    }
 }
 
 template <typename T, bool STREAM>
@@ -430,7 +435,7 @@ extern "C" int clg_top_logits(int dtype, const void *logits, int64_t row_stride,
     CLG_REQUIRE(temperature > 0 && temperature < 1e30, "clg_top_logits: the temperature must be positive and finite");
     if (!rows) return CLG_OK;
     CLG_REQUIRE(logits && values && columns, "clg_top_logits: null pointer");
-    TopArgs a{logits, rows, cols, row_stride, (int)k, temperature, values, columns, lse, parts_of(rows, cols, k), cols, nullptr, nullptr};
+    TopArgs a{logits, rows, cols, row_stride, 0, (int)k, temperature, values, columns, lse, parts_of(rows, cols, k), cols, nullptr, nullptr};
     if (a.parts > 1) {
         CLG_REQUIRE(scratch, "clg_top_logits: null scratch");
         a.width = clg_ceil_div(clg_ceil_div(cols, a.parts), 64) * 64;

@@ -355,6 +355,67 @@ def test_rows_through_and_past_the_caches(monkeypatch, dtype, past):
         check_balance(scores(70, experts, dtype, experts), 2)
 
 
+def test_rows_beyond_two_to_the_31_elements_and_threads():
+    # element 2^31 and more: the last rows as the same rows alone
+    rows, cols = 16500, 131072
+    z = torch.empty(rows, cols, dtype=torch.bfloat16, device=DEV)
+    z.normal_(generator=torch.Generator(device=DEV).manual_seed(1))
+    answers = C.top_logits(z, 5)
+    some = [0, 8000, rows - 2, rows - 1]
+    check_top(z[some], 5)
+    for got, want in zip(answers, C.top_logits(z[some], 5)):
+        assert torch.equal(got[some], want)
+    leaf = z.requires_grad_(True)
+    loss = C.distillation_loss(leaf, *answers, reduction="none")
+    grad, = torch.autograd.grad(loss.sum(), leaf)
+    alone = z.detach()[some].requires_grad_(True)
+    of_alone = C.distillation_loss(alone, *(t[some] for t in answers), reduction="none")
+    assert torch.equal(loss[some], of_alone) and torch.equal(grad[some], torch.autograd.grad(of_alone.sum(), alone)[0])
+    del z, leaf, grad, loss
+    # more rows than 2^32 threads have, of any of the teams that a row can get
+    rows = (1 << 28) + 6
+    z = (torch.arange(2 * rows, device=DEV, dtype=torch.int32) % 7).view(rows, 2).half()
+    values, columns = torch.zeros(rows, 1, dtype=torch.float16, device=DEV), torch.ones(rows, 1, dtype=torch.int32, device=DEV)
+    loss = C.distillation_loss(z, values, columns, reduction="none")
+    total = C.distillation_loss(z, values, columns, reduction="sum")
+    want = torch.nn.functional.softplus(torch.arange(-6, 7, device=DEV).double())      # log(1 + e^(z0 - z1))
+    for part in (slice(0, 1000), slice(rows // 2, rows // 2 + 1000), slice(rows - 1000, rows)):
+        d = (z[part, 0] - z[part, 1]).long() + 6
+        assert (loss[part].double() - want[d]).abs().max() <= 2.0 ** -24 * 400
+    assert abs(float(total) - float(loss.double().sum())) <= 1e-6 * float(total)
+    top = C.top_logits(z[: (1 << 25) + 70], 1)                        # (64 threads to a row)
+    assert torch.equal(top.values[-1000:, 0], z[(1 << 25) - 930:(1 << 25) + 70].max(1).values)
+
+
+@pytest.mark.parametrize("rows", [15, 16, 17, 1023, 16385, 70000, 200001])
+def test_the_mean_over_many_masked_rows(rows):
+    z = scores(rows, 3, torch.float32, 1)
+    values, columns, _ = teacher(rows, 3, 1, False, 1, 1.0)
+    kept = torch.rand(rows + 3, device=DEV)[3:] < 0.6
+    each = C.distillation_loss(z, values, columns, reduction="none").double()
+    for mask in (kept, torch.ones_like(kept), torch.zeros_like(kept)):
+        n = max(int(mask.sum()), 1)
+        for reduction, want in (("mean", each[mask].sum() / n), ("sum", each[mask].sum())):
+            assert abs(float(C.distillation_loss(z, values, columns, mask=mask, reduction=reduction)) - float(want)) <= 2.0 ** -22 * float(want)
+
+
+def test_what_autograd_offers_around_the_losses():
+    z = scores(8, 300, torch.float32, 1).requires_grad_(True)
+    t = teacher(8, 300, 5, True, 1, 1.0)
+    call = lambda x: C.distillation_loss(x, *t) + C.balance_loss(x, 3).loss
+    want, = torch.autograd.grad(call(z), z)
+    moved = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: moved.append(1) or s.cpu(), lambda s: s.to(DEV)):
+        got, = torch.autograd.grad(call(z), z)
+        half, = torch.autograd.grad(0.5 * call(z), z)
+    assert moved and torch.equal(got, want) and torch.equal(half * 2, want)
+    for one in (lambda x: C.distillation_loss(x, *(s[0] for s in t)), lambda x: C.balance_loss(x, 3).loss, lambda x: C.top_logits(x, 3).values):
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(one)(z.detach())
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError):
+        call(torch.autograd.forward_ad.make_dual(z.detach(), torch.ones_like(z)))
+
+
 # ---- balance -------------------------------------------------------------------------------------
 def check_balance(z, k, mask=None, weight=1.0):
     leaf = z.detach().requires_grad_(True)
