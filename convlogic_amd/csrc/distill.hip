@@ -6,6 +6,8 @@
 //     d loss / d z_v = tau [ M q_v - sum_{j: c_j = v} p_j ]  listed,    tau q_v [ M - p_r / q_r ]  not listed,        M = sum_j p_j + p_r
 // q_r is small where the student agrees with its teacher, so it is no difference of sums: listed columns leave the row first (a bit per column in
 // LDS), their few exponentials are added to the sum of the others afterwards.
+#include <stdlib.h>
+
 #include "row_tile.h"
 
 namespace {
@@ -26,7 +28,6 @@ struct DistillArgs {
     int upstream_rows, only_changed;
 };
 
-constexpr int kFewEntries = 32, kManyRows = 2048;
 constexpr int kFlagTwice = 1, kFlagListed = 2, kFlagBad = 4;
 
 // LDS of a team: reduction room (16 wavefronts of 4 doubles, for a workgroup), flags, entries (probability, logit, column), bits of a tile
@@ -309,14 +310,14 @@ template <typename T, int STREAM>
 void launch_rows(const DistillArgs &a, hipStream_t stream)
 {
     const int64_t pieces = (a.cols + Vec16<T>::N - 1) / Vec16<T>::N;
-    // 16 lanes to a row: what is done once for a row is done for four at a time, which is most of the work of short rows
-    if (a.k <= kFewEntries) {
-        if (pieces <= 16) return launch_as<T, 64, 16, 1, false, STREAM>(a, stream);
-        if (a.rows >= kManyRows) {
-            if (pieces <= 16 * 4) return launch_as<T, 64, 16, 4, false, STREAM>(a, stream);
-            if (pieces <= 16 * 16) return launch_as<T, 64, 16, 16, false, STREAM>(a, stream);
-        }
-    }
+    // 16 lanes to a row: what is done once for a row is done for four at a time, most of the work of short rows; with fewer rows than fill the chip so, longer
+    // ones are done sooner by 64 lanes each.  Float32 with gradient, 64 and 16 lanes: 8192 rows of 100 columns 21 and 13 us (2048: 13 and 12, 512: 11 and
+    // 11), 32768 of 500 62 and 44 (8192: 24 and 19, 2048: 13 and 15); entries beyond 32 take a lane as long as its part of 1000 columns (k = 64: 87 and 100).
+    const char *lanes = clg_knob(K_DISTILL_LANES);
+    const bool few = lanes ? atoi(lanes) == 16 : pieces <= 16 ? a.k <= 64 : pieces <= 64 ? a.k <= 64 && a.rows >= 2048 : a.k <= 32 && a.rows >= 8192;
+    if (few && pieces <= 16) return launch_as<T, 64, 16, 1, false, STREAM>(a, stream);
+    if (few && pieces <= 16 * 4) return launch_as<T, 64, 16, 4, false, STREAM>(a, stream);
+    if (few && pieces <= 16 * 16) return launch_as<T, 64, 16, 16, false, STREAM>(a, stream);
     if (pieces <= 64 * 4) return launch_as<T, 64, 64, 4, false, STREAM>(a, stream);
     if (pieces <= 64 * 16) return launch_as<T, 64, 64, 16, false, STREAM>(a, stream);
     if (pieces <= 256 * 16) return launch_as<T, 256, 256, 16, false, STREAM>(a, stream);

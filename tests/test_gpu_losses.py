@@ -320,8 +320,9 @@ def test_distillation_of_many_rows():
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rest", [False, True])
 @pytest.mark.parametrize("cols,k", [(9, 3), (100, 20), (250, 64), (251, 65), (900, 5), (2047, 7)])
-def test_distillation_of_many_short_rows(dtype, rest, cols, k):
-    # enough rows that several share a wavefront, the last one not full; some without entries, masked, with other rows' special values beside them
+def test_distillation_of_rows_that_share_a_wavefront(monkeypatch, dtype, rest, cols, k):
+    # the last wavefront not full; some rows without entries, masked, with other rows' special values beside them
+    set_knobs(monkeypatch, CLG_DISTILL_LANES=16)
     rows = 2050
     z = scores(rows, cols, dtype, cols)
     values, columns, lse = teacher(rows, cols, k, rest, k, 1.5)
