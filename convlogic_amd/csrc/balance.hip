@@ -41,6 +41,11 @@ __device__ __forceinline__ int of_lanes(int v)                        // (every 
     return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, true);
 }
 template <int CTRL>
+__device__ __forceinline__ uint32_t of_lanes(uint32_t v)
+{
+    return (uint32_t)of_lanes<CTRL>((int)v);
+}
+template <int CTRL>
 __device__ __forceinline__ float of_lanes(float v)
 {
     return __builtin_bit_cast(float, of_lanes<CTRL>(__builtin_bit_cast(int, v)));
@@ -155,6 +160,14 @@ __device__ __forceinline__ void choose(Part &part, int lane, int k, int (&c)[N])
     }
 }
 
+// order of a 16-bit logit, then of its expert, from the lowest; 0 for -inf
+__device__ __forceinline__ uint32_t choice_key(float x, int expert)
+{
+    const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f), ordered = x != x ? ~0u : u ^ (u >> 31 ? ~0u : 0x80000000u);
+    return x == lowest(0.f) ? 0 : (ordered & ~0x1FFFu) | (uint32_t)(0x1FFF - expert);
+}
+__device__ __forceinline__ uint32_t choice_key(double, int) { return 0; }                // (not of this type)
+
 // sums and counts of a workgroup's rows
 template <typename T, int G, int NV, bool STREAM>
 __global__ __launch_bounds__(kThreads) void balance_kernel(BalanceArgs a)
@@ -189,44 +202,77 @@ __global__ __launch_bounds__(kThreads) void balance_kernel(BalanceArgs a)
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) s[r] = part[r].exponentials(m[r], e[r]);
-        // The choice: k times the highest below the last one.  -inf is none, NaN is above everything.  Where values are equal, or too few are there,
-        // these are too many or too few experts, and the slow way takes one at a time, the lowest of the highest.
-        A least[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             kept[r] = kept[r] && !(s[r] == 0);
             n += kept[r];
-            least[r] = m[r];
-            odd |= s[r] != s[r];
         }
+        if constexpr (sizeof(T) == 2) {
+            // The choice of 16-bit logits, of which many are equal: the k highest keys of a logit's order and, in the bits that a float32 of it does not use,
+            // the expert.  No two are equal; -inf has none.
+            uint32_t key[R][N], least[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                least[r] = ~0u;
+#pragma unroll
+                for (int i = 0; i < N; ++i) key[r][i] = choice_key(part[r].x[i], Part::expert(lane, i));
+            }
 #pragma unroll 1
-        for (int pick = 1; pick < a.k; ++pick) {
+            for (int pick = 0; pick < a.k; ++pick)
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    uint32_t next = 0;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const uint32_t below = key[r][i] < least[r] ? key[r][i] : 0;
+                        next = below > next ? below : next;
+                    }
+                    least[r] = group_reduce<G>(next, [](uint32_t u, uint32_t v) { return u > v ? u : v; });
+                }
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                A next = lowest(A(0));
+                least[r] = least[r] == 0 ? 1 : least[r];
 #pragma unroll
-                for (int i = 0; i < N; ++i) next = max_of(next, part[r].x[i] < least[r] ? part[r].x[i] : lowest(A(0)));
-                least[r] = group_reduce<G>(next, Max());
+                for (int i = 0; i < N; ++i) c[i] += kept[r] && key[r][i] >= least[r];
             }
-        }
-        int want = 0, have = 0;                                       // of the wavefront
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            odd |= kept[r] && least[r] == lowest(A(0));
-            want += __popcll(__ballot(kept[r]));
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const bool it = kept[r] && part[r].x[i] >= least[r];
-                have += __popcll(__ballot(it));
-                c[i] += it;
-            }
-        }
-        if (__any(odd) || have * G != want * a.k) {
+        } else {
+            // The choice: k times the highest below the last one.  -inf is none, NaN is above everything.  Where values are equal, or too few are there,
+            // these are too many or too few experts, and the slow way takes one at a time, the lowest of the highest.
+            A least[R];
 #pragma unroll
             for (int r = 0; r < R; ++r) {
+                least[r] = m[r];
+                odd |= s[r] != s[r];
+            }
+#pragma unroll 1
+            for (int pick = 1; pick < a.k; ++pick) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) c[i] -= kept[r] && part[r].x[i] >= least[r];
-                if (kept[r]) choose(part[r], lane, a.k, c);
+                for (int r = 0; r < R; ++r) {
+                    A next = lowest(A(0));
+#pragma unroll
+                    for (int i = 0; i < N; ++i) next = max_of(next, part[r].x[i] < least[r] ? part[r].x[i] : lowest(A(0)));
+                    least[r] = group_reduce<G>(next, Max());
+                }
+            }
+            int want = 0, have = 0;                                   // of the wavefront
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                odd |= kept[r] && least[r] == lowest(A(0));
+                want += __popcll(__ballot(kept[r]));
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const bool it = kept[r] && part[r].x[i] >= least[r];
+                    have += __popcll(__ballot(it));
+                    c[i] += it;
+                }
+            }
+            if (__any(odd) || have * G != want * a.k) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) c[i] -= kept[r] && part[r].x[i] >= least[r];
+                    if (kept[r]) choose(part[r], lane, a.k, c);
+                }
             }
         }
 #pragma unroll
@@ -418,7 +464,8 @@ void with_part(int experts, F call)
     if (pieces <= 16) return call(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
     if (pieces <= 32) return call(std::integral_constant<int, 16>(), std::integral_constant<int, 2>());
     if (pieces <= 64) return call(std::integral_constant<int, 16>(), std::integral_constant<int, 4>());
-    return call(std::integral_constant<int, 64>(), std::integral_constant<int, kMaxExperts / 64 / Vec16<T>::N>());
+    if (pieces <= 128) return call(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+    call(std::integral_constant<int, 64>(), std::integral_constant<int, (kMaxExperts / 64 / Vec16<T>::N > 2 ? kMaxExperts / 64 / Vec16<T>::N : 2)>());
 }
 
 template <typename T>

@@ -89,7 +89,7 @@ __host__ __device__ __forceinline__ bool by_pieces(int k)
 }
 
 constexpr int kSpare = 512;                                           // candidates that there is room for beside the k best
-constexpr int kAllRanked = 128;                                       // columns of rows without a threshold
+constexpr int kAllRanked = 64;                                        // columns of rows without a threshold
 constexpr int kNoted = 1024;                                          // pieces that may be noted when a tile begins
 
 // LDS of a workgroup: reduction room, counters, candidates, the best k, maxima, noted pieces
@@ -206,11 +206,17 @@ __global__ __launch_bounds__(THREADS, sizeof(T) == 8 ? 2 : 6) void top_kernel(To
             maxima[tid] = ordered(m_t);
         }
     };
-    const auto search = [&]() {
+    const auto search = [&](const Tile &tile) {
         if (tid >= kWave) return;
         constexpr int PER = THREADS / kWave;
         K t;
-        if (pieces) {
+        if (!MULTI && THREADS == kWave && 2 * k > tile.whole) {       // (too many for maxima of pieces: of the elements, which this wavefront has)
+            K x[NV * Tile::VEC + 1];
+#pragma unroll
+            for (int i = 0; i < NV * Tile::VEC; ++i) x[i] = i / Tile::VEC * THREADS + tid < tile.whole ? ordered((A)tile.v[i / Tile::VEC][i % Tile::VEC]) : K(0);
+            x[NV * Tile::VEC] = tid < tile.tail ? ordered((A)tile.last) : K(0);
+            t = wave_threshold(x, k, k + k / 4 + 8);
+        } else if (pieces) {
             K x[PER * SEEN];
 #pragma unroll
             for (int i = 0; i < PER * SEEN; ++i) x[i] = maxima[i * kWave + tid];
@@ -265,7 +271,7 @@ __global__ __launch_bounds__(THREADS, sizeof(T) == 8 ? 2 : 6) void top_kernel(To
         if (base == 0) {
             show();
             __syncthreads();
-            search();
+            search(tile);
             __syncthreads();
             raise();
         }
@@ -283,7 +289,7 @@ __global__ __launch_bounds__(THREADS, sizeof(T) == 8 ? 2 : 6) void top_kernel(To
             const bool last = base + Tile::COLS >= cols, anew = base && (last || (tiles & (tiles - 1)) == 0);
             if (anew) show();
             __syncthreads();
-            if (anew) search();
+            if (anew) search(tile);
             const int n = *noted;
             if (n > kNoted && !last) {
                 take_all(n);
@@ -318,6 +324,51 @@ __global__ __launch_bounds__(THREADS, sizeof(T) == 8 ? 2 : 6) void top_kernel(To
     const double lse = (double)finite_or_zero(top[0]) / a.temperature + log(s[0]) + e.residue(top[0]);
     if (a.parts > 1) a.part_lse[row * a.parts + part] = lse;
     else static_cast<A *>(a.lse)[row] = (A)lse;
+}
+
+// Rows of up to 16 columns, 16 lanes each: a lane has an element and meets the others on its way around the row of lanes.
+template <int BY>
+__device__ __forceinline__ uint32_t rotated(uint32_t v)
+{
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + BY, 0xF, 0xF, true);           // row_ror
+}
+template <int BY>
+__device__ __forceinline__ uint64_t rotated(uint64_t v)
+{
+    return (uint64_t)rotated<BY>((uint32_t)(v >> 32)) << 32 | rotated<BY>((uint32_t)v);
+}
+template <int BY, typename K>
+__device__ __forceinline__ int count_before(K mine, int lane)
+{
+    if constexpr (BY == 16) {
+        return 0;
+    } else {
+        const K other = rotated<BY>(mine);                            // of lane - BY, around the row
+        return (other > mine || (other == mine && lane >= BY)) + count_before<BY + 1>(mine, lane);
+    }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void top_small_kernel(TopArgs a)
+{
+    typedef typename Wide<T>::type A;
+    const int lane = threadIdx.x % 16;
+    const int64_t row = a.first_row + (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
+    if (row >= a.rows) return;
+    const bool there = lane < a.cols;
+    const T z = there ? static_cast<const T *>(a.z)[row * a.row_stride + lane] : (T)lowest(0.f);
+    const int before = count_before<1>(there ? ordered((A)z) : typename Cand<A>::K(0), lane);
+    if (there && before < a.k) {
+        static_cast<T *>(a.values)[row * a.k + before] = z;
+        a.columns[row * a.k + before] = lane;
+    }
+    if (!a.lse) return;
+    A top[1] = {(A)z};
+    Team<256, 16>::reduce<false>(top, (A *)nullptr);
+    if (top[0] != top[0]) top[0] = 0;                                 // (NaN, as the sum will be)
+    const Exps<A> e(top[0], (A)Exps<A>::unit(a.temperature));
+    A s[1] = {e((A)z)};
+    Team<256, 16>::reduce<true>(s, (A *)nullptr);
+    if (lane == 0) static_cast<A *>(a.lse)[row] = (A)((double)finite_or_zero(top[0]) / a.temperature + log((double)s[0]) + e.residue(top[0]));
 }
 
 constexpr int kMostParts = 64, kMerged = 1024;                        // parts of a row, and their candidates
@@ -384,6 +435,13 @@ template <typename T, bool STREAM>
 void launch_rows(const TopArgs &a, hipStream_t stream)
 {
     const int64_t pieces = (a.width + Vec16<T>::N - 1) / Vec16<T>::N;
+    if (a.cols <= 16) {
+        TopArgs some = a;
+        constexpr int64_t kMost = (int64_t)1 << 27;                   // rows of a launch: 2^31 threads
+        for (; some.first_row < a.rows; some.first_row += kMost)
+            top_small_kernel<T><<<dim3((unsigned)clg_ceil_div(a.rows - some.first_row < kMost ? a.rows - some.first_row : kMost, 16)), dim3(256), 0, stream>>>(some);
+        return;
+    }
     if (pieces <= 64) launch_as<T, 64, 1, false, STREAM>(a, stream);
     else if (pieces <= 64 * 4) launch_as<T, 64, 4, false, STREAM>(a, stream);
     else if (pieces <= 256 * 4) launch_as<T, 256, 4, false, STREAM>(a, stream);
