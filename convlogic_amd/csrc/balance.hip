@@ -345,10 +345,21 @@ __global__ __launch_bounds__(1024) void balance_finish_kernel(FinishArgs a)
     double p = 0;
     int64_t c = 0;
     if (e < a.experts) {
-#pragma unroll 4
-        for (int w = first + tid / EACH; w < end; w += SLICES) {
-            p += (double)static_cast<const A *>(a.sums)[(int64_t)w * a.experts + e];
-            c += a.counts[(int64_t)w * (a.experts + 1) + e];
+        for (int w0 = first + tid / EACH; w0 < end; w0 += 8 * SLICES) {       // (eight rows of sums on their way at once)
+            A p8[8];
+            int c8[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int w = w0 + u * SLICES < end ? w0 + u * SLICES : w0;
+                p8[u] = static_cast<const A *>(a.sums)[(int64_t)w * a.experts + e];
+                c8[u] = a.counts[(int64_t)w * (a.experts + 1) + e];
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const bool there = w0 + u * SLICES < end;
+                p += there ? (double)p8[u] : 0.0;
+                c += there ? c8[u] : 0;
+            }
         }
     }
     sum_p[tid] = p;
