@@ -160,10 +160,10 @@ __device__ __forceinline__ void choose(Part &part, int lane, int k, int (&c)[N])
     }
 }
 
-// order of a 16-bit logit, then of its expert, from the lowest; 0 for -inf
+// order of a 16-bit logit, then of its expert, from the lowest; 0 for -inf, as +inf for NaN (and so never ~0)
 __device__ __forceinline__ uint32_t choice_key(float x, int expert)
 {
-    const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f), ordered = x != x ? ~0u : u ^ (u >> 31 ? ~0u : 0x80000000u);
+    const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f), ordered = x != x ? 0xFF800000u : u ^ (u >> 31 ? ~0u : 0x80000000u);
     return x == lowest(0.f) ? 0 : (ordered & ~0x1FFFu) | (uint32_t)(0x1FFF - expert);
 }
 __device__ __forceinline__ uint32_t choice_key(double, int) { return 0; }                // (not of this type)

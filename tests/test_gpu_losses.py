@@ -455,6 +455,21 @@ def test_balance_of_padded_and_masked_rows(dtype, experts, k):
     assert C.balance_loss(z, k).loss.isnan()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("experts,k", [(1, 1), (8, 1), (20, 3), (300, 5)])
+def test_balance_counts_a_nan_as_the_maximum(dtype, experts, k):
+    # a NaN at each expert in turn, alone, behind and in front of +inf, and between experts of -inf; rows of NaN: counts are integers, those of the plain form
+    z = scores(4 * experts + 1, experts, dtype, 11)
+    for e in range(experts):
+        z[4 * e:4 * e + 4, e] = NAN
+        z[4 * e + 1, e - 1] = INF
+        z[4 * e + 2, e // 2] = INF
+        z[4 * e + 3] = torch.where(z[4 * e + 3].isnan(), z[4 * e + 3], -INF)
+    z[-1] = NAN
+    for rows in (slice(None), slice(0, 1), slice(0, 4), slice(-1, None)):
+        assert torch.equal(C.balance_loss(z[rows], k).counts.cpu(), C.balance_loss(z[rows].cpu(), k).counts)
+
+
 @pytest.mark.parametrize("rows,experts,k,dtype", [(40000, 16, 1, torch.float32), (9000, 64, 8, torch.bfloat16), (20011, 5, 2, torch.float32)])
 def test_balance_of_many_rows(rows, experts, k, dtype):
     z = scores(rows, experts, dtype, 8)
