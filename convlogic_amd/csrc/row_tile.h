@@ -35,7 +35,8 @@ __device__ __forceinline__ A finite_or_zero(A m)
 
 // Exponentials of z / temperature relative to that of a value m.  Floats: 2^(scale z - at) in one multiply-add and the instruction for 2^x, with
 // scale = log2(e) / temperature and at = scale m as it is rounded; residue() is what that rounding moved, in 64 bits, for the few values that are not such
-// sums.  Beyond +-1e30 scale z would overflow, and two values that differ do so by more than any temperature reaches: there scale is 1.
+// sums.  It is at most 64 (a factor of 2^64 in every exponential of a row) while |at| < 2^31.  From there on another value than m is at least 2^-24 |m| away,
+// its exponential at most 2^-128 of m's: nothing next to it, whatever the scale, which is then the power of two that puts `at` between 2^31 and 2^32, exactly.
 template <typename A>
 struct Exps;
 template <>
@@ -46,14 +47,16 @@ struct Exps<float> {
     {
 #pragma clang fp contract(off)                                        // (`at` is the rounded product in all that is computed of it)
         m = finite_or_zero(m);
-        scale = __builtin_fabsf(m) > 1e30f ? 1.f : unit_;
+        const float whole = m * unit_;
+        const uint32_t power = (uint32_t)(127 + 31 + 127) << 23;          // (2^31 over the power of two in m)
+        scale = __builtin_fabsf(whole) < 0x1p31f ? unit_ : __builtin_bit_cast(float, power - (__builtin_bit_cast(uint32_t, m) & 0x7F800000u));
         at = m * scale;
     }
     __device__ __forceinline__ float operator()(float z) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(z, scale, -at)); }
     // the factor that makes a sum relative to this one of one relative to `to`, which is of a value no lower
-    __device__ __forceinline__ float factor(const Exps &to) const { return __builtin_amdgcn_exp2f(at - to.at); }
+    __device__ __forceinline__ float factor(const Exps &to) const { return scale == to.scale ? __builtin_amdgcn_exp2f(at - to.at) : 0.f; }
     // natural logarithm of the sum 1 relative to m
-    __device__ __forceinline__ double residue(float m) const { return scale == 1.f ? 0.0 : ((double)at - (double)finite_or_zero(m) * (double)scale) * 0.69314718055994530942; }
+    __device__ __forceinline__ double residue(float m) const { return ((double)at - (double)finite_or_zero(m) * (double)scale) * 0.69314718055994530942; }
 };
 template <>
 struct Exps<double> {

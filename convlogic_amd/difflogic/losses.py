@@ -136,7 +136,9 @@ def _distillation_plain(logits, values, indices, logsumexp, temperature, mask, w
     if mask is not None:
         keep = keep & mask
     # rows that do not count are rows of zeros from here on: no inf or NaN of theirs reaches a gradient
-    x = torch.where(keep.unsqueeze(-1), _wide(logits), 0.0).double() / temperature
+    x = torch.where(keep.unsqueeze(-1), _wide(logits), 0.0).double()
+    highest = x.detach().amax(-1, keepdim=True)                       # (subtracted first: x / temperature would be rounded in steps of its own size)
+    x = (x - torch.where(highest.isinf(), 0.0, highest)) / temperature
     x = x * torch.where(keep & bad, math.nan, 1.0).unsqueeze(-1)
     at = torch.where(there, indices, 0).long()
     t = torch.where(there, values.double() / temperature, -math.inf)

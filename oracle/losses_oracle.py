@@ -32,9 +32,8 @@ def distillation(z, values, columns, lse=None, temperature=1.0, mask=None, weigh
         if (cs >= cols).any():
             losses[r], grad[r] = np.nan, np.nan
             continue
-        u = z[r] / temperature
         with np.errstate(all="ignore"):
-            log_q = u - u.max()
+            log_q = (z[r] - z[r].max()) / temperature                 # (z / temperature first is off by half a step of itself: 2^-9 at 3e13)
             log_q = log_q - np.log(np.exp(log_q).sum())
         entries = [(values[r, j] / temperature, cs[j]) for j in range(len(cs)) if cs[j] >= 0]
         t = np.array([e[0] for e in entries])

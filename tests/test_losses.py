@@ -231,3 +231,17 @@ def refused_by_the_c_entry_points():
         args[at] = value
         assert lib.clg_balance_backward(*args) == -1 and b"clg_balance_backward" in lib.clg_last_error(), (at, value)
     assert lib.clg_balance_scratch_bytes(0, 0) == 0 and lib.clg_balance_scratch_bytes(0, 16) > 0 and lib.clg_distill_scratch_bytes(-1) == 0
+
+
+def test_distillation_of_close_logits_at_a_low_temperature():
+    # logits of 30 that differ in their last bits, over 1e-12: their differences count, not what is left of 3e13.  Probabilities in 50 digits
+    from decimal import Decimal, localcontext
+    z = 30.0 - 2.0 ** -48 * torch.tensor([[4.0, 1.0, 0.0, 7.0, 3.0]], dtype=torch.float64)
+    with localcontext() as context:
+        context.prec = 50
+        e = [(Decimal(float(x)) / Decimal(1e-12) - Decimal(30.0) / Decimal(1e-12)).exp() for x in z[0]]
+        want = [float(x / sum(e)) for x in e]
+    leaf = z.requires_grad_(True)
+    C.distillation_loss(leaf, torch.zeros(1, 1), torch.tensor([[2]]), temperature=1e-12, weight=1e12, reduction="sum").backward()
+    want[2] -= 1.0
+    assert np.abs(leaf.grad[0].numpy() - np.array(want)).max() <= 16 * 2.0 ** -53
