@@ -314,7 +314,7 @@ void launch_rows(const DistillArgs &a, hipStream_t stream)
     // ones are done sooner by 64 lanes each.  Float32 with gradient, 64 and 16 lanes: 8192 rows of 100 columns 21 and 13 us (2048: 13 and 12, 512: 11 and
     // 11), 32768 of 500 62 and 44 (8192: 24 and 19, 2048: 13 and 15); entries beyond 32 take a lane as long as its part of 1000 columns (k = 64: 87 and 100).
     const char *lanes = clg_knob(K_DISTILL_LANES);
-    const bool few = lanes ? atoi(lanes) == 16 : pieces <= 16 ? a.k <= 64 : pieces <= 64 ? a.k <= 64 && a.rows >= 2048 : a.k <= 32 && a.rows >= 8192;
+    const bool few = a.k <= 64 && (lanes ? atoi(lanes) == 16 : pieces <= 16 || (pieces <= 64 ? a.rows >= 2048 : a.k <= 32 && a.rows >= 8192));
     if (few && pieces <= 16) return launch_as<T, 64, 16, 1, false, STREAM>(a, stream);
     if (few && pieces <= 16 * 4) return launch_as<T, 64, 16, 4, false, STREAM>(a, stream);
     if (few && pieces <= 16 * 16) return launch_as<T, 64, 16, 16, false, STREAM>(a, stream);
