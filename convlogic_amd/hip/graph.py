@@ -20,6 +20,9 @@ class GraphedStep:
     are overwritten by every call.  Shapes, dtypes, training/eval mode, wiring buffers and environment knobs are
     those of the recording.  ``input_grads=True`` also keeps the gradients of floating-point inputs
     (``step.input_grads``).
+
+    Record while no eager autograd graph of the same parameters is alive: drop a loss that was not taken back to them, with whatever else holds its
+    graph, first.  Its accumulation nodes belong to the stream it was made on, and a recorded backward pass cannot run there.
     """
 
     def __init__(self, loss_fn, example_inputs, parameters, warmup=3, input_grads=False):
