@@ -4,8 +4,9 @@
 // logsumexp L over all columns, p_j = exp(t_j / tau - L), and p_r = 1 - sum p_j for everything else):
 //     loss = tau^2 [ sum_j p_j (log p_j - log q_{c_j}) + p_r (log p_r - log q_r) ],        q_r = sum of q over the columns that are not listed
 //     d loss / d z_v = tau [ M q_v - sum_{j: c_j = v} p_j ]  listed,    tau q_v [ M - p_r / q_r ]  not listed,        M = sum_j p_j + p_r
-// q_r is small where the student agrees with its teacher, so it is no difference of sums: listed columns leave the row first (a bit per column in
-// LDS), their few exponentials are added to the sum of the others afterwards.
+// q_r may be small, so it is no difference of sums: listed columns leave the row first (a bit per column in LDS), their few exponentials are added to the
+// sum of the others afterwards.  Where the student agrees with its teacher the loss is a small difference of its terms: those exponentials and what takes the
+// others' sum to the row's highest are 64-bit numbers, and a relative error d of that sum, in 32 bits, moves the loss by tau^2 (M q_r - p_r) d only.
 #include <stdlib.h>
 
 #include "row_tile.h"
@@ -31,10 +32,9 @@ struct DistillArgs {
 constexpr int kFlagTwice = 1, kFlagListed = 2, kFlagBad = 4;
 
 // LDS of a team: reduction room (16 wavefronts of 4 doubles, for a workgroup), flags, entries (probability, logit, column), bits of a tile
-template <typename A>
 __host__ __device__ inline int distill_lds(bool workgroup, int k, int cols_of_tile /* whole words of bits */)
 {
-    return ((workgroup ? 16 * 4 * 8 : 0) + 16 + k * (8 + (int)sizeof(A) + 4) + cols_of_tile / 32 * 4 + 15) & ~15;
+    return ((workgroup ? 16 * 4 * 8 : 0) + 16 + k * (8 + 8 + 4) + cols_of_tile / 32 * 4 + 15) & ~15;
 }
 
 // whether entry j is the first of its column, and with all the others' probabilities on it
@@ -66,9 +66,8 @@ __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
     static_assert(TEAMS == 1 || THREADS == kWave, "teams share a wavefront, where LDS is in order");
     extern __shared__ char lds[];
     const int tid = Mine::kWhole ? threadIdx.x : threadIdx.x % LANES, team = Mine::kWhole ? 0 : threadIdx.x / LANES, k = a.k;
-    double *room = reinterpret_cast<double *>(lds + team * distill_lds<A>(Mine::kWhole, k, Tile::COLS)), *prob = room + ROOM + 2;
+    double *room = reinterpret_cast<double *>(lds + team * distill_lds(Mine::kWhole, k, Tile::COLS)), *prob = room + ROOM + 2, *logit = prob + k;
     int *flags = reinterpret_cast<int *>(room + ROOM);
-    A *logit = reinterpret_cast<A *>(prob + k);
     int *column = reinterpret_cast<int *>(logit + k);
     uint32_t *bits = reinterpret_cast<uint32_t *>(column + k);
     const A unit = (A)Exps<A>::unit(a.temperature);
@@ -92,7 +91,7 @@ __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
         const double t = value_of_bits(value, a.values_type) * a.inv_tau;
         const A l = (A)logit_j;
         prob[j] = t;
-        logit[j] = l;
+        logit[j] = (double)l;
         tops[0] = max_of(tops[0], (A)t);
         tops[1] = max_of(tops[1], l);
     };
@@ -171,26 +170,29 @@ __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
     tops[2] = m_t;
     Mine::template reduce<false>(tops, reinterpret_cast<A *>(room));
     const A m_u = tops[2], m = max_of(tops[1], m_u);
-    const Exps<A> of_rest(m_u, unit), of_all(m, unit);
+    const Exps<A> of_rest(m_u, unit);
     __syncthreads();
 
-    // sums: the others' exponentials relative to m_u, the listed ones' relative to m; in 64 bits the teacher's, of which small differences are taken, and
-    // its share times the difference of the logarithms
-    A sums[2] = {rescaled(s_t, m_t, Exps<A>(m_t, unit), of_rest), 0};
-    double parts[2] = {0, 0};
+    // sums: the others' exponentials relative to m_u; in 64 bits the teacher's, its share times the difference of the logarithms, and the student's listed
+    // exponentials relative to m
+    A sums[1] = {rescaled(s_t, m_t, Exps<A>(m_t, unit), of_rest)};
+    double parts[3] = {0, 0, 0};
     const double base_t = a.lse ? value_of_bits(lse_bits, a.lse_type) : (double)finite_or_zero(tops[0]);
 #pragma unroll 1
     for (int j = tid; j < k; j += LANES) {
         if (column[j] < 0) continue;
-        const A l = logit[j];
-        if (!(flag & kFlagTwice) || first_of(column, j)) sums[1] += of_all(l);
-        const double u = ((double)l - (double)m) * a.inv_tau, t = prob[j] - base_t, e = exp(t);
+        const double l = logit[j], u = (l - (double)m) * a.inv_tau, t = prob[j] - base_t, e = exp(t), q = l == lowest(0.0) ? 0 : exp(u);
+        if (!(flag & kFlagTwice) || first_of(column, j)) parts[2] += q;
         parts[0] += e;
         if (e != 0) parts[1] += e * (t - u);
         prob[j] = e;
+        logit[j] = q;
     }
-    Mine::sums(sums, parts, reinterpret_cast<A *>(room), room + 32);
-    const double s_u = sums[0], mass_p = parts[0], total = (m_u == lowest(A(0)) ? s_u : s_u * (double)of_rest.factor(of_all)) + (double)sums[1];
+    // what makes an exponential of the others, as it is summed, one relative to m: by the first wavefront, beside the entries
+    const double log_of_u = ((double)m_u - (double)m) * a.inv_tau + of_rest.residue(m_u);
+    if (!Mine::kWhole || tid < kWave) room[ROOM + 1] = m_u == lowest(A(0)) ? 1 : exp(log_of_u);
+    Mine::sums(sums, parts, reinterpret_cast<A *>(room), room + 16, uniform(tid & ~63) < k);
+    const double s_u = sums[0], mass_p = parts[0], of_u = room[ROOM + 1], total = s_u * of_u + parts[2];
     bool all_listed = false;                                          // (then there is nothing else)
     if (a.lse && k >= a.cols) {
         A n[1] = {0};
@@ -205,18 +207,18 @@ __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
     // four logarithms and three inverses at once, one in a lane
     const int lane = tid & 63;
     const double value = lane == 0 ? total : lane == 1 ? s_u : lane == 2 ? rest : mass_p, logs = log(value), inverses = quick_inverse(value);
-    const double log_total = Mine::from(logs, 0) + of_all.residue(m);
+    const double log_total = Mine::from(logs, 0);
     double mass, loss, per = 1;                                       // per: of an entry's exponential
     if (a.lse) {
         mass = mass_p + rest;
         loss = parts[1] + mass_p * log_total;
-        if (rest != 0) loss += rest * (Mine::from(logs, 2) - (((double)m_u - (double)m) * a.inv_tau + Mine::from(logs, 1) + of_rest.residue(m_u) - log_total));
+        if (rest != 0) loss += rest * (Mine::from(logs, 2) - (log_of_u + Mine::from(logs, 1) - log_total));
     } else {
         per = mass_p == 0 ? 0 : Mine::from(inverses, 3);
         mass = mass_p * per;
         loss = mass_p == 0 ? 0 : parts[1] * per + log_total - Mine::from(logs, 3);
     }
-    if ((flag & kFlagBad) || total > 1e300) loss = mass = __builtin_nan("");             // (a logit of +inf)
+    if ((flag & kFlagBad) || m == -lowest(A(0))) loss = mass = __builtin_nan("");        // (a logit of +inf)
     const double factor = a.per_count ? *a.per_count : 1;
     if (tid == 0) {
         if (a.row_loss) a.row_loss[row] = loss * a.loss_scale;
@@ -227,7 +229,7 @@ __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
     const double g = a.grad_scale * factor * (double)up, of_listed = mass * Mine::from(inverses, 0);
     const A others = s_u == 0 && total > 0 && mass == mass
                          ? A(0)
-                         : (A)(g * (of_listed * (double)of_rest.factor(of_all) - (rest == 0 ? 0 : rest * Mine::from(inverses, 1))));
+                         : (A)(g * (of_listed * of_u - (rest == 0 ? 0 : rest * Mine::from(inverses, 1))));
     const auto of = [&](A x) { return of_rest(x) * others; };
     if (MULTI) {
         for (int64_t base = 0; base < a.cols; base += Tile::COLS) {
@@ -246,7 +248,7 @@ __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
             if (!first_of(column, j)) continue;
             p = all_of(column, prob, j, k);
         }
-        grad[column[j]] = (T)(A)(g * (of_listed * (double)of_all(logit[j]) - p * per));
+        grad[column[j]] = (T)(A)(g * (of_listed * logit[j] - p * per));
     }
 }
 
@@ -300,7 +302,7 @@ void launch_as(const DistillArgs &a, hipStream_t stream)
     typedef RowTile<T, LANES, NV, STREAM> Tile;
     static_assert(Tile::COLS % 32 == 0, "bits of a tile fill whole words");
     constexpr int TEAMS = THREADS / LANES;
-    const size_t lds = (size_t)TEAMS * distill_lds<typename Wide<T>::type>(TEAMS == 1, a.k, Tile::COLS);
+    const size_t lds = (size_t)TEAMS * distill_lds(TEAMS == 1, a.k, Tile::COLS);
     DistillArgs part = a;
     constexpr int64_t kMost = (int64_t)1 << 31;                       // threads of a launch
     for (; part.first_row < a.rows; part.first_row += kMost / LANES) {

@@ -246,14 +246,15 @@ __device__ __forceinline__ void block_reduce(A (&x)[COUNT], A *room)
     }
 }
 
-// The same for sums of two types at once.
+// The same for sums of two types at once; `some`, of a wavefront: whether its y are other than 0.
 template <int THREADS, int CA, int CB, typename A, typename B>
-__device__ __forceinline__ void block_sums(A (&x)[CA], B (&y)[CB], A *room_x, B *room_y)
+__device__ __forceinline__ void block_sums(A (&x)[CA], B (&y)[CB], A *room_x, B *room_y, bool some)
 {
 #pragma unroll
     for (int c = 0; c < CA; ++c) x[c] = wave_sum(x[c]);
+    if (some)
 #pragma unroll
-    for (int c = 0; c < CB; ++c) y[c] = wave_sum(y[c]);
+        for (int c = 0; c < CB; ++c) y[c] = wave_sum(y[c]);
     if constexpr (THREADS > kWave) {
         constexpr int WAVES = THREADS / kWave;
         if ((threadIdx.x & 63) == 0) {
@@ -287,10 +288,10 @@ struct Team {
         }
     }
     template <int CA, int CB, typename A>
-    __device__ __forceinline__ static void sums(A (&x)[CA], double (&y)[CB], A *room_x, double *room_y)
+    __device__ __forceinline__ static void sums(A (&x)[CA], double (&y)[CB], A *room_x, double *room_y, bool some)
     {
         if constexpr (kWhole) {
-            block_sums<THREADS>(x, y, room_x, room_y);
+            block_sums<THREADS>(x, y, room_x, room_y, some);
         } else {
             reduce<true>(x, room_x);
             reduce<true>(y, room_y);

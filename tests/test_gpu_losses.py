@@ -648,3 +648,70 @@ def test_calls_on_another_stream_and_refusals_on_the_gpu():
             call()
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(lambda a: C.top_logits(a, 2).values, z.detach()[:3, :5])
+
+
+# ---- students that are close to their teacher ----------------------------------------------------
+def check_close_student(z, values, columns, lse, temperature):
+    """Loss and gradient of each row within what 32 bits in the sum over the columns that are not listed can do, and nothing else.
+
+    That sum s has a relative error d of at most eps = (2 X + 4 + A) 2^-24: X, the mean of |x| = log2(e) (max - z) / temperature over the columns in it, weighted
+    with their shares (two roundings of x, of |x| 2^-24 each), 2 steps of the exponential itself, A additions in a row of half a step each: a thread's elements, 11
+    to join up to 1024 threads, one for each tile of a row in tiles.  Everything else of a row is in 64 bits, where the terms that cancel are off by 2^-44 of their
+    size.  With q_r the share of those columns, p_r the teacher's and M its whole mass:
+        loss = T^2 (... + M log(total) - p_r log(s)):  off by T^2 |M q_r - p_r| d, and d^2 of T^2 M q_r
+        gradient, listed: T (M q - p), off by T M q q_r d;  others: T q_v / q_r (M q_r - p_r), where M q_r is off by itself times d, the rest by d and
+        the error of its own exponential, (2 |x| + 4) 2^-24, and by two products in 32 bits
+    and results are rounded once to their type."""
+    leaf = z.detach().requires_grad_(True)
+    loss = C.distillation_loss(z, values, columns, lse, temperature=temperature, reduction="none")
+    grad, = torch.autograd.grad(C.distillation_loss(leaf, values, columns, lse, temperature=temperature, reduction="sum"), leaf)
+    args = (host(values), columns.cpu().numpy(), None if lse is None else host(lse), temperature, None, 1.0)
+    want_loss, want_grad, size, _ = L.distillation(host(z), *args, "none")
+    unit = 2.0 ** -53 if z.dtype == torch.float64 else 2.0 ** -24
+    for r, row in enumerate(host(z)):
+        listed = np.zeros(len(row), bool)
+        listed[columns[r].cpu().numpy()] = True
+        x = np.where(listed, -INF, (row - row[~listed].max()) / temperature * math.log2(math.e))
+        share = np.exp2(x) / np.exp2(x).sum()
+        q = np.exp((row - row.max()) / temperature)
+        q /= q.sum()
+        q_r = q[~listed].sum()
+        t = host(values)[r] / temperature
+        p = np.exp(t - host(lse)[r]) if lse is not None else np.exp(t - t.max()) / np.exp(t - t.max()).sum()
+        p_r = max(0.0, 1 - p.sum()) if lse is not None else 0.0
+        mass = p.sum() + p_r
+        x = np.where(listed, 0.0, -x)
+        eps = (2 * (share * x).sum() + 4 + min(129, len(row) // 16 + 16) + 11 + len(row) // 16384) * unit
+        bound = temperature ** 2 * (abs(mass * q_r - p_r) * eps + mass * q_r * eps ** 2) + 2.0 ** -44 * size[r]
+        half = torch.finfo(loss.dtype).eps / 2
+        off = abs(float(loss[r]) - want_loss[r])
+        assert off <= bound + half * abs(want_loss[r]) * (1 + 2.0 ** -10), ("loss", r, off, bound, want_loss[r])
+        own = np.where(listed, mass * q * q_r * eps, share * (abs(mass * q_r - p_r) * (eps + (2 * x + 6) * unit) + mass * q_r * eps))
+        half, least = torch.finfo(grad.dtype).eps / 2, torch.finfo(torch.float32).smallest_normal + torch.finfo(grad.dtype).smallest_normal * torch.finfo(grad.dtype).eps
+        bound = temperature * (own + 2.0 ** -44 * (mass * q + listed)) + half * np.abs(want_grad[r]) * (1 + 2.0 ** -10) + unit * np.abs(want_grad[r]) + least
+        off = np.abs(host(grad)[r] - want_grad[r])
+        assert (off <= bound).all(), ("grad", r, (off / bound).max(), np.argmax(off / bound))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("noise", [1e-2, 1e-1])
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("cols", [10, 100, 1000, 5000, 40000, 140000])
+def test_distillation_of_a_student_close_to_its_teacher(dtype, noise, rest, cols):
+    for rows in (1, 4):
+        for k in (1, 2, 8):
+            for temperature in (1.0, 4.0):
+                z = scores(rows, cols, dtype, cols + k)
+                own = z.float() + noise * scores(rows, cols, torch.float32, k, 1.0)
+                t = C.top_logits(own, k, temperature=temperature)
+                check_close_student(z, t.values, t.indices, t.logsumexp if rest else None, temperature)
+
+
+@pytest.mark.parametrize("lanes", [16, 64])
+def test_distillation_of_close_students_that_share_a_wavefront(monkeypatch, lanes):
+    set_knobs(monkeypatch, CLG_DISTILL_LANES=lanes)
+    for cols in (17, 100, 250, 1000):
+        z = scores(9, cols, torch.float32, cols)
+        t = C.top_logits(z + 0.01 * scores(9, cols, torch.float32, 1, 1.0), 4, temperature=4.0)
+        check_close_student(z, *t, 4.0)
+        check_close_student(z, t.values, t.indices, None, 4.0)
