@@ -83,17 +83,18 @@ __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
     // on to the row.  What this thread's first entry loads is taken up after the row is on its way.
     if (tid == 0) *flags = 0;
     __syncthreads();
-    A tops[3] = {lowest(A(0)), lowest(A(0)), lowest(A(0))};           // highest of the teacher, of the student's listed logits, of the others
+    A tops[2] = {lowest(A(0)), lowest(A(0))};                         // highest of the student's listed logits, of the others
+    double top_t[1] = {lowest(0.0)};                                  // of the teacher's values
     T first_logit = (T)0.f;
     uint64_t first_value = 0, lse_bits = 0;
     bool first_there = false;
     const auto enter = [&](int j, T logit_j, uint64_t value) {
-        const double t = value_of_bits(value, a.values_type) * a.inv_tau;
+        const double v = value_of_bits(value, a.values_type);
         const A l = (A)logit_j;
-        prob[j] = t;
+        prob[j] = v;
         logit[j] = (double)l;
-        tops[0] = max_of(tops[0], (A)t);
-        tops[1] = max_of(tops[1], l);
+        top_t[0] = max_of(top_t[0], v);
+        tops[0] = max_of(tops[0], l);
     };
     if (kept) {
         int seen = 0;
@@ -167,9 +168,11 @@ __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
         }
         return;
     }
-    tops[2] = m_t;
+    tops[1] = m_t;
     Mine::template reduce<false>(tops, reinterpret_cast<A *>(room));
-    const A m_u = tops[2], m = max_of(tops[1], m_u);
+    // (the teacher's highest is exact: relative to one that was rounded, or rounded over the temperature, its exponentials may all be 0, or infinite)
+    if (!a.lse) Mine::template reduce<false>(top_t, room + 32);
+    const A m_u = tops[1], m = max_of(tops[0], m_u);
     const Exps<A> of_rest(m_u, unit);
     __syncthreads();
 
@@ -177,11 +180,11 @@ __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
     // exponentials relative to m
     A sums[1] = {rescaled(s_t, m_t, Exps<A>(m_t, unit), of_rest)};
     double parts[3] = {0, 0, 0};
-    const double base_t = a.lse ? value_of_bits(lse_bits, a.lse_type) : (double)finite_or_zero(tops[0]);
+    const double lse = a.lse ? value_of_bits(lse_bits, a.lse_type) : 0, base_t = a.lse ? 0 : finite_or_zero(top_t[0]);
 #pragma unroll 1
     for (int j = tid; j < k; j += LANES) {
         if (column[j] < 0) continue;
-        const double l = logit[j], u = (l - (double)m) * a.inv_tau, t = prob[j] - base_t, e = exp(t), q = l == lowest(0.0) ? 0 : exp(u);
+        const double l = logit[j], u = (l - (double)m) * a.inv_tau, t = (prob[j] - base_t) * a.inv_tau - lse, e = exp(t), q = l == lowest(0.0) ? 0 : exp(u);
         if (!(flag & kFlagTwice) || first_of(column, j)) parts[2] += q;
         parts[0] += e;
         if (e != 0) parts[1] += e * (t - u);

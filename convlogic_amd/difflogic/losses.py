@@ -141,14 +141,14 @@ def _distillation_plain(logits, values, indices, logsumexp, temperature, mask, w
     x = (x - torch.where(highest.isinf(), 0.0, highest)) / temperature
     x = x * torch.where(keep & bad, math.nan, 1.0).unsqueeze(-1)
     at = torch.where(there, indices, 0).long()
-    t = torch.where(there, values.double() / temperature, -math.inf)
+    t = torch.where(there, values.double(), -math.inf)
     if logsumexp is None:
         highest = t.amax(-1, keepdim=True)
-        highest = torch.where(highest.isinf(), 0.0, highest)
-        total = (t - highest).exp().sum(-1, keepdim=True)
-        log_p = t - highest - torch.where(total == 0, 0.0, total.log())
+        t = (t - torch.where(highest.isinf(), 0.0, highest)) / temperature
+        total = t.exp().sum(-1, keepdim=True)
+        log_p = t - torch.where(total == 0, 0.0, total.log())
     else:
-        log_p = t - logsumexp.double().unsqueeze(-1)
+        log_p = t / temperature - logsumexp.double().unsqueeze(-1)
     p = log_p.exp()
     log_q = torch.log_softmax(x, -1)
     used = there & (p != 0)

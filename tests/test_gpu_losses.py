@@ -715,3 +715,42 @@ def test_distillation_of_close_students_that_share_a_wavefront(monkeypatch, lane
         t = C.top_logits(z + 0.01 * scores(9, cols, torch.float32, 1, 1.0), 4, temperature=4.0)
         check_close_student(z, *t, 4.0)
         check_close_student(z, t.values, t.indices, None, 4.0)
+
+
+def far_values(kind, rows, k, low, high):
+    # the two highest equal, one far below, the others in between or far below too
+    v = torch.full((rows, k), low, dtype=kind)
+    v[:, :2] = high
+    return v.to(DEV)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [10, 600, 9000, 140000])
+@pytest.mark.parametrize("kind,high,low,temperature", [
+    (torch.float32, 3.3e30, -3.3e30, 1.5), (torch.float32, -1e30, -3.3e30, 1.5), (torch.float32, 1e30, 9e29, 1.5), (torch.float32, -3.4028234663852886e38, -INF, 0.9),
+    (torch.float32, 3.4028234663852886e38, -3.4028234663852886e38, 0.9), (torch.float32, 30.0, 29.9, 1e-10), (torch.float32, -7.3, -7.4, 1e-10),
+    (torch.bfloat16, 3.3895313892515355e38, 1.0, 0.9), (torch.float16, 65504.0, -65504.0, 1e-7), (torch.float64, 1e300, -1e300, 0.9), (torch.float64, -1e100, -1.1e100, 1.5)])
+def test_distillation_from_values_far_beyond_what_an_exponential_takes(dtype, cols, kind, high, low, temperature):
+    # (differences of the values over the temperature are 0 or beyond 1000, so that each has its probability, 1/2 or 0)
+    z = scores(3, cols, dtype, 5)
+    columns = torch.arange(4, device=DEV).repeat(3, 1)
+    values = far_values(kind, 3, 4, low, high)
+    columns[2, 1] = -1                                                # (one of the two alone)
+    loss, _ = check_distill(z, values, columns, None, temperature, weight=max(1.0, 1.0 / temperature), reduction="none", upstream=torch.ones(3, device=DEV, dtype=C.distillation_loss(z, values, columns).dtype))
+    assert loss.isfinite().all() and (loss[:2] != 0).all()            # (the last is 0 where an all but certain student has the one answer of its teacher)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [10, 600, 9000])
+def test_distillation_from_close_values_at_a_low_temperature(dtype, cols):
+    # float64 values of 30 that differ in their last bits, over 1e-12; an undecided student.  The teacher's probabilities in 50 digits
+    from decimal import Decimal, localcontext
+    values = 30.0 - 2.0 ** -48 * torch.tensor([[4.0, 1.0, 0.0, 7.0, 3.0]], dtype=torch.float64)
+    with localcontext() as context:
+        context.prec = 50
+        e = [((Decimal(float(v)) - 30) / Decimal(1e-12)).exp() for v in values[0]]
+        p = [x / sum(e) for x in e]
+        want = float(sum(x * x.ln() for x in p) + Decimal(cols).ln())
+    loss = C.distillation_loss(torch.zeros(1, cols, dtype=dtype, device=DEV), values.to(DEV), torch.arange(5, device=DEV)[None], temperature=1e-12, weight=1e24, reduction="sum")
+    # (equal logits: their exponentials are 1 and sums of them whole numbers; the rest is in 64 bits, and T^2 weight is 1 but for 3 roundings)
+    assert abs(float(loss) - want) <= torch.finfo(loss.dtype).eps / 2 * want + 2.0 ** -46 * (want + 10)

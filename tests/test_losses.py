@@ -245,3 +245,16 @@ def test_distillation_of_close_logits_at_a_low_temperature():
     C.distillation_loss(leaf, torch.zeros(1, 1), torch.tensor([[2]]), temperature=1e-12, weight=1e12, reduction="sum").backward()
     want[2] -= 1.0
     assert np.abs(leaf.grad[0].numpy() - np.array(want)).max() <= 16 * 2.0 ** -53
+
+
+def test_distillation_from_close_values_at_a_low_temperature():
+    # float64 values of 30 that differ in their last bits, over 1e-12: their differences count.  The teacher's probabilities in 50 digits, an undecided student
+    from decimal import Decimal, localcontext
+    values = 30.0 - 2.0 ** -48 * torch.tensor([[4.0, 1.0, 0.0, 7.0, 3.0]], dtype=torch.float64)
+    with localcontext() as context:
+        context.prec = 50
+        e = [((Decimal(float(v)) - 30) / Decimal(1e-12)).exp() for v in values[0]]
+        p = [x / sum(e) for x in e]
+        want = float(sum(x * x.ln() for x in p) + Decimal(10).ln())
+    loss = C.distillation_loss(torch.zeros(1, 10, dtype=torch.float64), values, torch.arange(5)[None], temperature=1e-12, weight=1e24, reduction="sum")
+    assert abs(float(loss) - want) <= 2.0 ** -46 * (want + 10)
