@@ -154,7 +154,7 @@ def _distillation_plain(logits, values, indices, logsumexp, temperature, mask, w
     used = there & (p != 0)
     loss = torch.where(used, p * (torch.where(used, log_p, 0.0) - torch.where(used, log_q.gather(-1, at), 0.0)), 0.0).sum(-1)
     if logsumexp is not None:
-        listed = torch.zeros(x.shape, dtype=torch.uint8).scatter_add_(-1, at, there.to(torch.uint8)) > 0
+        listed = torch.zeros(x.shape, dtype=torch.int32).scatter_add_(-1, at, there.to(torch.int32)) > 0
         rest = (1.0 - p.sum(-1)).clamp(min=0.0)
         rest = torch.where(listed.all(-1) | ~keep, 0.0, rest)
         log_rest = torch.logsumexp(log_q.masked_fill(listed, -math.inf), -1)

@@ -258,3 +258,16 @@ def test_distillation_from_close_values_at_a_low_temperature():
         want = float(sum(x * x.ln() for x in p) + Decimal(10).ln())
     loss = C.distillation_loss(torch.zeros(1, 10, dtype=torch.float64), values, torch.arange(5)[None], temperature=1e-12, weight=1e24, reduction="sum")
     assert abs(float(loss) - want) <= 2.0 ** -46 * (want + 10)
+
+
+@pytest.mark.parametrize("times", [255, 256, 257, 512, 1024])
+def test_distillation_of_a_column_listed_many_times(times):
+    z = scores(2, 3, torch.float64, 2).requires_grad_(True)
+    columns = torch.full((2, times), 1)
+    columns[1, -1] = 2
+    values, lse = torch.full((2, times), -8.0, dtype=torch.float64), torch.zeros(2, dtype=torch.float64)
+    loss = C.distillation_loss(z, values, columns, lse)
+    grad, = torch.autograd.grad(loss, z)
+    want = L.distillation(z.detach().numpy(), values.numpy(), columns.numpy(), lse.numpy())
+    close(loss, want[0], want[2], "loss")
+    close(grad, want[1], want[3], "grad")
