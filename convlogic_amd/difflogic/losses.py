@@ -157,7 +157,10 @@ def _distillation_plain(logits, values, indices, logsumexp, temperature, mask, w
         listed = torch.zeros(x.shape, dtype=torch.int32).scatter_add_(-1, at, there.to(torch.int32)) > 0
         rest = (1.0 - p.sum(-1)).clamp(min=0.0)
         rest = torch.where(listed.all(-1) | ~keep, 0.0, rest)
-        log_rest = torch.logsumexp(log_q.masked_fill(listed, -math.inf), -1)
+        # (nothing beside the listed columns: a constant -inf less the logarithm of the whole, which keeps its gradient)
+        others = x.masked_fill(listed, -math.inf)
+        none = (others == -math.inf).all(-1)
+        log_rest = torch.where(none, -math.inf, torch.logsumexp(torch.where(none.unsqueeze(-1), 0.0, others), -1)) - torch.logsumexp(x, -1)
         some = rest != 0
         loss = loss + torch.where(some, torch.special.xlogy(rest, rest) - rest * torch.where(some, log_rest, 0.0), 0.0)
     loss = torch.where(keep, loss, 0.0)

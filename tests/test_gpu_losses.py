@@ -754,3 +754,20 @@ def test_distillation_from_close_values_at_a_low_temperature(dtype, cols):
     loss = C.distillation_loss(torch.zeros(1, cols, dtype=dtype, device=DEV), values.to(DEV), torch.arange(5, device=DEV)[None], temperature=1e-12, weight=1e24, reduction="sum")
     # (equal logits: their exponentials are 1 and sums of them whole numbers; the rest is in 64 bits, and T^2 weight is 1 but for 3 roundings)
     assert abs(float(loss) - want) <= torch.finfo(loss.dtype).eps / 2 * want + 2.0 ** -46 * (want + 10)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [10, 600, 9000, 140000])
+def test_distillation_of_a_student_with_nothing_beside_the_listed_columns(dtype, cols):
+    # the teacher has mass elsewhere: the loss is inf, the gradient is that of the listed columns
+    values, columns, lse = teacher(3, cols, 5, True, 1, 1.0)
+    z = torch.full((3, cols), -INF, dtype=dtype, device=DEV)
+    z.scatter_(1, columns, scores(3, 5, dtype, 2))
+    z[2] = scores(1, cols, dtype, 3)[0]
+    leaf = z.requires_grad_(True)
+    loss = C.distillation_loss(leaf, values, columns, lse, reduction="none")
+    grad, = torch.autograd.grad(loss, leaf, torch.ones_like(loss))
+    want = L.distillation(host(z), host(values), columns.cpu().numpy(), host(lse), reduction="none")
+    assert loss.tolist()[:2] == [INF, INF] and want[0].tolist()[:2] == [INF, INF]
+    close(loss[2], want[0][2], want[2][2], z, "loss")
+    close(grad, want[1], want[3], z, "grad")

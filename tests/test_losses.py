@@ -271,3 +271,19 @@ def test_distillation_of_a_column_listed_many_times(times):
     want = L.distillation(z.detach().numpy(), values.numpy(), columns.numpy(), lse.numpy())
     close(loss, want[0], want[2], "loss")
     close(grad, want[1], want[3], "grad")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16])
+def test_distillation_of_a_student_with_nothing_beside_the_listed_columns(dtype):
+    # the teacher has mass elsewhere: the loss is inf, the gradient is that of the listed columns; a row that lists every column; an ordinary one
+    z = scores(4, 4, dtype, 1)
+    z[0, 1:], z[1, 0], z[1, 3] = -INF, -INF, -INF
+    columns = torch.tensor([[0, -1, -1, -1], [2, 1, -1, -1], [3, 0, 1, 2], [1, 2, -1, -1]])
+    values, lse = torch.zeros(4, 4), torch.full((4,), 1.5)
+    leaf = z.requires_grad_(True)
+    loss = C.distillation_loss(leaf, values, columns, lse, reduction="none")
+    grad, = torch.autograd.grad(loss, leaf, torch.ones_like(loss))
+    want = L.distillation(z.detach().double().numpy(), values.numpy(), columns.numpy(), lse.numpy(), reduction="none")
+    assert loss.tolist()[:2] == [INF, INF] and want[0].tolist()[:2] == [INF, INF] and loss[2:].isfinite().all()
+    close(loss[2:], want[0][2:], want[2][2:], "loss")
+    close(grad, want[1], want[3], "grad")
