@@ -24,7 +24,15 @@ void check(int rc)
     TORCH_CHECK(rc == CLG_OK, clg_last_error());
 }
 void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
-bool recording() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
+// the graph that the current stream is recorded into, 0 for none
+int64_t recording()
+{
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return 0;
+    hipStreamCaptureStatus status;
+    unsigned long long id = 0;
+    C10_HIP_CHECK(hipStreamGetCaptureInfo(c10::hip::getCurrentHIPStream().stream(), &status, &id));
+    return (int64_t)id + 1;
+}
 int code_of(const Tensor &t)
 {
     switch (t.scalar_type()) {
@@ -102,7 +110,8 @@ struct DistillCall {
 
 // The forward call leaves the gradient for an upstream gradient of 1, from the same pass over the logits.  The first backward pass hands that
 // tensor on -- the kernel looks at the upstream gradient and computes the rows again where it is another -- and later ones through a retained graph
-// compute one of their own, since the first one's receiver may have changed it.
+// compute one of their own, since the first one's receiver may have changed it.  So does a backward pass of which only one side
+// is recorded, or each into a graph of its own: one can be replayed without the other, and the tensor be written by nobody in between.
 struct Distill : torch::autograd::Function<Distill> {
     static Tensor forward(AutogradContext *ctx, const Tensor &logits, const DistillCall *c)
     {
@@ -143,7 +152,7 @@ struct Distill : torch::autograd::Function<Distill> {
             auto &kept = ctx->saved_data;
             c.temperature = kept.at("temperature").toDouble(), c.weight = kept.at("weight").toDouble(), c.reduction = kept.at("reduction").toInt();
             const auto it = kept.find("grad");
-            if (it != kept.end() && kept.at("recorded").toBool() == recording()) {
+            if (it != kept.end() && kept.at("recorded").toInt() == recording()) {
                 grad = it->second.toTensor();
                 applied = kept.at("applied").toTensor();
                 scratch = kept.at("scratch").toTensor();

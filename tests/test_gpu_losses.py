@@ -771,3 +771,42 @@ def test_distillation_of_a_student_with_nothing_beside_the_listed_columns(dtype,
     assert loss.tolist()[:2] == [INF, INF] and want[0].tolist()[:2] == [INF, INF]
     close(loss[2], want[0][2], want[2][2], z, "loss")
     close(grad, want[1], want[3], z, "grad")
+
+
+def test_a_recorded_backward_pass_replays_without_its_forward_pass():
+    # forward and backward pass in a graph each: the second is replayed again after its gradient was changed by its receiver
+    z = scores(12, 300, torch.float32, 1).requires_grad_(True)
+    t = teacher(12, 300, 5, True, 1, 1.0)
+    want, = torch.autograd.grad(C.distillation_loss(z, *t), z)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    forward, backward = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(forward, stream=stream):
+        loss = C.distillation_loss(z, *t)
+    up = torch.ones_like(loss)
+    with torch.cuda.graph(backward, pool=forward.pool(), stream=stream):
+        grad, = torch.autograd.grad(loss, z, up, retain_graph=True)
+    for i in range(4):
+        if i % 2 == 0:
+            forward.replay()
+        backward.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, want), i
+        with torch.no_grad():
+            grad.mul_(7)                                              # (the receiver's to change)
+        torch.cuda.synchronize()
+
+
+def test_forward_and_backward_passes_in_graphs_of_their_own():
+    # as torch.cuda.make_graphed_callables records them
+    z = scores(12, 300, torch.float32, 1).requires_grad_(True)
+    t = teacher(12, 300, 5, True, 1, 1.0)
+    call = torch.cuda.make_graphed_callables(lambda x: C.distillation_loss(x, *t), (z.detach().clone().requires_grad_(True),))
+    for i in range(3):
+        x = scores(12, 300, torch.float32, 2 + i).requires_grad_(True)
+        for factor in (1.0, 0.5):
+            loss = call(x)
+            got, = torch.autograd.grad(loss * factor, x)
+            want, = torch.autograd.grad(C.distillation_loss(x, *t) * factor, x)
+            torch.cuda.synchronize()
+            assert torch.equal(loss, C.distillation_loss(x, *t)) and torch.equal(got, want)
