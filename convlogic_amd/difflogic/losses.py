@@ -225,6 +225,8 @@ def gate_balance(gates, weight=1.0):
     the layer's logits, with a neuron's most probable gate as its choice, and counts int64 [layers, 16], the neurons whose choice is each gate (what
     a layer evaluates with).  gates: a layer, a network (its LogicLayers, ConvLogicLayers and TreeLogicLayers in the order of modules()), or a
     sequence of logits [..., 16].  Up to 16 layers go in one launch."""
+    if isinstance(gates, torch.Tensor):
+        raise RuntimeError(f"gate_balance takes a module or a sequence of logits, got a tensor of {tuple(gates.shape)}: [logits] for one layer")
     tensors = _gate_logits(gates) if isinstance(gates, torch.nn.Module) else list(gates)
     weight = _check_number(weight, "weight")
     if not tensors:

@@ -287,3 +287,11 @@ def test_distillation_of_a_student_with_nothing_beside_the_listed_columns(dtype)
     assert loss.tolist()[:2] == [INF, INF] and want[0].tolist()[:2] == [INF, INF] and loss[2:].isfinite().all()
     close(loss[2:], want[0][2:], want[2][2:], "loss")
     close(grad, want[1], want[3], "grad")
+
+
+def test_gate_balance_refuses_a_bare_tensor():
+    # (its rows would each be a layer of one neuron)
+    for logits in (torch.zeros(12, 16), torch.nn.Parameter(torch.zeros(3, 7, 16))):
+        with pytest.raises(RuntimeError, match="sequence"):
+            C.gate_balance(logits)
+    assert C.gate_balance([torch.zeros(12, 16)]).counts.tolist() == [[12] + [0] * 15] and C.gate_balance(iter([torch.zeros(12, 16)])).loss == 1
