@@ -810,3 +810,64 @@ def test_forward_and_backward_passes_in_graphs_of_their_own():
             want, = torch.autograd.grad(C.distillation_loss(x, *t) * factor, x)
             torch.cuda.synchronize()
             assert torch.equal(loss, C.distillation_loss(x, *t)) and torch.equal(got, want)
+
+
+def overlapping_rows(rows, cols):
+    # row r is elements r .. r + cols - 1 of one buffer: many rows in little memory
+    base = (torch.arange(rows + cols, device=DEV, dtype=torch.int32) * 7919 % 1009).half()
+    return base.as_strided((rows, cols), (1, 1))
+
+
+@pytest.mark.parametrize("cols,most", [(17, 1 << 25), (2, 1 << 27)])
+def test_top_logits_of_more_rows_than_a_launch_has(cols, most):
+    # 2^31 threads: 2^25 rows of 64 threads, 2^27 of 16
+    rows = most + 70
+    z = overlapping_rows(rows, cols)
+    got = C.top_logits(z, 1)
+    for part in (slice(0, 100), slice(most - 100, most + 70)):
+        want = C.top_logits(z[part].cpu(), 1)
+        assert torch.equal(got.values[part].cpu(), want.values) and torch.equal(got.indices[part].cpu(), want.indices)
+        close(got.logsumexp[part], want.logsumexp.double().numpy(), 1.0 + np.abs(want.logsumexp.double().numpy()) / 128, z[part], "logsumexp")   # (`want` is rounded too)
+
+
+def test_distillation_of_more_rows_than_a_launch_of_64_lanes_has(monkeypatch):
+    set_knobs(monkeypatch, CLG_DISTILL_LANES=64)
+    most = 1 << 25
+    rows = most + 6
+    z = (overlapping_rows(rows, 17) / 128).requires_grad_(True)
+    columns = (torch.arange(rows, device=DEV, dtype=torch.int32) % 17)[:, None]
+    loss = C.distillation_loss(z, torch.zeros(rows, 1, dtype=torch.float16, device=DEV), columns, reduction="none")
+    grad, = torch.autograd.grad(loss, z, torch.ones_like(loss))
+    for part in (slice(0, 20), slice(most - 20, most + 6)):
+        x = z[part].detach()
+        want = L.distillation(host(x), np.zeros((len(x), 1)), columns[part].cpu().numpy(), reduction="none")
+        close(loss[part], want[0], want[2], x, "loss")
+        close(grad[part], want[1], want[3], x, "grad")
+
+
+def test_balance_on_two_streams_at_once():
+    # several workgroups end the sums of each call, the last of them by a ticket that the launch before resets
+    some = [scores(4000, 60, torch.float32, 1), scores(4000, 60, torch.float32, 2)]
+    gates = [[scores(n, 16, torch.float32, n + i) for n in (700, 33, 5000)] for i in range(2)]
+
+    def call(i):
+        leaf = some[i].detach().requires_grad_(True)
+        leaves = [g.detach().requires_grad_(True) for g in gates[i]]
+        loss, counts = C.balance_loss(leaf, 4)
+        even, of_gates = C.gate_balance(leaves)
+        return [loss.detach(), counts, even.detach(), of_gates, *torch.autograd.grad(loss, leaf), *torch.autograd.grad(even, leaves)]
+
+    want = [call(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for one in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(one, want[i]))
