@@ -53,9 +53,10 @@ __device__ __forceinline__ double all_of(const int *column, const double *prob, 
 
 // A team of LANES threads per row: a workgroup, or 16 lanes where there are many short rows.  A row that fits its registers (COLS columns) is read from memory
 // once, for the sum and for the gradient; longer ones (MULTI) tile by tile, twice.
-// 4096 rows of 131072 bfloat16 with gradient: 474 to 504 us, 4.3 to 4.5 TB/s of the 5.1 that a copy reaches; 123 registers of 1024 threads are all that a CU
-// has, so a row's loads, sums and stores follow one another (vector units 62 % of the time).  777 of 50001 float16, 3 rows to a CU and two at a time: 46 us.
-// 10000 of 1000 float32 without gradient, 16 lanes each: 14 us, of instruction issue.
+// 4096 rows of 131072 bfloat16 with gradient: 465 to 508 us, 4.2 to 4.6 TB/s of the 5.1 that a copy reaches; 122 registers of 1024 threads are all that a CU
+// has, so a row's loads, sums and stores follow one another (vector units 60 % of the time).  777 of 50001 float16, 3 rows to a CU and two at a time: 47 us.
+// 10000 of 1000 float32 without gradient, 16 lanes each: 16 us, of latency: 2500 wavefronts are 2.4 to a SIMD, each once through its chain of loads, sums and
+// logarithms; they wait half of their time, the vector units are busy 44 % of it.
 template <typename T, int THREADS, int LANES, int NV, bool MULTI, int STREAM>
 __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillArgs a)
 {
@@ -274,7 +275,8 @@ __global__ __launch_bounds__(1024) void count_kept_kernel(const uint8_t *mask, i
     if (threadIdx.x == 0) *per_count = n[0] == 0 ? 0 : 1 / n[0];
 }
 
-// The sum of the rows' losses, in a fixed order: of all rows, or of kSlice to a workgroup first.  (One workgroup, 10000 rows: 3.9 us, of loads that wait.)
+// The sum of the rows' losses, in a fixed order: of all rows, or of kSlice to a workgroup first.  (One workgroup: 3 us for 10000 rows, 6 for 40000, 9 for
+// 65536, of loads that wait; in slices 5 for 65537, two launches.)
 constexpr int kSlice = 16384;
 __device__ __forceinline__ double sum_of(const double *v, int64_t n, double *room)
 {
@@ -319,8 +321,12 @@ void launch_rows(const DistillArgs &a, hipStream_t stream)
 {
     const int64_t pieces = (a.cols + Vec16<T>::N - 1) / Vec16<T>::N;
     // 16 lanes to a row: what is done once for a row is done for four at a time, most of the work of short rows; with fewer rows than fill the chip so, longer
-    // ones are done sooner by 64 lanes each.  Float32 with gradient, 64 and 16 lanes: 8192 rows of 100 columns 21 and 13 us (2048: 13 and 12, 512: 11 and
-    // 11), 32768 of 500 62 and 44 (8192: 24 and 19, 2048: 13 and 15); entries beyond 32 take a lane as long as its part of 1000 columns (k = 64: 87 and 100).
+    // ones are done sooner by 64 lanes each.  A pass in us by 64 and by 16 lanes, float32 with gradient: 8192 rows of 100 columns 23 and 15 (2048: 13 and 12,
+    // 512: 12 and 11), 32768 of 500 66 and 50 (8192: 25 and 21, 2048: 15 and 17), 8192 of 1000 29 and 26 (2048: 16 and 19); entries beyond 32 take a lane as long as
+    // its part of 1000 columns (32768 rows, k = 33: 80 and 91).  The loss alone: 8192 of 100 17 and 10, of 500 18 and 14 (2048: 10 and 11), of 1000 21 and
+    // 18 (2048: 11 and 12).  bfloat16 with gradient: 8192 of 1000 27 and 24 (2048: 15 and 18), 32768 of 2000 84 and 82; with k = 33, where the rule takes
+    // 64 lanes, 32768 of 1000 78 and 66.  float64: 8192 of 500 33 and 33, 32768 91 and 88 (2048: 18 and 24).  16 pieces in 16 lanes are all 128 registers and
+    // 28 to 44 bytes of scratch beyond.
     const char *lanes = clg_knob(K_DISTILL_LANES);
     const bool few = a.k <= 64 && (lanes ? atoi(lanes) == 16 : pieces <= 16 || (pieces <= 64 ? a.rows >= 2048 : a.k <= 32 && a.rows >= 8192));
     if (few && pieces <= 16) return launch_as<T, 64, 16, 1, false, STREAM>(a, stream);

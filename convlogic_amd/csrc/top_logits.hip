@@ -79,7 +79,9 @@ __device__ __forceinline__ K wave_threshold(const K (&x)[PER], int want, int eno
     return t;
 }
 
-// Maxima that the threshold is made of: the threads' own, or where k is more than a third of the threads up to four of each.
+// Maxima that the threshold is made of: the threads' own, or where k is more than a third of the threads up to four of each.  5000 rows of 8000 bfloat16, 256
+// threads, us by threads and by pieces: k = 60 39 and 44, 85 42 and 46, 120 49 and 51, 200 606 and 72; 20000 of 1000 float32, 64 threads: k = 15 34 and 37,
+// 22 37 and 39, 30 44 and 42, 60 607 and 58.
 template <int THREADS, int NV>
 constexpr int kSeen = THREADS >= 1024 ? 1 : NV < 4 ? NV : 4;
 template <int THREADS, int NV>
@@ -89,7 +91,7 @@ __host__ __device__ __forceinline__ bool by_pieces(int k)
 }
 
 constexpr int kSpare = 512;                                           // candidates that there is room for beside the k best
-constexpr int kAllRanked = 64;                                        // columns of rows without a threshold
+constexpr int kAllRanked = 64;                                        // columns of rows without a threshold (20000 of 64 float32 20 us, 23 with one; of 20 17, 24)
 constexpr int kNoted = 1024;                                          // pieces that may be noted when a tile begins
 
 // LDS of a workgroup: reduction room, counters, candidates, the best k, maxima, noted pieces
@@ -107,6 +109,8 @@ struct TopRoom {
 
 // One workgroup per row; MULTI: of more than one tile.  The best 64 of 65536 bfloat16, 4096 rows: 113 us, 4.8 TB/s with the vector units busy 71 % of the time
 // under the counters; the best 20 of 131071 in one row, 31 parts: 8 us and 7 to merge them, two launches that wait for their loads.
+// Registers for six wavefronts to a SIMD: 4096 x 65536 bfloat16 125 us, for four 136, for eight 132 (20000 x 3000 95, 94, 88; 20000 x 1000 float32 33, 33, 35).
+// float64, for two: 1000 x 65536 148 to 154 us, for four 139; 20000 x 1000 148 and 149.
 template <typename T, int THREADS, int NV, bool MULTI, bool STREAM>
 __global__ __launch_bounds__(THREADS, sizeof(T) == 8 ? 2 : 6) void top_kernel(TopArgs a)
 {
@@ -447,6 +451,8 @@ void launch_rows(const TopArgs &a, hipStream_t stream)
     if (pieces <= 64) launch_as<T, 64, 1, false, STREAM>(a, stream);
     else if (pieces <= 64 * 4) launch_as<T, 64, 4, false, STREAM>(a, stream);
     else if (pieces <= 256 * 4) launch_as<T, 256, 4, false, STREAM>(a, stream);
+    // (1024 threads where there are few workgroups.  bfloat16, 256 and 1024 threads: 256 x 131072 36 and 28 us, 128 34 and 24, 1 29 and 20; 1024 58 and 95, 600 47 and 70.
+    // 256 threads are sooner from more rows than one to a CU on, which this takes as 512 workgroups: 384 x 131072 40 and 49, 300 x 20000 15 and 22)
     else if (a.rows * a.parts > 512) launch_as<T, 256, 8, true, STREAM>(a, stream);
     else launch_as<T, sizeof(T) == 8 ? 256 : 1024, 8, true, STREAM>(a, stream);
     if (a.parts > 1)
@@ -461,7 +467,10 @@ void launch(const TopArgs &a, hipStream_t stream)
     else launch_rows<T, false>(a, stream);
 }
 
-// Few long rows are shared out among workgroups, whose best are merged by a second launch.
+// Few long rows are shared out among workgroups, whose best are merged by a second launch.  In us whole and in parts, bfloat16, k = 20: 1 row of 131072 20 and 15,
+// 64 23 and 19 (of 200000 34 and 21), 128 25 and 23 (36 and 28), 192 26 and 28 (38 and 34): rows up to 64, well before the crossing.  1 row of 65536 13 and 15,
+// of 80000 18 and 15.  The width of a part hardly counts: 1 row of 131072, k = 8, 14 us from 1024 to 8192 columns, 17 at 16384.  What a part finds does, by which the merge
+// gets longer: of 131072 columns in 10 parts (k = 100) 23 and 22, in 5 (k = 200) 25 and 27, in 4 (k = 256) 27 and 33, in 3 (k = 300) 28 and 36.
 int parts_of(int64_t rows, int64_t cols, int64_t k)
 {
     if (rows > 64 || rows == 0) return 1;

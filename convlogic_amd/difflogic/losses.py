@@ -72,7 +72,10 @@ def _wide(t):
 def top_logits(logits, k, temperature=1.0):
     """The k highest logits of each row of [..., columns], highest first: values [..., k], indices int64 [..., k] (of equal logits the lowest index
     first; a NaN counts as the maximum), and the logsumexp of the whole row at `temperature`, log sum exp(logits / temperature), in float32 (float64
-    of float64 logits).  1 <= k <= 1024.  Constants for autograd, whatever the logits are."""
+    of float64 logits).  1 <= k <= 1024.  Constants for autograd, whatever the logits are.
+
+    As a float32 number the logsumexp is off by up to 2^-24 of itself, and so is the logarithm of every probability that is taken relative to it: 10^-6
+    at 20, more than the probabilities themselves from about 10^7 on.  Logits that are far from 0 go in less a constant per row, or in float64."""
     _check_scores(logits, "logits")
     k, temperature = int(k), _check_number(temperature, "temperature", positive=True)
     if not 1 <= k <= min(MAX_ENTRIES, logits.shape[-1]):
@@ -99,7 +102,7 @@ def distillation_loss(logits, values, indices, logsumexp=None, *, temperature=1.
 
     Without `logsumexp` the teacher's probabilities are the softmax of values / temperature.  With it -- [...], of the teacher's whole row at this
     temperature, as top_logits() returns it -- they are exp(values / temperature - logsumexp), and all columns that are not listed are one answer more,
-    whose probability is what is left of 1 on both sides.
+    whose probability is what is left of 1 on both sides.  The logsumexp is taken as it is, with the rounding of its type.
 
     Rows with mask (bool [...]) False, and rows without an entry, have loss 0 and gradient 0, whatever their logits are.  reduction: "mean" over the rows
     that the mask keeps (0 if it keeps none), "sum", or "none" for a loss per row.  The loss is float32 (float64 of float64 logits), the gradient has the
