@@ -131,6 +131,11 @@ def distillation_loss(logits, values, indices, logsumexp=None, *, temperature=1.
     return _distillation_plain(logits, values, indices, logsumexp, temperature, mask, weight, reduction)
 
 
+def _finite_highest(t):
+    highest = t.detach().amax(-1, keepdim=True)
+    return torch.where(highest.isinf(), 0.0, highest)
+
+
 def _distillation_plain(logits, values, indices, logsumexp, temperature, mask, weight, reduction):
     cols, lead = logits.shape[-1], logits.shape[:-1]
     there = (indices >= 0) & (indices < cols)
@@ -139,15 +144,14 @@ def _distillation_plain(logits, values, indices, logsumexp, temperature, mask, w
     if mask is not None:
         keep = keep & mask
     # rows that do not count are rows of zeros from here on: no inf or NaN of theirs reaches a gradient
-    x = torch.where(keep.unsqueeze(-1), _wide(logits), 0.0).double()
-    highest = x.detach().amax(-1, keepdim=True)                       # (subtracted first: x / temperature would be rounded in steps of its own size)
-    x = (x - torch.where(highest.isinf(), 0.0, highest)) / temperature
+    z = torch.where(keep.unsqueeze(-1), _wide(logits), 0.0).double()
+    highest = _finite_highest(z)                                      # (subtracted first: z / temperature would be rounded in steps of its own size)
+    x = (z - highest) / temperature
     x = x * torch.where(keep & bad, math.nan, 1.0).unsqueeze(-1)
     at = torch.where(there, indices, 0).long()
     t = torch.where(there, values.double(), -math.inf)
     if logsumexp is None:
-        highest = t.amax(-1, keepdim=True)
-        t = (t - torch.where(highest.isinf(), 0.0, highest)) / temperature
+        t = (t - _finite_highest(t)) / temperature
         total = t.exp().sum(-1, keepdim=True)
         log_p = t - torch.where(total == 0, 0.0, total.log())
     else:
@@ -160,10 +164,13 @@ def _distillation_plain(logits, values, indices, logsumexp, temperature, mask, w
         listed = torch.zeros(x.shape, dtype=torch.int32).scatter_add_(-1, at, there.to(torch.int32)) > 0
         rest = (1.0 - p.sum(-1)).clamp(min=0.0)
         rest = torch.where(listed.all(-1) | ~keep, 0.0, rest)
-        # (nothing beside the listed columns: a constant -inf less the logarithm of the whole, which keeps its gradient)
-        others = x.masked_fill(listed, -math.inf)
+        # relative to their own highest; nothing beside the listed columns: a constant -inf less the logarithm of the whole, which keeps its gradient
+        others = z.masked_fill(listed, -math.inf)
         none = (others == -math.inf).all(-1)
-        log_rest = torch.where(none, -math.inf, torch.logsumexp(torch.where(none.unsqueeze(-1), 0.0, others), -1)) - torch.logsumexp(x, -1)
+        others = torch.where(none.unsqueeze(-1), 0.0, others)
+        highest_other = _finite_highest(others)
+        log_others = torch.logsumexp((others - highest_other) / temperature, -1) + ((highest_other - highest) / temperature).squeeze(-1)
+        log_rest = torch.where(none, -math.inf, log_others) - torch.logsumexp(x, -1)
         some = rest != 0
         loss = loss + torch.where(some, torch.special.xlogy(rest, rest) - rest * torch.where(some, log_rest, 0.0), 0.0)
     loss = torch.where(keep, loss, 0.0)

@@ -295,3 +295,17 @@ def test_gate_balance_refuses_a_bare_tensor():
         with pytest.raises(RuntimeError, match="sequence"):
             C.gate_balance(logits)
     assert C.gate_balance([torch.zeros(12, 16)]).counts.tolist() == [[12] + [0] * 15] and C.gate_balance(iter([torch.zeros(12, 16)])).loss == 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_distillation_of_a_listed_logit_far_above_the_others(dtype):
+    # the gradient of the columns that are not listed goes by their differences among themselves: T (M q_v - p_r q_v / q_r), here -T p_r times their softmax
+    z = scores(2, 9, dtype, 3)
+    z[:, 4] = torch.tensor([1e30, torch.finfo(dtype).max / 4], dtype=dtype)     # (as float32 the second would be inf)
+    leaf = z.requires_grad_(True)
+    columns, values, lse = torch.tensor([[4, 0], [4, 0]]), torch.tensor([[1.0, 0.5], [1.0, 0.5]]), torch.full((2,), 2.0)
+    grad, = torch.autograd.grad(C.distillation_loss(leaf, values, columns, lse, temperature=1.5, reduction="sum", weight=1e-3), leaf)
+    others = [1, 2, 3, 5, 6, 7, 8]
+    rest = 1.0 - (values.double() / 1.5 - 2.0).exp().sum(1, keepdim=True)
+    want = -1.5e-3 * rest * torch.softmax(z.detach()[:, others].double() / 1.5, 1)
+    assert (grad[:, others].double() - want).abs().max() <= torch.finfo(dtype).eps * want.abs().max()
