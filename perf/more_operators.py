@@ -168,7 +168,7 @@ def _coded(x):
     low, high = padded.amin(1, keepdim=True), padded.amax(1, keepdim=True)
     size = high.double() - low.double()
     step = (size / 255.0).to(wide)
-    codes = ((padded.double() - low.double()) * torch.where(size > 0, 255.0 / size, 0.0)).round()
+    codes = ((padded.double() - low.double()) * 255.0 / torch.where(size > 0, size, 1.0)).round()
     return (codes * step.double() + low.double()).to(wide).view(-1)[:n].view(x.shape)
 
 
@@ -269,7 +269,7 @@ def _exact_coded(x):
         t = flat[begin:end].view(-1, min(GROUP, end - begin))
         low = t.min(1, keepdim=True).values
         size = t.max(1, keepdim=True).values - low
-        codes = torch.where(size > 0, torch.round((t - low) * (255.0 / size)), 0.0)
+        codes = torch.where(size > 0, torch.round((t - low) * 255.0 / size), 0.0)
         out[begin:end] = (low + codes * (size / 255.0)).view(-1)
     return out.view(x.shape)
 
