@@ -7,6 +7,7 @@ import torch
 from torch import nn
 from torch.autograd import Function
 
+from ..difflogic.activation_codes import check_bits
 from ..difflogic.functional import GradFactor, bin_op_s
 from ..difflogic.packbitstensor import PackBitsTensor
 from ..hip import _lib, convlogic_hip
@@ -202,12 +203,19 @@ class ConvLogicLayer(nn.Module):
     """Logic-gate convolution: every output channel reads 8 taps (from at most two input channels of
     its group) inside its receptive field and combines them with 4 gates, or with the complete
     4 -> 2 -> 1 tree followed by 2x2 OR(max)-pooling when complete=True
-    (src/convlogic/convlogic_layer.py:85-160)."""
+    (src/convlogic/convlogic_layer.py:85-160).
+
+    checkpoint_bits=8 (no counterpart in the reference; complete float32 blocks on the GPU): a training step keeps the input in 8 bits (encode_activations)
+    instead of the input itself.  The output, and which element of a window the pooling takes, are those of the input; both gradients are computed from
+    the values that the codes stand for.  (A block on 0/1 inputs keeps a bit per tap anyway.)"""
 
     def __init__(self, in_channels: int, out_channels: int, stride=1, padding=1, kernel=3, groups: int = 1,
                  selection=None, residual_init: bool = False, implementation: str = "cuda", grad_factor: float = 1.0,
-                 complete: bool = False, return_intermediate: bool = False, return_indices: bool = False):
+                 complete: bool = False, return_intermediate: bool = False, return_indices: bool = False, checkpoint_bits: int = None):
         super().__init__()
+        self.checkpoint_bits = check_bits(checkpoint_bits)
+        if checkpoint_bits is not None and (implementation != "cuda" or not complete or return_intermediate or return_indices):
+            raise ValueError("checkpoint_bits is for complete blocks with implementation='cuda' that return their output alone")
         self.in_channels, self.out_channels = in_channels, out_channels
         self.stride, self.padding, self.kernel = _pair(stride), _pair(padding), _pair(kernel)
         self.groups, self.grad_factor, self.complete = groups, grad_factor, complete
@@ -313,7 +321,7 @@ class ConvLogicLayer(nn.Module):
         difflogic_hip.fold_many), or None when the layer's training path does not take the result."""
         w = self._parameters["weights"]
         if (self.implementation == "cuda" and self.complete and self.training and not self.return_intermediate
-                and not self.return_indices and not self.__dict__.get("binary_input", False) and w.is_cuda and w.is_contiguous()
+                and not self.return_indices and not self.__dict__.get("binary_input", False) and self.__dict__.get("checkpoint_bits") is None and w.is_cuda and w.is_contiguous()
                 and w.dtype in (torch.float32, torch.float64)):
             return w
         return None
@@ -411,12 +419,17 @@ class ConvLogicLayer(nn.Module):
                 return _FullConvLogicBinaryFunction.apply(x, weights, sel, *geo, True, flag)
             w_prob = kernel_probabilities(self.weights, self.training, x.dtype)
             return _FullConvLogicBinaryFunction.apply(x, w_prob, sel, *geo, False, flag)
+        codes = (self.__dict__.get("checkpoint_bits") is not None and self.training and torch.is_grad_enabled()
+                 and (x.requires_grad or weights.requires_grad))
+        if codes and not (self.complete and not self.return_intermediate and not self.return_indices and x.is_cuda and x.dtype == weights.dtype == torch.float32
+                          and weights.is_contiguous() and weights.device == x.device and sel.device == x.device and not _lib.traced()):
+            raise RuntimeError("checkpoint_bits needs float32 activations and weights on one GPU, and a call that is not traced")
         if (self.complete and self.training and not self.return_intermediate and not self.return_indices and x.is_cuda
                 and weights.dtype == x.dtype and x.dtype in (torch.float32, torch.float64) and weights.is_contiguous()
                 and weights.device == x.device and sel.device == x.device):
             plan = self._backward_plan(x, sel)
             if x.dtype == torch.float32 and not _lib.traced():
-                return _lib.nodes().block(x, weights, sel, geo, self.__dict__.get("feature_major_output", False), *plan, self._take_prefold(weights))
+                return _lib.nodes().block(x, weights, sel, geo, self.__dict__.get("feature_major_output", False), *plan, self._take_prefold(weights), codes)
             return _FullConvLogicLogitsFunction.apply(x, weights, sel, *geo, self.__dict__.get("feature_major_output", False), plan,
                                                       self._take_prefold(weights) if plan is not None else None)
         w_prob = kernel_probabilities(self.weights, self.training, x.dtype)

@@ -220,23 +220,23 @@ def _block(c_in, c_out, implementation, **kw):
                           implementation=implementation, **kw)
 
 
-def _head(dims, tau, implementation):
-    fc = [LogicLayer(a, b, grad_factor=1, residual_init=True, implementation=implementation) for a, b in zip(dims, dims[1:])]
+def _head(dims, tau, implementation, **kw):
+    fc = [LogicLayer(a, b, grad_factor=1, residual_init=True, implementation=implementation, **kw) for a, b in zip(dims, dims[1:])]
     return [nn.Flatten(), *fc, GroupSum(k=10, tau=tau)]
 
 
 class ConvLogicCifarModel(nn.Module):
     """Four 3x3 / padding 1 blocks of k, 4k, 16k, 32k kernels (each halves the image), then three
     LogicLayers of 10, 5 and 2.5 times the flattened width (doubled from k = 1024) and a 10-class
-    GroupSum (src/convlogic/model.py:11-60)."""
+    GroupSum (src/convlogic/model.py:11-60).  checkpoint_bits: of all layers (ConvLogicLayer, LogicLayer)."""
 
-    def __init__(self, k_param=32, input_channels=3, input_size=32, tau=20, implementation="cuda"):
+    def __init__(self, k_param=32, input_channels=3, input_size=32, tau=20, implementation="cuda", checkpoint_bits=None):
         super().__init__()
         self.input_size = input_size
         self.k_param = k_param
         self.extra_layers = 2 if k_param >= 1024 else 1
         widths = [input_channels] + [m * k_param for m in (1, 4, 16, 32)]
-        blocks = [_block(a, b, implementation, padding=1, groups=1) for a, b in zip(widths, widths[1:])]
+        blocks = [_block(a, b, implementation, padding=1, groups=1, checkpoint_bits=checkpoint_bits) for a, b in zip(widths, widths[1:])]
         side = input_size // 2 ** len(blocks)
         flat = widths[-1] * side * side
         m = self.extra_layers
@@ -246,7 +246,7 @@ class ConvLogicCifarModel(nn.Module):
         blocks[-1].feature_major_output = implementation == "cuda"
         # the network's input is the thresholded image (src/convlogic/data.py:46-50): every element is 0 or 1
         blocks[0].binary_input = implementation == "cuda"
-        self.network = nn.Sequential(*blocks, *_head(dims, tau, implementation))
+        self.network = nn.Sequential(*blocks, *_head(dims, tau, implementation, checkpoint_bits=checkpoint_bits))
 
     def forward(self, x):
         return _forward(self, x)
@@ -255,16 +255,17 @@ class ConvLogicCifarModel(nn.Module):
 class ConvLogicMnistModel(nn.Module):
     """A 5x5 / padding 0 block of k kernels (28 -> 24 -> 12), two 3x3 / padding 1 blocks of 3k and 9k
     kernels (-> 6 -> 3), then LogicLayers 81k -> 1280k -> 640k -> 320k and a 10-class GroupSum
-    (src/convlogic/model.py:63-108)."""
+    (src/convlogic/model.py:63-108).  checkpoint_bits: of all layers (ConvLogicLayer, LogicLayer)."""
 
-    def __init__(self, input_channels=1, input_size=28, k_param=32, tau=6.5, implementation="cuda"):
+    def __init__(self, input_channels=1, input_size=28, k_param=32, tau=6.5, implementation="cuda", checkpoint_bits=None):
         super().__init__()
         k = k_param
-        blocks = [_block(input_channels, k, implementation, kernel=5, padding=0),
-                  _block(k, 3 * k, implementation, kernel=3, padding=1),
-                  _block(3 * k, 9 * k, implementation, kernel=3, padding=1)]
+        keep = {"checkpoint_bits": checkpoint_bits}
+        blocks = [_block(input_channels, k, implementation, kernel=5, padding=0, **keep),
+                  _block(k, 3 * k, implementation, kernel=3, padding=1, **keep),
+                  _block(3 * k, 9 * k, implementation, kernel=3, padding=1, **keep)]
         blocks[0].binary_input = implementation == "cuda"          # binarised digits, as in the CIFAR topology
-        self.network = nn.Sequential(*blocks, *_head([81 * k, 1280 * k, 640 * k, 320 * k], tau, implementation))
+        self.network = nn.Sequential(*blocks, *_head([81 * k, 1280 * k, 640 * k, 320 * k], tau, implementation, **keep))
 
     def forward(self, x):
         return _forward(self, x)

@@ -41,6 +41,8 @@ def train(net, tail, plan, x, called_for_itself):
     if type(x) is not torch.Tensor or x.dim() != 4 or x.shape[0] > fc_tree.MAX_BATCH or not x.is_contiguous() or _lib.traced() or layers[0]._parameters["weights"].device != x.device:
         return None
     blocks = blocks_of(net, called_for_itself, x.device)
+    if any(m.__dict__.get("checkpoint_bits") is not None for m in (*(blocks or ()), layers[0])):
+        return None
     if blocks is None or 16 * 7 * (plan.roots + sum(m.out_channels for m in blocks)) > MAX_LOGITS:
         return None
     n, c, h, w = x.shape

@@ -212,6 +212,18 @@ __device__ __forceinline__ T row16_sum(T v)
     v += dpp_zero<0x140, 0xF>(v);
     return v;
 }
+// Sum over each group of LPR lanes: valid in the last 16 lanes of the group.
+template <typename T, int LPR>
+__device__ __forceinline__ T lane_group_sum(T v)
+{
+    if constexpr (LPR == 64) {
+        return wave_sum(v);
+    } else {
+        v = row16_sum(v);
+        if constexpr (LPR == 32) v += dpp_zero<0x142, 0xA>(v);   // row_bcast15: rows 1 and 3 add the row before them
+        return v;
+    }
+}
 // The sums over a wavefront of 28 values, four for each of seven gates.  Every exchange between lane groups halves the number of values that a
 // lane holds.  The lane that gets a sum returns it and which one in `at`; the others get at = -1.
 __device__ __forceinline__ float wave_sums28(const float (&v)[28], int lane, int &at)

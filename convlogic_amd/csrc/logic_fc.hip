@@ -165,19 +165,6 @@ __global__ __launch_bounds__(kBlock) void fc_forward_kernel(const S *__restrict_
     }
 }
 
-// Sum over each group of LPR lanes: valid in the last 16 lanes of the group.
-template <typename T, int LPR>
-__device__ __forceinline__ T lane_group_sum(T v)
-{
-    if constexpr (LPR == 64) {
-        return wave_sum(v);
-    } else {
-        v = row16_sum(v);
-        if constexpr (LPR == 32) v += dpp_zero<0x142, 0xA>(v);   // row_bcast15: rows 1 and 3 add the row before them
-        return v;
-    }
-}
-
 // A neuron's row takes LPR lanes x VEC samples per pass, a wavefront 64/LPR neurons; the last 16 lanes of each
 // group hold the four sums and write the 16 gate gradients.
 template <typename S, int VEC, int LPR>

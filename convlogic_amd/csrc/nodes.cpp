@@ -5,6 +5,7 @@
 // per launch.  Forward and backward of one block 82 us on a quiet host and 146 with the hand-off by the Python
 // functions, of a LogicLayer 64 and 124.
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_cpp_function.h>
@@ -64,6 +65,59 @@ struct FeatureMajor : torch::autograd::Function<FeatureMajor> {
     }
 };
 Tensor feature_major(const Tensor &x) { return FeatureMajor::apply(x); }
+
+// ---- activations in 8 bits ---------------------------------------------------------------------------------------------------
+int code_of(at::ScalarType t)
+{
+    switch (t) {
+    case at::kFloat: return CLG_F32;
+    case at::kDouble: return CLG_F64;
+    case at::kHalf: return CLG_F16;
+    case at::kBFloat16: return CLG_BF16;
+    default: TORCH_CHECK(false, "float32, float64, float16 or bfloat16 expected, got ", t);
+    }
+}
+struct Codes {
+    Tensor codes, scales;
+    // of a tensor without gaps, in the order in which it lies in memory
+    static Codes of(const Tensor &x)
+    {
+        const int64_t n = x.numel();
+        Codes c{at::empty({n}, x.options().dtype(at::kByte)),
+                at::empty({clg_codes_groups(n), 2}, x.options().dtype(x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat))};
+        check(clg_codes_encode(code_of(x.scalar_type()), x.data_ptr(), n, static_cast<uint8_t *>(c.codes.data_ptr()), c.scales.data_ptr(), stream_of(x)));
+        return c;
+    }
+    void into(const Tensor &x) const
+    {
+        check(clg_codes_decode(code_of(x.scalar_type()), static_cast<const uint8_t *>(codes.data_ptr()), scales.data_ptr(), x.numel(), x.data_ptr(), stream_of(x)));
+    }
+    Tensor values(at::IntArrayRef shape) const                        // float32, dense
+    {
+        const Tensor x = at::empty(shape, scales.options());
+        into(x);
+        return x;
+    }
+};
+// x without gaps -> codes and scales
+std::pair<Tensor, Tensor> encode(const Tensor &x)
+{
+    const c10::OptionalDeviceGuard guard(x.device());
+    TORCH_CHECK(x.is_non_overlapping_and_dense(), "activations without gaps in memory expected");
+    const Codes c = Codes::of(x);
+    return {c.codes, c.scales};
+}
+Tensor decode(const Tensor &codes, const Tensor &scales, std::vector<int64_t> shape, std::vector<int64_t> stride, at::ScalarType type)
+{
+    const c10::OptionalDeviceGuard guard(codes.device());
+    const Tensor x = at::empty_strided(shape, stride, scales.options().dtype(type));
+    TORCH_CHECK(codes.scalar_type() == at::kByte && codes.is_contiguous() && codes.numel() == x.numel() && scales.is_contiguous() &&
+                    scales.device() == codes.device() && scales.scalar_type() == (type == at::kDouble ? at::kDouble : at::kFloat) &&
+                    scales.numel() == 2 * clg_codes_groups(x.numel()) && x.is_non_overlapping_and_dense(),
+                "codes and scales are not those of activations ", shape, " of ", type);
+    Codes{codes, scales}.into(x);
+    return x;
+}
 
 // ---- LogicLayer ------------------------------------------------------------------------------------------------------------
 struct FcLayer : torch::autograd::Function<FcLayer> {
@@ -130,11 +184,50 @@ struct FcLayer : torch::autograd::Function<FcLayer> {
         return {gx, Tensor(), Tensor(), gl, Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
+// The same, with the input kept in codes.
+struct FcLayerCodes : torch::autograd::Function<FcLayerCodes> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x_in, const Tensor &a, const Tensor &b, const Tensor &logits, const Tensor &start,
+                          const Tensor &flat, bool sole, bool sample_major)
+    {
+        const c10::OptionalDeviceGuard guard(x_in.device());
+        const Tensor x = sample_major ? transposed(x_in) : x_in;
+        const int64_t out_dim = logits.size(0), in_dim = x.size(0), batch = x.size(1);
+        const Tensor y = floats(x, {out_dim, batch}), probs = floats(x, {out_dim, 16}), folded = floats(x, {out_dim, 4});
+        check(clg_fc_forward_logits(CLG_F32, x.data_ptr(), idx(a), idx(b), logits.data_ptr(), probs.data_ptr(), folded.data_ptr(), y.data_ptr(), in_dim,
+                                    out_dim, batch, stream_of(x)));
+        const Codes c = Codes::of(x);
+        ctx->save_for_backward({c.codes, c.scales, a, b, probs, folded, start, flat});
+        ctx->saved_data["sole"] = sole;
+        ctx->saved_data["sample_major"] = sample_major;
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const auto saved = ctx->get_saved_variables();
+        const c10::OptionalDeviceGuard guard(saved[0].device());
+        const Tensor &codes = saved[0], &scales = saved[1], &a = saved[2], &b = saved[3], &probs = saved[4], &folded = saved[5], &start = saved[6], &flat = saved[7];
+        const bool sole = ctx->saved_data["sole"].toBool(), sample_major = ctx->saved_data["sample_major"].toBool();
+        const bool need_x = ctx->needs_input_grad(0), need_l = ctx->needs_input_grad(3);
+        const int64_t in_dim = start.numel() - 1, out_dim = folded.size(0), batch = codes.numel() / in_dim;
+        const Tensor gy = contiguous_2d(grads[0]);
+        need(gy, folded, "grad_y", {out_dim, batch});
+        Tensor gx, gl, scratch;
+        if (need_x) gx = floats(folded, {in_dim, batch});
+        if (need_l) gl = floats(folded, {out_dim, 16});
+        if (need_x && need_l && !sole) scratch = bytes(folded, clg_fc_codes_scratch_bytes(out_dim, batch));
+        check(clg_fc_codes_backward(static_cast<const uint8_t *>(codes.data_ptr()), scales.data_ptr(), idx(a), idx(b), folded.data_ptr<float>(), probs.data_ptr<float>(),
+                                    gy.data_ptr<float>(), idx(start), idx(flat), static_cast<float *>(ptr(gx)), static_cast<float *>(ptr(gl)), in_dim, out_dim, batch,
+                                    sole, ptr(scratch), stream_of(codes)));
+        if (sample_major && need_x) gx = transposed(gx);
+        return {gx, Tensor(), Tensor(), gl, Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
 // x [batch, in] where sample_major, else [in, batch]; -> [batch, out], a transposed view of [out, batch]
 Tensor fc_layer(const Tensor &x, const Tensor &a, const Tensor &b, const Tensor &logits, const Tensor &start, const Tensor &flat, bool sole,
-                bool sample_major)
+                bool sample_major, bool codes)
 {
     need(logits, x, "weights", {a.numel(), 16});
+    if (codes) return FcLayerCodes::apply(x, a, b, logits, start, flat, sole, sample_major).transpose(0, 1);
     return FcLayer::apply(x, a, b, logits, start, flat, sole, sample_major).transpose(0, 1);
 }
 
@@ -291,15 +384,24 @@ std::pair<Tensor, Tensor> block_backward(const BlockState &state, const Conv &co
     return {gx, gl};
 }
 struct Block : torch::autograd::Function<Block> {
+    // codes: x is kept in 8 bits, and a padded copy of it not at all
     static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &logits, const Tensor &sel, const Conv *conv, bool want_fm,
-                          const Tensor *plan, int64_t signature, const std::pair<Tensor, Tensor> *pair, bool need_x)
+                          const Tensor *plan, int64_t signature, const std::pair<Tensor, Tensor> *pair, bool need_x, bool codes)
     {
         BlockState state;
-        const Tensor y = block_forward(x, logits, sel, *conv, want_fm, signature, pair, need_x, state);
+        const Tensor y = block_forward(x, logits, sel, *conv, want_fm, signature, pair, need_x && !codes, state);
+        std::vector<int64_t> more{want_fm, signature};
+        Codes kept;
+        if (codes) {
+            more.insert(more.end(), state.x.sizes().begin(), state.x.sizes().end());
+            kept = Codes::of(state.x);
+            state.x = kept.codes;
+        }
         variable_list saved;
         state.save(saved);
+        saved.push_back(kept.scales);
         ctx->save_for_backward(std::move(saved));
-        ctx->saved_data["conv"] = conv->saved({want_fm, signature});
+        ctx->saved_data["conv"] = conv->saved(std::move(more));
         ctx->saved_data["plan"] = *plan;
         return want_fm ? y.permute({3, 0, 1, 2}) : y;
     }
@@ -307,17 +409,20 @@ struct Block : torch::autograd::Function<Block> {
     {
         const auto saved = ctx->get_saved_variables();
         const auto ints = ctx->saved_data["conv"].toIntVector();
-        const auto g = block_backward(BlockState::from(saved.data()), Conv::from(ints), ints[6], ctx->saved_data["plan"].toTensor(), ints[7], grads[0],
+        BlockState state = BlockState::from(saved.data());
+        if (const Tensor &scales = saved[BlockState::kTensors]; scales.defined()) state.x = Codes{state.x, scales}.values(at::IntArrayRef(ints).slice(8));
+        const auto g = block_backward(state, Conv::from(ints), ints[6], ctx->saved_data["plan"].toTensor(), ints[7], grads[0],
                                       ctx->needs_input_grad(0), ctx->needs_input_grad(1));
-        return {g.first, g.second, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        return {g.first, g.second, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 Tensor block(const Tensor &x, const Tensor &logits, const Tensor &sel, std::array<int64_t, 6> conv, bool want_fm, const Tensor &plan,
-             int64_t signature, const std::optional<std::pair<Tensor, Tensor>> &prefolded)
+             int64_t signature, const std::optional<std::pair<Tensor, Tensor>> &prefolded, bool codes)
 {
     need(logits, x, "weights", {sel.size(0), 7, 16});
     const Conv cv{conv[0], conv[1], conv[2], conv[3], conv[4], conv[5]};
-    return Block::apply(x, logits, sel, &cv, want_fm, &plan, signature, prefolded ? &*prefolded : nullptr, at::GradMode::is_enabled() && x.requires_grad());
+    return Block::apply(x, logits, sel, &cv, want_fm, &plan, signature, prefolded ? &*prefolded : nullptr, at::GradMode::is_enabled() && x.requires_grad(),
+                        codes);
 }
 
 // The block on 0/1 inputs, from the logits.  flag: device address of the layer's BinaryFlag.  It keeps taps and keep; x itself is not needed
@@ -438,11 +543,13 @@ std::array<Tensor, 4> trees_backward(const Tensor &x, const Tensor &start, const
     return g;
 }
 struct Trees : torch::autograd::Function<Trees> {
-    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &l0, const Tensor &l1, const Tensor &l2, const TreeArgs *t, bool need_l)
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &l0, const Tensor &l1, const Tensor &l2, const TreeArgs *t, bool need_l, bool codes)
     {
         Tensor coef, probs;
         const Tensor out = trees_forward(x, l0, l1, l2, *t, need_l, coef, probs);
-        variable_list saved = {x, t->start, coef, probs};
+        Codes kept;
+        if (codes) kept = Codes::of(x);
+        variable_list saved = {codes ? kept.codes : x, t->start, coef, probs, kept.scales};
         saved.insert(saved.end(), t->wiring.begin(), t->wiring.end());
         ctx->save_for_backward(std::move(saved));
         ctx->saved_data["tables"] = std::vector<Tensor>{t->rows, t->pos, t->slot};
@@ -453,20 +560,22 @@ struct Trees : torch::autograd::Function<Trees> {
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
         const auto saved = ctx->get_saved_variables();
-        const auto g = trees_backward(saved[0], saved[1], saved[2], saved[3], ctx->saved_data["tables"].toTensorVector(), ctx->saved_data["k"].toInt(),
+        const int64_t in_dim = saved[1].numel() - 1;
+        const Tensor x = saved[4].defined() ? Codes{saved[0], saved[4]}.values({in_dim, saved[0].numel() / in_dim}) : saved[0];
+        const auto g = trees_backward(x, saved[1], saved[2], saved[3], ctx->saved_data["tables"].toTensorVector(), ctx->saved_data["k"].toInt(),
                                       ctx->saved_data["tau"].toDouble(), grads[0],
                                       {ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2), ctx->needs_input_grad(3)});
-        return {g[0], g[1], g[2], g[3], Tensor(), Tensor()};
+        return {g[0], g[1], g[2], g[3], Tensor(), Tensor(), Tensor()};
     }
 };
 Tensor trees(const Tensor &x, const Tensor &l0, const Tensor &l1, const Tensor &l2, const Tensor &start, std::vector<Tensor> wiring, const Tensor &rows,
-             const Tensor &pos, const Tensor &ids, const Tensor &slot, int64_t roots, int64_t k, double tau)
+             const Tensor &pos, const Tensor &ids, const Tensor &slot, int64_t roots, int64_t k, double tau, bool codes)
 {
     need(l0, x, "weights", {4 * roots, 16});
     need(l1, x, "weights", {2 * roots, 16});
     need(l2, x, "weights", {roots, 16});
     const TreeArgs t{start, rows, pos, ids, slot, std::move(wiring), roots, k, tau};
-    return Trees::apply(x, l0, l1, l2, &t, at::GradMode::is_enabled() && (l0.requires_grad() || l1.requires_grad() || l2.requires_grad()));
+    return Trees::apply(x, l0, l1, l2, &t, at::GradMode::is_enabled() && (l0.requires_grad() || l1.requires_grad() || l2.requires_grad()), codes);
 }
 
 // ---- a network: blocks, flattening, trees -------------------------------------------------------------------------------------
@@ -641,12 +750,15 @@ PYBIND11_MODULE(_nodes, m)
     const auto no_gil = py::call_guard<py::gil_scoped_release>();
     name_node<FeatureMajor>("_FeatureMajorBackward");
     name_node<FcLayer>("_LogicLayerLogitsFunctionBackward");
+    name_node<FcLayerCodes>("_LogicLayerCodesFunctionBackward");
     name_node<Block>("_FullConvLogicLogitsFunctionBackward");
     name_node<BinaryBlock>("_FullConvLogicBinaryFunctionBackward");
     name_node<Trees>("_TreeFunctionBackward");
     name_node<Network>("_TreeNetworkFunctionBackward");
     m.def("feature_major", &feature_major, no_gil);
     m.def("fc_layer", &fc_layer, no_gil);
+    m.def("encode", &encode, no_gil);
+    m.def("decode", &decode, no_gil);
     m.def("block", &block, no_gil);
     m.def("binary_block", &binary_block, no_gil);
     m.def("trees", &trees, no_gil);

@@ -14,6 +14,7 @@ import torch
 
 from ..hip import _lib, difflogic_hip
 from . import fc_tree
+from .activation_codes import RecomputedFromCodes, check_bits
 from .functional import GradFactor, bin_op_s, get_unique_connections
 from .packbitstensor import PackBitsTensor
 
@@ -38,11 +39,15 @@ def _reverse_wiring(idx0, idx1, in_dim):
 
 
 class LogicLayer(torch.nn.Module):
-    """out_dim two-input logic gate neurons over in_dim features (src/difflogic/difflogic.py:14-90)."""
+    """out_dim two-input logic gate neurons over in_dim features (src/difflogic/difflogic.py:14-90).
+
+    checkpoint_bits=8 (no counterpart in the reference): a training step keeps the input in 8 bits (encode_activations) instead of the input itself.  The
+    output is that of the input; both gradients are those at the values that the codes stand for."""
 
     def __init__(self, in_dim: int, out_dim: int, grad_factor: float = 1.0, implementation: str = None,
-                 connections: str = "random", residual_init: bool = False):
+                 connections: str = "random", residual_init: bool = False, checkpoint_bits: int = None):
         super().__init__()
+        self.checkpoint_bits = check_bits(checkpoint_bits)
         if residual_init:                       # gate 3 ("A") gets logit 5 -> p = 0.908
             logits = torch.zeros(out_dim, 16)
             logits[:, 3] = 5.0
@@ -94,9 +99,19 @@ class LogicLayer(torch.nn.Module):
 
     def forward_python(self, x):
         assert x.shape[-1] == self.in_dim, (x.shape[-1], self.in_dim)
+        if self._keeps_codes(x):
+            return RecomputedFromCodes.apply(x, self.weights, self._evaluate_python)
         a, b = x[..., self.indices_0], x[..., self.indices_1]
         w = self._gate_weights(torch.float32 if not self.training else self.weights.dtype)
         return bin_op_s(a, b, w)
+
+    def _evaluate_python(self, x, weights):
+        return bin_op_s(x[..., self.indices_0], x[..., self.indices_1], torch.nn.functional.softmax(weights, dim=-1))
+
+    def _keeps_codes(self, x):
+        """True for a call whose backward pass reads the input from codes."""
+        return (self.__dict__.get("checkpoint_bits") is not None and self.training and torch.is_grad_enabled()
+                and (x.requires_grad or self._parameters["weights"].requires_grad))
 
     def forward_cuda(self, x):
         if self.training:
@@ -105,6 +120,8 @@ class LogicLayer(torch.nn.Module):
         assert x.shape[1] == self.in_dim, (tuple(x.shape[::-1]), self.in_dim)
         key = self._check_wiring()
         weights, buffers = self._parameters["weights"], self._buffers
+        if self._keeps_codes(x):
+            return self._forward_codes(x, key)
         if (self.training and weights.dtype == x.dtype and x.dtype in (torch.float32, torch.float64)
                 and weights.is_contiguous() and weights.device == x.device):
             # a sample-major batch is transposed inside the Function (and its gradient on the way back): one autograd
@@ -114,7 +131,7 @@ class LogicLayer(torch.nn.Module):
             if prefolded is None and x.dtype == torch.float32 and not _lib.traced():
                 return _lib.nodes().fc_layer(x if inside else _feature_major(x), buffers["indices_0"], buffers["indices_1"], weights,
                                              buffers["given_x_indices_of_y_start"], buffers["given_x_indices_of_y"], self._sole_consumers(key),
-                                             inside)
+                                             inside, False)
             return _LogicLayerLogitsFunction.apply(x if inside else _feature_major(x), buffers["indices_0"], buffers["indices_1"],
                                                    weights, buffers["given_x_indices_of_y_start"],
                                                    buffers["given_x_indices_of_y"], self._sole_consumers(key), inside,
@@ -127,11 +144,26 @@ class LogicLayer(torch.nn.Module):
         with torch.no_grad():
             return LogicLayerCudaFunction.apply(*args).transpose(0, 1)
 
+    def _forward_codes(self, x, key):
+        if _lib.traced():
+            raise RuntimeError("a layer with checkpoint_bits cannot be traced in training")
+        weights, buffers = self._parameters["weights"], self._buffers
+        if x.dtype == torch.float32 and weights.dtype == x.dtype and weights.is_contiguous() and weights.device == x.device and x.numel() > 0:
+            inside = _transposes_with_kernel(x)
+            return _lib.nodes().fc_layer(x if inside else _feature_major(x), buffers["indices_0"], buffers["indices_1"], weights,
+                                         buffers["given_x_indices_of_y_start"], buffers["given_x_indices_of_y"], self._sole_consumers(key), inside, True)
+        return RecomputedFromCodes.apply(_feature_major(x), weights, self._evaluate_probabilities).transpose(0, 1)
+
+    def _evaluate_probabilities(self, x, weights):
+        buffers = self._buffers
+        return LogicLayerCudaFunction.apply(x, buffers["indices_0"], buffers["indices_1"], torch.nn.functional.softmax(weights, dim=-1).to(x.dtype),
+                                            buffers["given_x_indices_of_y_start"], buffers["given_x_indices_of_y"])
+
     def prefold_candidate(self):
         """The logits a network may fold for this layer ahead of its forward call (one launch for all its layers,
         difflogic_hip.fold_many), or None when the layer's training path does not take the result."""
         w = self._parameters["weights"]
-        if (self.implementation == "cuda" and self.training and w.is_cuda and w.is_contiguous()
+        if (self.implementation == "cuda" and self.training and self.__dict__.get("checkpoint_bits") is None and w.is_cuda and w.is_contiguous()
                 and w.dtype in (torch.float32, torch.float64)):
             return w
         return None
@@ -477,7 +509,7 @@ def logic_layer_group_sum(layer, group_sum, x):
     weights = layer._parameters["weights"]
     if (isinstance(layer, LogicLayer) and isinstance(group_sum, GroupSum) and layer.implementation == "cuda" and layer.training
             and torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.is_cuda and x.ndim == 2 and x.shape[1] == layer.in_dim
-            and layer.grad_factor == 1.0 and weights.dtype == x.dtype and x.dtype in (torch.float32, torch.float64)
+            and layer.grad_factor == 1.0 and layer.__dict__.get("checkpoint_bits") is None and weights.dtype == x.dtype and x.dtype in (torch.float32, torch.float64)
             and weights.is_contiguous() and weights.device == x.device and layer.out_dim % group_sum.k == 0 and x.shape[0] > 0
             and group_sum.tau != 0 and not _has_forward_hooks(layer) and not _has_forward_hooks(group_sum)):
         key = layer._check_wiring()

@@ -183,11 +183,16 @@ def tree_eval(layers, group_sum, x, plan):
 
 
 def tree_train(layers, group_sum, x, plan):
-    """group_sum(third(second(first(x)))) in training; x feature-major [features, B]."""
+    """group_sum(third(second(first(x)))) in training; x feature-major [features, B].  The trees keep no input but x: in codes where the first layer has
+    checkpoint_bits."""
     first, second, third = layers
+    codes = (first.__dict__.get("checkpoint_bits") is not None and torch.is_grad_enabled()
+             and (x.requires_grad or any(layer.weights.requires_grad for layer in layers)))
+    if codes and _lib.traced():
+        raise RuntimeError("a layer with checkpoint_bits cannot be traced in training")
     if not _lib.traced():
         return _lib.nodes().trees(x, first.weights, second.weights, third.weights, first._buffers["given_x_indices_of_y_start"], wiring_of(*layers),
-                                  plan.rows, plan.pos, plan.ids, plan.slot, plan.roots, group_sum.k, float(group_sum.tau))
+                                  plan.rows, plan.pos, plan.ids, plan.slot, plan.roots, group_sum.k, float(group_sum.tau), codes)
     return _TreeFunction.apply(x, first.weights, second.weights, third.weights, first._buffers["given_x_indices_of_y_start"],
                                wiring_of(*layers), plan, group_sum.k, group_sum.tau)
 

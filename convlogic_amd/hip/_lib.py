@@ -145,6 +145,11 @@ SIGNATURES = {
     "clg_balance_scratch_bytes": (_i64, [_i, _i64]),
     "clg_balance_forward": (_i, [_i, _i, _p, _p, _p, _i64, _i64, _p, _f64, _p, _p, _p, _p, _p]),
     "clg_balance_backward": (_i, [_i, _i, _p, _p, _p, _i64, _p, _p, _p, _p, _p]),
+    "clg_codes_groups": (_i64, [_i64]),
+    "clg_codes_encode": (_i, [_i, _p, _i64, _p, _p, _p]),
+    "clg_codes_decode": (_i, [_i, _p, _p, _i64, _p, _p]),
+    "clg_fc_codes_scratch_bytes": (_i64, [_i64, _i64]),
+    "clg_fc_codes_backward": (_i, [_p] * 11 + [_i64, _i64, _i64, _i, _p, _p]),
     "clg_net_packed": (_i, [_p, _i] + [_p] * 9 + [_f64, _i64, _i64, _i64, _i64, _p, _p]),
 }
 

@@ -715,6 +715,28 @@ int clg_balance_forward(int dtype, int n, const void *const *logits, const int64
 int clg_balance_backward(int dtype, int n, const void *const *logits, const int64_t *rows, const int64_t *row_strides, int64_t experts,
                          const uint8_t *mask, const void *coefs, const void *upstream, void *const *grads, void *stream);
 
+/* ---------------------------------------------------------------------------------
+ * activations in 8 bits (no counterpart in the reference)
+ * ------------------------------------------------------------------------------- */
+
+/* 128 elements, in the order in which they lie in memory (the last ones may be fewer), share their lowest value and a step: element i is kept as codes[i] and
+ * stands for scales[i / 128][0] + codes[i] scales[i / 128][1], codes[i] = rint((x[i] - lowest) 255 / (highest - lowest)) in 64-bit arithmetic, a half to
+ * the even code.  Elements of a group with a NaN or an infinity all stand for NaN, and so do those of a float64 group with 255 times its range beyond float64.
+ * dtype: CLG_F32, CLG_F64, CLG_F16 or CLG_BF16; scales [clg_codes_groups(n), 2] float32, float64 for CLG_F64.  codes aligned to 8 bytes, scales to 16,
+ * x to an element. */
+int64_t clg_codes_groups(int64_t n);
+int clg_codes_encode(int dtype, const void *x /*[n]*/, int64_t n, uint8_t *codes /*[n]*/, void *scales, void *stream);
+int clg_codes_decode(int dtype, const uint8_t *codes, const void *scales, int64_t n, void *x, void *stream);
+
+/* Backward pass of a float32 LogicLayer whose input [in_dim, batch] was kept in codes: as clg_fc_backward_x_folded and clg_fc_backward_logits, at the
+ * values that the codes stand for.  Either gradient may be NULL (probs then too, or the reverse map).  sole: every input is read by exactly one operand.
+ * scratch: clg_fc_codes_scratch_bytes() bytes, NULL where that is 0. */
+int64_t clg_fc_codes_scratch_bytes(int64_t out_dim, int64_t batch);
+int clg_fc_codes_backward(const uint8_t *codes, const void *scales, const int64_t *a, const int64_t *b, const float *folded /*[out,4]*/,
+                          const float *probs /*[out,16]*/, const float *grad_y /*[out,batch]*/, const int64_t *csr_start, const int64_t *csr_list,
+                          float *grad_x /*[in,batch]*/, float *grad_logits /*[out,16]*/, int64_t in_dim, int64_t out_dim, int64_t batch, int sole,
+                          void *scratch, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
