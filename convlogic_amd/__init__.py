@@ -9,10 +9,10 @@ differentiable logic gate networks.
 from .convlogic import (ConvLogicCifarModel, ConvLogicFunction, ConvLogicLayer, ConvLogicMnistModel, FullConvLogicFunction, PoolLogicLayer, TreeLogicFunction,
                         TreeLogicLayer)
 from .difflogic import (ActivationCodes, GradFactor, GroupSum, LogicLayer, LogicLayerCudaFunction, PackBitsTensor, balance_loss, decode_activations,
-                        distillation_loss, encode_activations, gate_balance, top_logits)
+                        distillation_loss, encode_activations, gate_balance, group_cross_entropy, top_logits)
 from .hip import GraphedStep
 
 __all__ = ["ConvLogicLayer", "ConvLogicFunction", "FullConvLogicFunction", "PoolLogicLayer", "TreeLogicLayer",
            "TreeLogicFunction", "LogicLayer", "GroupSum", "LogicLayerCudaFunction", "PackBitsTensor", "GradFactor", "ConvLogicCifarModel",
-           "ConvLogicMnistModel", "GraphedStep", "top_logits", "distillation_loss", "balance_loss", "gate_balance", "ActivationCodes",
+           "ConvLogicMnistModel", "GraphedStep", "top_logits", "distillation_loss", "balance_loss", "gate_balance", "group_cross_entropy", "ActivationCodes",
            "encode_activations", "decode_activations"]

@@ -9,7 +9,7 @@
 // others' sum to the row's highest are 64-bit numbers, and a relative error d of that sum, in 32 bits, moves the loss by tau^2 (M q_r - p_r) d only.
 #include <stdlib.h>
 
-#include "row_tile.h"
+#include "row_sums.h"
 
 namespace {
 
@@ -275,32 +275,6 @@ __global__ __launch_bounds__(1024) void count_kept_kernel(const uint8_t *mask, i
     if (threadIdx.x == 0) *per_count = n[0] == 0 ? 0 : 1 / n[0];
 }
 
-// The sum of the rows' losses, in a fixed order: of all rows, or of kSlice to a workgroup first.  (One workgroup: 3 us for 10000 rows, 6 for 40000, 9 for
-// 65536, of loads that wait; in slices 5 for 65537, two launches.)
-constexpr int kSlice = 16384;
-__device__ __forceinline__ double sum_of(const double *v, int64_t n, double *room)
-{
-    double s[1] = {0};
-#pragma unroll 4
-    for (int64_t i = threadIdx.x; i < n; i += 1024) s[0] += v[i];
-    block_reduce<true, 1024>(s, room);
-    return s[0];
-}
-__global__ __launch_bounds__(1024) void sum_slices_kernel(const double *row_loss, int64_t rows, double *slices)
-{
-    __shared__ double room[16];
-    const int64_t first = (int64_t)blockIdx.x * kSlice;
-    const double s = sum_of(row_loss + first, rows - first < kSlice ? rows - first : kSlice, room);
-    if (threadIdx.x == 0) slices[blockIdx.x] = s;
-}
-template <typename A>
-__global__ __launch_bounds__(1024) void sum_rows_kernel(const double *row_loss, int64_t rows, const double *per_count, A *out)
-{
-    __shared__ double room[16];
-    const double s = sum_of(row_loss, rows, room);
-    if (threadIdx.x == 0) *out = (A)(s * (per_count ? *per_count : 1));
-}
-
 template <typename T, int THREADS, int LANES, int NV, bool MULTI, int STREAM>
 void launch_as(const DistillArgs &a, hipStream_t stream)
 {
@@ -411,18 +385,7 @@ extern "C" int clg_distill_forward(int dtype, const void *logits, int64_t row_st
         CLG_CHECK_LAUNCH("clg_distill_forward");
     }
     if (reduction == CLG_REDUCE_NONE) return CLG_OK;
-    const double *terms = row_loss;
-    int64_t n = rows;
-    if (rows > 4 * kSlice) {
-        n = clg_ceil_div(rows, kSlice);
-        sum_slices_kernel<<<dim3((unsigned)n), dim3(1024), 0, clg_stream(stream)>>>(row_loss, rows, per_count + 1);
-        CLG_CHECK_LAUNCH("clg_distill_forward");
-        terms = per_count + 1;
-    }
-    if (dtype == CLG_F64) sum_rows_kernel<double><<<dim3(1), dim3(1024), 0, clg_stream(stream)>>>(terms, n, a.per_count, static_cast<double *>(loss));
-    else sum_rows_kernel<float><<<dim3(1), dim3(1024), 0, clg_stream(stream)>>>(terms, n, a.per_count, static_cast<float *>(loss));
-    CLG_CHECK_LAUNCH("clg_distill_forward");
-    return CLG_OK;
+    return sum_rows("clg_distill_forward", dtype, row_loss, rows, per_count + 1, a.per_count, loss, clg_stream(stream));
 }
 
 extern "C" int clg_distill_backward(int dtype, const void *logits, int64_t row_stride, const void *values, int values_dtype, const void *columns,

@@ -250,6 +250,83 @@ std::tuple<Tensor, Tensor> balance(const std::vector<Tensor> &logits, int64_t k,
     return {out[0], out[1]};
 }
 
+// ---- cross entropy of group sums --------------------------------------------------------------------------------------------
+struct GroupCeCall {
+    Tensor targets;
+    int64_t k;
+    double tau, smoothing, weight;
+    int64_t reduction;
+    bool wanted;
+};
+// x [..., features] as the kernels read it: rows of dense features, or [features, rows] behind a transposed view
+bool in_columns(const Tensor &x) { return x.dim() == 2 && !x.is_contiguous() && x.stride(0) == 1 && x.stride(1) == x.size(0); }
+Tensor like_features(const Tensor &x)
+{
+    return in_columns(x) ? at::empty({x.size(1), x.size(0)}, x.options()).t() : at::empty(x.sizes(), x.options());
+}
+struct GroupCe : torch::autograd::Function<GroupCe> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const GroupCeCall *c)
+    {
+        const c10::OptionalDeviceGuard guard(x.device());
+        const bool per_row = c->reduction == CLG_REDUCE_NONE, columns = in_columns(x);
+        const Rows r(x);
+        const auto room = [&](int64_t n) { return at::empty({n}, x.options().dtype(at::kByte)); };
+        Tensor loss = at::empty(per_row ? x.sizes().slice(0, x.dim() - 1) : at::IntArrayRef(), wide(x)), grad;
+        const Tensor kept = room(clg_group_ce_kept_bytes(code_of(x), columns, r.rows, r.cols, c->k)),
+                     scratch = room(clg_group_ce_scratch_bytes(code_of(x), columns, r.rows, r.cols, c->k));
+        if (c->wanted && !per_row) grad = like_features(x);
+        check(clg_group_ce_forward(code_of(x), r.at, columns ? -1 : r.stride, r.rows, r.cols, c->k, c->targets.data_ptr(), 8 * (int)c->targets.element_size(),
+                                   c->tau, c->smoothing, c->weight, (int)c->reduction, loss.data_ptr(), grad.defined() ? grad.data_ptr() : nullptr,
+                                   kept.data_ptr(), scratch.data_ptr(), stream_of(x)));
+        if (!c->wanted) return loss;
+        ctx->save_for_backward({x, c->targets, kept});
+        auto &data = ctx->saved_data;
+        data["k"] = c->k;
+        data["tau"] = c->tau;
+        data["smoothing"] = c->smoothing;
+        data["weight"] = c->weight;
+        data["reduction"] = c->reduction;
+        if (!per_row) {                                               // (handed on to the first backward pass, as Distill does)
+            data["grad"] = grad;
+            data["recorded"] = recording();
+        }
+        return loss;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        static std::mutex taking;
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &targets = saved[1], &kept = saved[2];
+        const c10::OptionalDeviceGuard guard(x.device());
+        const Tensor up = grads[0].contiguous();
+        TORCH_CHECK(up.scalar_type() == wide(x).dtype() && up.device() == x.device(), "the loss's gradient must be ", wide(x).dtype(), " on ", x.device());
+        Tensor grad;
+        GroupCeCall c;
+        {
+            const std::lock_guard<std::mutex> lock(taking);
+            auto &data = ctx->saved_data;
+            c.k = data.at("k").toInt(), c.tau = data.at("tau").toDouble(), c.smoothing = data.at("smoothing").toDouble(), c.weight = data.at("weight").toDouble();
+            c.reduction = data.at("reduction").toInt();
+            const auto it = data.find("grad");
+            if (it != data.end() && data.at("recorded").toInt() == recording()) {
+                grad = it->second.toTensor();
+                data.erase("grad");
+            }
+        }
+        const bool has_grad = grad.defined();
+        if (!has_grad) grad = like_features(x);
+        const Rows r(x);
+        check(clg_group_ce_backward(code_of(x), r.at, in_columns(x) ? -1 : r.stride, r.rows, r.cols, c.k, targets.data_ptr(), 8 * (int)targets.element_size(), c.tau,
+                                    c.smoothing, c.weight, (int)c.reduction, up.data_ptr(), grad.data_ptr(), has_grad, kept.data_ptr(), stream_of(x)));
+        return once({grad, Tensor()});
+    }
+};
+Tensor group_ce(const Tensor &x, const Tensor &targets, int64_t k, double tau, double smoothing, double weight, int64_t reduction)
+{
+    const GroupCeCall c{targets.contiguous(), k, tau, smoothing, weight, reduction, x.requires_grad() && at::GradMode::is_enabled()};
+    return GroupCe::apply(in_columns(x) ? x : rows_of(x), &c);
+}
+
 template <typename F>
 void name_node(const char *name)
 {
@@ -265,6 +342,8 @@ void add_loss_nodes(pybind11::module_ &m)
     const auto no_gil = pybind11::call_guard<pybind11::gil_scoped_release>();
     name_node<Distill>("_DistillationBackward");
     name_node<Balance>("_BalanceBackward");
+    name_node<GroupCe>("_GroupCrossEntropyBackward");
+    m.def("group_ce", &group_ce, no_gil);
     m.def("top_logits", &top_logits, no_gil);
     m.def("distillation", &distillation, no_gil);
     m.def("balance", &balance, no_gil);

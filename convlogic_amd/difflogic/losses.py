@@ -1,11 +1,12 @@
 """Losses on the scores of a network and on the logits of its gates, and what they need of a teacher: its highest logits.
 
+  group_cross_entropy cross entropy of a network's GroupSum, from the features that it sums
   top_logits          the highest logits of each row, their columns and the logsumexp of the row: what a teacher's answers are stored as
   distillation_loss   the loss of a student against such answers
   balance_loss        how evenly rows choose among experts, and how many rows chose each
   gate_balance        the same for the gates of a layer or a whole network, 16 to a neuron
 
-Tensors on the GPU go through HIP kernels (csrc/top_logits.hip, csrc/distill.hip, csrc/balance.hip) and raise if the compiled library is missing;
+Tensors on the GPU go through HIP kernels (csrc/group_ce.hip, csrc/top_logits.hip, csrc/distill.hip, csrc/balance.hip) and raise if the compiled library is missing;
 tensors on the CPU, as networks with implementation="python" have them, through plain torch operations.  No counterpart in the reference."""
 import math
 from typing import NamedTuple
@@ -181,6 +182,51 @@ def _distillation_plain(logits, values, indices, logsumexp, temperature, mask, w
         return loss.to(_wide(logits).dtype)
     count = lead.numel() if mask is None else int(mask.sum())
     return (loss.sum() / (max(count, 1) if reduction == "mean" else 1)).to(_wide(logits).dtype)
+
+
+# ---- cross entropy of group sums -----------------------------------------------------------------
+def group_cross_entropy(x, targets, k, tau=1.0, *, label_smoothing=0.0, weight=1.0, reduction="mean"):
+    """weight * cross_entropy(GroupSum(k, tau)(x), targets, label_smoothing=...) of x [..., features], without scores in memory beyond the call: a class is
+    features / k features in a row, its score their sum over tau, and k = features takes x as scores.
+
+    targets int32 or int64 [...]: a row with a negative one does not count -- loss 0 and gradient 0, whatever its features are -- and one of k or more makes
+    the loss and gradient of its row NaN.  reduction: "mean" over the rows that count (0 if none does), "sum", or "none" for a loss per row.  Sums over features
+    are 64-bit numbers.  The loss is float32 (float64 of float64 features), the gradient has the type of the features, and their layout where x is the
+    transposed view that a LogicLayer returns.
+
+    As with distillation_loss, the gradient is computed along with the loss, for an upstream gradient of 1: a factor that is known goes into `weight`."""
+    _check_scores(x, "x")
+    k, tau, weight = int(k), _check_number(tau, "tau", positive=True), _check_number(weight, "weight")
+    label_smoothing = _check_number(label_smoothing, "label_smoothing")
+    if not isinstance(targets, torch.Tensor) or targets.dtype not in (torch.int32, torch.int64) or targets.shape != x.shape[:-1]:
+        raise RuntimeError(f"targets must be an int32 or int64 tensor of shape {tuple(x.shape[:-1])}, got "
+                           + (f"{targets.dtype} {tuple(targets.shape)}" if isinstance(targets, torch.Tensor) else f"{type(targets)}"))
+    _lib.check_same_device(x, targets)
+    if k < 1 or x.shape[-1] % k:
+        raise ValueError(f"k must be a divisor of the {x.shape[-1]} features, got {k}")
+    if not 0 <= label_smoothing <= 1:
+        raise ValueError(f"label_smoothing must be between 0 and 1, got {label_smoothing}")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    if x.is_cuda:
+        return _nodes("group_cross_entropy").group_ce(x, targets, k, tau, label_smoothing, weight, _REDUCTIONS[reduction])
+    return _group_ce_plain(x, targets, k, tau, label_smoothing, weight, reduction)
+
+
+def _group_ce_plain(x, targets, k, tau, smoothing, weight, reduction):
+    keep, bad = targets >= 0, targets >= k
+    # rows that do not count are rows of zeros from here on: no inf or NaN of theirs reaches a gradient
+    rows = torch.where(keep.unsqueeze(-1), _wide(x), 0.0).double()
+    scores = rows.reshape(*x.shape[:-1], k, x.shape[-1] // k).sum(-1) / tau
+    scores = scores * torch.where(bad, math.nan, 1.0).unsqueeze(-1)
+    log_p = torch.log_softmax(scores, -1)
+    loss = -log_p.gather(-1, torch.where(keep & ~bad, targets, 0).long().unsqueeze(-1)).squeeze(-1)
+    if smoothing:
+        loss = (1 - smoothing) * loss - smoothing * log_p.mean(-1)
+    loss = torch.where(keep, loss, 0.0) * weight
+    if reduction == "mean":
+        loss = loss / max(int(keep.sum()), 1)
+    return (loss if reduction == "none" else loss.sum()).to(_wide(x).dtype)
 
 
 # ---- balance -------------------------------------------------------------------------------------

@@ -715,6 +715,25 @@ int clg_balance_forward(int dtype, int n, const void *const *logits, const int64
 int clg_balance_backward(int dtype, int n, const void *const *logits, const int64_t *rows, const int64_t *row_strides, int64_t experts,
                          const uint8_t *mask, const void *coefs, const void *upstream, void *const *grads, void *stream);
 
+/* Softmax cross entropy of group sums: features / k features of a row are a class, its score their sum over tau (what a GroupSum computes), and with
+ * smoothing e the loss of a row is weight times (1 - e) (logsumexp - score of its target) + e (logsumexp - mean score).  A row with a negative target does not
+ * count: loss 0 and gradient 0, whatever its features are; a target of k or more makes its row NaN.  CLG_REDUCE_MEAN divides by the number of rows that count
+ * (none: 0).
+ *   x         rows of dense features, row_stride elements apart, or for row_stride -1 "columns": [features, rows] dense
+ *   loss      one value, or [rows] for CLG_REDUCE_NONE; float32, float64 for CLG_F64
+ *   grad      NULL, or of x's shape, dense: the gradient for an upstream gradient of 1 (not for CLG_REDUCE_NONE)
+ *   kept      clg_group_ce_kept_bytes() bytes, as the forward call left them, for clg_group_ce_backward; scratch: clg_group_ce_scratch_bytes(), free afterwards
+ * clg_group_ce_backward: upstream is one value, or [rows] for CLG_REDUCE_NONE.  With has_grad, grad is what the forward call left, and stays as it is for
+ * an upstream gradient of 1. */
+int64_t clg_group_ce_kept_bytes(int dtype, int columns, int64_t rows, int64_t features, int64_t k);
+int64_t clg_group_ce_scratch_bytes(int dtype, int columns, int64_t rows, int64_t features, int64_t k);
+int clg_group_ce_forward(int dtype, const void *x, int64_t row_stride, int64_t rows, int64_t features, int64_t k, const void *targets /*[rows]*/,
+                         int targets_bits /*32 or 64*/, double tau, double smoothing, double weight, int reduction, void *loss, void *grad, void *kept,
+                         void *scratch, void *stream);
+int clg_group_ce_backward(int dtype, const void *x, int64_t row_stride, int64_t rows, int64_t features, int64_t k, const void *targets, int targets_bits,
+                          double tau, double smoothing, double weight, int reduction, const void *upstream, void *grad, int has_grad, const void *kept,
+                          void *stream);
+
 /* ---------------------------------------------------------------------------------
  * activations in 8 bits (no counterpart in the reference)
  * ------------------------------------------------------------------------------- */
