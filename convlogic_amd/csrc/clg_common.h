@@ -256,6 +256,38 @@ __device__ __forceinline__ T row16_max(T v)
 template <typename T>
 __device__ __forceinline__ T softmax16_backward(T g, T p) { return p * (g - row16_sum(p * g)); }
 
+// Softmax and fold of 16 logits by the 16 lanes of a row, lane q with logit q: the coefficients, in all lanes, as dot products with the integer patterns of
+// fold16 (c_1 = the sum of gates 8 to 15), and the lane's probability.
+template <typename T>
+struct Fold16 {
+    T w_ab, w_a, w_b, w_1;
+    __device__ __forceinline__ explicit Fold16(int q)
+    {
+        constexpr int kAb[16] = {0, 1, -1, 0, -1, 0, -2, -1, 1, 2, 0, 1, 0, 1, -1, 0};
+        constexpr int kA[16] = {0, 0, 1, 1, 0, 0, 1, 1, -1, -1, 0, 0, -1, -1, 0, 0};
+        constexpr int kB[16] = {0, 0, 0, 0, 1, 1, 1, 1, -1, -1, -1, -1, 0, 0, 0, 0};
+        int ab = 0, aa = 0, bb = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {                                // selects, not a table in memory
+            ab = q == i ? kAb[i] : ab;
+            aa = q == i ? kA[i] : aa;
+            bb = q == i ? kB[i] : bb;
+        }
+        w_ab = (T)ab, w_a = (T)aa, w_b = (T)bb, w_1 = q >= 8 ? T(1) : T(0);
+    }
+    __device__ __forceinline__ Coef<T> operator()(T logit, T &p) const
+    {
+        const T e = exp(logit - row16_max(logit));
+        p = e * (T(1) / row16_sum(e));
+        Coef<T> c;
+        c.ab = row16_sum(p * w_ab);
+        c.a = row16_sum(p * w_a);
+        c.b = row16_sum(p * w_b);
+        c.one = row16_sum(p * w_1);
+        return c;
+    }
+};
+
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // A wiring / reverse-map entry as the kernels use it: forced into 0..n-1, so that a corrupted index buffer (the host checks

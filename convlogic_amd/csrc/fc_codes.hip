@@ -7,6 +7,8 @@
 namespace {
 
 constexpr int kWaves = 4, kBlock = kWaves * kWave;
+constexpr int64_t kFull = 256 * 32, kTurns = 4;                       // wavefronts that the chip holds; items that one takes, from there on
+constexpr int kWalk = 8;                                              // lanes' worth of a walk over the wiring
 typedef float f32x4_row __attribute__((ext_vector_type(4), aligned(4)));
 
 template <int VEC>
@@ -27,14 +29,11 @@ __device__ __forceinline__ void store_floats(float *__restrict__ p, const float 
     else *p = v[0];
 }
 
-// Coefficients of a neuron as clg_fc_fold leaves them.
-struct Gate {
-    float ab, a, b;
-    __device__ __forceinline__ explicit Gate(const float *__restrict__ folded)
-    {
-        const float4 v = *reinterpret_cast<const float4 *>(folded);
-        ab = v.x, a = v.y, b = v.z;
-    }
+// What a backward pass needs of a neuron, in one line of memory (its wiring and its coefficients in tables of their own were three lines for each visit): the inputs
+// of its operands and the coefficients, as the forward pass leaves them.
+struct __attribute__((aligned(16))) Neuron {
+    int32_t in_a, in_b;
+    float ab, a, b, one, unused[2];
 };
 
 // The lane's samples: VEC of them from `at` on.  The last lane of a row that VEC does not divide steps back to its last VEC samples, of which `again` are its
@@ -76,18 +75,116 @@ struct Sums {
         b = lane_group_sum<float, LPR>(b);
         one = lane_group_sum<float, LPR>(one);
     }
+    // their sums over LPR lanes, of which l is this one, at `to`: every exchange between rows of 16 lanes halves the number of values that a row has
+    template <int LPR>
+    __device__ __forceinline__ void store(float4 *to, int l) const
+    {
+        float *at = reinterpret_cast<float *>(to);
+        if constexpr (LPR == 64) {
+            const float v = row16_sum(swap_add16(swap_add32(ab, b), swap_add32(a, one)));      // row 0: ab, 1: a, 2: b, 3: one
+            if ((l & 15) == 0) at[l >> 4] = v;
+        } else if constexpr (LPR == 32) {
+            const float u = row16_sum(swap_add16(ab, a)), v = row16_sum(swap_add16(b, one));
+            if ((l & 15) == 0) at[l >> 4] = u, at[2 + (l >> 4)] = v;
+        } else {
+            const float4 v = {row16_sum(ab), row16_sum(a), row16_sum(b), row16_sum(one)};
+            if (l == 0) *to = v;
+        }
+    }
     __device__ __forceinline__ float of_logit(int q, float p) const { return softmax16_backward(coef_transpose_row<float>(q, ab, a, b, one), p); }
 };
 
 struct Layer {
-    const uint8_t *codes;
-    const CodeScale<float> *scales;
+    uint8_t *codes;
+    CodeScale<float> *scales;
+    Neuron *neurons;
     const int64_t *a, *b, *start, *list;
-    const float *folded, *probs, *gy;
-    float *gx, *gl;
+    const float *x, *logits, *gy;
+    float *probs, *y, *gx, *gl;
     float4 *sums;                                                     // [chunks][out_dim]
     int64_t in_dim, out_dim, batch;
 };
+
+// The 128 samples that 32 lanes have of an input become codes.
+__device__ __forceinline__ float over_rows(float v, bool highest)     // of two rows of 16 lanes, the same in both
+{
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    const float p = __builtin_bit_cast(float, (unsigned)r[0]), q = __builtin_bit_cast(float, (unsigned)r[1]);
+    return highest ? max_of(p, q) : min_of(p, q);
+}
+__device__ __forceinline__ void encode_row(const Layer &L, int64_t at, const float (&v)[4])
+{
+    float low = min_of(min_of(v[0], v[1]), min_of(v[2], v[3])), high = max_of(max_of(v[0], v[1]), max_of(v[2], v[3]));
+    low = over_rows(-row16_max(-low), false);
+    high = over_rows(row16_max(high), true);
+    const Coder code((double)low, (double)high);
+    bool bad = !(code.size * 255.0 <= __DBL_MAX__);
+    uint32_t c[1];
+    code(v, c, bad);
+    bad = (uint32_t)(__ballot(bad) >> (threadIdx.x & 32)) != 0;
+    *reinterpret_cast<uint32_t *>(L.codes + at) = bad ? 0 : c[0];
+    if ((threadIdx.x & 31) == 0) L.scales[at / kCodeGroup] = scale_of(low, code, bad);
+}
+
+// Forward pass from the logits, with the arithmetic of clg_fc_forward_logits; a neuron takes LPR lanes.  ENCODE: every input is read by one operand only, whose
+// neuron also makes its codes, and the batch is a multiple of 128, so that a row of 32 lanes has a group (x is then read once, not twice: 163840 inputs, batch
+// 256, forward pass and codes 110 -> 68 us).  Else the workgroups from neuron_blocks on make them.  The wiring and the logits of a wavefront's next neurons are on
+// their way while the rows of these are.
+template <int VEC, bool RAGGED, int LPR, bool ENCODE>
+__global__ __launch_bounds__(kBlock) void forward_kernel(Layer L, int neuron_blocks)
+{
+    constexpr int ROWS = kWave / LPR;
+    if (!ENCODE && (int)blockIdx.x >= neuron_blocks) {
+        encode_groups(L.x, L.in_dim * L.batch, L.codes, L.scales, (int64_t)(blockIdx.x - neuron_blocks) * (kBlock / kCodeLanes) + threadIdx.x / kCodeLanes,
+                      (int64_t)(gridDim.x - neuron_blocks) * (kBlock / kCodeLanes));
+        return;
+    }
+    const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x >> 6), sub = lane / LPR, l = lane % LPR, q = lane & 15;
+    const Fold16<float> fold(q);
+    const int64_t step = (int64_t)neuron_blocks * kWaves * ROWS;
+    struct Wiring {
+        int64_t a, b;
+        float logit;
+        __device__ __forceinline__ Wiring(const Layer &L, int64_t j, int q) : a(L.a[j]), b(L.b[j]), logit(L.logits[j * 16 + q]) {}
+    };
+    int64_t j0 = ((int64_t)blockIdx.x * kWaves + wave) * ROWS;
+    if (j0 >= L.out_dim) return;
+    const auto neuron = [&](int64_t first) { return first + sub < L.out_dim ? first + sub : L.out_dim - 1; };
+    for (Wiring next(L, neuron(j0), q); j0 < L.out_dim; j0 += step) {
+        const bool valid = j0 + sub < L.out_dim;
+        const int64_t j = neuron(j0);                                 // every lane takes part in the sums
+        const int32_t ia = (int32_t)clamp_index(next.a, L.in_dim), ib = (int32_t)clamp_index(next.b, L.in_dim);
+        const float logit = next.logit;
+        float x[VEC], y[VEC], out[VEC];
+        int64_t s = (int64_t)l * VEC;
+        Samples<VEC, RAGGED> mine(s, L.batch);
+        load_floats(L.x + ia * L.batch + mine.at, x);
+        load_floats(L.x + ib * L.batch + mine.at, y);
+        if (j0 + step < L.out_dim) next = Wiring(L, neuron(j0 + step), q);
+        float p;
+        const Coef<float> c = fold(logit, p);
+        if (valid && l < 16) {
+            L.probs[j * 16 + q] = p;
+            const float wiring = __builtin_bit_cast(float, q == 0 ? ia : ib), coef = q == 2 ? c.ab : q == 3 ? c.a : q == 4 ? c.b : c.one;
+            if (q < 6) reinterpret_cast<float *>(L.neurons + j)[q] = q < 2 ? wiring : coef;
+        }
+        if (!valid) continue;
+        while (s < L.batch) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) out[k] = gate(c, x[k], y[k]);
+            store_floats(L.y + j * L.batch + mine.at, out);
+            if constexpr (ENCODE) {
+                encode_row(L, ia * L.batch + mine.at, x);
+                encode_row(L, ib * L.batch + mine.at, y);
+            }
+            s += LPR * VEC;
+            if (s >= L.batch) break;
+            mine = Samples<VEC, RAGGED>(s, L.batch);
+            load_floats(L.x + ia * L.batch + mine.at, x);
+            load_floats(L.x + ib * L.batch + mine.at, y);
+        }
+    }
+}
 
 // A neuron takes LPR lanes, which go through its three rows; with GX every input is read by one operand only, whose neuron writes its gradient.
 template <int VEC, bool RAGGED, int LPR, bool GX>
@@ -98,16 +195,19 @@ __global__ __launch_bounds__(kBlock) void neurons_kernel(Layer L)
     for (int64_t j0 = ((int64_t)blockIdx.x * kWaves + wave) * ROWS; j0 < L.out_dim; j0 += (int64_t)gridDim.x * kWaves * ROWS) {
         const bool valid = j0 + sub < L.out_dim;
         const int64_t j = valid ? j0 + sub : L.out_dim - 1;           // every lane takes part in the sums
-        const int64_t ia = clamp_index(L.a[j], L.in_dim) * L.batch, ib = clamp_index(L.b[j], L.in_dim) * L.batch;
-        const Gate c(L.folded + j * 4);
+        const Neuron c = L.neurons[j];
+        const int64_t ia = c.in_a * L.batch, ib = c.in_b * L.batch;
         const float p = L.probs[j * 16 + q];
         Sums sums;
         for (int64_t s = (int64_t)l * VEC; s < L.batch; s += LPR * VEC) {
             const Samples<VEC, RAGGED> mine(s, L.batch);
             float x[VEC], y[VEC], g[VEC];
             load_floats(L.gy + j * L.batch + mine.at, g);
-            decode_at<VEC, RAGGED>(L.codes, L.scales, ia + mine.at, x);
-            decode_at<VEC, RAGGED>(L.codes, L.scales, ib + mine.at, y);
+            Coded<VEC, RAGGED> cx, cy;
+            cx.load(L.codes, L.scales, ia + mine.at);
+            cy.load(L.codes, L.scales, ib + mine.at);
+            cx.values(x);
+            cy.values(y);
             sums.add(g, x, y, mine.again);
             if (GX && valid) {
                 float ga[VEC], gb[VEC];
@@ -128,127 +228,211 @@ __global__ __launch_bounds__(kBlock) void neurons_kernel(Layer L)
     }
 }
 
-// An input takes LPR lanes, which walk the operands it is (`list`) for LPR * VEC samples.  With SUMS != kNoSums the visit that reaches a neuron through its first
-// operand has all its rows and forms its sums as well: the gradient of its logits if the samples are the whole batch (kWhole), else for gradients_kernel (kParts).
-// A neuron wired to an input twice is listed twice, and is its second operand the second time.
-// Operands go by fours, with a sum of their own per place: the rows of four are fetched and used while the wiring of the next four and the list entries of
-// those behind are on their way.  All loads are from valid addresses, and what does not count is dropped afterwards: a load under a lane's condition
-// would be waited for at the end of its branch.
+// value of lane `at` of the LPR lanes of a row, in all of them
+template <int LPR>
+__device__ __forceinline__ int32_t from_lane(int32_t v, int at)
+{
+    if constexpr (LPR == kWave) return __builtin_amdgcn_readlane(v, at);
+    else return __shfl(v, at, LPR);
+}
+template <int LPR>
+__device__ __forceinline__ float from_lane(float v, int at) { return __builtin_bit_cast(float, from_lane<LPR>(__builtin_bit_cast(int32_t, v), at)); }
+template <int LPR>
+__device__ __forceinline__ uint32_t from_lane(uint32_t v, int at) { return (uint32_t)from_lane<LPR>((int32_t)v, at); }
+template <int LPR>
+__device__ __forceinline__ uint64_t from_lane(uint64_t v, int at)
+{
+    return (uint64_t)from_lane<LPR>((uint32_t)(v >> 32), at) << 32 | from_lane<LPR>((uint32_t)v, at);
+}
+
+// LPR lanes take `each` inputs one after the other and go through the operands these are, which follow one another in `list`, for LPR * VEC samples.  The
+// visit that reaches a neuron through its first operand has all its rows and forms its sums as well (SUMS): the gradient of its logits if the samples are the
+// whole batch (kWhole), else for gradients_kernel (kParts).  A neuron wired to an input twice is listed twice, and is its second operand the second time.
+// The way to a row -- list entry, neuron, row -- is three trips to memory: the lanes first go it for as many operands as they are, one each, and then
+// take these one by one, with the rows of the next two on their way (of the next four: 28 to 57 registers more, and 8000 -> 8000 neurons, batch 100, 9.7 us, not
+// 7.9).  I: what holds an index into x and gy.
+// 131072 -> 1310720 neurons, batch 128: 365 us for 1.3 GB of gradients that are read twice, 0.3 of codes and 0.2 of the rest, 5 TB/s; a walk operand by operand, with
+// the wiring and the coefficients in tables of their own, took 623.
 enum { kNoSums, kWhole, kParts };
-template <int VEC, bool RAGGED, int LPR, int SUMS>
-__global__ __launch_bounds__(kBlock) void inputs_kernel(Layer L)
+constexpr int kEachMost = 15;
+template <int VEC, bool RAGGED, int LPR, int SUMS, typename I>
+__global__ __launch_bounds__(kBlock) void inputs_kernel(Layer L, int each)
 {
     constexpr int ROWS = kWave / LPR;
-    struct Operands {
-        int32_t j[4], other[4];                                       // neuron (-1: none), input of its other operand
-        float c_ab[4], c_own[4], p[4];
-        bool first[4];
-    };
+    constexpr int kOwner = 15, kFirst = 16, kLast = 32;
     const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x >> 6), sub = lane / LPR, l = lane % LPR, q = lane & 15;
-    const int64_t groups = (L.in_dim + ROWS - 1) / ROWS, last = 2 * L.out_dim - 1;
+    const int64_t groups = (L.in_dim + each - 1) / each, most = 2 * L.out_dim;
+    const I batch = (I)L.batch;
     const Samples<VEC, RAGGED> mine(((int64_t)blockIdx.y * LPR + l) * VEC, L.batch);
-    for (int64_t it = (int64_t)blockIdx.x * kWaves + wave; it < groups; it += (int64_t)gridDim.x * kWaves) {
-        const bool valid = it * ROWS + sub < L.in_dim;
-        const int64_t i = valid ? it * ROWS + sub : L.in_dim - 1;
-        const int64_t begin = clamp_index(L.start[i], last + 2), end = valid ? clamp_index(L.start[i + 1], last + 2) : begin;
-        const bool live = valid && mine.live;
-        const auto entries = [&](int64_t at, int32_t (&j)[4]) {
+    const I mine_at = (I)mine.at;
+    struct Rows {
+        Coded<VEC, RAGGED> x, own;
+        float g[VEC];
+        int mark;
+    };
+    for (int64_t it = ((int64_t)blockIdx.x * kWaves + wave) * ROWS; it < groups; it += (int64_t)gridDim.x * kWaves * ROWS) {
+        const bool valid = it + sub < groups;
+        const int64_t i0 = valid ? (it + sub) * each : 0;
+        const int count = !valid ? 0 : L.in_dim - i0 < each ? (int)(L.in_dim - i0) : each;
+        const int64_t begin = clamp_index(L.start[i0], most + 1);
+        const int ends = (int)(clamp_index(L.start[i0 + (l < count ? l + 1 : count)], most + 1) - begin);       // lane l: behind input l, from `begin` on
+        const int edges = valid ? max(from_lane<LPR>(ends, count > 0 ? count - 1 : 0), 0) : 0;
+        int longest = edges;                                          // of the rows of a wavefront
+        if constexpr (LPR <= 32) longest = max(longest, __shfl_xor(longest, 32));
+        if constexpr (LPR <= 16) longest = max(longest, __shfl_xor(longest, 16));
+        longest = uniform(longest);
+        const I own_at = (I)i0 * batch + mine_at;                     // the first input's
+        float acc[VEC];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int32_t v = (int32_t)clamp_index(L.list[at + u < last ? at + u : last], L.out_dim);
-                j[u] = at + u < end ? v : -1;
+        for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+        for (int base = 0; base < longest; base += LPR) {
+            // an operand for each lane
+            const int at = base + l;
+            const bool there = at < edges;
+            const int64_t place = begin + (there ? at : 0);
+            const int32_t j = (int32_t)clamp_index(L.list[place < most ? place : most - 1], L.out_dim);
+            const int32_t before = (int32_t)L.list[place > 0 ? (place < most ? place : most - 1) - 1 : 0];
+            const Neuron n = L.neurons[j];
+            int owner = 0, opened = 0, closed = edges;                // input, from the first; its operands are opened .. closed
+            for (int k = 0; k < each; ++k) {
+                const int e = from_lane<LPR>(ends, k);
+                if (k < count - 1 && e <= at) owner = k + 1, opened = e;
             }
-        };
-        const auto wiring = [&](const int32_t (&j)[4], int32_t before, Operands &m) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int64_t jj = j[u] < 0 ? 0 : j[u];
-                const int64_t ja = clamp_index(L.a[jj], L.in_dim), jb = clamp_index(L.b[jj], L.in_dim);
-                const Gate c(L.folded + jj * 4);
-                if (SUMS == kWhole) m.p[u] = L.probs[jj * 16 + q];
-                const bool as_a = ja == i && !(jb == i && before == j[u]);
-                m.j[u] = j[u];
-                m.first[u] = j[u] >= 0 && as_a;
-                m.other[u] = (int32_t)(as_a ? jb : ja);
-                m.c_ab[u] = j[u] >= 0 ? c.ab : 0.f;
-                m.c_own[u] = j[u] >= 0 ? (as_a ? c.a : c.b) : 0.f;
-                before = j[u];
+            for (int k = each - 1; k >= 0; --k) {
+                const int e = from_lane<LPR>(ends, k);
+                if (k < count && k >= owner) closed = e;
             }
-        };
-        float own[VEC];
-        if (SUMS != kNoSums) decode_at<VEC, RAGGED>(L.codes, L.scales, i * L.batch + mine.at, own);
-        float part[4][VEC];
+            const int32_t i = (int32_t)i0 + owner;
+            const bool as_a = n.in_a == i && !(n.in_b == i && at > opened && before == j);
+            const int mark = owner | (there && as_a ? kFirst : 0) | (there && at + 1 == closed ? kLast : 0);
+            const I row_x = there ? (I)(as_a ? n.in_b : n.in_a) * batch : I(0), row_g = there ? (I)j * batch : I(0);
+            const float c_ab = there ? n.ab : 0.f, c_own = there ? (as_a ? n.a : n.b) : 0.f;
+            const int steps = longest - base < LPR ? longest - base : LPR;
+            const auto load = [&](int e, Rows &r) {
+                const int from = e < LPR ? e : LPR - 1;               // (what is behind the last of a row is dropped)
+                r.mark = from_lane<LPR>(mark, from);
+                const float *g = L.gy + (from_lane<LPR>(row_g, from) + mine_at);
+                load_floats(g, r.g);
+                r.x.load(L.codes, L.scales, (I)(from_lane<LPR>(row_x, from) + mine_at));
+                if (SUMS != kNoSums) r.own.load(L.codes, L.scales, (I)(own_at + (I)(r.mark & kOwner) * batch));
+            };
+            const auto take = [&](int e, const Rows &r) {
+                if (e >= steps) return;
+                const float ab = from_lane<LPR>(c_ab, e), lin = from_lane<LPR>(c_own, e);
+                float x[VEC];
+                r.x.values(x);
+                // (an operand that is not there has coefficients 0, and a gradient that may be infinite)
+                if (LPR == kWave || base + e < edges) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+                    for (int k = 0; k < VEC; ++k) acc[k] = __builtin_fmaf(__builtin_fmaf(ab, x[k], lin), r.g[k], acc[k]);
+                }
+                if (SUMS != kNoSums) {
+                    const int32_t to = from_lane<LPR>(j, e);
+                    if (r.mark & kFirst) {                            // uniform over the lanes of a row
+                        float own[VEC];
+                        r.own.values(own);
+                        Sums sums;
+                        sums.add(r.g, own, x, mine.live ? mine.again : VEC);
+                        if constexpr (SUMS == kWhole) {
+                            sums.over_lanes<LPR>();
+                            if (l >= LPR - 16) L.gl[(int64_t)to * 16 + q] = sums.of_logit(q, L.probs[(int64_t)to * 16 + q]);
+                        } else {
+                            sums.store<LPR>(L.sums + (int64_t)blockIdx.y * L.out_dim + to, l);
+                        }
+                    }
+                }
+                if (r.mark & kLast) {
+                    if (mine.live) store_floats(L.gx + (own_at + (I)(r.mark & kOwner) * batch), acc);
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) part[u][k] = 0.f;
-        int32_t next[4], after[4];
-        Operands now, then;
-        entries(begin, next);
-        wiring(next, -1, now);
-        entries(begin + 4, next);
-        for (int64_t at = begin; at < end; at += 4) {                 // (the lanes of a row leave the loop together)
-            float x[4][VEC], g[4][VEC];
+                    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+                }
+            };
+            constexpr int AHEAD = 2;
+            Rows rows[AHEAD];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                decode_at<VEC, RAGGED>(L.codes, L.scales, (int64_t)now.other[u] * L.batch + mine.at, x[u]);
-                load_floats(L.gy + (int64_t)(now.j[u] < 0 ? 0 : now.j[u]) * L.batch + mine.at, g[u]);
-            }
-            wiring(next, now.j[3], then);
-            entries(at + 8, after);
+            for (int u = 0; u < AHEAD; ++u) load(u, rows[u]);
+            for (int e = 0; e < steps; e += AHEAD) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (now.j[u] < 0) continue;
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) part[u][k] = __builtin_fmaf(__builtin_fmaf(now.c_ab[u], x[u][k], now.c_own[u]), g[u][k], part[u][k]);
-                if (SUMS != kNoSums && now.first[u]) {                // uniform over the lanes of a row
-                    Sums sums;
-                    sums.add(g[u], own, x[u], mine.live ? mine.again : VEC);
-                    sums.over_lanes<LPR>();
-                    if (SUMS == kWhole && l >= LPR - 16) L.gl[(int64_t)now.j[u] * 16 + q] = sums.of_logit(q, now.p[u]);
-                    if (SUMS == kParts && l == LPR - 1) L.sums[(int64_t)blockIdx.y * L.out_dim + now.j[u]] = float4{sums.ab, sums.a, sums.b, sums.one};
+                for (int u = 0; u < AHEAD; ++u) {
+                    take(e + u, rows[u]);
+                    load(e + u + AHEAD, rows[u]);
                 }
             }
-            now = then;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) next[u] = after[u];
         }
-        float sum[VEC];
+        // inputs that nobody reads
+        for (int k = 0; k < each; ++k) {
+            const int e = from_lane<LPR>(ends, k), b = k ? from_lane<LPR>(ends, k - 1) : 0;
+            if (k < count && e <= b && mine.live) {
+                float none[VEC];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) sum[k] = (part[0][k] + part[1][k]) + (part[2][k] + part[3][k]);
-        if (live) store_floats(L.gx + i * L.batch + mine.at, sum);
+                for (int v = 0; v < VEC; ++v) none[v] = 0.f;
+                store_floats(L.gx + (own_at + (I)k * batch), none);
+            }
+        }
     }
 }
 
-// The gradient of the logits from the sums of inputs_kernel's parts of the batch, added in their order: 16 lanes to a neuron.
-__global__ __launch_bounds__(kBlock) void gradients_kernel(const float4 *__restrict__ sums, const float *__restrict__ probs, float *__restrict__ gl, int64_t out_dim,
+// The gradient of the logits from the sums of inputs_kernel's parts of the batch, added in their order: four lanes to a neuron, with four logits each.
+__global__ __launch_bounds__(kBlock) void gradients_kernel(const float4 *__restrict__ sums, const float4 *__restrict__ probs, float4 *__restrict__ gl, int64_t out_dim,
                                                          int chunks)
 {
-    for (int64_t e = (int64_t)blockIdx.x * kBlock + threadIdx.x; e < out_dim * 16; e += (int64_t)gridDim.x * kBlock) {
-        Sums s;
-        for (int c = 0; c < chunks; ++c) {
-            const float4 v = sums[c * out_dim + e / 16];
-            s.ab += v.x, s.a += v.y, s.b += v.z, s.one += v.w;
+    const int i = (threadIdx.x & 3) * 4;
+    for (int64_t e = (int64_t)blockIdx.x * kBlock + threadIdx.x; e < out_dim * 4; e += (int64_t)gridDim.x * kBlock) {
+        const float4 v = probs[e];
+        float4 s = sums[e / 4];
+        for (int c = 1; c < chunks; ++c) {
+            const float4 u = sums[c * out_dim + e / 4];
+            s.x += u.x, s.y += u.y, s.z += u.z, s.w += u.w;
         }
-        gl[e] = s.of_logit((int)(e & 15), probs[e]);
+        const float p[4] = {v.x, v.y, v.z, v.w};
+        float g[4], mean = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) g[k] = coef_transpose_row<float>(i + k, s.x, s.y, s.z, s.w), mean = __builtin_fmaf(p[k], g[k], mean);
+        mean += dpp_zero<0xB1, 0xF>(mean);
+        mean += dpp_zero<0x4E, 0xF>(mean);
+        gl[e] = float4{p[0] * (g[0] - mean), p[1] * (g[1] - mean), p[2] * (g[2] - mean), p[3] * (g[3] - mean)};
     }
 }
 
 // Four samples to a lane from 17 samples on, or where they divide the batch.
 bool fours(int64_t batch) { return batch % 4 == 0 || batch > 16; }
+// Lanes of a row: as many as it takes, up to a wavefront.
 int lanes_of(int64_t batch)
 {
     const int64_t lanes = fours(batch) ? clg_ceil_div(batch, 4) : batch;
     return lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64;
 }
-int64_t chunks_of(int64_t batch) { return clg_ceil_div(batch, (int64_t)lanes_of(batch) * (fours(batch) ? 4 : 1)); }
+// Where rows go in chunks of the batch, each with a walk over the wiring of its own: lanes that few of them leave idle.
+int chunk_lanes(int64_t batch)
+{
+    int best = lanes_of(batch);
+    const auto cost = [&](int lanes) { return clg_ceil_div(batch, (int64_t)lanes * 4) * (lanes + kWalk); };
+    if (batch > 256)
+        for (int lanes = 32; lanes >= 16; lanes /= 2)
+            if (cost(lanes) < cost(best)) best = lanes;
+    return best;
+}
+int64_t chunks_of(int64_t batch) { return clg_ceil_div(batch, (int64_t)chunk_lanes(batch) * (fours(batch) ? 4 : 1)); }
+
+// Whether gradients_kernel ends the sums, also those of one chunk: with and without it 34.8 + 3.9 and 39.2 us for 30001 -> 60000 neurons, batch 256, 69.0 + 4.7 and
+// 78.6 for 100000 -> 100000; batch 64 14.5 + 3.8 and 16.1, 24.8 + 4.1 and 26.7.
+bool in_parts(int64_t out_dim, int64_t batch) { return chunks_of(batch) > 1 || out_dim * batch >= 1 << 24; }
+
+// Inputs that a row of lanes takes: about 16 operands, worth the way to them, and rows enough to fill the chip.  1, 4 and 15 inputs each: 100000 -> 100000 neurons,
+// batch 256, 94, 70 and 71 us; 30001 -> 60000, batch 333, 85, 77 and 77; 8000 -> 8000, batch 100, 8, 11 and 27; 131072 -> 1310720, batch 128, 369, 372 and 427.
+int inputs_each(int64_t in_dim, int64_t out_dim, int64_t chunks, int rows)
+{
+    const int64_t fan = clg_ceil_div(2 * out_dim, in_dim), by_fan = 16 / fan, by_rows = in_dim * chunks / (rows * 4096);
+    const int64_t each = by_fan < by_rows ? by_fan : by_rows;
+    return (int)(each < 1 ? 1 : each > kEachMost ? kEachMost : each);
+}
 
 // call(VEC, RAGGED, LPR) of the batch as integral constants
 template <typename F>
-void with_rows(int64_t batch, F call)
+void with_rows(int64_t batch, int row_lanes, F call)
 {
     const auto lanes = [&](auto vec, auto ragged) {
-        switch (lanes_of(batch)) {
+        switch (row_lanes) {
         case 16: return call(vec, ragged, std::integral_constant<int, 16>());
         case 32: return call(vec, ragged, std::integral_constant<int, 32>());
         default: return call(vec, ragged, std::integral_constant<int, 64>());
@@ -272,44 +456,90 @@ unsigned blocks_of(int64_t wavefronts)
 extern "C" int64_t clg_fc_codes_scratch_bytes(int64_t out_dim, int64_t batch)
 {
     if (out_dim <= 0 || batch <= 0) return 0;
-    const int64_t chunks = chunks_of(batch);
-    return chunks > 1 ? chunks * out_dim * (int64_t)sizeof(float4) : 0;
+    return in_parts(out_dim, batch) ? chunks_of(batch) * out_dim * (int64_t)sizeof(float4) : 0;
 }
 
-extern "C" int clg_fc_codes_backward(const uint8_t *codes, const void *scales, const int64_t *a, const int64_t *b, const float *folded, const float *probs,
-                                     const float *grad_y, const int64_t *csr_start, const int64_t *csr_list, float *grad_x, float *grad_logits, int64_t in_dim,
-                                     int64_t out_dim, int64_t batch, int sole, void *scratch, void *stream)
+static int check_layer(const char *name, int64_t in_dim, int64_t out_dim, int64_t batch, int sole)
 {
-    const char *name = "clg_fc_codes_backward";
     CLG_REQUIRE(in_dim > 0 && out_dim > 0 && batch > 0, "%s: in_dim, out_dim and batch must be positive (%lld, %lld, %lld)", name, (long long)in_dim,
                 (long long)out_dim, (long long)batch);
-    CLG_REQUIRE(in_dim < (1ll << 31) && out_dim < (1ll << 30) && chunks_of(batch) <= 65535, "%s: 2^31 inputs, 2^30 neurons and batches of more than 65535 times 256 are not supported", name);
-    CLG_REQUIRE(codes && scales && a && b && folded && grad_y && (grad_x || grad_logits), "%s: null pointer argument", name);
+    CLG_REQUIRE(in_dim < (1ll << 31) && out_dim < (1ll << 30), "%s: 2^31 inputs and 2^30 neurons are not supported", name);
+    CLG_REQUIRE(chunks_of(batch) <= 65535, "%s: a batch of %lld is not supported", name, (long long)batch);
+    CLG_REQUIRE(!sole || 2 * out_dim == in_dim, "%s: sole needs 2 out_dim == in_dim, got %lld and %lld", name, (long long)out_dim, (long long)in_dim);
+    return CLG_OK;
+}
+
+extern "C" int clg_fc_codes_forward(const float *x, const int64_t *a, const int64_t *b, const float *logits, float *probs, void *neurons, float *y, uint8_t *codes,
+                                    void *scales, int64_t in_dim, int64_t out_dim, int64_t batch, int sole, void *stream)
+{
+    const char *name = "clg_fc_codes_forward";
+    if (const int rc = check_layer(name, in_dim, out_dim, batch, sole)) return rc;
+    CLG_REQUIRE(x && a && b && logits && probs && neurons && y && codes && scales, "%s: null pointer argument", name);
+    CLG_REQUIRE(reinterpret_cast<uintptr_t>(neurons) % 16 == 0 && reinterpret_cast<uintptr_t>(codes) % 8 == 0, "%s: neurons must be aligned to 16 bytes, codes to 8", name);
+    Layer L{};
+    L.codes = codes, L.scales = static_cast<CodeScale<float> *>(scales), L.neurons = static_cast<Neuron *>(neurons), L.a = a, L.b = b;
+    L.x = x, L.logits = logits, L.probs = probs, L.y = y, L.in_dim = in_dim, L.out_dim = out_dim, L.batch = batch;
+    hipStream_t st = clg_stream(stream);
+    const bool encode = sole && batch % kCodeGroup == 0;
+    with_rows(batch, lanes_of(batch), [&](auto vec, auto ragged, auto lpr) {
+        constexpr int VEC = decltype(vec)::value, LPR = decltype(lpr)::value;
+        constexpr bool RAGGED = decltype(ragged)::value;
+        // (up to four neurons one after the other, from where the chip is full)
+        const int64_t wavefronts = clg_ceil_div(out_dim, (int64_t)(kWave / LPR)), turns = wavefronts / kFull;
+        const int neurons = (int)blocks_of(clg_ceil_div(wavefronts, turns < 1 ? 1 : turns > kTurns ? kTurns : turns));
+        const int coders = encode ? 0 : (int)blocks_of(clg_ceil_div(in_dim * batch, 4 * (int64_t)kCodeLanes * kCodeEach));
+        const dim3 grid((unsigned)(neurons + coders));
+        if constexpr (!RAGGED && LPR >= 32)
+            if (encode) return forward_kernel<VEC, RAGGED, LPR, true><<<grid, dim3(kBlock), 0, st>>>(L, neurons);
+        forward_kernel<VEC, RAGGED, LPR, false><<<grid, dim3(kBlock), 0, st>>>(L, neurons);
+    });
+    CLG_CHECK_LAUNCH(name);
+    return CLG_OK;
+}
+
+extern "C" int clg_fc_codes_backward(const uint8_t *codes, const void *scales, const void *neurons, const float *probs, const float *grad_y, const int64_t *csr_start,
+                                     const int64_t *csr_list, float *grad_x, float *grad_logits, int64_t in_dim, int64_t out_dim, int64_t batch, int sole,
+                                     void *scratch, void *stream)
+{
+    const char *name = "clg_fc_codes_backward";
+    if (const int rc = check_layer(name, in_dim, out_dim, batch, sole)) return rc;
+    CLG_REQUIRE(codes && scales && neurons && grad_y && (grad_x || grad_logits), "%s: null pointer argument", name);
     CLG_REQUIRE(!grad_x || (csr_start && csr_list), "%s: null pointer argument", name);
     CLG_REQUIRE(!grad_logits || probs, "%s: null pointer argument", name);
-    CLG_REQUIRE(!sole || 2 * out_dim == in_dim, "%s: sole needs 2 out_dim == in_dim, got %lld and %lld", name, (long long)out_dim, (long long)in_dim);
-    const bool parts = grad_x && grad_logits && !sole && chunks_of(batch) > 1;
+    const bool parts = grad_x && grad_logits && !sole && in_parts(out_dim, batch);
     CLG_REQUIRE(!parts || scratch, "%s: null scratch", name);
-    const Layer L{codes, static_cast<const CodeScale<float> *>(scales), a, b, csr_start, csr_list, folded, probs, grad_y, grad_x, grad_logits, static_cast<float4 *>(scratch),
-                  in_dim, out_dim, batch};
+    Layer L{};
+    L.codes = const_cast<uint8_t *>(codes), L.scales = static_cast<CodeScale<float> *>(const_cast<void *>(scales));
+    L.neurons = static_cast<Neuron *>(const_cast<void *>(neurons)), L.start = csr_start, L.list = csr_list;
+    L.probs = const_cast<float *>(probs), L.gy = grad_y, L.gx = grad_x, L.gl = grad_logits, L.sums = static_cast<float4 *>(scratch);
+    L.in_dim = in_dim, L.out_dim = out_dim, L.batch = batch;
     hipStream_t st = clg_stream(stream);
-    with_rows(batch, [&](auto vec, auto ragged, auto lpr) {
+    const bool by_neurons = !grad_x || (sole && grad_logits);
+    with_rows(batch, by_neurons ? lanes_of(batch) : chunk_lanes(batch), [&](auto vec, auto ragged, auto lpr) {
         constexpr int VEC = decltype(vec)::value, LPR = decltype(lpr)::value, ROWS = kWave / LPR;
         constexpr bool RAGGED = decltype(ragged)::value;
-        if (!grad_x || (sole && grad_logits)) {
+        if (by_neurons) {
             const dim3 grid(blocks_of(clg_ceil_div(out_dim, (int64_t)ROWS)));
             if (grad_x) neurons_kernel<VEC, RAGGED, LPR, true><<<grid, dim3(kBlock), 0, st>>>(L);
             else neurons_kernel<VEC, RAGGED, LPR, false><<<grid, dim3(kBlock), 0, st>>>(L);
             return;
         }
-        const dim3 grid(blocks_of(clg_ceil_div(in_dim, (int64_t)ROWS)), (unsigned)chunks_of(batch));
-        if (!grad_logits) inputs_kernel<VEC, RAGGED, LPR, kNoSums><<<grid, dim3(kBlock), 0, st>>>(L);
-        else if (parts) inputs_kernel<VEC, RAGGED, LPR, kParts><<<grid, dim3(kBlock), 0, st>>>(L);
-        else inputs_kernel<VEC, RAGGED, LPR, kWhole><<<grid, dim3(kBlock), 0, st>>>(L);
+        const int each = inputs_each(in_dim, out_dim, chunks_of(batch), ROWS);
+        const dim3 grid(blocks_of(clg_ceil_div(clg_ceil_div(in_dim, each), (int64_t)ROWS)), (unsigned)chunks_of(batch));
+        const auto launch = [&](auto index) {
+            typedef decltype(index) I;
+            if (!grad_logits) inputs_kernel<VEC, RAGGED, LPR, kNoSums, I><<<grid, dim3(kBlock), 0, st>>>(L, each);
+            else if (parts) inputs_kernel<VEC, RAGGED, LPR, kParts, I><<<grid, dim3(kBlock), 0, st>>>(L, each);
+            else inputs_kernel<VEC, RAGGED, LPR, kWhole, I><<<grid, dim3(kBlock), 0, st>>>(L, each);
+        };
+        // (the batch behind the last row: what lanes that are dropped read is in front of it)
+        if ((in_dim > out_dim ? in_dim : out_dim) * batch < 1ll << 30) launch(uint32_t());
+        else launch(uint64_t());
     });
     CLG_CHECK_LAUNCH(name);
     if (parts) {
-        gradients_kernel<<<dim3(blocks_of(clg_ceil_div(out_dim, 4))), dim3(kBlock), 0, st>>>(L.sums, probs, grad_logits, out_dim, (int)chunks_of(batch));
+        gradients_kernel<<<dim3(blocks_of(clg_ceil_div(out_dim, 16))), dim3(kBlock), 0, st>>>(L.sums, reinterpret_cast<const float4 *>(probs),
+                                                                                         reinterpret_cast<float4 *>(grad_logits), out_dim, (int)chunks_of(batch));
         CLG_CHECK_LAUNCH(name);
     }
     return CLG_OK;

@@ -415,31 +415,14 @@ __global__ __launch_bounds__(kBlock) void fc_forward_logits_kernel(const T *__re
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
     const int rows = kWave >> lpr_log2, sub = lane >> lpr_log2, l = lane & ((1 << lpr_log2) - 1);
     const int q = lane & 15;
-    // fold16 as dot products with integer patterns; c_1 = sum of gates 8..15
-    constexpr int kAb[16] = {0, 1, -1, 0, -1, 0, -2, -1, 1, 2, 0, 1, 0, 1, -1, 0};
-    constexpr int kA[16] = {0, 0, 1, 1, 0, 0, 1, 1, -1, -1, 0, 0, -1, -1, 0, 0};
-    constexpr int kB[16] = {0, 0, 0, 0, 1, 1, 1, 1, -1, -1, -1, -1, 0, 0, 0, 0};
-    int ab = 0, aa = 0, bb = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {                                    // selects, not a table in memory
-        ab = q == i ? kAb[i] : ab;
-        aa = q == i ? kA[i] : aa;
-        bb = q == i ? kB[i] : bb;
-    }
-    const T w_ab = (T)ab, w_a = (T)aa, w_b = (T)bb, w_1 = q >= 8 ? T(1) : T(0);
+    const Fold16<T> fold(q);
     const int64_t pass = (int64_t)VEC << lpr_log2;
     for (int64_t j0 = ((int64_t)blockIdx.x * kWavesPerBlock + wave) * rows; j0 < out_dim;
          j0 += (int64_t)gridDim.x * kWavesPerBlock * rows) {
         const bool valid = j0 + sub < out_dim;
         const int64_t j = valid ? j0 + sub : out_dim - 1;            // every lane takes part in the reductions
-        const T lg = logits[j * 16 + q];
-        const T e = exp(lg - row16_max(lg));
-        const T p = e * (T(1) / row16_sum(e));
-        Coef<T> c;
-        c.ab = row16_sum(p * w_ab);
-        c.a = row16_sum(p * w_a);
-        c.b = row16_sum(p * w_b);
-        c.one = row16_sum(p * w_1);
+        T p;
+        const Coef<T> c = fold(logits[j * 16 + q], p);
         if (valid && l < 16) {
             probs[j * 16 + q] = p;
             if (q < 4) folded[j * 4 + q] = q == 0 ? c.ab : (q == 1 ? c.a : (q == 2 ? c.b : c.one));

@@ -80,12 +80,16 @@ int code_of(at::ScalarType t)
 struct Codes {
     Tensor codes, scales;
     // of a tensor without gaps, in the order in which it lies in memory
-    static Codes of(const Tensor &x)
+    static Codes room(const Tensor &x)
     {
         const int64_t n = x.numel();
-        Codes c{at::empty({n}, x.options().dtype(at::kByte)),
+        return {at::empty({n}, x.options().dtype(at::kByte)),
                 at::empty({clg_codes_groups(n), 2}, x.options().dtype(x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat))};
-        check(clg_codes_encode(code_of(x.scalar_type()), x.data_ptr(), n, static_cast<uint8_t *>(c.codes.data_ptr()), c.scales.data_ptr(), stream_of(x)));
+    }
+    static Codes of(const Tensor &x)
+    {
+        const Codes c = room(x);
+        check(clg_codes_encode(code_of(x.scalar_type()), x.data_ptr(), x.numel(), static_cast<uint8_t *>(c.codes.data_ptr()), c.scales.data_ptr(), stream_of(x)));
         return c;
     }
     void into(const Tensor &x) const
@@ -192,11 +196,11 @@ struct FcLayerCodes : torch::autograd::Function<FcLayerCodes> {
         const c10::OptionalDeviceGuard guard(x_in.device());
         const Tensor x = sample_major ? transposed(x_in) : x_in;
         const int64_t out_dim = logits.size(0), in_dim = x.size(0), batch = x.size(1);
-        const Tensor y = floats(x, {out_dim, batch}), probs = floats(x, {out_dim, 16}), folded = floats(x, {out_dim, 4});
-        check(clg_fc_forward_logits(CLG_F32, x.data_ptr(), idx(a), idx(b), logits.data_ptr(), probs.data_ptr(), folded.data_ptr(), y.data_ptr(), in_dim,
-                                    out_dim, batch, stream_of(x)));
-        const Codes c = Codes::of(x);
-        ctx->save_for_backward({c.codes, c.scales, a, b, probs, folded, start, flat});
+        const Tensor y = floats(x, {out_dim, batch}), probs = floats(x, {out_dim, 16}), neurons = floats(x, {out_dim, 8});
+        const Codes c = Codes::room(x);
+        check(clg_fc_codes_forward(x.data_ptr<float>(), idx(a), idx(b), logits.data_ptr<float>(), probs.data_ptr<float>(), neurons.data_ptr(), y.data_ptr<float>(),
+                                   static_cast<uint8_t *>(c.codes.data_ptr()), c.scales.data_ptr(), in_dim, out_dim, batch, sole, stream_of(x)));
+        ctx->save_for_backward({c.codes, c.scales, a, b, probs, neurons, start, flat});     // (a, b: for autograd's check that the wiring was not written)
         ctx->saved_data["sole"] = sole;
         ctx->saved_data["sample_major"] = sample_major;
         return y;
@@ -205,19 +209,20 @@ struct FcLayerCodes : torch::autograd::Function<FcLayerCodes> {
     {
         const auto saved = ctx->get_saved_variables();
         const c10::OptionalDeviceGuard guard(saved[0].device());
-        const Tensor &codes = saved[0], &scales = saved[1], &a = saved[2], &b = saved[3], &probs = saved[4], &folded = saved[5], &start = saved[6], &flat = saved[7];
+        const Tensor &codes = saved[0], &scales = saved[1], &probs = saved[4], &neurons = saved[5], &start = saved[6], &flat = saved[7];
         const bool sole = ctx->saved_data["sole"].toBool(), sample_major = ctx->saved_data["sample_major"].toBool();
         const bool need_x = ctx->needs_input_grad(0), need_l = ctx->needs_input_grad(3);
-        const int64_t in_dim = start.numel() - 1, out_dim = folded.size(0), batch = codes.numel() / in_dim;
+        const int64_t in_dim = start.numel() - 1, out_dim = probs.size(0), batch = codes.numel() / in_dim;
         const Tensor gy = contiguous_2d(grads[0]);
-        need(gy, folded, "grad_y", {out_dim, batch});
+        need(gy, probs, "grad_y", {out_dim, batch});
         Tensor gx, gl, scratch;
-        if (need_x) gx = floats(folded, {in_dim, batch});
-        if (need_l) gl = floats(folded, {out_dim, 16});
-        if (need_x && need_l && !sole) scratch = bytes(folded, clg_fc_codes_scratch_bytes(out_dim, batch));
-        check(clg_fc_codes_backward(static_cast<const uint8_t *>(codes.data_ptr()), scales.data_ptr(), idx(a), idx(b), folded.data_ptr<float>(), probs.data_ptr<float>(),
-                                    gy.data_ptr<float>(), idx(start), idx(flat), static_cast<float *>(ptr(gx)), static_cast<float *>(ptr(gl)), in_dim, out_dim, batch,
-                                    sole, ptr(scratch), stream_of(codes)));
+        if (need_x) gx = floats(probs, {in_dim, batch});
+        if (need_l) gl = floats(probs, {out_dim, 16});
+        const int64_t room = need_x && need_l && !sole ? clg_fc_codes_scratch_bytes(out_dim, batch) : 0;
+        if (room) scratch = bytes(probs, room);
+        check(clg_fc_codes_backward(static_cast<const uint8_t *>(codes.data_ptr()), scales.data_ptr(), neurons.data_ptr(), probs.data_ptr<float>(), gy.data_ptr<float>(),
+                                    idx(start), idx(flat), static_cast<float *>(ptr(gx)), static_cast<float *>(ptr(gl)), in_dim, out_dim, batch, sole, ptr(scratch),
+                                    stream_of(codes)));
         if (sample_major && need_x) gx = transposed(gx);
         return {gx, Tensor(), Tensor(), gl, Tensor(), Tensor(), Tensor(), Tensor()};
     }

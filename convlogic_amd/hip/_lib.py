@@ -149,7 +149,8 @@ SIGNATURES = {
     "clg_codes_encode": (_i, [_i, _p, _i64, _p, _p, _p]),
     "clg_codes_decode": (_i, [_i, _p, _p, _i64, _p, _p]),
     "clg_fc_codes_scratch_bytes": (_i64, [_i64, _i64]),
-    "clg_fc_codes_backward": (_i, [_p] * 11 + [_i64, _i64, _i64, _i, _p, _p]),
+    "clg_fc_codes_forward": (_i, [_p] * 9 + [_i64, _i64, _i64, _i, _p]),
+    "clg_fc_codes_backward": (_i, [_p] * 9 + [_i64, _i64, _i64, _i, _p, _p]),
     "clg_group_ce_kept_bytes": (_i64, [_i, _i, _i64, _i64, _i64]),
     "clg_group_ce_scratch_bytes": (_i64, [_i, _i, _i64, _i64, _i64]),
     "clg_group_ce_forward": (_i, [_i, _p, _i64, _i64, _i64, _i64, _p, _i, _f64, _f64, _f64, _i] + [_p] * 5),

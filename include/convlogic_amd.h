@@ -747,14 +747,17 @@ int64_t clg_codes_groups(int64_t n);
 int clg_codes_encode(int dtype, const void *x /*[n]*/, int64_t n, uint8_t *codes /*[n]*/, void *scales, void *stream);
 int clg_codes_decode(int dtype, const uint8_t *codes, const void *scales, int64_t n, void *x, void *stream);
 
-/* Backward pass of a float32 LogicLayer whose input [in_dim, batch] was kept in codes: as clg_fc_backward_x_folded and clg_fc_backward_logits, at the
- * values that the codes stand for.  Either gradient may be NULL (probs then too, or the reverse map).  sole: every input is read by exactly one operand.
+/* A float32 LogicLayer that keeps its input [in_dim, batch] in codes.  Forward: y and probs as clg_fc_forward_logits; neurons [out, 32 bytes], the wiring and the
+ * coefficients together, codes and scales for the backward pass.  Backward: as clg_fc_backward_x_folded and clg_fc_backward_logits, at the values that the codes
+ * stand for; either gradient may be NULL (probs then too, or the reverse map).  sole: every input is read by exactly one operand.
  * scratch: clg_fc_codes_scratch_bytes() bytes, NULL where that is 0. */
 int64_t clg_fc_codes_scratch_bytes(int64_t out_dim, int64_t batch);
-int clg_fc_codes_backward(const uint8_t *codes, const void *scales, const int64_t *a, const int64_t *b, const float *folded /*[out,4]*/,
-                          const float *probs /*[out,16]*/, const float *grad_y /*[out,batch]*/, const int64_t *csr_start, const int64_t *csr_list,
-                          float *grad_x /*[in,batch]*/, float *grad_logits /*[out,16]*/, int64_t in_dim, int64_t out_dim, int64_t batch, int sole,
-                          void *scratch, void *stream);
+int clg_fc_codes_forward(const float *x /*[in,batch]*/, const int64_t *a, const int64_t *b, const float *logits /*[out,16]*/, float *probs /*[out,16]*/,
+                         void *neurons, float *y /*[out,batch]*/, uint8_t *codes, void *scales, int64_t in_dim, int64_t out_dim, int64_t batch, int sole,
+                         void *stream);
+int clg_fc_codes_backward(const uint8_t *codes, const void *scales, const void *neurons, const float *probs, const float *grad_y /*[out,batch]*/,
+                          const int64_t *csr_start, const int64_t *csr_list, float *grad_x /*[in,batch]*/, float *grad_logits /*[out,16]*/, int64_t in_dim,
+                          int64_t out_dim, int64_t batch, int sole, void *scratch, void *stream);
 
 #ifdef __cplusplus
 }
