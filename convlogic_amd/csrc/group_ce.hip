@@ -12,9 +12,19 @@
 
 namespace {
 
-// exp(x - m) as the sums take it: the difference in 64 bits, the exponential in A
-__device__ __forceinline__ float exp_of(double x, double m, float) { return __builtin_amdgcn_exp2f((float)((x - m) * 1.4426950408889634074)); }
-__device__ __forceinline__ double exp_of(double x, double m, double) { return exp(x - m); }
+// Exponentials of scores, as the sums take them: of differences of scores times `unit`, which are 64-bit numbers, rounded to A; 2^x by one instruction for float.
+template <typename A>
+struct Unit;
+template <>
+struct Unit<float> {
+    static constexpr double unit = 1.4426950408889634074;
+    __device__ __forceinline__ static float power(float u) { return __builtin_amdgcn_exp2f(u); }
+};
+template <>
+struct Unit<double> {
+    static constexpr double unit = 1.0;
+    __device__ __forceinline__ static double power(double u) { return exp(u); }
+};
 
 struct CeArgs {
     const void *x;
@@ -26,7 +36,7 @@ struct CeArgs {
     double inv_tau, smoothing, scale;                                 // scale: weight, over the rows where their number is known to be all
     int reduction, count;                                             // count: to be counted here (1), or in per_count (2)
     double *per_count, *row_loss;                                     // 1 / rows that count; [rows]
-    double *final;                                                    // [rows][3]: M, O, Z
+    double *final;                                                    // [rows][4]: M in units, O, Z
     void *out;                                                        // [rows] in A, or NULL
     const void *upstream;                                             // in A, [rows] for CLG_REDUCE_NONE, or NULL for 1
     int if_changed;                                                   // nothing to do for an upstream gradient of 1
@@ -56,56 +66,74 @@ __device__ __forceinline__ double per_row(const CeArgs &a, double *room)
     return n[0] == 0 ? 0 : 1 / n[0];
 }
 
-// The statistics of a part of a row's classes.
+// The statistics of a part of a row's classes, of scores in units: the highest, O and the sum of (highest - score) relative to it, and the number of classes.  A
+// thread holds scores relative to its first one, as A.
+template <typename A>
 struct Stats {
-    double m = lowest(0.0), others = 0, down = 0, n = 0;             // highest, O and sum of (m - s) relative to it, classes
-    template <typename A>
-    __device__ __forceinline__ void add(double s, bool is_target, A type)
+    double base = 0, others = 0, down = 0, n = 0;
+    A m = lowest(A(0));
+    bool started = false;
+    // -> the score as it is held
+    __device__ __forceinline__ double add(double score, bool is_target, bool smooth)
     {
-        if (!(s <= m)) raise(s == s ? s : m, type);
-        const double e = s == m ? 1.0 : (double)exp_of(s, m, type);
-        others += is_target ? 0.0 : s == s ? e : s;
-        down += m - s;
-        n += 1;
+        if (!started) {
+            base = __builtin_fabs(score) <= __DBL_MAX__ ? score : 0;
+            started = true;
+        }
+        const A u = (A)(score - base);
+        if (u > m) raise(u);
+        const A e = u == lowest(A(0)) ? A(0) : Unit<A>::power(u - m);
+        others += is_target ? 0.0 : (double)e;
+        if (smooth) {
+            down += u == lowest(A(0)) ? -lowest(0.0) : (double)(m - u);
+            n += 1;
+        }
+        return base + (double)u;
     }
-    template <typename A>
-    __device__ __forceinline__ void raise(double to, A type)
+    __device__ __forceinline__ void raise(A to)
     {
         if (!(to > m)) return;
-        if (m != lowest(0.0)) {
-            others *= (double)exp_of(m, to, type);
-            down += n * (to - m);
-        } else {
-            others = others == others ? 0.0 : others;
-            down = n == 0 ? 0.0 : -lowest(0.0);                       // (classes of -inf)
+        if (m != lowest(A(0))) {
+            others *= (double)Unit<A>::power(m - to);
+            down += n * (double)(to - m);
         }
         m = to;
     }
-    template <typename A>
-    __device__ __forceinline__ void join(const Stats &o, A type)
+};
+// The same of several threads, relative to `m`.
+template <typename A>
+struct Joint {
+    double m = lowest(0.0), others = 0, down = 0, n = 0;
+    __device__ __forceinline__ Joint() {}
+    __device__ __forceinline__ explicit Joint(const Stats<A> &s) : m(s.base + (double)s.m), others(s.others), down(s.down), n(s.n) {}
+    __device__ __forceinline__ explicit Joint(const double *p) : m(p[0]), others(p[1]), down(p[2]), n(p[3]) {}
+    __device__ __forceinline__ void store(double *p) const { p[0] = m, p[1] = others, p[2] = down, p[3] = n; }
+    __device__ __forceinline__ void raise(double to)
     {
-        Stats b = o;
-        raise(b.m, type);
-        b.raise(m, type);
+        if (!(to > m)) return;
+        if (m != lowest(0.0)) {
+            others *= (double)Unit<A>::power((A)(m - to));
+            down += n * (to - m);
+        }
+        m = to;
+    }
+    __device__ __forceinline__ void join(Joint b)
+    {
+        raise(b.m);
+        b.raise(m);
         others += b.others;
         down += b.down;
         n += b.n;
-    }
-    __device__ __forceinline__ void store(double *p) const { p[0] = m, p[1] = others, p[2] = down, p[3] = n; }
-    __device__ __forceinline__ static Stats load(const double *p)
-    {
-        Stats s;
-        s.m = p[0], s.others = p[1], s.down = p[2], s.n = p[3];
-        return s;
     }
 };
 
 // What a row's loss and gradient are made of.
 struct Row {
-    double m, others, total;
-    __device__ __forceinline__ double loss(double s_target, double down, int k, double smoothing) const
+    double others, total;
+    // margin: M - s_t, down: sum of M - s_c
+    __device__ __forceinline__ double loss(double margin, double down, int k, double smoothing) const
     {
-        const double margin = m - s_target, log_total = margin == 0 ? log1p(others) : log(total);
+        const double log_total = margin == 0 ? log1p(others) : log(total);
         double l = margin + log_total;
         if (smoothing != 0) l = (1 - smoothing) * l + smoothing * (log_total + down / k);
         return l;
@@ -198,6 +226,48 @@ struct Classes {
             }
         }
     }
+    // every feature of class c of `to` = value(c, sum of c's features in `row`)
+    template <typename F>
+    __device__ __forceinline__ void both(const T *__restrict__ row, T *__restrict__ to, int first, int end, F value) const
+    {
+        if constexpr (PACK == 0) {
+            sums(row, first, end, [&](int c, double s, bool) { fill(to + (int64_t)c * group, (T)value(c, s)); });
+        } else {
+            const T *p = row + (int64_t)first * PACK;
+            T *o = to + (int64_t)first * PACK;
+            const int pieces = (end - first) / EACH;
+            const auto of = [&](int i, V v) {
+#pragma unroll
+                for (int q = 0; q < EACH; ++q) {
+                    double s = 0;
+#pragma unroll
+                    for (int j = 0; j < PACK; ++j) s += (double)(typename Wide<T>::type)v[q * PACK + j];
+                    const T u = (T)value(first + i * EACH + q, s);
+#pragma unroll
+                    for (int j = 0; j < PACK; ++j) v[q * PACK + j] = u;
+                }
+                reinterpret_cast<V *>(o)[i] = v;
+            };
+            int i = threadIdx.x;
+            for (; i + 3 * THREADS < pieces; i += 4 * THREADS) {
+                V v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = reinterpret_cast<const V *>(p)[i + u * THREADS];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) of(i + u * THREADS, v[u]);
+            }
+            for (; i < pieces; i += THREADS) of(i, reinterpret_cast<const V *>(p)[i]);
+            const int c = first + pieces * EACH + (int)threadIdx.x;
+            if (c < end) {
+                double s = 0;
+#pragma unroll
+                for (int j = 0; j < PACK; ++j) s += (double)(typename Wide<T>::type)row[(int64_t)c * PACK + j];
+                const T u = (T)value(c, s);
+#pragma unroll
+                for (int j = 0; j < PACK; ++j) to[(int64_t)c * PACK + j] = u;
+            }
+        }
+    }
     // every feature of class c = value(c)
     template <typename F>
     __device__ __forceinline__ void store(T *__restrict__ row, int first, int end, F value) const
@@ -227,23 +297,18 @@ struct Classes {
     }
 };
 
-// A workgroup per row.  The scores are in LDS as the arguments of their exponentials, relative to a value near them (of the first features of class 0): as 32-bit
-// numbers they are then as exact as a 32-bit exponential can tell.
-template <typename T, int THREADS, int PACK>
+// A workgroup per row.  Its scores, in units, are in LDS as S.  Those of up to 64 features to a class are floats relative to the score of class 0: as exact as a
+// 32-bit exponential can tell, and twice as many.
+constexpr int kNear = 64;
+template <typename T, int THREADS, int PACK, typename S>
 __global__ __launch_bounds__(THREADS) void rows_kernel(CeArgs a)
 {
     typedef typename Wide<T>::type A;
     extern __shared__ char lds[];
     __shared__ double room[32], shared[2];
-    A *score = reinterpret_cast<A *>(lds);
-    constexpr bool kFloat = sizeof(A) == 4;
-    constexpr double kUnit = kFloat ? 1.4426950408889634074 : 1.0;    // exponentials are 2^x, or e^x
-    const auto power = [](A x) {
-        if constexpr (kFloat) return __builtin_amdgcn_exp2f(x);
-        else return exp(x);
-    };
+    S *score = reinterpret_cast<S *>(lds);
+    constexpr double kUnit = Unit<A>::unit;
     const Classes<T, THREADS, PACK> classes(a.group, a.lanes_log2);
-    const int lane = threadIdx.x & 63;
     const double per = per_row<THREADS>(a, room);
     if (a.count == 1 && blockIdx.x == 0 && threadIdx.x == 0) *a.per_count = per;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -259,20 +324,24 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(CeArgs a)
             if (grad) classes.store(grad, 0, a.k, [&](int) { return (A)v; });
             continue;
         }
-        const int near = a.group < 64 ? a.group : 64;
-        double pivot = kFloat ? wave_sum(lane < near ? (double)(A)x[lane] : 0.0) * ((double)a.group / near) * a.inv_tau * kUnit : 0.0;
-        if (!(__builtin_fabs(pivot) <= __DBL_MAX__)) pivot = 0;
-        A m[1] = {lowest(A(0))};
+        double pivot = 0;
+        if constexpr (sizeof(S) == 4) {                               // (each wavefront adds up class 0 for itself)
+            const int lane = threadIdx.x & 63;
+            pivot = wave_sum(lane < a.group ? (double)(A)x[lane] : 0.0) * (a.inv_tau * kUnit);
+            if (!(__builtin_fabs(pivot) <= __DBL_MAX__)) pivot = 0;
+        }
+        S m[1] = {lowest(S(0))};
         classes.sums(x, 0, a.k, [&](int c, double s, bool mine) {
-            const A u = (A)(s * (a.inv_tau * kUnit) - pivot);
+            const S u = (S)(s * (a.inv_tau * kUnit) - pivot);
             if (mine) score[c] = u;
             m[0] = max_of(m[0], u);
         });
         __syncthreads();                                              // (also: room is free again)
-        block_reduce<false, THREADS>(m, reinterpret_cast<A *>(room));
+        block_reduce<false, THREADS>(m, reinterpret_cast<S *>(room));
         double sums[2] = {0, 0};
         for (int c = threadIdx.x; c < a.k; c += THREADS) {
-            const A u = score[c], e = power(u - m[0]);
+            const S u = score[c];
+            const A e = Unit<A>::power((A)(u - m[0]));
             if (c == t) {
                 shared[0] = (double)u;
                 shared[1] = (double)e;
@@ -280,37 +349,103 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(CeArgs a)
                 sums[0] += (double)e;
             }
             if (a.smoothing != 0) sums[1] += (double)m[0] - (double)u;
-            score[c] = e;
+            score[c] = (S)e;
         }
         __syncthreads();
         block_reduce<true, THREADS>(sums, room);
         __syncthreads();
-        const Row r{((double)m[0] + pivot) / kUnit, sums[0], sums[0] + shared[1]};
-        const double margin = ((double)m[0] - shared[0]) / kUnit;
+        const Row r{sums[0], sums[0] + shared[1]};
         const double scale = a.scale * per;
         const Grad g(r, scale * a.inv_tau, a.smoothing, a.k);
         if (threadIdx.x == 0) {
-            const double loss = Row{margin, r.others, r.total}.loss(0, sums[1] / kUnit, a.k, a.smoothing) * scale;
+            const double loss = r.loss(((double)m[0] - shared[0]) / kUnit, sums[1] / kUnit, a.k, a.smoothing) * scale;
             if (a.row_loss) a.row_loss[row] = loss;
             if (a.out) static_cast<A *>(a.out)[row] = (A)loss;
-            if (a.final) a.final[3 * row] = r.m, a.final[3 * row + 1] = r.others, a.final[3 * row + 2] = r.total;
+            double *f = a.final + 4 * row;
+            f[0] = (double)m[0] + pivot, f[1] = r.others, f[2] = r.total;
         }
         if (grad) {
             const A factor = (A)g.factor, off = (A)g.off, target = (A)g.target;
             const int at = (int)t;
-            classes.store(grad, 0, a.k, [&](int c) { return c == at ? target : __builtin_elementwise_fma(score[c], factor, -off); });
+            classes.store(grad, 0, a.k, [&](int c) { return c == at ? target : __builtin_elementwise_fma((A)score[c], factor, -off); });
         }
         __syncthreads();                                              // the scores are read
     }
 }
 
+// Few short rows, by one workgroup: 16 lanes to a row, a lane has classes l, l + 16, ...  The whole call is one launch: 100 rows of 10 classes 4 us.
+constexpr int kFewClasses = 64, kFewFeatures = 1 << 15, kFewRow = 1024;
+template <typename T>
+__global__ __launch_bounds__(1024) void few_rows_kernel(CeArgs a, void *out_sum)
+{
+    typedef typename Wide<T>::type A;
+    constexpr int EACH = kFewClasses / 16;
+    __shared__ double room[16], more[16];
+    const double per = per_row<1024>(a, room);
+    if (a.count == 1 && threadIdx.x == 0) *a.per_count = per;
+    const int l = threadIdx.x % 16;
+    double sum[1] = {0};
+    for (int64_t row = threadIdx.x / 16; row < a.rows; row += 64) {
+        const T *x = static_cast<const T *>(a.x) + row * a.stride;
+        T *grad = a.grad ? static_cast<T *>(a.grad) + row * ((int64_t)a.k * a.group) : nullptr;
+        const int64_t t = target_of(a, row);
+        double s[EACH], s_target = lowest(0.0), m = lowest(0.0), others = 0, of_target = 0, down = 0;
+        A e[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int c = l + 16 * i;
+            s[i] = 0;
+            if (c >= a.k) continue;
+            for (int j = 0; j < a.group; ++j) s[i] += (double)(A)x[c * a.group + j];
+            s[i] *= a.inv_tau;
+            m = max_of(m, s[i]);
+            if (c == t) s_target = s[i];
+        }
+        m = row16_max(m);
+        // (one lane has the target's; a NaN there is found by the exponential)
+        s_target = row16_max(s_target);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int c = l + 16 * i;
+            e[i] = c < a.k ? Unit<A>::power((A)((s[i] - m) * Unit<A>::unit)) : A(0);
+            if (c >= a.k) continue;
+            if (c == t) of_target = (double)e[i];
+            else others += (double)e[i];
+            down += m - s[i];
+        }
+        others = row16_sum(others), of_target = row16_sum(of_target), down = row16_sum(down);
+        const Row r{others, others + of_target};
+        const bool counts = t >= 0 && t < a.k;
+        const double scale = a.scale * per, none = t < 0 ? 0.0 : __builtin_nan("");
+        const Grad g(r, scale * a.inv_tau, a.smoothing, a.k);
+        const double loss = counts ? r.loss(m - s_target, down, a.k, a.smoothing) * scale : none;
+        if (l < 3) a.final[4 * row + l] = l == 0 ? m * Unit<A>::unit : l == 1 ? r.others : r.total;
+        if (l == 0) {
+            sum[0] += loss;
+            if (a.out) static_cast<A *>(a.out)[row] = (A)loss;
+        }
+        if (!grad) continue;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int c = l + 16 * i;
+            if (c >= a.k) continue;
+            const A v = !counts ? (A)none : c == t ? (A)g.target : __builtin_elementwise_fma(e[i], (A)g.factor, -(A)g.off);
+            for (int j = 0; j < a.group; ++j) grad[c * a.group + j] = (T)v;
+        }
+    }
+    if (!out_sum) return;
+    block_reduce<true, 1024>(sum, more);
+    if (threadIdx.x == 0) *static_cast<A *>(out_sum) = (A)sum[0];
+}
+
 // Statistics over THREADS threads, valid in thread 0.
 template <int THREADS, typename A>
-__device__ __forceinline__ Stats block_stats(Stats s, double *room, A type)
+__device__ __forceinline__ Joint<A> block_stats(const Stats<A> &mine, double *room)
 {
+    Joint<A> s(mine);
     double m[1] = {s.m};
     block_reduce<false, THREADS>(m, room);
-    s.raise(m[0], type);
+    s.raise(m[0]);
     double sums[3] = {s.others, s.down, s.n};
     __syncthreads();
     block_reduce<true, THREADS>(sums, room);
@@ -327,59 +462,89 @@ __global__ __launch_bounds__(kPart) void row_stats_kernel(CeArgs a)
     typedef typename Wide<T>::type A;
     __shared__ double room[3 * kPart / kWave];
     const Classes<T, kPart, PACK> classes(a.group, a.lanes_log2);
+    const bool smooth = a.smoothing != 0;
     for (int64_t task = blockIdx.x; task < a.rows * a.pieces; task += gridDim.x) {
         const int64_t row = task / a.pieces;
         const int piece = (int)(task % a.pieces), first = piece * a.per_piece, end = first + a.per_piece < a.k ? first + a.per_piece : a.k;
         const int64_t t = target_of(a, row);
-        Stats s;
+        const T *x = static_cast<const T *>(a.x) + row * a.stride;
+        Stats<A> s;
         if (t >= 0 && t < a.k) {
-            classes.sums(static_cast<const T *>(a.x) + row * a.stride, first, end, [&](int c, double sum, bool mine) {
+            const double unit = a.inv_tau * Unit<A>::unit;
+            classes.sums(x, first, end, [&](int c, double sum, bool mine) {
                 if (!mine) return;
-                const double v = sum * a.inv_tau;
-                if (c == t) a.target_score[row] = v;
-                s.add(v, c == t, A());
+                const double held = s.add(sum * unit, c == t, smooth);
+                if (c == t) a.target_score[row] = held;
             });
-            s = block_stats<kPart>(s, room, A());
         }
-        if (threadIdx.x == 0) s.store(a.stats + 4 * ((int64_t)piece * a.rows + row));
+        const Joint<A> all = block_stats<kPart>(s, room);
+        if (threadIdx.x == 0) all.store(a.stats + 4 * ((int64_t)piece * a.rows + row));
     }
 }
 
-// The statistics of a row's pieces into M, O, Z and the loss: a thread per row.  (One workgroup also counts the rows.)
-__global__ __launch_bounds__(1024) void join_kernel(CeArgs a, int dtype)
-{
-    __shared__ double room[16];
-    const double per = per_row<1024>(a, room);
-    if (a.count == 1 && threadIdx.x == 0) *a.per_count = per;
-    const int64_t row = (int64_t)blockIdx.x * 1024 + threadIdx.x;
-    if (row >= a.rows) return;
-    const int64_t t = target_of(a, row);
-    double loss = t < 0 ? 0.0 : __builtin_nan("");
-    if (t >= 0 && t < a.k) {
-        Stats s;
-        const auto join = [&](auto type) {
-            for (int p = 0; p < a.pieces; ++p) s.join(Stats::load(a.stats + 4 * ((int64_t)p * a.rows + row)), type);
-            return (double)exp_of(a.target_score[row], s.m, type);
-        };
-        const double of_target = dtype == CLG_F64 ? join(double()) : join(float());
-        if (__builtin_isinf(s.m)) s.others = __builtin_nan("");
-        const Row r{s.m, s.others, s.others + of_target};
-        loss = r.loss(a.target_score[row], s.down, a.k, a.smoothing) * a.scale * per;
-        if (a.final) a.final[3 * row] = r.m, a.final[3 * row + 1] = r.others, a.final[3 * row + 2] = r.total;
-    }
-    if (a.row_loss) a.row_loss[row] = loss;
-    if (a.out && dtype == CLG_F64) static_cast<double *>(a.out)[row] = loss;
-    else if (a.out) static_cast<float *>(a.out)[row] = (float)loss;
-}
-
-// Gradient of a row from its M, O and Z.
+// A row's loss from its statistics, which become M, O and Z.
 template <typename A>
-__device__ __forceinline__ Grad grad_of(const CeArgs &a, int64_t row)
+__device__ __forceinline__ double row_of(const CeArgs &a, int64_t row, Joint<A> s, double target, double per)
 {
-    const Row r{a.final[3 * row], a.final[3 * row + 1], a.final[3 * row + 2]};
-    const double up = a.upstream ? (double)static_cast<const A *>(a.upstream)[a.reduction == CLG_REDUCE_NONE ? row : 0] : 1.0;
-    return Grad(r, a.scale * (a.count ? *a.per_count : 1.0) * a.inv_tau * up, a.smoothing, a.k);
+    if (__builtin_isinf(s.m)) s.others = __builtin_nan("");
+    const Row r{s.others, s.others + (double)Unit<A>::power((A)(target - s.m))};
+    a.final[4 * row] = s.m, a.final[4 * row + 1] = r.others, a.final[4 * row + 2] = r.total;
+    return r.loss((s.m - target) / Unit<A>::unit, s.down / Unit<A>::unit, a.k, a.smoothing) * a.scale * per;
 }
+// The statistics of a row's pieces into M, O, Z and the loss: LANES to a row.  One workgroup for all rows (`out_sum`) also adds their losses.
+template <typename A, int LANES>
+__global__ __launch_bounds__(1024) void join_kernel(CeArgs a, void *out_sum)
+{
+    constexpr int ROWS = 1024 / LANES;
+    __shared__ double room[16], more[16];
+    const double per = per_row<1024>(a, room);
+    if (a.count == 1 && blockIdx.x == 0 && threadIdx.x == 0) *a.per_count = per;
+    const int l = threadIdx.x % LANES;
+    double sum[1] = {0};
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * ROWS) {
+        const int64_t t = target_of(a, row);
+        double loss = t < 0 ? 0.0 : __builtin_nan("");
+        if (t >= 0 && t < a.k) {
+            Joint<A> s;
+            for (int p = l; p < a.pieces; p += LANES) s.join(Joint<A>(a.stats + 4 * ((int64_t)p * a.rows + row)));
+            if constexpr (LANES == 16) {
+                s.raise(row16_max(s.m));
+                s.others = row16_sum(s.others), s.down = row16_sum(s.down);
+            } else {
+                s.raise(wave_max(s.m));
+                s.others = wave_sum(s.others), s.down = wave_sum(s.down);
+            }
+            if (l == 0) loss = row_of(a, row, s, a.target_score[row], per);
+        }
+        if (l != 0) continue;
+        sum[0] += loss;
+        if (a.row_loss) a.row_loss[row] = loss;
+        if (a.out) static_cast<A *>(a.out)[row] = (A)loss;
+    }
+    if (!out_sum) return;
+    block_reduce<true, 1024>(sum, more);
+    if (threadIdx.x == 0) *static_cast<A *>(out_sum) = (A)sum[0];
+}
+
+// What a gradient is computed from: M and the factors.
+template <typename A>
+struct GradOf {
+    double m, unit;
+    A factor, off, target;
+    __device__ __forceinline__ GradOf(const CeArgs &a, int64_t row)
+    {
+        const double *f = a.final + 4 * row;
+        const double up = a.upstream ? (double)static_cast<const A *>(a.upstream)[a.reduction == CLG_REDUCE_NONE ? row : 0] : 1.0;
+        const Grad g(Row{f[1], f[2]}, a.scale * (a.count ? *a.per_count : 1.0) * a.inv_tau * up, a.smoothing, a.k);
+        m = f[0], unit = a.inv_tau * Unit<A>::unit;
+        factor = (A)g.factor, off = (A)g.off, target = (A)g.target;
+    }
+    __device__ __forceinline__ A operator()(double sum, bool is_target) const
+    {
+        const A e = Unit<A>::power((A)__builtin_fma(sum, unit, -m));
+        return is_target ? target : __builtin_elementwise_fma(e, factor, -off);
+    }
+};
 
 template <typename T, int PACK>
 __global__ __launch_bounds__(kPart) void row_grad_kernel(CeArgs a)
@@ -397,18 +562,8 @@ __global__ __launch_bounds__(kPart) void row_grad_kernel(CeArgs a)
             classes.store(grad, first, end, [&](int) { return v; });
             continue;
         }
-        const Grad g = grad_of<A>(a, row);
-        const double m = a.final[3 * row];
-        const A factor = (A)g.factor, off = (A)g.off, target = (A)g.target;
-        classes.sums(static_cast<const T *>(a.x) + row * a.stride, first, end, [&](int c, double sum, bool) {
-            const A v = c == t ? target : __builtin_elementwise_fma(exp_of(sum * a.inv_tau, m, A()), factor, -off);
-            if constexpr (PACK == 0) {
-                classes.fill(grad + (int64_t)c * a.group, (T)v);
-            } else {
-#pragma unroll
-                for (int j = 0; j < PACK; ++j) grad[(int64_t)c * PACK + j] = (T)v;
-            }
-        });
+        const GradOf<A> g(a, row);
+        classes.both(static_cast<const T *>(a.x) + row * a.stride, grad, first, end, [&](int c, double sum) { return g(sum, c == t); });
     }
 }
 
@@ -445,16 +600,52 @@ __device__ __forceinline__ double column_sum(const CeArgs &a, const Column &col,
     for (int by = 1 << a.lanes_log2; by < 64; by <<= 1) s += __shfl_xor(s, by);
     return s;
 }
-// statistics of the workgroup's wavefronts, a sample each lane
-template <typename A>
-__device__ __forceinline__ void store_stats(const CeArgs &a, const Column &col, const Stats &s, double (&room)[kPart / kWave][kWave][4], A type)
+// f(class, sum) for the classes from `first` to `end` whose features are rows of x one after the other, with the next 8 rows on their way, or 16 (a sample each lane)
+template <typename T, typename F>
+__device__ __forceinline__ void column_stream(const CeArgs &a, const Column &col, const T *x, int first, int64_t from, int64_t to, int group, F f)
 {
-    s.store(room[col.wave][threadIdx.x & 63]);
+    typedef typename Wide<T>::type A;
+    constexpr int U = sizeof(T) == 2 ? 16 : 8;
+    x += col.row;
+    const auto load = [&](int64_t i, T (&v)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = x[(i + u < to ? i + u : to - 1) * a.rows];
+    };
+    T now[U], then[U];
+    int c = first, left = group;
+    double s = 0;
+    load(from, now);
+    for (int64_t i = from; i < to; i += U) {
+        if (i + U < to) load(i + U, then);
+        if (left > U && i + U <= to) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) s += (double)(A)now[u];
+            left -= U;
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (i + u >= to) break;
+                s += (double)(A)now[u];
+                if (--left == 0) {
+                    f(c, s);
+                    ++c, left = group, s = 0;
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) now[u] = then[u];
+    }
+}
+// Statistics of the workgroup's wavefronts, a sample each lane: valid in the first wavefront's, after which `finish` is called for each sample.
+template <typename A, int WAVES, typename F>
+__device__ __forceinline__ void column_finish(const Column &col, const Stats<A> &s, double (&room)[WAVES][kWave][4], F finish)
+{
+    Joint<A> all(s);
+    all.store(room[col.wave][threadIdx.x & 63]);
     __syncthreads();
     if (col.wave != 0 || col.sub != 0 || !col.live) return;
-    Stats all = s;
-    for (int w = 1; w < kPart / kWave; ++w) all.join(Stats::load(room[w][threadIdx.x & 63]), type);
-    all.store(a.stats + 4 * ((int64_t)blockIdx.y * a.rows + col.row));
+    for (int w = 1; w < WAVES; ++w) all.join(Joint<A>(room[w][threadIdx.x & 63]));
+    finish(all);
 }
 
 // Sums over the features of a class, or a slice of them; statistics of the classes of a piece where the sums are whole.
@@ -467,46 +658,60 @@ __global__ __launch_bounds__(kPart) void column_sums_kernel(CeArgs a)
     const int first = (int)blockIdx.y * a.per_piece, end = first + a.per_piece < a.k ? first + a.per_piece : a.k, slice = blockIdx.z;
     const int64_t from = (int64_t)a.group * slice / a.slices, to = (int64_t)a.group * (slice + 1) / a.slices;
     const int64_t t = target_of(a, col.row);
-    Stats s;
-    for (int c = first + col.wave; c < end; c += kPart / kWave) {
-        const double sum = column_sum<T>(a, col, (int64_t)c * a.group + from, (int64_t)c * a.group + to);
+    const bool smooth = a.smoothing != 0, store = col.live && col.sub == 0;
+    const double unit = a.inv_tau * Unit<A>::unit;
+    Stats<A> s;
+    const auto score = [&](int c, double sum) {
         if (a.slices > 1) {
-            if (col.live && col.sub == 0) a.partial[((int64_t)slice * a.k + c) * a.rows + col.row] = sum;
-            continue;
+            if (store) a.partial[((int64_t)slice * a.k + c) * a.rows + col.row] = sum;
+            return;
         }
-        const double v = sum * a.inv_tau;
-        if (col.live && col.sub == 0) {
-            if (a.scores) a.scores[(int64_t)c * a.rows + col.row] = v;
-            if (c == t) a.target_score[col.row] = v;
-        }
-        s.add(v, c == t, A());
+        const double held = s.add(sum * unit, c == t, smooth);
+        if (store && a.scores) a.scores[(int64_t)c * a.rows + col.row] = sum;
+        if (store && c == t) a.target_score[col.row] = held;
+    };
+    const T *x = static_cast<const T *>(a.x);
+    const int run = (end - first + kPart / kWave - 1) / (kPart / kWave), c0 = first + col.wave * run, c1 = c0 + run < end ? c0 + run : end;
+    if (col.subs > 1) {
+        for (int c = c0; c < c1; ++c) score(c, column_sum<T>(a, col, (int64_t)c * a.group + from, (int64_t)c * a.group + to));
+    } else if (a.slices > 1) {
+        for (int c = c0; c < c1; ++c) column_stream(a, col, x, c, (int64_t)c * a.group + from, (int64_t)c * a.group + to, (int)(to - from), score);
+    } else if (c0 < c1) {
+        column_stream(a, col, x, c0, (int64_t)c0 * a.group, (int64_t)c1 * a.group, a.group, score);
     }
-    if (a.slices == 1) store_stats(a, col, s, room, A());
+    if (a.slices == 1)
+        column_finish(col, s, room, [&](const Joint<A> &all) { all.store(a.stats + 4 * ((int64_t)blockIdx.y * a.rows + col.row)); });
 }
-// the same from the sums of the slices
-template <typename A>
-__global__ __launch_bounds__(kPart) void column_stats_kernel(CeArgs a)
+// The same from the sums of the slices, of all classes by one workgroup, which ends the rows' losses too.
+template <typename T>
+__global__ __launch_bounds__(1024) void column_stats_kernel(CeArgs a)
 {
-    __shared__ double room[kPart / kWave][kWave][4];
+    typedef typename Wide<T>::type A;
+    constexpr int WAVES = 1024 / kWave;
+    __shared__ double room[WAVES][kWave][4], more[WAVES];
+    const double per = per_row<1024>(a, more);
+    if (a.count == 1 && blockIdx.x == 0 && threadIdx.x == 0) *a.per_count = per;
     const Column col(a);
-    const int first = (int)blockIdx.y * a.per_piece, end = first + a.per_piece < a.k ? first + a.per_piece : a.k;
     const int64_t t = target_of(a, col.row);
-    Stats s;
-    for (int c = first + col.wave; c < end; c += kPart / kWave) {
+    const bool smooth = a.smoothing != 0, store = col.live && col.sub == 0;
+    const double unit = a.inv_tau * Unit<A>::unit;
+    Stats<A> s;
+    for (int c = col.wave; c < a.k; c += WAVES) {
         double sum = 0;
 #pragma unroll 8
         for (int i = col.sub; i < a.slices; i += col.subs) sum += a.partial[((int64_t)i * a.k + c) * a.rows + col.row];
         for (int by = 1 << a.lanes_log2; by < 64; by <<= 1) sum += __shfl_xor(sum, by);
-        const double v = sum * a.inv_tau;
-        if (col.live && col.sub == 0) {
-            a.scores[(int64_t)c * a.rows + col.row] = v;
-            if (c == t) a.target_score[col.row] = v;
-        }
-        s.add(v, c == t, A());
+        const double held = s.add(sum * unit, c == t, smooth);
+        if (store) a.scores[(int64_t)c * a.rows + col.row] = sum;
+        if (store && c == t) a.target_score[col.row] = held;
     }
-    store_stats(a, col, s, room, A());
+    column_finish(col, s, room, [&](const Joint<A> &all) {            // (behind a barrier: the target's score is there)
+        const double loss = t < 0 ? 0.0 : t >= a.k ? __builtin_nan("") : row_of(a, col.row, all, a.target_score[col.row], per);
+        if (a.row_loss) a.row_loss[col.row] = loss;
+        if (a.out) static_cast<A *>(a.out)[col.row] = (A)loss;
+    });
 }
-// Gradient from the scores, or from the features again.
+// Gradient from the sums of the classes, or from the features again.
 template <typename T>
 __global__ __launch_bounds__(kPart) void column_grad_kernel(CeArgs a)
 {
@@ -517,17 +722,24 @@ __global__ __launch_bounds__(kPart) void column_grad_kernel(CeArgs a)
     const int64_t from = (int64_t)a.group * slice / a.slices, to = (int64_t)a.group * (slice + 1) / a.slices;
     const int64_t t = target_of(a, col.row);
     const bool counts = t >= 0 && t < a.k;
-    const Grad g = grad_of<A>(a, counts ? col.row : 0);
-    const double m = a.final[3 * col.row];
-    const A factor = (A)g.factor, off = (A)g.off, target = (A)g.target;
+    const GradOf<A> g(a, col.row);
     T *grad = static_cast<T *>(a.grad) + col.row;
-    for (int c = first + col.wave; c < end; c += kPart / kWave) {
-        const double s = a.scores ? a.scores[(int64_t)c * a.rows + col.row] : column_sum<T>(a, col, (int64_t)c * a.group, (int64_t)(c + 1) * a.group) * a.inv_tau;
-        A v = c == t ? target : __builtin_elementwise_fma(exp_of(s, m, A()), factor, -off);
+    const auto store = [&](int c, double sum) {
+        A v = g(sum, c == t);
         if (!counts) v = t < 0 ? A(0) : (A)__builtin_nan("");
-        if (!col.live) continue;
+        if (!col.live) return;
         const T u = (T)v;
-        for (int64_t i = (int64_t)c * a.group + from + col.sub; i < (int64_t)c * a.group + to; i += col.subs) grad[i * a.rows] = u;
+        T *p = grad + ((int64_t)c * a.group + from + col.sub) * a.rows;
+        for (int64_t i = from + col.sub; i < to; i += col.subs, p += col.subs * a.rows) *p = u;
+    };
+    const int run = (end - first + kPart / kWave - 1) / (kPart / kWave), c0 = first + col.wave * run, c1 = c0 + run < end ? c0 + run : end;
+    if (c0 >= c1) return;
+    if (a.scores && col.subs == 1) {
+        column_stream(a, col, a.scores, c0, c0, c1, 1, store);
+    } else if (col.subs == 1) {
+        column_stream(a, col, static_cast<const T *>(a.x), c0, (int64_t)c0 * a.group, (int64_t)c1 * a.group, a.group, store);
+    } else {
+        for (int c = c0; c < c1; ++c) store(c, a.scores ? a.scores[(int64_t)c * a.rows + col.row] : column_sum<T>(a, col, (int64_t)c * a.group, (int64_t)(c + 1) * a.group));
     }
 }
 
@@ -547,7 +759,7 @@ constexpr int64_t kMostBlocks = 1 << 20;
 
 // How a call goes, by its sizes alone.
 struct Plan {
-    bool rows, whole;                                                 // layout; a workgroup per row
+    bool rows, whole, few;                                            // layout; a workgroup per row, or for all
     int64_t n, k, group, features;
     int size;                                                         // bytes of an element
     int lanes_log2, pieces, per_piece, slices;
@@ -566,17 +778,18 @@ int packed(const Plan &p)
 }
 Plan plan_of(int dtype, bool rows, int64_t n, int64_t features, int64_t k)
 {
-    Plan p{rows, false, n, k, features / k, features, clg_elem_bytes(dtype), 0, 1, (int)k, 1, false, false};
+    Plan p{rows, false, false, n, k, features / k, features, clg_elem_bytes(dtype), 0, 1, (int)k, 1, false, false};
     const auto cut = [&](int64_t pieces, int64_t unit) {              // pieces of a multiple of `unit` classes
         const int64_t each = clg_ceil_div(clg_ceil_div(k, pieces < 1 ? 1 : pieces), unit) * unit;
         p.per_piece = (int)(each < k ? each : k);
         p.pieces = (int)clg_ceil_div(k, p.per_piece);
     };
+    p.few = rows && k <= kFewClasses && features <= kFewRow && n <= kCounted && n * features <= kFewFeatures;
     if (rows) {
         const int64_t pieces = clg_ceil_div(p.group, 16 / p.size);    // of a class; a lane takes about four
         p.lanes_log2 = pieces <= 4 ? 0 : log2_up(clg_ceil_div(pieces, 4));
         if (p.lanes_log2 > 6) p.lanes_log2 = 6;
-        const int64_t lds = k * (dtype == CLG_F64 ? 8 : 4);
+        const int64_t lds = k * (dtype == CLG_F64 || p.group > kNear ? 8 : 4);
         p.whole = lds <= kLds && (n >= 128 || features * p.size <= 64 << 10);
         // else about 1024 workgroups, of 16 KiB of features at least
         int64_t want = clg_ceil_div(1024, n), most = clg_ceil_div(features * p.size, 16 << 10);
@@ -585,7 +798,8 @@ Plan plan_of(int dtype, bool rows, int64_t n, int64_t features, int64_t k)
         p.lanes_log2 = log2_up(n < 64 ? n : 64);
         const int64_t chunks = clg_ceil_div(n, 1ll << p.lanes_log2), want = clg_ceil_div(1024, chunks);
         cut(want < clg_ceil_div(k, 4) ? want : clg_ceil_div(k, 4), 4);
-        const int64_t slices = clg_ceil_div(1024, chunks * p.pieces), most = p.group / 64;
+        // (few classes: the workgroup that joins the slices has all of them)
+        const int64_t slices = clg_ceil_div(1024, chunks * p.pieces), most = k <= 256 ? p.group / 64 : 1;
         p.slices = (int)(slices < most ? slices : most);
         if (p.slices < 1) p.slices = 1;
         if (p.slices > 64) p.slices = 64;
@@ -610,10 +824,11 @@ Rooms rooms_of(const Plan &p, CeArgs *a, void *kept, void *scratch)
     CeArgs none;
     CeArgs &r = a ? *a : none;
     r.per_count = take(kept, 2);
-    r.final = take(kept, 3 * p.n);
+    r.final = take(kept, 4 * p.n);
     if (p.kept_scores) r.scores = take(kept, p.k * p.n);
     const int64_t bytes = at * 8;
     at = 0;
+    if (p.few) return {bytes, 0};
     r.row_loss = take(scratch, p.n);
     take(scratch, clg_ceil_div(p.n, kSlice));
     if (!p.whole) {
@@ -643,32 +858,44 @@ void with_pack(int pack, F call)
 
 unsigned blocks(int64_t n) { return (unsigned)(n < kMostBlocks ? n : kMostBlocks); }
 
-template <typename T, int THREADS, int PACK>
+template <typename T, int THREADS, int PACK, typename S>
 int launch_rows(const char *name, const CeArgs &a, hipStream_t stream)
 {
-    const size_t lds = a.k * sizeof(typename Wide<T>::type);
+    const size_t lds = a.k * sizeof(S);
     if (lds > 48 << 10) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(rows_kernel<T, THREADS, PACK>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(rows_kernel<T, THREADS, PACK, S>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) {
             clg_set_error("%s: %s", name, hipGetErrorString(e));
             return CLG_ELAUNCH;
         }
     }
-    rows_kernel<T, THREADS, PACK><<<dim3(blocks(a.rows)), dim3(THREADS), lds, stream>>>(a);
+    rows_kernel<T, THREADS, PACK, S><<<dim3(blocks(a.rows)), dim3(THREADS), lds, stream>>>(a);
     CLG_CHECK_LAUNCH(name);
     return CLG_OK;
 }
+template <typename T, int PACK, typename S>
+int launch_rows(const char *name, const CeArgs &a, hipStream_t stream)
+{
+    const int64_t features = (int64_t)a.k * a.group;
+    if (features <= 2048) return launch_rows<T, 64, PACK, S>(name, a, stream);
+    if (features <= 16384) return launch_rows<T, 256, PACK, S>(name, a, stream);
+    return launch_rows<T, 1024, PACK, S>(name, a, stream);
+}
 
 template <typename T>
-int forward(const char *name, const Plan &p, CeArgs a, int dtype, hipStream_t stream)
+int forward(const char *name, const Plan &p, const CeArgs &a, void *out_sum, hipStream_t stream)
 {
     int rc = CLG_OK;
-    if (p.rows && p.whole) {
+    if (p.few) {
+        few_rows_kernel<T><<<dim3(1), dim3(1024), 0, stream>>>(a, out_sum);
+        CLG_CHECK_LAUNCH(name);
+        return CLG_OK;
+    }
+    if (p.whole) {
         with_pack<T>(packed(p), [&](auto pack) {
             constexpr int PACK = decltype(pack)::value;
-            if (p.features <= 2048) rc = launch_rows<T, 64, PACK>(name, a, stream);
-            else if (p.features <= 16384) rc = launch_rows<T, 256, PACK>(name, a, stream);
-            else rc = launch_rows<T, 1024, PACK>(name, a, stream);
+            if (p.group > kNear) rc = launch_rows<T, 0, double>(name, a, stream);
+            else rc = launch_rows<T, PACK, typename Wide<T>::type>(name, a, stream);
         });
         return rc;
     }
@@ -678,10 +905,17 @@ int forward(const char *name, const Plan &p, CeArgs a, int dtype, hipStream_t st
     } else {
         column_sums_kernel<T><<<columns, dim3(kPart), 0, stream>>>(a);
         CLG_CHECK_LAUNCH(name);
-        if (p.slices > 1) column_stats_kernel<typename Wide<T>::type><<<dim3(columns.x, columns.y), dim3(kPart), 0, stream>>>(a);
+        if (p.slices > 1) {                                           // 16 samples to a workgroup, so that there are some of them
+            CeArgs b = a;
+            b.lanes_log2 = p.lanes_log2 < 4 ? p.lanes_log2 : 4;
+            column_stats_kernel<T><<<dim3((unsigned)clg_ceil_div(p.n, 1ll << b.lanes_log2)), dim3(1024), 0, stream>>>(b);
+        }
     }
     CLG_CHECK_LAUNCH(name);
-    join_kernel<<<dim3((unsigned)clg_ceil_div(p.n, 1024)), dim3(1024), 0, stream>>>(a, dtype);
+    if (!p.rows && p.slices > 1) return CLG_OK;
+    typedef typename Wide<T>::type A;
+    if (p.pieces <= 32) join_kernel<A, 16><<<dim3(out_sum ? 1 : (unsigned)clg_ceil_div(p.n, 1024 / 16)), dim3(1024), 0, stream>>>(a, out_sum);
+    else join_kernel<A, 64><<<dim3(out_sum ? 1 : (unsigned)clg_ceil_div(p.n, 1024 / 64)), dim3(1024), 0, stream>>>(a, out_sum);
     CLG_CHECK_LAUNCH(name);
     return CLG_OK;
 }
@@ -738,13 +972,14 @@ extern "C" int clg_group_ce_forward(int dtype, const void *x, int64_t row_stride
     const char *name = "clg_group_ce_forward";
     if (const int rc = check_call(name, dtype, x, row_stride, rows, features, k, targets, targets_bits, tau, smoothing, reduction)) return rc;
     CLG_REQUIRE(loss || (reduction == CLG_REDUCE_NONE && !rows), "%s: null pointer", name);
-    CLG_REQUIRE(!rows || (kept && scratch), "%s: null workspace", name);
+    CLG_REQUIRE(!rows || kept, "%s: null workspace", name);
     CLG_REQUIRE(!grad || reduction != CLG_REDUCE_NONE, "%s: the gradient of a loss per row is clg_group_ce_backward's", name);
     hipStream_t st = clg_stream(stream);
     if (!rows) return reduction == CLG_REDUCE_NONE ? CLG_OK : sum_rows(name, dtype, nullptr, 0, nullptr, nullptr, loss, st);
     const Plan p = plan_of(dtype, row_stride >= 0, rows, features, k);
     CeArgs a = args_of(p, x, row_stride, targets, targets_bits, tau, smoothing, weight, reduction);
-    rooms_of(p, &a, kept, scratch);
+    const Rooms rooms = rooms_of(p, &a, kept, scratch);
+    CLG_REQUIRE(!rooms.scratch || scratch, "%s: null workspace", name);
     double *row_loss = a.row_loss;
     if (reduction == CLG_REDUCE_NONE) a.out = loss, a.row_loss = nullptr;
     if (reduction == CLG_REDUCE_MEAN) {
@@ -756,16 +991,19 @@ extern "C" int clg_group_ce_forward(int dtype, const void *x, int64_t row_stride
             CLG_CHECK_LAUNCH(name);
         }
     }
-    if (p.whole) a.grad = grad;
-    int rc = clg_with_type(dtype, [&](auto t) { return forward<decltype(t)>(name, p, a, dtype, st); });
+    const bool at_once = p.whole || p.few;                            // gradient and all
+    // one workgroup also adds the losses: all of few rows, or the joint statistics of so many
+    const bool add = reduction != CLG_REDUCE_NONE && (p.few || (!p.whole && p.slices == 1 && rows <= (p.pieces <= 32 ? 64 : 16)));
+    if (at_once) a.grad = grad;
+    int rc = clg_with_type(dtype, [&](auto t) { return forward<decltype(t)>(name, p, a, add ? loss : nullptr, st); });
     if (rc) return rc;
-    if (grad && !p.whole) {
+    if (grad && !at_once) {
         a.grad = grad;
         if (a.count) a.count = 2;
         rc = clg_with_type(dtype, [&](auto t) { return gradient<decltype(t)>(name, p, a, st); });
         if (rc) return rc;
     }
-    return reduction == CLG_REDUCE_NONE ? CLG_OK : sum_rows(name, dtype, row_loss, rows, row_loss + rows, nullptr, loss, st);
+    return reduction == CLG_REDUCE_NONE || add ? CLG_OK : sum_rows(name, dtype, row_loss, rows, row_loss + rows, nullptr, loss, st);
 }
 
 extern "C" int clg_group_ce_backward(int dtype, const void *x, int64_t row_stride, int64_t rows, int64_t features, int64_t k, const void *targets, int targets_bits,
