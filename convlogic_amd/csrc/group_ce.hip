@@ -184,17 +184,74 @@ struct Classes {
         for (int by = lanes >> 1; by > 0; by >>= 1) s += __shfl_xor(s, by);
         return s;
     }
+    // the first N of `count` elements and the last N: all of N to 2 N
+    template <int N>
+    __device__ __forceinline__ static void fill_twice(T *p, int count, T value)
+    {
+        typedef T P __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+        *reinterpret_cast<P *>(p) = (P)value;
+        *reinterpret_cast<P *>(p + count - N) = (P)value;
+    }
+    // the class's features = value; the end of its last 16 bytes is written along with what is in front of it, with the same
     __device__ __forceinline__ void fill(T *__restrict__ p, T value) const
     {
         const int pieces = group / E;
-        for (int i = lane; i < pieces; i += lanes) reinterpret_cast<V *>(p)[i] = (V)value;
-        for (int i = pieces * E + lane; i < group; i += lanes) p[i] = value;
+        if (pieces > 0) {
+            for (int i = lane; i * E < group; i += lanes) *reinterpret_cast<V *>(p + (i < pieces ? i * E : group - E)) = (V)value;
+            return;
+        }
+        if (lane != 0) return;
+        if constexpr (E >= 4)
+            if (group >= E / 2) return fill_twice<E / 2>(p, group, value);
+        if constexpr (E >= 8)
+            if (group >= E / 4) return fill_twice<E / 4>(p, group, value);
+        for (int i = 0; i < group; ++i) p[i] = value;
     }
+    // f(c, sum) in all lanes of a team for the classes from `first` to `end` of at most a piece of 16 bytes for each lane, with the pieces of four classes on their way
+    // at once.  What is left behind a class's whole pieces is the end of its last 16 bytes; a class of less than a piece is a part of one.  last: features of the row.
+    template <typename F>
+    __device__ __forceinline__ void short_sums(const T *__restrict__ row, int first, int end, int64_t last, F f) const
+    {
+        typedef typename Wide<T>::type A;
+        constexpr int U = sizeof(T) == 8 ? 2 : 4;
+        const int pieces = group / E, rest = group - pieces * E;
+        const auto place = [&](int64_t at) {                          // of the lane's piece of the class at `at`
+            if (pieces > 0) return at + (lane < pieces ? lane * E : group - E);
+            return at + E <= last ? at : last - E;
+        };
+        if (last < E) {
+            for (int c = first + team; c < end; c += teams) f(c, sum(row + (int64_t)c * group));
+            return;
+        }
+        for (int c0 = first + team; c0 < end; c0 += U * teams) {
+            V v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const V *>(row + place((int64_t)(c0 + u * teams < end ? c0 + u * teams : end - 1) * group));
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int c = c0 + u * teams;
+                if (c >= end) break;
+                int from = 0, to = E;                                 // elements of the piece that are the lane's
+                if (pieces == 0) {
+                    from = (int)((int64_t)c * group - place((int64_t)c * group)), to = from + group;
+                } else if (lane >= pieces) {
+                    from = lane == pieces ? E - rest : E;
+                }
+                double s = 0;
+#pragma unroll
+                for (int j = 0; j < E; ++j) s += j >= from && j < to ? (double)(A)v[u][j] : 0.0;
+                for (int by = lanes >> 1; by > 0; by >>= 1) s += __shfl_xor(s, by);
+                f(c, s);
+            }
+        }
+    }
+    __device__ __forceinline__ bool is_short() const { return group <= lanes * E; }
     // f(c, sum of the features, whether this thread is to account for it) for the classes from `first` to `end`; every lane of a team calls it
     template <typename F>
-    __device__ __forceinline__ void sums(const T *__restrict__ row, int first, int end, F f) const
+    __device__ __forceinline__ void sums(const T *__restrict__ row, int first, int end, int64_t last, F f) const
     {
         if constexpr (PACK == 0) {
+            if (is_short()) return short_sums(row, first, end, last, [&](int c, double s) { f(c, s, lane == 0); });
             for (int c = first + team; c < end; c += teams) f(c, sum(row + (int64_t)c * group), lane == 0);
         } else {
             const T *p = row + (int64_t)first * PACK;
@@ -228,10 +285,10 @@ struct Classes {
     }
     // every feature of class c of `to` = value(c, sum of c's features in `row`)
     template <typename F>
-    __device__ __forceinline__ void both(const T *__restrict__ row, T *__restrict__ to, int first, int end, F value) const
+    __device__ __forceinline__ void both(const T *__restrict__ row, T *__restrict__ to, int first, int end, int64_t last, F value) const
     {
         if constexpr (PACK == 0) {
-            sums(row, first, end, [&](int c, double s, bool) { fill(to + (int64_t)c * group, (T)value(c, s)); });
+            sums(row, first, end, last, [&](int c, double s, bool) { fill(to + (int64_t)c * group, (T)value(c, s)); });
         } else {
             const T *p = row + (int64_t)first * PACK;
             T *o = to + (int64_t)first * PACK;
@@ -331,7 +388,7 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(CeArgs a)
             if (!(__builtin_fabs(pivot) <= __DBL_MAX__)) pivot = 0;
         }
         S m[1] = {lowest(S(0))};
-        classes.sums(x, 0, a.k, [&](int c, double s, bool mine) {
+        classes.sums(x, 0, a.k, (int64_t)a.k * a.group, [&](int c, double s, bool mine) {
             const S u = (S)(s * (a.inv_tau * kUnit) - pivot);
             if (mine) score[c] = u;
             m[0] = max_of(m[0], u);
@@ -471,7 +528,7 @@ __global__ __launch_bounds__(kPart) void row_stats_kernel(CeArgs a)
         Stats<A> s;
         if (t >= 0 && t < a.k) {
             const double unit = a.inv_tau * Unit<A>::unit;
-            classes.sums(x, first, end, [&](int c, double sum, bool mine) {
+            classes.sums(x, first, end, (int64_t)a.k * a.group, [&](int c, double sum, bool mine) {
                 if (!mine) return;
                 const double held = s.add(sum * unit, c == t, smooth);
                 if (c == t) a.target_score[row] = held;
@@ -531,6 +588,7 @@ template <typename A>
 struct GradOf {
     double m, unit;
     A factor, off, target;
+    __device__ __forceinline__ GradOf() {}
     __device__ __forceinline__ GradOf(const CeArgs &a, int64_t row)
     {
         const double *f = a.final + 4 * row;
@@ -563,27 +621,35 @@ __global__ __launch_bounds__(kPart) void row_grad_kernel(CeArgs a)
             continue;
         }
         const GradOf<A> g(a, row);
-        classes.both(static_cast<const T *>(a.x) + row * a.stride, grad, first, end, [&](int c, double sum) { return g(sum, c == t); });
+        classes.both(static_cast<const T *>(a.x) + row * a.stride, grad, first, end, (int64_t)a.k * a.group, [&](int c, double sum) { return g(sum, c == t); });
     }
 }
 
 // ---- columns: x [k G][rows] ----------------------------------------------------------------------------------------------------
-// A wavefront has 1 << lanes_log2 samples side by side and, beside them, as many features of a class as its lanes hold; the wavefronts of a workgroup have a class each.
+// A wavefront has 64 V samples, V to a lane; or (V = 1) 1 << lanes_log2 samples side by side and, beside them, as many features of a class as its lanes hold.  The
+// wavefronts of a workgroup have a class each.  The last lanes of a row that V does not divide take the last V samples, some of them twice.
+template <int V>
 struct Column {
-    int64_t row;                                                      // sample
+    int64_t row;                                                      // the first sample
     int sub, subs, wave;
     bool live;
     __device__ __forceinline__ explicit Column(const CeArgs &a)
     {
         const int lane = threadIdx.x & 63;
-        row = ((int64_t)blockIdx.x << a.lanes_log2) + (lane & ((1 << a.lanes_log2) - 1));
-        sub = lane >> a.lanes_log2, subs = 64 >> a.lanes_log2, wave = uniform(threadIdx.x >> 6);
+        wave = uniform(threadIdx.x >> 6);
+        if constexpr (V == 1) {
+            row = ((int64_t)blockIdx.x << a.lanes_log2) + (lane & ((1 << a.lanes_log2) - 1));
+            sub = lane >> a.lanes_log2, subs = 64 >> a.lanes_log2;
+        } else {
+            row = ((int64_t)blockIdx.x * 64 + lane) * V;
+            sub = 0, subs = 1;
+        }
         live = row < a.rows;
-        if (!live) row = a.rows - 1;
+        if (row + V > a.rows) row = a.rows - V;
     }
 };
 template <typename T>
-__device__ __forceinline__ double column_sum(const CeArgs &a, const Column &col, int64_t from, int64_t to)
+__device__ __forceinline__ double column_sum(const CeArgs &a, const Column<1> &col, int64_t from, int64_t to)
 {
     typedef typename Wide<T>::type A;
     const T *x = static_cast<const T *>(a.x) + col.row;
@@ -600,35 +666,67 @@ __device__ __forceinline__ double column_sum(const CeArgs &a, const Column &col,
     for (int by = 1 << a.lanes_log2; by < 64; by <<= 1) s += __shfl_xor(s, by);
     return s;
 }
-// f(class, sum) for the classes from `first` to `end` whose features are rows of x one after the other, with the next 8 rows on their way, or 16 (a sample each lane)
-template <typename T, typename F>
-__device__ __forceinline__ void column_stream(const CeArgs &a, const Column &col, const T *x, int first, int64_t from, int64_t to, int group, F f)
+// V values of a row, at any element's address
+template <typename T, int V>
+struct Some {
+    typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+};
+template <typename T>
+struct Some<T, 1> {
+    typedef T type;
+};
+template <int V, typename U>
+__device__ __forceinline__ auto part_of(const U &v, int i)
+{
+    if constexpr (V == 1) return v;
+    else return v[i];
+}
+template <int V, typename T, typename S>
+__device__ __forceinline__ void store_part(T *p, const S (&s)[V])
+{
+    typename Some<T, V>::type v;
+    if constexpr (V == 1) v = (T)s[0];
+    else
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = (T)s[i];
+    *reinterpret_cast<typename Some<T, V>::type *>(p) = v;
+}
+
+// f(class, sums) for the classes from `first` on whose features are rows `from` to `to` of x one after the other, `group` each, with the next rows on their way
+template <int V, typename T, typename F>
+__device__ __forceinline__ void column_stream(const CeArgs &a, const Column<V> &col, const T *x, int first, int64_t from, int64_t to, int group, F f)
 {
     typedef typename Wide<T>::type A;
-    constexpr int U = sizeof(T) == 2 ? 16 : 8;
+    typedef typename Some<T, V>::type P;
+    constexpr int U = V * sizeof(T) >= 16 ? 4 : V * sizeof(T) <= 2 ? 16 : 8;
     x += col.row;
-    const auto load = [&](int64_t i, T (&v)[U]) {
+    const auto load = [&](int64_t i, P (&v)[U]) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = x[(i + u < to ? i + u : to - 1) * a.rows];
+        for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const P *>(x + (i + u < to ? i + u : to - 1) * a.rows);
     };
-    T now[U], then[U];
+    P now[U], then[U];
     int c = first, left = group;
-    double s = 0;
+    double s[V] = {};
     load(from, now);
     for (int64_t i = from; i < to; i += U) {
         if (i + U < to) load(i + U, then);
         if (left > U && i + U <= to) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) s += (double)(A)now[u];
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int v = 0; v < V; ++v) s[v] += (double)(A)part_of<V>(now[u], v);
             left -= U;
         } else {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (i + u >= to) break;
-                s += (double)(A)now[u];
+#pragma unroll
+                for (int v = 0; v < V; ++v) s[v] += (double)(A)part_of<V>(now[u], v);
                 if (--left == 0) {
                     f(c, s);
-                    ++c, left = group, s = 0;
+                    ++c, left = group;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) s[v] = 0;
                 }
             }
         }
@@ -636,51 +734,64 @@ __device__ __forceinline__ void column_stream(const CeArgs &a, const Column &col
         for (int u = 0; u < U; ++u) now[u] = then[u];
     }
 }
-// Statistics of the workgroup's wavefronts, a sample each lane: valid in the first wavefront's, after which `finish` is called for each sample.
-template <typename A, int WAVES, typename F>
-__device__ __forceinline__ void column_finish(const Column &col, const Stats<A> &s, double (&room)[WAVES][kWave][4], F finish)
+// Statistics of the workgroup's wavefronts, V samples a lane: valid in the first wavefront's, after which `finish` is called for each sample.
+template <typename A, int V, int WAVES, typename F>
+__device__ __forceinline__ void column_finish(const Column<V> &col, const Stats<A> (&s)[V], double (&room)[WAVES][V][kWave][4], F finish)
 {
-    Joint<A> all(s);
-    all.store(room[col.wave][threadIdx.x & 63]);
+#pragma unroll
+    for (int v = 0; v < V; ++v) Joint<A>(s[v]).store(room[col.wave][v][threadIdx.x & 63]);
     __syncthreads();
     if (col.wave != 0 || col.sub != 0 || !col.live) return;
-    for (int w = 1; w < WAVES; ++w) all.join(Joint<A>(room[w][threadIdx.x & 63]));
-    finish(all);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        Joint<A> all(s[v]);
+        for (int w = 1; w < WAVES; ++w) all.join(Joint<A>(room[w][v][threadIdx.x & 63]));
+        finish(v, all);
+    }
 }
 
 // Sums over the features of a class, or a slice of them; statistics of the classes of a piece where the sums are whole.
-template <typename T>
+template <typename T, int V>
 __global__ __launch_bounds__(kPart) void column_sums_kernel(CeArgs a)
 {
     typedef typename Wide<T>::type A;
-    __shared__ double room[kPart / kWave][kWave][4];
-    const Column col(a);
+    __shared__ double room[kPart / kWave][V][kWave][4];
+    const Column<V> col(a);
     const int first = (int)blockIdx.y * a.per_piece, end = first + a.per_piece < a.k ? first + a.per_piece : a.k, slice = blockIdx.z;
     const int64_t from = (int64_t)a.group * slice / a.slices, to = (int64_t)a.group * (slice + 1) / a.slices;
-    const int64_t t = target_of(a, col.row);
+    int64_t t[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) t[v] = target_of(a, col.row + v);
     const bool smooth = a.smoothing != 0, store = col.live && col.sub == 0;
     const double unit = a.inv_tau * Unit<A>::unit;
-    Stats<A> s;
-    const auto score = [&](int c, double sum) {
+    Stats<A> s[V];
+    const auto score = [&](int c, const double (&sum)[V]) {
         if (a.slices > 1) {
-            if (store) a.partial[((int64_t)slice * a.k + c) * a.rows + col.row] = sum;
+            if (store) store_part<V>(a.partial + ((int64_t)slice * a.k + c) * a.rows + col.row, sum);
             return;
         }
-        const double held = s.add(sum * unit, c == t, smooth);
-        if (store && a.scores) a.scores[(int64_t)c * a.rows + col.row] = sum;
-        if (store && c == t) a.target_score[col.row] = held;
+        if (store && a.scores) store_part<V>(a.scores + (int64_t)c * a.rows + col.row, sum);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const double held = s[v].add(sum[v] * unit, c == t[v], smooth);
+            if (store && c == t[v]) a.target_score[col.row + v] = held;
+        }
     };
     const T *x = static_cast<const T *>(a.x);
     const int run = (end - first + kPart / kWave - 1) / (kPart / kWave), c0 = first + col.wave * run, c1 = c0 + run < end ? c0 + run : end;
-    if (col.subs > 1) {
-        for (int c = c0; c < c1; ++c) score(c, column_sum<T>(a, col, (int64_t)c * a.group + from, (int64_t)c * a.group + to));
+    if (V == 1 && col.subs > 1) {
+        if constexpr (V == 1)
+            for (int c = c0; c < c1; ++c) {
+                const double sum[1] = {column_sum<T>(a, col, (int64_t)c * a.group + from, (int64_t)c * a.group + to)};
+                score(c, sum);
+            }
     } else if (a.slices > 1) {
         for (int c = c0; c < c1; ++c) column_stream(a, col, x, c, (int64_t)c * a.group + from, (int64_t)c * a.group + to, (int)(to - from), score);
     } else if (c0 < c1) {
         column_stream(a, col, x, c0, (int64_t)c0 * a.group, (int64_t)c1 * a.group, a.group, score);
     }
     if (a.slices == 1)
-        column_finish(col, s, room, [&](const Joint<A> &all) { all.store(a.stats + 4 * ((int64_t)blockIdx.y * a.rows + col.row)); });
+        column_finish(col, s, room, [&](int v, const Joint<A> &all) { all.store(a.stats + 4 * ((int64_t)blockIdx.y * a.rows + col.row + v)); });
 }
 // The same from the sums of the slices, of all classes by one workgroup, which ends the rows' losses too.
 template <typename T>
@@ -688,58 +799,65 @@ __global__ __launch_bounds__(1024) void column_stats_kernel(CeArgs a)
 {
     typedef typename Wide<T>::type A;
     constexpr int WAVES = 1024 / kWave;
-    __shared__ double room[WAVES][kWave][4], more[WAVES];
+    __shared__ double room[WAVES][1][kWave][4], more[WAVES];
     const double per = per_row<1024>(a, more);
     if (a.count == 1 && blockIdx.x == 0 && threadIdx.x == 0) *a.per_count = per;
-    const Column col(a);
+    const Column<1> col(a);
     const int64_t t = target_of(a, col.row);
     const bool smooth = a.smoothing != 0, store = col.live && col.sub == 0;
     const double unit = a.inv_tau * Unit<A>::unit;
-    Stats<A> s;
+    Stats<A> s[1];
     for (int c = col.wave; c < a.k; c += WAVES) {
         double sum = 0;
 #pragma unroll 8
         for (int i = col.sub; i < a.slices; i += col.subs) sum += a.partial[((int64_t)i * a.k + c) * a.rows + col.row];
         for (int by = 1 << a.lanes_log2; by < 64; by <<= 1) sum += __shfl_xor(sum, by);
-        const double held = s.add(sum * unit, c == t, smooth);
+        const double held = s[0].add(sum * unit, c == t, smooth);
         if (store) a.scores[(int64_t)c * a.rows + col.row] = sum;
         if (store && c == t) a.target_score[col.row] = held;
     }
-    column_finish(col, s, room, [&](const Joint<A> &all) {            // (behind a barrier: the target's score is there)
+    column_finish(col, s, room, [&](int, const Joint<A> &all) {       // (behind a barrier: the target's score is there)
         const double loss = t < 0 ? 0.0 : t >= a.k ? __builtin_nan("") : row_of(a, col.row, all, a.target_score[col.row], per);
         if (a.row_loss) a.row_loss[col.row] = loss;
         if (a.out) static_cast<A *>(a.out)[col.row] = (A)loss;
     });
 }
 // Gradient from the sums of the classes, or from the features again.
-template <typename T>
+template <typename T, int V>
 __global__ __launch_bounds__(kPart) void column_grad_kernel(CeArgs a)
 {
     typedef typename Wide<T>::type A;
     if (nothing_to_do<A>(a)) return;
-    const Column col(a);
+    const Column<V> col(a);
     const int first = (int)blockIdx.y * a.per_piece, end = first + a.per_piece < a.k ? first + a.per_piece : a.k, slice = blockIdx.z;
     const int64_t from = (int64_t)a.group * slice / a.slices, to = (int64_t)a.group * (slice + 1) / a.slices;
-    const int64_t t = target_of(a, col.row);
-    const bool counts = t >= 0 && t < a.k;
-    const GradOf<A> g(a, col.row);
+    int64_t t[V];
+    GradOf<A> g[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) t[v] = target_of(a, col.row + v), g[v] = GradOf<A>(a, col.row + v);
     T *grad = static_cast<T *>(a.grad) + col.row;
-    const auto store = [&](int c, double sum) {
-        A v = g(sum, c == t);
-        if (!counts) v = t < 0 ? A(0) : (A)__builtin_nan("");
+    const auto store = [&](int c, const double (&sum)[V]) {
+        A value[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            value[v] = g[v](sum[v], c == t[v]);
+            if (t[v] < 0 || t[v] >= a.k) value[v] = t[v] < 0 ? A(0) : (A)__builtin_nan("");
+        }
         if (!col.live) return;
-        const T u = (T)v;
         T *p = grad + ((int64_t)c * a.group + from + col.sub) * a.rows;
-        for (int64_t i = from + col.sub; i < to; i += col.subs, p += col.subs * a.rows) *p = u;
+        for (int64_t i = from + col.sub; i < to; i += col.subs, p += col.subs * a.rows) store_part<V>(p, value);
     };
     const int run = (end - first + kPart / kWave - 1) / (kPart / kWave), c0 = first + col.wave * run, c1 = c0 + run < end ? c0 + run : end;
     if (c0 >= c1) return;
-    if (a.scores && col.subs == 1) {
-        column_stream(a, col, a.scores, c0, c0, c1, 1, store);
-    } else if (col.subs == 1) {
-        column_stream(a, col, static_cast<const T *>(a.x), c0, (int64_t)c0 * a.group, (int64_t)c1 * a.group, a.group, store);
-    } else {
-        for (int c = c0; c < c1; ++c) store(c, a.scores ? a.scores[(int64_t)c * a.rows + col.row] : column_sum<T>(a, col, (int64_t)c * a.group, (int64_t)(c + 1) * a.group));
+    if (V > 1 || col.subs == 1) {
+        if (a.scores) column_stream(a, col, a.scores, c0, c0, c1, 1, store);
+        else column_stream(a, col, static_cast<const T *>(a.x), c0, (int64_t)c0 * a.group, (int64_t)c1 * a.group, a.group, store);
+    } else if constexpr (V == 1) {
+        for (int c = c0; c < c1; ++c) {
+            const double sum[1] = {a.scores ? a.scores[(int64_t)c * a.rows + col.row]
+                                            : column_sum<T>(a, col, (int64_t)c * a.group, (int64_t)(c + 1) * a.group)};
+            store(c, sum);
+        }
     }
 }
 
@@ -756,13 +874,14 @@ __global__ __launch_bounds__(1024) void count_kernel(CeArgs a)
 constexpr int64_t kCounted = 1024;                                    // rows that every workgroup counts for itself
 constexpr int kLds = 144 << 10;                                       // of a row's scores
 constexpr int64_t kMostBlocks = 1 << 20;
+constexpr int64_t kSliced = 256;                                      // classes whose features may go in slices
 
 // How a call goes, by its sizes alone.
 struct Plan {
     bool rows, whole, few;                                            // layout; a workgroup per row, or for all
     int64_t n, k, group, features;
     int size;                                                         // bytes of an element
-    int lanes_log2, pieces, per_piece, slices;
+    int lanes_log2, samples, pieces, per_piece, slices;               // samples: of a lane ("columns")
     bool scores, kept_scores;                                         // "columns"
 };
 int log2_up(int64_t v)
@@ -771,6 +890,7 @@ int log2_up(int64_t v)
     while ((1ll << l) < v) ++l;
     return l;
 }
+int64_t chunks_of(const Plan &p) { return clg_ceil_div(p.n, p.samples > 1 ? 64ll * p.samples : 1ll << p.lanes_log2); }
 int packed(const Plan &p)
 {
     const int e = 16 / p.size;
@@ -778,7 +898,7 @@ int packed(const Plan &p)
 }
 Plan plan_of(int dtype, bool rows, int64_t n, int64_t features, int64_t k)
 {
-    Plan p{rows, false, false, n, k, features / k, features, clg_elem_bytes(dtype), 0, 1, (int)k, 1, false, false};
+    Plan p{rows, false, false, n, k, features / k, features, clg_elem_bytes(dtype), 0, 1, 1, (int)k, 1, false, false};
     const auto cut = [&](int64_t pieces, int64_t unit) {              // pieces of a multiple of `unit` classes
         const int64_t each = clg_ceil_div(clg_ceil_div(k, pieces < 1 ? 1 : pieces), unit) * unit;
         p.per_piece = (int)(each < k ? each : k);
@@ -786,8 +906,10 @@ Plan plan_of(int dtype, bool rows, int64_t n, int64_t features, int64_t k)
     };
     p.few = rows && k <= kFewClasses && features <= kFewRow && n <= kCounted && n * features <= kFewFeatures;
     if (rows) {
-        const int64_t pieces = clg_ceil_div(p.group, 16 / p.size);    // of a class; a lane takes about four
-        p.lanes_log2 = pieces <= 4 ? 0 : log2_up(clg_ceil_div(pieces, 4));
+        // a lane for each piece of a class, up to a wavefront: what the lanes load at once is then in one place (a lane for four pieces, two lanes to a class
+        // of 61 bfloat16 features: 2.1 TB/s)
+        const int e = 16 / p.size;
+        p.lanes_log2 = p.group < e ? 0 : log2_up(clg_ceil_div(p.group, e));
         if (p.lanes_log2 > 6) p.lanes_log2 = 6;
         const int64_t lds = k * (dtype == CLG_F64 || p.group > kNear ? 8 : 4);
         p.whole = lds <= kLds && (n >= 128 || features * p.size <= 64 << 10);
@@ -796,10 +918,16 @@ Plan plan_of(int dtype, bool rows, int64_t n, int64_t features, int64_t k)
         cut(want < most ? want : most, 16);
     } else {
         p.lanes_log2 = log2_up(n < 64 ? n : 64);
-        const int64_t chunks = clg_ceil_div(n, 1ll << p.lanes_log2), want = clg_ceil_div(1024, chunks);
+        // several samples to a lane where that leaves few lanes idle and workgroups enough (4 to a lane and 1: 4802 rows of 1759 classes of 27 float32 543
+        // and 657 us, but the sums of 256 rows of 10 classes of 8192 28 and 21)
+        for (int v = dtype == CLG_F64 ? 2 : 4; v > 1 && p.samples == 1; v /= 2)
+            if (n >= v * 64 && clg_ceil_div(n, v * 64) * v * 64 * 3 <= n * 4 &&
+                clg_ceil_div(n, v * 64) * clg_ceil_div(k, 4) * (p.group < 128 || k > kSliced ? 1 : p.group > 4096 ? 64 : p.group / 64) >= 768)
+                p.samples = v;
+        const int64_t chunks = chunks_of(p), want = clg_ceil_div(1024, chunks);
         cut(want < clg_ceil_div(k, 4) ? want : clg_ceil_div(k, 4), 4);
         // (few classes: the workgroup that joins the slices has all of them)
-        const int64_t slices = clg_ceil_div(1024, chunks * p.pieces), most = k <= 256 ? p.group / 64 : 1;
+        const int64_t slices = clg_ceil_div(1024, chunks * p.pieces), most = k <= kSliced ? p.group / 64 : 1;
         p.slices = (int)(slices < most ? slices : most);
         if (p.slices < 1) p.slices = 1;
         if (p.slices > 64) p.slices = 64;
@@ -856,6 +984,14 @@ void with_pack(int pack, F call)
     }
 }
 
+template <typename T, typename F>
+void with_samples(int samples, F call)
+{
+    if (samples == 1) call(std::integral_constant<int, 1>());
+    else if (sizeof(T) == 8 || samples == 2) call(std::integral_constant<int, 2>());
+    else call(std::integral_constant<int, sizeof(T) == 8 ? 2 : 4>());
+}
+
 unsigned blocks(int64_t n) { return (unsigned)(n < kMostBlocks ? n : kMostBlocks); }
 
 template <typename T, int THREADS, int PACK, typename S>
@@ -899,11 +1035,11 @@ int forward(const char *name, const Plan &p, const CeArgs &a, void *out_sum, hip
         });
         return rc;
     }
-    const dim3 columns((unsigned)clg_ceil_div(p.n, 1ll << p.lanes_log2), (unsigned)p.pieces, (unsigned)p.slices);
+    const dim3 columns((unsigned)chunks_of(p), (unsigned)p.pieces, (unsigned)p.slices);
     if (p.rows) {
         with_pack<T>(packed(p), [&](auto pack) { row_stats_kernel<T, decltype(pack)::value><<<dim3(blocks(p.n * p.pieces)), dim3(kPart), 0, stream>>>(a); });
     } else {
-        column_sums_kernel<T><<<columns, dim3(kPart), 0, stream>>>(a);
+        with_samples<T>(p.samples, [&](auto v) { column_sums_kernel<T, decltype(v)::value><<<columns, dim3(kPart), 0, stream>>>(a); });
         CLG_CHECK_LAUNCH(name);
         if (p.slices > 1) {                                           // 16 samples to a workgroup, so that there are some of them
             CeArgs b = a;
@@ -923,7 +1059,9 @@ template <typename T>
 int gradient(const char *name, const Plan &p, const CeArgs &a, hipStream_t stream)
 {
     if (p.rows) with_pack<T>(packed(p), [&](auto pack) { row_grad_kernel<T, decltype(pack)::value><<<dim3(blocks(p.n * p.pieces)), dim3(kPart), 0, stream>>>(a); });
-    else column_grad_kernel<T><<<dim3((unsigned)clg_ceil_div(p.n, 1ll << p.lanes_log2), (unsigned)p.pieces, (unsigned)p.slices), dim3(kPart), 0, stream>>>(a);
+    else with_samples<T>(p.samples, [&](auto v) {
+            column_grad_kernel<T, decltype(v)::value><<<dim3((unsigned)chunks_of(p), (unsigned)p.pieces, (unsigned)p.slices), dim3(kPart), 0, stream>>>(a);
+        });
     CLG_CHECK_LAUNCH(name);
     return CLG_OK;
 }
