@@ -1,11 +1,8 @@
 // Autograd nodes of the losses on scores and gate logits (difflogic/losses.py checks their arguments and has their plain forms for CPU tensors).
 #include "loss_nodes.h"
 
-#include <ATen/ATen.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_cpp_function.h>
 
 #include <mutex>
@@ -62,15 +59,7 @@ Tensor rows_of(const Tensor &t)
     return t.contiguous();
 }
 
-// gradients that cannot be differentiated again
-variable_list once(variable_list grads)
-{
-    if (!at::GradMode::is_enabled()) return grads;
-    for (Tensor &g : grads)
-        if (g.defined()) g = g.detach().requires_grad_(true);
-    auto error = std::make_shared<torch::autograd::DelayedError>("the gradient of this loss cannot be differentiated", (int64_t)grads.size());
-    return (*error)(std::move(grads));
-}
+variable_list once(variable_list grads) { return once_only(std::move(grads), "the gradient of this loss cannot be differentiated"); }
 
 // ---- top logits ------------------------------------------------------------------------------------------------------------
 std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor &logits_in, int64_t k, double temperature)

@@ -88,12 +88,14 @@ struct Codes {
     }
     static Codes of(const Tensor &x)
     {
+        const c10::OptionalDeviceGuard guard(x.device());
         const Codes c = room(x);
         check(clg_codes_encode(code_of(x.scalar_type()), x.data_ptr(), x.numel(), static_cast<uint8_t *>(c.codes.data_ptr()), c.scales.data_ptr(), stream_of(x)));
         return c;
     }
     void into(const Tensor &x) const
     {
+        const c10::OptionalDeviceGuard guard(x.device());
         check(clg_codes_decode(code_of(x.scalar_type()), static_cast<const uint8_t *>(codes.data_ptr()), scales.data_ptr(), x.numel(), x.data_ptr(), stream_of(x)));
     }
     Tensor values(at::IntArrayRef shape) const                        // float32, dense
@@ -106,14 +108,12 @@ struct Codes {
 // x without gaps -> codes and scales
 std::pair<Tensor, Tensor> encode(const Tensor &x)
 {
-    const c10::OptionalDeviceGuard guard(x.device());
     TORCH_CHECK(x.is_non_overlapping_and_dense(), "activations without gaps in memory expected");
     const Codes c = Codes::of(x);
     return {c.codes, c.scales};
 }
 Tensor decode(const Tensor &codes, const Tensor &scales, std::vector<int64_t> shape, std::vector<int64_t> stride, at::ScalarType type)
 {
-    const c10::OptionalDeviceGuard guard(codes.device());
     const Tensor x = at::empty_strided(shape, stride, scales.options().dtype(type));
     TORCH_CHECK(codes.scalar_type() == at::kByte && codes.is_contiguous() && codes.numel() == x.numel() && scales.is_contiguous() &&
                     scales.device() == codes.device() && scales.scalar_type() == (type == at::kDouble ? at::kDouble : at::kFloat) &&
@@ -224,7 +224,7 @@ struct FcLayerCodes : torch::autograd::Function<FcLayerCodes> {
                                     idx(start), idx(flat), static_cast<float *>(ptr(gx)), static_cast<float *>(ptr(gl)), in_dim, out_dim, batch, sole, ptr(scratch),
                                     stream_of(codes)));
         if (sample_major && need_x) gx = transposed(gx);
-        return {gx, Tensor(), Tensor(), gl, Tensor(), Tensor(), Tensor(), Tensor()};
+        return once_only({gx, Tensor(), Tensor(), gl, Tensor(), Tensor(), Tensor(), Tensor()}, "the gradient of a layer with checkpoint_bits cannot be differentiated");
     }
 };
 // x [batch, in] where sample_major, else [in, batch]; -> [batch, out], a transposed view of [out, batch]

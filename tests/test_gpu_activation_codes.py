@@ -307,6 +307,52 @@ def test_a_recorded_step_of_layers():
         torch.cuda.synchronize()
 
 
+def test_the_gradient_of_a_layer_cannot_be_differentiated():
+    layer = layer_of(12, 9)
+    x = activations((12, 20)).to(DEV).t().requires_grad_(True)
+    g, = torch.autograd.grad(layer(x).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        g.sum().backward()
+
+
+def test_codes_of_more_than_2_to_the_31_elements():
+    n = (1 << 31) + 300
+    x = torch.zeros(n, dtype=torch.float16, device=DEV)
+    x[-300:] = activations((300,), torch.float16).to(DEV)
+    x[5] = 1.0
+    back = C.encode_activations(x).decode()
+    assert back[5] == 1 and back[:1000].sum() == 1
+    assert torch.equal(back[-300:], C.encode_activations(x[(n - 300) // 128 * 128:]).decode()[-300:])
+
+
+def test_layer_of_more_than_2_to_the_30_elements():
+    # 0/1 inputs, which the codes keep, in the last rows and samples alone, so that a few of them can be checked one by one
+    inputs, neurons, batch = 66000, 33000, 17000
+    layer = layer_of(inputs, neurons)
+    with torch.no_grad():                                             # (no input is read once only)
+        layer.indices_0[-1], layer.indices_1[-1], layer.indices_0[-2] = inputs - 1, inputs - 2, inputs - 1
+        if layer.indices_0[0] == layer.indices_0[1]:
+            layer.indices_0[0] += 1
+        layer.indices_0[0] = layer.indices_0[1]
+    xt = torch.zeros(inputs, batch, device=DEV)
+    xt[-2:, -5:] = torch.tensor([[0.0, 1, 0, 1, 1], [1, 1, 0, 0, 1]], device=DEV)
+    x = xt.t().requires_grad_(True)
+    y = layer(x)
+    up = torch.zeros(neurons, batch, device=DEV)
+    up[-1, -5:] = torch.tensor([1.0, 2, 3, 4, 5], device=DEV)
+    gx, gl = torch.autograd.grad(y, (x, layer.weights), up.t())
+    p = torch.softmax(layer.weights[-1].detach().double(), 0).cpu().numpy()
+    a, b, g = xt[-1, -5:].cpu().double().numpy(), xt[-2, -5:].cpu().double().numpy(), np.array([1.0, 2, 3, 4, 5])
+    value, da, db = K.gates(a, b)
+    want = p * ((value * g).sum(1) - (p[:, None] * value * g).sum())
+    # (five samples; coefficients and softmax as in the other tests)
+    assert np.abs(host(gl[-1]) - want).max() <= 64 * 2.0 ** -24 * 15 and (gl[:-1] == 0).all()
+    got = host(gx[-5:, -2:])
+    assert np.abs(got[:, 1] - (p[:, None] * da).sum(0) * g).max() <= 64 * 2.0 ** -24 * 10
+    assert np.abs(got[:, 0] - (p[:, None] * db).sum(0) * g).max() <= 64 * 2.0 ** -24 * 10
+    assert int((gx != 0).sum()) == int((gx[-5:, -2:] != 0).sum())     # (counted: sums of both in float32 differ in the order of their terms)
+
+
 # ---- blocks and networks -------------------------------------------------------------------------
 def block_of(seed=0, **kw):
     torch.manual_seed(seed)
@@ -367,3 +413,19 @@ def test_networks(make, shape):
     assert all((u - v).norm() <= 0.05 * v.norm() + 1e-8 for u, v in zip(got, ref))
     net.eval(), plain.eval()
     assert torch.equal(net(x), plain(x))
+
+
+def test_a_recorded_step_of_a_network():
+    torch.manual_seed(0)
+    net = C.ConvLogicMnistModel(k_param=4, checkpoint_bits=8).to(DEV)
+    x, t = (activations((16, 1, 28, 28)) > 0.5).float().to(DEV), torch.randint(0, 10, (16,), device=DEV)
+    step = C.GraphedStep(lambda x, t: C.group_cross_entropy(net(x), t, 10), (x, t), net.parameters())
+    for seed in range(3):
+        x, t = (activations((16, 1, 28, 28), seed=seed) > 0.5).float().to(DEV), torch.randint(0, 10, (16,), device=DEV)
+        value = float(step(x, t))
+        grads = [p.grad.clone() for p in net.parameters()]
+        loss = C.group_cross_entropy(net(x), t, 10)
+        want = torch.autograd.grad(loss, list(net.parameters()))
+        assert value == float(loss.detach()) and all(torch.equal(u, v) for u, v in zip(grads, want))
+        del loss
+        torch.cuda.synchronize()

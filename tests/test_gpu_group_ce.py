@@ -233,6 +233,37 @@ def test_int32_targets_and_shapes():
         loss.sum().backward()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["rows", "columns"])
+@pytest.mark.parametrize("group", [2, 3, 5, 6, 7, 9, 13, 15, 17, 31, 33, 61, 63, 65, 127, 255, 513])
+def test_groups_of_every_kind(group, layout, dtype):
+    check(features(150, 5, group, dtype), labels(150, 5), 5, layout, tau=0.3 * group ** 0.5)
+    check(features(4, 600, group, dtype), labels(4, 600), 600, layout, tau=0.3 * group ** 0.5, reduction="none")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [63, 64, 65, 128, 129, 191, 256, 257, 300, 511, 700, 1025])
+def test_columns_of_every_width(rows, dtype):
+    check(features(rows, 6, 20, dtype), labels(rows, 6, masked=True), 6, "columns", tau=1.5)
+    check(features(rows, 770, 2, dtype), labels(rows, 770, masked=True), 770, "columns", tau=0.5, reduction="none")
+
+
+def test_features_of_more_than_2_to_the_31_elements():
+    rows, k, group = 70000, 32768, 1
+    x = torch.zeros(rows, k, device=DEV, dtype=torch.bfloat16)
+    x[-1, 7] = 5.0
+    t = torch.zeros(rows, dtype=torch.int64, device=DEV)
+    t[-1] = 7
+    for leaf in (x.requires_grad_(True), x.detach().t().contiguous().t().requires_grad_(True)):
+        loss = C.group_cross_entropy(leaf, t, k, reduction="none")
+        grad, = torch.autograd.grad(loss.sum(), leaf)
+        assert abs(float(loss[0].detach()) - math.log(k)) <= 1e-5 and abs(float(loss[-1].detach()) - math.log1p((k - 1) * math.exp(-5))) <= 1e-5
+        p = 1 / (1 + (k - 1) * math.exp(-5))
+        assert abs(float(grad[-1, 7]) - (p - 1)) <= 2.0 ** -8 and abs(float(grad[-1, -1]) - p * math.exp(-5)) <= 2.0 ** -8 * p * math.exp(-5)
+        assert abs(float(grad[-2, 0]) - (1 / k - 1)) <= 2.0 ** -8 and abs(float(grad[-2, -1]) - 1 / k) <= 2.0 ** -8 / k
+        del grad, loss
+
+
 def test_many_rows():
     check(features(70001, 3, 1), labels(70001, 3, masked=True), 3, "rows")
     check(features(70001, 3, 2), labels(70001, 3, masked=True), 3, "columns", smoothing=0.1)
@@ -252,7 +283,7 @@ def test_refusals():
 
 
 @pytest.mark.parametrize("layout", ["rows", "columns"])
-@pytest.mark.parametrize("rows,k,group", [(40, 10, 1), (40, 10, 50), (3, 4, 3000)])
+@pytest.mark.parametrize("rows,k,group", [(40, 10, 1), (40, 10, 50), (3, 4, 3000), (130, 20000, 1)])
 def test_retained_graphs_streams_and_recordings(rows, k, group, layout):
     x, t = on_gpu(features(rows, k, group), layout), labels(rows, k).to(DEV)
     leaf = x.clone().requires_grad_(True) if layout == "rows" else x.t().clone().t().requires_grad_(True)
