@@ -8,7 +8,7 @@ namespace {
 
 constexpr int kWaves = 4, kBlock = kWaves * kWave;
 constexpr int64_t kFull = 256 * 32, kTurns = 4;                       // wavefronts that the chip holds; items that one takes, from there on
-constexpr int kWalk = 8;                                              // lanes' worth of a walk over the wiring
+constexpr int kWay = 24;                                              // lanes' worth of the way to the rows
 typedef float f32x4_row __attribute__((ext_vector_type(4), aligned(4)));
 
 template <int VEC>
@@ -394,7 +394,8 @@ __global__ __launch_bounds__(kBlock) void gradients_kernel(const float4 *__restr
     }
 }
 
-// Four samples to a lane from 17 samples on, or where they divide the batch.
+// Four samples to a lane from 17 samples on, or where they divide the batch (up to 16, one to a lane is one pass as well: 30001 -> 60000 neurons, batch 9, 23 us and
+// 27 with four).
 bool fours(int64_t batch) { return batch % 4 == 0 || batch > 16; }
 // Lanes of a row: as many as it takes, up to a wavefront.
 int lanes_of(int64_t batch)
@@ -402,15 +403,12 @@ int lanes_of(int64_t batch)
     const int64_t lanes = fours(batch) ? clg_ceil_div(batch, 4) : batch;
     return lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64;
 }
-// Where rows go in chunks of the batch, each with a walk over the wiring of its own: lanes that few of them leave idle.
+// Where rows go in chunks of the batch, each with a way to them of its own: 32 lanes where 64 would leave many of them idle.  30001 -> 60000 neurons with 64 and 32
+// lanes, the whole step: batch 333 138 and 132 us, 300 110 and 114, 512 139 and 152, 700 207 and 236.
 int chunk_lanes(int64_t batch)
 {
-    int best = lanes_of(batch);
-    const auto cost = [&](int lanes) { return clg_ceil_div(batch, (int64_t)lanes * 4) * (lanes + kWalk); };
-    if (batch > 256)
-        for (int lanes = 32; lanes >= 16; lanes /= 2)
-            if (cost(lanes) < cost(best)) best = lanes;
-    return best;
+    const auto cost = [&](int lanes) { return clg_ceil_div(batch, (int64_t)lanes * 4) * (lanes + kWay); };
+    return batch > 256 && cost(32) < cost(64) ? 32 : lanes_of(batch);
 }
 int64_t chunks_of(int64_t batch) { return clg_ceil_div(batch, (int64_t)chunk_lanes(batch) * (fours(batch) ? 4 : 1)); }
 

@@ -7,7 +7,8 @@
 //
 // Rows in memory ("rows", features dense): a workgroup has a row, whose scores stay in LDS from the sums to the gradient, so the features are read once (rows_kernel);
 // rows of more classes than LDS holds, or too few rows to fill the chip, go in pieces of the classes, once for the sums and the highest (row_stats_kernel) and once
-// more for the gradient (row_grad_kernel).  A feature per row in memory ("columns"): lanes are samples, in pieces of the classes likewise.
+// more for the gradient (row_grad_kernel).  A feature per row in memory ("columns"): lanes are samples, in pieces of the classes likewise; where a class has few
+// features the gradient is from the features again, else from the classes' sums, and large classes in a few of them go in slices (column_stats_kernel joins these).
 #include "row_sums.h"
 
 namespace {
@@ -430,13 +431,14 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(CeArgs a)
     }
 }
 
-// Few short rows, by one workgroup: 16 lanes to a row, a lane has classes l, l + 16, ...  The whole call is one launch: 100 rows of 10 classes 4 us.
-constexpr int kFewClasses = 64, kFewFeatures = 1 << 15, kFewRow = 1024;
+// Few short rows, by one workgroup: 16 lanes to a row, a lane has classes l, l + 16, ...  The call is one launch, not two: 100 rows of 10 classes with gradient 9.3 us
+// in all, 10.6 with a workgroup for each row and one that adds their losses; 128 rows of 64 13 and 10, and a launch less for the host; 256 of 10 17 and 11.
+constexpr int kFewRows = 128, kFewFeatures = 64;
 template <typename T>
 __global__ __launch_bounds__(1024) void few_rows_kernel(CeArgs a, void *out_sum)
 {
     typedef typename Wide<T>::type A;
-    constexpr int EACH = kFewClasses / 16;
+    constexpr int EACH = kFewFeatures / 16;
     __shared__ double room[16], more[16];
     const double per = per_row<1024>(a, room);
     if (a.count == 1 && threadIdx.x == 0) *a.per_count = per;
@@ -904,7 +906,7 @@ Plan plan_of(int dtype, bool rows, int64_t n, int64_t features, int64_t k)
         p.per_piece = (int)(each < k ? each : k);
         p.pieces = (int)clg_ceil_div(k, p.per_piece);
     };
-    p.few = rows && k <= kFewClasses && features <= kFewRow && n <= kCounted && n * features <= kFewFeatures;
+    p.few = rows && n <= kFewRows && features <= kFewFeatures;
     if (rows) {
         // a lane for each piece of a class, up to a wavefront: what the lanes load at once is then in one place (a lane for four pieces, two lanes to a class
         // of 61 bfloat16 features: 2.1 TB/s)
@@ -912,7 +914,9 @@ Plan plan_of(int dtype, bool rows, int64_t n, int64_t features, int64_t k)
         p.lanes_log2 = p.group < e ? 0 : log2_up(clg_ceil_div(p.group, e));
         if (p.lanes_log2 > 6) p.lanes_log2 = 6;
         const int64_t lds = k * (dtype == CLG_F64 || p.group > kNear ? 8 : 4);
-        p.whole = lds <= kLds && (n >= 128 || features * p.size <= 64 << 10);
+        // a workgroup for a row of 256 KB (1000 classes of 64 float32) takes 26, 28, 28 and 33 us for 32, 64, 96 and 192 of them, pieces 22, 26, 36 and 50; for
+        // rows of 240 KB (30000 of 4 bfloat16) 23, 25 and 31 for 32, 64 and 192, pieces 19, 25 and 45; for 16 and 96 of 32 KB 15 and 15, pieces 16 and 21
+        p.whole = lds <= kLds && (n > 64 || features * p.size <= 64 << 10);
         // else about 1024 workgroups, of 16 KiB of features at least
         int64_t want = clg_ceil_div(1024, n), most = clg_ceil_div(features * p.size, 16 << 10);
         cut(want < most ? want : most, 16);
@@ -931,6 +935,9 @@ Plan plan_of(int dtype, bool rows, int64_t n, int64_t features, int64_t k)
         p.slices = (int)(slices < most ? slices : most);
         if (p.slices < 1) p.slices = 1;
         if (p.slices > 64) p.slices = 64;
+        // The sums of the classes are written out for the gradient where that is less than to read the features again: without and with, 1024 rows of 4096 classes
+        // of 4 float32 features 66 and 69 us, of 5 71 and 67, of 16 190 and 157; of 8 bfloat16 69 and 66, of 16 118 and 92.  Those that are no more than a
+        // sixteenth of the features are kept for a backward pass with another upstream gradient.
         p.kept_scores = p.slices > 1 || p.group * p.size >= 128;
         p.scores = p.kept_scores || p.group * p.size > 16;
     }
@@ -1009,12 +1016,16 @@ int launch_rows(const char *name, const CeArgs &a, hipStream_t stream)
     CLG_CHECK_LAUNCH(name);
     return CLG_OK;
 }
+// Threads of a row.  64, 256 and 1024 of them, 2000 rows of 4 KB of float32 19, 21 and 45 us, of 16 KB 24, 27 and 48, of 64 KB 68, 66 and 86, of 256 KB 278, 248
+// and 224, of bfloat16 32 KB 46, 38 and 68, 128 KB 160, 130 and 139; 500 rows of 4 KB 14, 12 and 17, of 64 KB 49, 25 and 28, of 256 KB 180, 70 and 64; 150 rows of 4
+// KB 13, 11 and 12, of 64 KB 44, 21 and 17.
 template <typename T, int PACK, typename S>
 int launch_rows(const char *name, const CeArgs &a, hipStream_t stream)
 {
-    const int64_t features = (int64_t)a.k * a.group;
-    if (features <= 2048) return launch_rows<T, 64, PACK, S>(name, a, stream);
-    if (features <= 16384) return launch_rows<T, 256, PACK, S>(name, a, stream);
+    const int64_t bytes = (int64_t)a.k * a.group * sizeof(T);
+    const bool many = a.rows >= 1024;
+    if (bytes <= (many ? 16 << 10 : 2 << 10)) return launch_rows<T, 64, PACK, S>(name, a, stream);
+    if (bytes <= (many ? 128 << 10 : 32 << 10)) return launch_rows<T, 256, PACK, S>(name, a, stream);
     return launch_rows<T, 1024, PACK, S>(name, a, stream);
 }
 
@@ -1050,6 +1061,7 @@ int forward(const char *name, const Plan &p, const CeArgs &a, void *out_sum, hip
     CLG_CHECK_LAUNCH(name);
     if (!p.rows && p.slices > 1) return CLG_OK;
     typedef typename Wide<T>::type A;
+    // (16 and 64 lanes to a row, the whole call: 32 pieces of 64 rows 16 and 22 us, 64 22 and 20, 256 34 and 24; 256 pieces of 1024 rows 46 and 37)
     if (p.pieces <= 32) join_kernel<A, 16><<<dim3(out_sum ? 1 : (unsigned)clg_ceil_div(p.n, 1024 / 16)), dim3(1024), 0, stream>>>(a, out_sum);
     else join_kernel<A, 64><<<dim3(out_sum ? 1 : (unsigned)clg_ceil_div(p.n, 1024 / 64)), dim3(1024), 0, stream>>>(a, out_sum);
     CLG_CHECK_LAUNCH(name);

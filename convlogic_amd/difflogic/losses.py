@@ -186,7 +186,7 @@ def _distillation_plain(logits, values, indices, logsumexp, temperature, mask, w
 
 # ---- cross entropy of group sums -----------------------------------------------------------------
 def group_cross_entropy(x, targets, k, tau=1.0, *, label_smoothing=0.0, weight=1.0, reduction="mean"):
-    """weight * cross_entropy(GroupSum(k, tau)(x), targets, label_smoothing=...) of x [..., features], without scores in memory beyond the call: a class is
+    """weight * cross_entropy(GroupSum(k, tau)(x), targets, label_smoothing=...) of x [..., features] in one node, which keeps no probabilities: a class is
     features / k features in a row, its score their sum over tau, and k = features takes x as scores.
 
     targets int32 or int64 [...]: a row with a negative one does not count -- loss 0 and gradient 0, whatever its features are -- and one of k or more makes
