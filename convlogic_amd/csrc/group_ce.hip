@@ -930,11 +930,13 @@ Plan plan_of(int dtype, bool rows, int64_t n, int64_t features, int64_t k)
                 p.samples = v;
         const int64_t chunks = chunks_of(p), want = clg_ceil_div(1024, chunks);
         cut(want < clg_ceil_div(k, 4) ? want : clg_ceil_div(k, 4), 4);
-        // (few classes: the workgroup that joins the slices has all of them)
-        const int64_t slices = clg_ceil_div(1024, chunks * p.pieces), most = k <= kSliced ? p.group / 64 : 1;
+        // Slices of 64 features at least, for up to three workgroups to a CU (few classes: the workgroup that joins the slices has all of them).  768, 1024 and 1536
+        // workgroups: 512 rows of 10 classes of 8192 float32 88, 94 and 96 us, 1000 of 7 of 3000 54, 54 and 59; up to 64 and 256 slices: 64 rows of 2 of 65536
+        // 115 and 50.
+        const int64_t slices = 768 / (chunks * p.pieces), most = k <= kSliced ? p.group / 64 : 1;
         p.slices = (int)(slices < most ? slices : most);
         if (p.slices < 1) p.slices = 1;
-        if (p.slices > 64) p.slices = 64;
+        if (p.slices > 256) p.slices = 256;
         // The sums of the classes are written out for the gradient where that is less than to read the features again: without and with, 1024 rows of 4096 classes
         // of 4 float32 features 66 and 69 us, of 5 71 and 67, of 16 190 and 157; of 8 bfloat16 69 and 66, of 16 118 and 92.  Those that are no more than a
         // sixteenth of the features are kept for a backward pass with another upstream gradient.
@@ -1052,9 +1054,11 @@ int forward(const char *name, const Plan &p, const CeArgs &a, void *out_sum, hip
     } else {
         with_samples<T>(p.samples, [&](auto v) { column_sums_kernel<T, decltype(v)::value><<<columns, dim3(kPart), 0, stream>>>(a); });
         CLG_CHECK_LAUNCH(name);
-        if (p.slices > 1) {                                           // 16 samples to a workgroup, so that there are some of them
+        // 4 samples to a workgroup, and 16 lanes to a class's slices: this kernel of 256 rows of 10 classes in 64 slices 7.5 us, with 16 samples 10.9; of 1024 rows
+        // of 256 classes in 5 slices 20.9 and 18.2
+        if (p.slices > 1) {
             CeArgs b = a;
-            b.lanes_log2 = p.lanes_log2 < 4 ? p.lanes_log2 : 4;
+            b.lanes_log2 = p.lanes_log2 < 2 ? p.lanes_log2 : 2;
             column_stats_kernel<T><<<dim3((unsigned)clg_ceil_div(p.n, 1ll << b.lanes_log2)), dim3(1024), 0, stream>>>(b);
         }
     }
