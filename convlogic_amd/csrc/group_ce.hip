@@ -551,12 +551,12 @@ __device__ __forceinline__ double row_of(const CeArgs &a, int64_t row, Joint<A> 
     return r.loss((s.m - target) / Unit<A>::unit, s.down / Unit<A>::unit, a.k, a.smoothing) * a.scale * per;
 }
 // The statistics of a row's pieces into M, O, Z and the loss: LANES to a row.  One workgroup for all rows (`out_sum`) also adds their losses.
-template <typename A, int LANES>
-__global__ __launch_bounds__(1024) void join_kernel(CeArgs a, void *out_sum)
+template <typename A, int LANES, int THREADS>
+__global__ __launch_bounds__(THREADS) void join_kernel(CeArgs a, void *out_sum)
 {
-    constexpr int ROWS = 1024 / LANES;
+    constexpr int ROWS = THREADS / LANES;
     __shared__ double room[16], more[16];
-    const double per = per_row<1024>(a, room);
+    const double per = per_row<THREADS>(a, room);
     if (a.count == 1 && blockIdx.x == 0 && threadIdx.x == 0) *a.per_count = per;
     const int l = threadIdx.x % LANES;
     double sum[1] = {0};
@@ -581,7 +581,7 @@ __global__ __launch_bounds__(1024) void join_kernel(CeArgs a, void *out_sum)
         if (a.out) static_cast<A *>(a.out)[row] = (A)loss;
     }
     if (!out_sum) return;
-    block_reduce<true, 1024>(sum, more);
+    block_reduce<true, THREADS>(sum, more);
     if (threadIdx.x == 0) *static_cast<A *>(out_sum) = (A)sum[0];
 }
 
@@ -1065,9 +1065,12 @@ int forward(const char *name, const Plan &p, const CeArgs &a, void *out_sum, hip
     CLG_CHECK_LAUNCH(name);
     if (!p.rows && p.slices > 1) return CLG_OK;
     typedef typename Wide<T>::type A;
-    // (16 and 64 lanes to a row, the whole call: 32 pieces of 64 rows 16 and 22 us, 64 22 and 20, 256 34 and 24; 256 pieces of 1024 rows 46 and 37)
-    if (p.pieces <= 32) join_kernel<A, 16><<<dim3(out_sum ? 1 : (unsigned)clg_ceil_div(p.n, 1024 / 16)), dim3(1024), 0, stream>>>(a, out_sum);
-    else join_kernel<A, 64><<<dim3(out_sum ? 1 : (unsigned)clg_ceil_div(p.n, 1024 / 64)), dim3(1024), 0, stream>>>(a, out_sum);
+    // In one workgroup that adds the losses too, 16 lanes to a row, or 64 where it has more than 32 pieces (then of up to 16 rows): 40 rows of 16 pieces 5.2 and 8.4
+    // us, 16 of them 4.6 and 5.5.  Else four rows to a workgroup, 64 lanes each: 100 rows of 256 pieces 5.9 us, with 16 lanes 10.9; 1024 rows of 256 7.2 and 11.2,
+    // with 16 rows to a workgroup, whose lanes have a line of memory each, 10.2.
+    if (!out_sum) join_kernel<A, 64, 256><<<dim3(blocks(clg_ceil_div(p.n, 4))), dim3(256), 0, stream>>>(a, nullptr);
+    else if (p.pieces <= 32) join_kernel<A, 16, 1024><<<dim3(1), dim3(1024), 0, stream>>>(a, out_sum);
+    else join_kernel<A, 64, 1024><<<dim3(1), dim3(1024), 0, stream>>>(a, out_sum);
     CLG_CHECK_LAUNCH(name);
     return CLG_OK;
 }
@@ -1149,6 +1152,7 @@ extern "C" int clg_group_ce_forward(int dtype, const void *x, int64_t row_stride
     // one workgroup also adds the losses: all of few rows, or the joint statistics of so many
     const bool add = reduction != CLG_REDUCE_NONE && (p.few || (!p.whole && p.slices == 1 && rows <= (p.pieces <= 32 ? 64 : 16)));
     if (at_once) a.grad = grad;
+    if (!grad && !p.kept_scores) a.scores = nullptr;
     int rc = clg_with_type(dtype, [&](auto t) { return forward<decltype(t)>(name, p, a, add ? loss : nullptr, st); });
     if (rc) return rc;
     if (grad && !at_once) {
