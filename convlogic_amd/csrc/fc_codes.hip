@@ -127,9 +127,10 @@ __device__ __forceinline__ void encode_row(const Layer &L, int64_t at, const flo
 }
 
 // Forward pass from the logits, with the arithmetic of clg_fc_forward_logits; a neuron takes LPR lanes.  ENCODE: every input is read by one operand only, whose
-// neuron also makes its codes, and the batch is a multiple of 128, so that a row of 32 lanes has a group (x is then read once, not twice: 163840 inputs, batch
-// 256, forward pass and codes 110 -> 68 us).  Else the workgroups from neuron_blocks on make them.  The wiring and the logits of a wavefront's next neurons are on
-// their way while the rows of these are.
+// neuron also makes its codes, and the batch is a multiple of 128, so that a row of 32 lanes has a group: x is then read once, not twice (163840 inputs, batch 256,
+// forward pass and codes 76 us, not 95; with 64 lanes, two groups at a time, 79; batch 384 109, 143 and 117).  Else the workgroups from neuron_blocks on make them.
+// The wiring and the logits of a wavefront's next neurons are on their way while the rows of these are.  131072 -> 1310720 neurons, batch 128: 350 us for 0.95 GB
+// and 1.3 of rows of x that the XCDs fetch from the memory side, 6.4 TB/s.
 template <int VEC, bool RAGGED, int LPR, bool ENCODE>
 __global__ __launch_bounds__(kBlock) void forward_kernel(Layer L, int neuron_blocks)
 {
@@ -479,7 +480,7 @@ extern "C" int clg_fc_codes_forward(const float *x, const int64_t *a, const int6
     L.x = x, L.logits = logits, L.probs = probs, L.y = y, L.in_dim = in_dim, L.out_dim = out_dim, L.batch = batch;
     hipStream_t st = clg_stream(stream);
     const bool encode = sole && batch % kCodeGroup == 0;
-    with_rows(batch, lanes_of(batch), [&](auto vec, auto ragged, auto lpr) {
+    with_rows(batch, encode ? 32 : lanes_of(batch), [&](auto vec, auto ragged, auto lpr) {
         constexpr int VEC = decltype(vec)::value, LPR = decltype(lpr)::value;
         constexpr bool RAGGED = decltype(ragged)::value;
         // (up to four neurons one after the other, from where the chip is full)
@@ -487,7 +488,7 @@ extern "C" int clg_fc_codes_forward(const float *x, const int64_t *a, const int6
         const int neurons = (int)blocks_of(clg_ceil_div(wavefronts, turns < 1 ? 1 : turns > kTurns ? kTurns : turns));
         const int coders = encode ? 0 : (int)blocks_of(clg_ceil_div(in_dim * batch, 4 * (int64_t)kCodeLanes * kCodeEach));
         const dim3 grid((unsigned)(neurons + coders));
-        if constexpr (!RAGGED && LPR >= 32)
+        if constexpr (!RAGGED && LPR == 32)
             if (encode) return forward_kernel<VEC, RAGGED, LPR, true><<<grid, dim3(kBlock), 0, st>>>(L, neurons);
         forward_kernel<VEC, RAGGED, LPR, false><<<grid, dim3(kBlock), 0, st>>>(L, neurons);
     });
