@@ -8,7 +8,6 @@ namespace {
 
 constexpr int kWaves = 4, kBlock = kWaves * kWave;
 constexpr int64_t kFull = 256 * 32, kTurns = 4;                       // wavefronts that the chip holds; items that one takes, from there on
-constexpr int kWay = 24;                                              // lanes' worth of the way to the rows
 typedef float f32x4_row __attribute__((ext_vector_type(4), aligned(4)));
 
 template <int VEC>
@@ -246,17 +245,17 @@ __device__ __forceinline__ uint64_t from_lane(uint64_t v, int at)
     return (uint64_t)from_lane<LPR>((uint32_t)(v >> 32), at) << 32 | from_lane<LPR>((uint32_t)v, at);
 }
 
-// LPR lanes take `each` inputs one after the other and go through the operands these are, which follow one another in `list`, for LPR * VEC samples.  The
+// LPR lanes take `each` inputs one after the other and go through the operands these are, which follow one another in `list`, for PARTS * LPR * VEC samples.  The
 // visit that reaches a neuron through its first operand has all its rows and forms its sums as well (SUMS): the gradient of its logits if the samples are the
 // whole batch (kWhole), else for gradients_kernel (kParts).  A neuron wired to an input twice is listed twice, and is its second operand the second time.
 // The way to a row -- list entry, neuron, row -- is three trips to memory: the lanes first go it for as many operands as they are, one each, and then
 // take these one by one, with the rows of the next two on their way (of the next four: 28 to 57 registers more, and 8000 -> 8000 neurons, batch 100, 9.7 us, not
 // 7.9).  I: what holds an index into x and gy.
-// 131072 -> 1310720 neurons, batch 128: 365 us for 1.3 GB of gradients that are read twice, 0.3 of codes and 0.2 of the rest, 5 TB/s; a walk operand by operand, with
-// the wiring and the coefficients in tables of their own, took 623.
+// 131072 -> 1310720 neurons, batch 128: 395 us for 1.3 GB of gradients that are read twice, 0.3 of codes and 0.2 of the rest, 4.6 TB/s; a walk operand by operand,
+// with the wiring and the coefficients in tables of their own, took 623.
 enum { kNoSums, kWhole, kParts };
 constexpr int kEachMost = 15;
-template <int VEC, bool RAGGED, int LPR, int SUMS, typename I>
+template <int VEC, bool RAGGED, int LPR, int PARTS, int SUMS, typename I>
 __global__ __launch_bounds__(kBlock) void inputs_kernel(Layer L, int each)
 {
     constexpr int ROWS = kWave / LPR;
@@ -264,11 +263,19 @@ __global__ __launch_bounds__(kBlock) void inputs_kernel(Layer L, int each)
     const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x >> 6), sub = lane / LPR, l = lane % LPR, q = lane & 15;
     const int64_t groups = (L.in_dim + each - 1) / each, most = 2 * L.out_dim;
     const I batch = (I)L.batch;
-    const Samples<VEC, RAGGED> mine(((int64_t)blockIdx.y * LPR + l) * VEC, L.batch);
-    const I mine_at = (I)mine.at;
+    struct Part {
+        I at;
+        int again;
+        bool live;
+    } part[PARTS];                                                    // LPR * VEC samples apart
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        const Samples<VEC, RAGGED> s((((int64_t)blockIdx.y * PARTS + p) * LPR + l) * VEC, L.batch);
+        part[p] = {(I)s.at, s.live ? s.again : VEC, s.live};
+    }
     struct Rows {
-        Coded<VEC, RAGGED> x, own;
-        float g[VEC];
+        Coded<VEC, RAGGED> x[PARTS], own[PARTS];
+        float g[PARTS][VEC];
         int mark;
     };
     for (int64_t it = ((int64_t)blockIdx.x * kWaves + wave) * ROWS; it < groups; it += (int64_t)gridDim.x * kWaves * ROWS) {
@@ -282,10 +289,8 @@ __global__ __launch_bounds__(kBlock) void inputs_kernel(Layer L, int each)
         if constexpr (LPR <= 32) longest = max(longest, __shfl_xor(longest, 32));
         if constexpr (LPR <= 16) longest = max(longest, __shfl_xor(longest, 16));
         longest = uniform(longest);
-        const I own_at = (I)i0 * batch + mine_at;                     // the first input's
-        float acc[VEC];
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+        const I own_at = (I)i0 * batch;                               // the first input's
+        float acc[PARTS][VEC] = {};
         for (int base = 0; base < longest; base += LPR) {
             // an operand for each lane
             const int at = base + l;
@@ -312,28 +317,37 @@ __global__ __launch_bounds__(kBlock) void inputs_kernel(Layer L, int each)
             const auto load = [&](int e, Rows &r) {
                 const int from = e < LPR ? e : LPR - 1;               // (what is behind the last of a row is dropped)
                 r.mark = from_lane<LPR>(mark, from);
-                const float *g = L.gy + (from_lane<LPR>(row_g, from) + mine_at);
-                load_floats(g, r.g);
-                r.x.load(L.codes, L.scales, (I)(from_lane<LPR>(row_x, from) + mine_at));
-                if (SUMS != kNoSums) r.own.load(L.codes, L.scales, (I)(own_at + (I)(r.mark & kOwner) * batch));
+                const I at_g = from_lane<LPR>(row_g, from), at_x = from_lane<LPR>(row_x, from), at_own = own_at + (I)(r.mark & kOwner) * batch;
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    load_floats(L.gy + (at_g + part[p].at), r.g[p]);
+                    r.x[p].load(L.codes, L.scales, (I)(at_x + part[p].at));
+                    if (SUMS != kNoSums) r.own[p].load(L.codes, L.scales, (I)(at_own + part[p].at));
+                }
             };
             const auto take = [&](int e, const Rows &r) {
                 if (e >= steps) return;
                 const float ab = from_lane<LPR>(c_ab, e), lin = from_lane<LPR>(c_own, e);
-                float x[VEC];
-                r.x.values(x);
+                float x[PARTS][VEC];
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) r.x[p].values(x[p]);
                 // (an operand that is not there has coefficients 0, and a gradient that may be infinite)
                 if (LPR == kWave || base + e < edges) {
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) acc[k] = __builtin_fmaf(__builtin_fmaf(ab, x[k], lin), r.g[k], acc[k]);
+                    for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k) acc[p][k] = __builtin_fmaf(__builtin_fmaf(ab, x[p][k], lin), r.g[p][k], acc[p][k]);
                 }
                 if (SUMS != kNoSums) {
                     const int32_t to = from_lane<LPR>(j, e);
                     if (r.mark & kFirst) {                            // uniform over the lanes of a row
-                        float own[VEC];
-                        r.own.values(own);
                         Sums sums;
-                        sums.add(r.g, own, x, mine.live ? mine.again : VEC);
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p) {
+                            float own[VEC];
+                            r.own[p].values(own);
+                            sums.add(r.g[p], own, x[p], part[p].again);
+                        }
                         if constexpr (SUMS == kWhole) {
                             sums.over_lanes<LPR>();
                             if (l >= LPR - 16) L.gl[(int64_t)to * 16 + q] = sums.of_logit(q, L.probs[(int64_t)to * 16 + q]);
@@ -343,9 +357,12 @@ __global__ __launch_bounds__(kBlock) void inputs_kernel(Layer L, int each)
                     }
                 }
                 if (r.mark & kLast) {
-                    if (mine.live) store_floats(L.gx + (own_at + (I)(r.mark & kOwner) * batch), acc);
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+                    for (int p = 0; p < PARTS; ++p) {
+                        if (part[p].live) store_floats(L.gx + (own_at + (I)(r.mark & kOwner) * batch + part[p].at), acc[p]);
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k) acc[p][k] = 0.f;
+                    }
                 }
             };
             constexpr int AHEAD = 2;
@@ -363,11 +380,11 @@ __global__ __launch_bounds__(kBlock) void inputs_kernel(Layer L, int each)
         // inputs that nobody reads
         for (int k = 0; k < each; ++k) {
             const int e = from_lane<LPR>(ends, k), b = k ? from_lane<LPR>(ends, k - 1) : 0;
-            if (k < count && e <= b && mine.live) {
-                float none[VEC];
+            if (k < count && e <= b) {
+                const float none[VEC] = {};
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) none[v] = 0.f;
-                store_floats(L.gx + (own_at + (I)k * batch), none);
+                for (int p = 0; p < PARTS; ++p)
+                    if (part[p].live) store_floats(L.gx + (own_at + (I)k * batch + part[p].at), none);
             }
         }
     }
@@ -404,21 +421,34 @@ int lanes_of(int64_t batch)
     const int64_t lanes = fours(batch) ? clg_ceil_div(batch, 4) : batch;
     return lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64;
 }
-// Where rows go in chunks of the batch, each with a way to them of its own: 32 lanes where 64 would leave many of them idle.  30001 -> 60000 neurons with 64 and 32
-// lanes, the whole step: batch 333 138 and 132 us, 300 110 and 114, 512 139 and 152, 700 207 and 236.
-int chunk_lanes(int64_t batch)
+// How inputs_kernel takes a batch: LANES to a row, PARTS of LANES x 4 samples to a lane, so that up to 512 samples go one way to their rows.  inputs_kernel alone,
+// with the shape taken and the next best: 30001 -> 60000 neurons, batch 150 36.8 us and 41.9 (64 lanes), 190 40.6 and 46.6, 200 39.9 and 46.7 (16 lanes, 3 parts),
+// 300 48.6 and 55.1 (64, 2), 333 67.2 and 72.2 (16, 3, two chunks of the batch), 400 59.8 and 65.2 (64, two chunks); 300000 -> 500000, batch 300 439 and 479, with
+// three chunks of 32 lanes 588.  Two parts where one does: batch 256 43.0 us for 41.0, batch 128 23.6 for 22.1.  Behind 512 samples chunks of 64 lanes: batch 700
+// 109 us, with three parts of 32 lanes 111, with two of 64 115.
+struct Shape {
+    int lanes, parts;
+};
+Shape shape_of(int64_t batch)
 {
-    const auto cost = [&](int lanes) { return clg_ceil_div(batch, (int64_t)lanes * 4) * (lanes + kWay); };
-    return batch > 256 && cost(32) < cost(64) ? 32 : lanes_of(batch);
+    if (batch > 128 && batch <= 192) return {16, 3};
+    if (batch > 256 && batch <= 384) return {32, 3};
+    if (batch > 384 && batch <= 512) return {64, 2};
+    return {lanes_of(batch), 1};
 }
-int64_t chunks_of(int64_t batch) { return clg_ceil_div(batch, (int64_t)chunk_lanes(batch) * (fours(batch) ? 4 : 1)); }
+int64_t chunks_of(int64_t batch)
+{
+    const Shape s = shape_of(batch);
+    return clg_ceil_div(batch, (int64_t)s.lanes * s.parts * (fours(batch) ? 4 : 1));
+}
 
 // Whether gradients_kernel ends the sums, also those of one chunk: with and without it 34.8 + 3.9 and 39.2 us for 30001 -> 60000 neurons, batch 256, 69.0 + 4.7 and
 // 78.6 for 100000 -> 100000; batch 64 14.5 + 3.8 and 16.1, 24.8 + 4.1 and 26.7.
 bool in_parts(int64_t out_dim, int64_t batch) { return chunks_of(batch) > 1 || out_dim * batch >= 1 << 24; }
 
-// Inputs that a row of lanes takes: about 16 operands, worth the way to them, and rows enough to fill the chip.  1, 4 and 15 inputs each: 100000 -> 100000 neurons,
-// batch 256, 94, 70 and 71 us; 30001 -> 60000, batch 333, 85, 77 and 77; 8000 -> 8000, batch 100, 8, 11 and 27; 131072 -> 1310720, batch 128, 369, 372 and 427.
+// Inputs that a row of lanes takes: about 16 operands, worth the way to them, and rows enough to fill the chip.  inputs_kernel with 1, 4 and 15 inputs each: 100000
+// -> 100000 neurons, batch 256, 94, 70 and 72 us; 30001 -> 60000, batch 150, 37, 34 and 77; batch 333 73, 69 and 72; 8000 -> 8000, batch 100, 8, 11 and 27; 131072
+// -> 1310720, batch 128, 389, 397 and 453.
 int inputs_each(int64_t in_dim, int64_t out_dim, int64_t chunks, int rows)
 {
     const int64_t fan = clg_ceil_div(2 * out_dim, in_dim), by_fan = 16 / fan, by_rows = in_dim * chunks / (rows * 4096);
@@ -514,7 +544,8 @@ extern "C" int clg_fc_codes_backward(const uint8_t *codes, const void *scales, c
     L.in_dim = in_dim, L.out_dim = out_dim, L.batch = batch;
     hipStream_t st = clg_stream(stream);
     const bool by_neurons = !grad_x || (sole && grad_logits);
-    with_rows(batch, by_neurons ? lanes_of(batch) : chunk_lanes(batch), [&](auto vec, auto ragged, auto lpr) {
+    const Shape shape = shape_of(batch);
+    with_rows(batch, by_neurons ? lanes_of(batch) : shape.lanes, [&](auto vec, auto ragged, auto lpr) {
         constexpr int VEC = decltype(vec)::value, LPR = decltype(lpr)::value, ROWS = kWave / LPR;
         constexpr bool RAGGED = decltype(ragged)::value;
         if (by_neurons) {
@@ -527,9 +558,15 @@ extern "C" int clg_fc_codes_backward(const uint8_t *codes, const void *scales, c
         const dim3 grid(blocks_of(clg_ceil_div(clg_ceil_div(in_dim, each), (int64_t)ROWS)), (unsigned)chunks_of(batch));
         const auto launch = [&](auto index) {
             typedef decltype(index) I;
-            if (!grad_logits) inputs_kernel<VEC, RAGGED, LPR, kNoSums, I><<<grid, dim3(kBlock), 0, st>>>(L, each);
-            else if (parts) inputs_kernel<VEC, RAGGED, LPR, kParts, I><<<grid, dim3(kBlock), 0, st>>>(L, each);
-            else inputs_kernel<VEC, RAGGED, LPR, kWhole, I><<<grid, dim3(kBlock), 0, st>>>(L, each);
+            const auto with = [&](auto n) {
+                constexpr int PARTS = decltype(n)::value;
+                if (!grad_logits) inputs_kernel<VEC, RAGGED, LPR, PARTS, kNoSums, I><<<grid, dim3(kBlock), 0, st>>>(L, each);
+                else if (parts) inputs_kernel<VEC, RAGGED, LPR, PARTS, kParts, I><<<grid, dim3(kBlock), 0, st>>>(L, each);
+                else inputs_kernel<VEC, RAGGED, LPR, PARTS, kWhole, I><<<grid, dim3(kBlock), 0, st>>>(L, each);
+            };
+            if constexpr (VEC == 4)
+                if (shape.parts > 1) return with(std::integral_constant<int, LPR == 64 ? 2 : 3>());
+            with(std::integral_constant<int, 1>());
         };
         // (the batch behind the last row: what lanes that are dropped read is in front of it)
         if ((in_dim > out_dim ? in_dim : out_dim) * batch < 1ll << 30) launch(uint32_t());

@@ -179,6 +179,17 @@ def test_layer_of_which_one_gradient_is_wanted(need, batch):
     check_layer(layer_of(40, 20), batch, need=need)
 
 
+@pytest.mark.parametrize("batch", [150, 191, 192, 193, 300, 383, 384, 385, 400, 511, 513])
+@pytest.mark.parametrize("inputs,neurons", [(3, 5), (33, 700), (300, 150)])
+def test_layer_with_several_samples_of_a_row_to_a_lane(inputs, neurons, batch):
+    check_layer(layer_of(inputs, neurons), batch, seed=batch)
+
+
+@pytest.mark.parametrize("inputs,neurons,batch", [(2001, 90000, 187), (2001, 90000, 192), (50000, 45000, 377), (2001, 45000, 384), (2001, 33000, 511)])
+def test_large_layer_whose_sums_are_ended_apart(inputs, neurons, batch):
+    check_layer(layer_of(inputs, neurons), batch, seed=batch)
+
+
 @pytest.mark.parametrize("batch", [1, 33, 128, 300])
 def test_layer_on_samples_in_rows(batch):
     check_layer(layer_of(50, 37), batch, sample_major=True)
