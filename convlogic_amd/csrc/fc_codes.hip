@@ -128,8 +128,8 @@ __device__ __forceinline__ void encode_row(const Layer &L, int64_t at, const flo
 // Forward pass from the logits, with the arithmetic of clg_fc_forward_logits; a neuron takes LPR lanes.  ENCODE: every input is read by one operand only, whose
 // neuron also makes its codes, and the batch is a multiple of 128, so that a row of 32 lanes has a group: x is then read once, not twice (163840 inputs, batch 256,
 // forward pass and codes 76 us, not 95; with 64 lanes, two groups at a time, 79; batch 384 109, 143 and 117).  Else the workgroups from neuron_blocks on make them.
-// The wiring and the logits of a wavefront's next neurons are on their way while the rows of these are.  131072 -> 1310720 neurons, batch 128: 350 us for 0.95 GB
-// and 1.3 of rows of x that the XCDs fetch from the memory side, 6.4 TB/s.
+// The wiring and the logits of a wavefront's next neurons are on their way while the rows of these are.  131072 -> 1310720 neurons, batch 128: 350 us for 1.5 GB read,
+// 1.3 of them rows of x, which are in no XCD's cache, and 0.8 written, 6.6 TB/s.
 template <int VEC, bool RAGGED, int LPR, bool ENCODE>
 __global__ __launch_bounds__(kBlock) void forward_kernel(Layer L, int neuron_blocks)
 {
@@ -250,16 +250,17 @@ __device__ __forceinline__ uint64_t from_lane(uint64_t v, int at)
 // whole batch (kWhole), else for gradients_kernel (kParts).  A neuron wired to an input twice is listed twice, and is its second operand the second time.
 // The way to a row -- list entry, neuron, row -- is three trips to memory: the lanes first go it for as many operands as they are, one each, and then
 // take these one by one, with the rows of the next two on their way (of the next four: 28 to 57 registers more, and 8000 -> 8000 neurons, batch 100, 9.7 us, not
-// 7.9).  I: what holds an index into x and gy.
-// 131072 -> 1310720 neurons, batch 128: 395 us for 1.3 GB of gradients that are read twice, 0.3 of codes and 0.2 of the rest, 4.6 TB/s; a walk operand by operand,
-// with the wiring and the coefficients in tables of their own, took 623.
+// 7.9); an input's own row is read with its first operand's and stays in registers (with every operand's: 30001 -> 60000, batch 333, 67 us, not 58).  I: what holds
+// an index into x and gy.
+// 131072 -> 1310720 neurons, batch 128: 370 us for 2.2 GB that leave the memory side -- 1.3 of gradients, each read twice, 0.3 of codes, the rest wiring and
+// coefficients by the line -- 6 TB/s; a walk operand by operand, with the wiring and the coefficients in tables of their own, took 623.
 enum { kNoSums, kWhole, kParts };
 constexpr int kEachMost = 15;
 template <int VEC, bool RAGGED, int LPR, int PARTS, int SUMS, typename I>
 __global__ __launch_bounds__(kBlock) void inputs_kernel(Layer L, int each)
 {
     constexpr int ROWS = kWave / LPR;
-    constexpr int kOwner = 15, kFirst = 16, kLast = 32;
+    constexpr int kOwner = 15, kFirst = 16, kLast = 32, kOpens = 64;
     const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x >> 6), sub = lane / LPR, l = lane % LPR, q = lane & 15;
     const int64_t groups = (L.in_dim + each - 1) / each, most = 2 * L.out_dim;
     const I batch = (I)L.batch;
@@ -290,7 +291,7 @@ __global__ __launch_bounds__(kBlock) void inputs_kernel(Layer L, int each)
         if constexpr (LPR <= 16) longest = max(longest, __shfl_xor(longest, 16));
         longest = uniform(longest);
         const I own_at = (I)i0 * batch;                               // the first input's
-        float acc[PARTS][VEC] = {};
+        float acc[PARTS][VEC] = {}, own[PARTS][VEC];                  // gradient and values of the input that has its turn
         for (int base = 0; base < longest; base += LPR) {
             // an operand for each lane
             const int at = base + l;
@@ -310,7 +311,7 @@ __global__ __launch_bounds__(kBlock) void inputs_kernel(Layer L, int each)
             }
             const int32_t i = (int32_t)i0 + owner;
             const bool as_a = n.in_a == i && !(n.in_b == i && at > opened && before == j);
-            const int mark = owner | (there && as_a ? kFirst : 0) | (there && at + 1 == closed ? kLast : 0);
+            const int mark = owner | (there && as_a ? kFirst : 0) | (there && at + 1 == closed ? kLast : 0) | (at == opened ? kOpens : 0);
             const I row_x = there ? (I)(as_a ? n.in_b : n.in_a) * batch : I(0), row_g = there ? (I)j * batch : I(0);
             const float c_ab = there ? n.ab : 0.f, c_own = there ? (as_a ? n.a : n.b) : 0.f;
             const int steps = longest - base < LPR ? longest - base : LPR;
@@ -322,7 +323,7 @@ __global__ __launch_bounds__(kBlock) void inputs_kernel(Layer L, int each)
                 for (int p = 0; p < PARTS; ++p) {
                     load_floats(L.gy + (at_g + part[p].at), r.g[p]);
                     r.x[p].load(L.codes, L.scales, (I)(at_x + part[p].at));
-                    if (SUMS != kNoSums) r.own[p].load(L.codes, L.scales, (I)(at_own + part[p].at));
+                    if (SUMS != kNoSums && r.mark & kOpens) r.own[p].load(L.codes, L.scales, (I)(at_own + part[p].at));
                 }
             };
             const auto take = [&](int e, const Rows &r) {
@@ -340,14 +341,14 @@ __global__ __launch_bounds__(kBlock) void inputs_kernel(Layer L, int each)
                 }
                 if (SUMS != kNoSums) {
                     const int32_t to = from_lane<LPR>(j, e);
+                    if (r.mark & kOpens) {
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p) r.own[p].values(own[p]);
+                    }
                     if (r.mark & kFirst) {                            // uniform over the lanes of a row
                         Sums sums;
 #pragma unroll
-                        for (int p = 0; p < PARTS; ++p) {
-                            float own[VEC];
-                            r.own[p].values(own);
-                            sums.add(r.g[p], own, x[p], part[p].again);
-                        }
+                        for (int p = 0; p < PARTS; ++p) sums.add(r.g[p], own[p], x[p], part[p].again);
                         if constexpr (SUMS == kWhole) {
                             sums.over_lanes<LPR>();
                             if (l >= LPR - 16) L.gl[(int64_t)to * 16 + q] = sums.of_logit(q, L.probs[(int64_t)to * 16 + q]);
