@@ -248,6 +248,30 @@ def test_columns_of_every_width(rows, dtype):
     check(features(rows, 770, 2, dtype), labels(rows, 770, masked=True), 770, "columns", tau=0.5, reduction="none")
 
 
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("layout,rows,k,group", [
+    ("rows", 128, 64, 1), ("rows", 129, 64, 1), ("rows", 128, 13, 5), ("rows", 64, 300, 60), ("rows", 65, 300, 60), ("rows", 64, 250, 64),                # one workgroup, pieces, whole rows
+    ("rows", 70, 512, 1), ("rows", 70, 513, 1), ("rows", 70, 1024, 8), ("rows", 70, 1025, 8), ("rows", 1024, 512, 8), ("rows", 1024, 1025, 4),            # threads
+    ("columns", 3, 2, 65536), ("columns", 17, 3, 20001), ("columns", 64, 10, 2048), ("columns", 70, 256, 130), ("columns", 70, 257, 130),                 # slices
+    ("columns", 16, 140, 3), ("columns", 17, 140, 3), ("columns", 64, 128, 2), ("columns", 65, 128, 2), ("columns", 1030, 1500, 2), ("rows", 20, 2000, 64)])  # joins
+def test_borders_of_the_shapes(layout, rows, k, group, reduction):
+    check(features(rows, k, group), labels(rows, k, masked=True), k, layout, tau=0.3 * group ** 0.5, smoothing=0.1, reduction=reduction)
+    check(features(rows, k, group), labels(rows, k), k, layout, tau=0.3 * group ** 0.5, reduction=reduction, grad=False)
+
+
+@pytest.mark.parametrize("bits", [None, 8])
+def test_a_topology_without_its_group_sum(bits):
+    torch.manual_seed(0)
+    net = C.ConvLogicCifarModel(k_param=4, checkpoint_bits=bits).to(DEV)
+    x, t = (torch.rand(20, 3, 32, 32, device=DEV) > 0.5).float(), torch.randint(0, 10, (20,), device=DEV)
+    loss = C.group_cross_entropy(net.network[:-1](x), t, k=10, tau=20.0, label_smoothing=0.1)
+    other = torch.nn.functional.cross_entropy(net(x), t, label_smoothing=0.1)
+    assert abs(float(loss - other)) <= 1e-5 * float(other)
+    got, want = (torch.autograd.grad(v, list(net.parameters())) for v in (loss, other))
+    # (with codes the layers of the end keep their inputs' codes, its trees those of the first layer's input alone)
+    assert all((u - v).norm() <= (1e-4 if bits is None else 0.05) * v.norm() + 1e-9 for u, v in zip(got, want))
+
+
 def test_features_of_more_than_2_to_the_31_elements():
     rows, k, group = 70000, 32768, 1
     x = torch.zeros(rows, k, device=DEV, dtype=torch.bfloat16)
