@@ -208,6 +208,16 @@ def test_layer_with_inputs_that_few_or_all_neurons_read():
     check_layer(layer_of(1, 1), 7)
 
 
+@pytest.mark.parametrize("batch", [3, 16, 60, 128, 130, 192, 250, 280, 333, 384, 450, 600])
+def test_layer_with_long_and_empty_lists_of_readers(batch):
+    layer = layer_of(40, 300)
+    with torch.no_grad():
+        layer.indices_0.copy_((torch.arange(300) ** 2) % 11 * 3)      # every third input up to 30 by many, the others by none
+        layer.indices_1.copy_(torch.where(torch.arange(300) % 5 == 0, layer.indices_0.cpu(), 3 * (torch.arange(300) % 13)))
+    check_layer(layer, batch)
+    check_layer(layer, batch, need=(True, False))
+
+
 def test_layer_with_groups_of_one_value_and_gradients_that_are_not_finite():
     layer = layer_of(40, 30)
     x = torch.full((40, 128), 0.25)
