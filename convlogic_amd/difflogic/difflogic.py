@@ -148,7 +148,7 @@ class LogicLayer(torch.nn.Module):
         if _lib.traced():
             raise RuntimeError("a layer with checkpoint_bits cannot be traced in training")
         weights, buffers = self._parameters["weights"], self._buffers
-        if x.dtype == torch.float32 and weights.dtype == x.dtype and weights.is_contiguous() and weights.device == x.device and x.numel() > 0:
+        if x.dtype == torch.float32 and weights.dtype == x.dtype and weights.is_contiguous() and weights.device == x.device:
             inside = _transposes_with_kernel(x)
             return _lib.nodes().fc_layer(x if inside else _feature_major(x), buffers["indices_0"], buffers["indices_1"], weights,
                                          buffers["given_x_indices_of_y_start"], buffers["given_x_indices_of_y"], self._sole_consumers(key), inside, True)

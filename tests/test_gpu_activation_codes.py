@@ -218,6 +218,13 @@ def test_layer_with_long_and_empty_lists_of_readers(batch):
     check_layer(layer, batch, need=(True, False))
 
 
+@pytest.mark.parametrize("bits", [None, 8])
+def test_a_layer_without_samples_is_refused_by_its_forward_pass(bits):
+    layer = C.LogicLayer(16, 8, implementation="cuda", checkpoint_bits=bits).to(DEV)
+    with pytest.raises(RuntimeError, match="batch must be positive"):
+        layer(torch.rand(0, 16, device=DEV))
+
+
 def test_layer_with_groups_of_one_value_and_gradients_that_are_not_finite():
     layer = layer_of(40, 30)
     x = torch.full((40, 128), 0.25)
