@@ -67,38 +67,27 @@ __device__ __forceinline__ double per_row(const CeArgs &a, double *room)
     return n[0] == 0 ? 0 : 1 / n[0];
 }
 
-// The statistics of a part of a row's classes, of scores in units: the highest, O and the sum of (highest - score) relative to it, and the number of classes.  A
-// thread holds scores relative to its first one, as A.
+// The statistics of a part of a row's classes, of scores in units: the highest so far, O and the sum of (highest - score) relative to it, and the number of
+// classes.  Differences are taken in 64 bits before anything is rounded to A: relative to a score that is not the highest -- a masked class's, the first one's --
+// those of all others would lose their digits.
 template <typename A>
 struct Stats {
-    double base = 0, others = 0, down = 0, n = 0;
-    A m = lowest(A(0));
-    bool started = false;
-    // -> the score as it is held
-    __device__ __forceinline__ double add(double score, bool is_target, bool smooth)
+    double m = lowest(0.0), others = 0, down = 0, n = 0;
+    __device__ __forceinline__ void add(double score, bool is_target, bool smooth)
     {
-        if (!started) {
-            base = __builtin_fabs(score) <= __DBL_MAX__ ? score : 0;
-            started = true;
+        if (score > m) {
+            if (m != lowest(0.0)) {
+                others *= (double)Unit<A>::power((A)(m - score));
+                down += n * (score - m);
+            }
+            m = score;
         }
-        const A u = (A)(score - base);
-        if (u > m) raise(u);
-        const A e = u == lowest(A(0)) ? A(0) : Unit<A>::power(u - m);
+        const A e = score == lowest(0.0) ? A(0) : Unit<A>::power((A)(score - m));
         others += is_target ? 0.0 : (double)e;
         if (smooth) {
-            down += u == lowest(A(0)) ? -lowest(0.0) : (double)(m - u);
+            down += score == lowest(0.0) ? -lowest(0.0) : m - score;
             n += 1;
         }
-        return base + (double)u;
-    }
-    __device__ __forceinline__ void raise(A to)
-    {
-        if (!(to > m)) return;
-        if (m != lowest(A(0))) {
-            others *= (double)Unit<A>::power(m - to);
-            down += n * (double)(to - m);
-        }
-        m = to;
     }
 };
 // The same of several threads, relative to `m`.
@@ -106,7 +95,7 @@ template <typename A>
 struct Joint {
     double m = lowest(0.0), others = 0, down = 0, n = 0;
     __device__ __forceinline__ Joint() {}
-    __device__ __forceinline__ explicit Joint(const Stats<A> &s) : m(s.base + (double)s.m), others(s.others), down(s.down), n(s.n) {}
+    __device__ __forceinline__ explicit Joint(const Stats<A> &s) : m(s.m), others(s.others), down(s.down), n(s.n) {}
     __device__ __forceinline__ explicit Joint(const double *p) : m(p[0]), others(p[1]), down(p[2]), n(p[3]) {}
     __device__ __forceinline__ void store(double *p) const { p[0] = m, p[1] = others, p[2] = down, p[3] = n; }
     __device__ __forceinline__ void raise(double to)
@@ -534,8 +523,8 @@ __global__ __launch_bounds__(kPart) void row_stats_kernel(CeArgs a)
             const double unit = a.inv_tau * Unit<A>::unit;
             classes.sums(x, first, end, (int64_t)a.k * a.group, [&](int c, double sum, bool mine) {
                 if (!mine) return;
-                const double held = s.add(sum * unit, c == t, smooth);
-                if (c == t) a.target_score[row] = held;
+                s.add(sum * unit, c == t, smooth);
+                if (c == t) a.target_score[row] = sum * unit;
             });
         }
         const Joint<A> all = block_stats<kPart>(s, room);
@@ -778,8 +767,8 @@ __global__ __launch_bounds__(kPart) void column_sums_kernel(CeArgs a)
         if (store && a.scores) store_part<V>(a.scores + (int64_t)c * a.rows + col.row, sum);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const double held = s[v].add(sum[v] * unit, c == t[v], smooth);
-            if (store && c == t[v]) a.target_score[col.row + v] = held;
+            s[v].add(sum[v] * unit, c == t[v], smooth);
+            if (store && c == t[v]) a.target_score[col.row + v] = sum[v] * unit;
         }
     };
     const T *x = static_cast<const T *>(a.x);
@@ -817,9 +806,9 @@ __global__ __launch_bounds__(1024) void column_stats_kernel(CeArgs a)
 #pragma unroll 8
         for (int i = col.sub; i < a.slices; i += col.subs) sum += a.partial[((int64_t)i * a.k + c) * a.rows + col.row];
         for (int by = 1 << a.lanes_log2; by < 64; by <<= 1) sum += __shfl_xor(sum, by);
-        const double held = s[0].add(sum * unit, c == t, smooth);
+        s[0].add(sum * unit, c == t, smooth);
         if (store) a.scores[(int64_t)c * a.rows + col.row] = sum;
-        if (store && c == t) a.target_score[col.row] = held;
+        if (store && c == t) a.target_score[col.row] = sum * unit;
     }
     column_finish(col, s, room, [&](int, const Joint<A> &all) {       // (behind a barrier: the target's score is there)
         const double loss = t < 0 ? 0.0 : t >= a.k ? __builtin_nan("") : row_of(a, col.row, all, a.target_score[col.row], per);

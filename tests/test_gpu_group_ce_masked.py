@@ -1,0 +1,141 @@
+"""Cross entropy of group sums on the GPU where classes are masked with finite values, against its definition in 64 bits (oracle/keep_oracle.py).
+
+Bounds, per class and relative to the row's highest score alone.  With d = log2(e) times a class's distance from the highest, the argument of its 32-bit exponential is
+off by at most (2 d + 2 `held`) 2^-24 powers of two: the roundings of its score and of the difference from the highest.  `held` is the distance from the highest up to
+which a kernel may hold scores in 32 bits relative to another value: 128 where it has a row's scores in 32 bits, else 0.  The exponential is off by 2 steps more, and
+what becomes of it -- the factor, the product, the rounding -- by 6: (ln 2 (2 d + 2 held) + 8) 2^-24 of itself in all, and the instruction for 2^x gives 0 for results
+under 2^-126.  A total is off by its classes' parts, a gradient by its class's and the total's.  A loss is the margin, off by the two scores that it is a difference of,
+and the logarithm of the total, or of 1 + the others where the target is the highest.  2^-53 for float64, whose scores are off by the additions of their features too.
+Half a step of the type on top."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import convlogic_amd as C
+from oracle import keep_oracle as K
+from tests.gpu_util import DEV
+
+pytestmark = pytest.mark.gpu
+
+LN2 = 0.6932
+
+
+def host(t):
+    return t.detach().double().cpu().numpy()
+
+
+def masked(rows, k, group, dtype, value, seed=0):
+    """features with masked classes -- by the row: none, the first one, the first half and every third one, all but one -- and which ones are not"""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.rand(rows, k, group, generator=g, dtype=torch.float64) + torch.randn(rows, k, 1, generator=g, dtype=torch.float64) * (3.0 / group)
+    row, c = torch.arange(rows)[:, None] % 4, torch.arange(k)[None, :]
+    free = torch.ones(rows, k, dtype=torch.bool)
+    free &= ~((row == 1) & (c == 0))
+    free &= ~((row == 2) & ((c < k // 2) | (c % 3 == 0)) & (c != k - 1))
+    free &= ~((row == 3) & (c != 7 * torch.arange(rows)[:, None] % k))
+    x = torch.where(free[:, :, None], x, value)
+    return x.view(rows, k * group).to(dtype), free
+
+
+def targets(free, seed=0):
+    """a class that is not masked"""
+    score = torch.rand(free.shape, generator=torch.Generator().manual_seed(seed + 1))
+    return torch.where(free, score, -1.0).argmax(1)
+
+
+def held_of(x, k, layout):
+    """where scores are in 32 bits: rows of up to 64 features to a class, by a workgroup each, but for the few short ones"""
+    rows, features = x.shape
+    in_lds = layout == "rows" and x.dtype != torch.float64 and features <= 64 * k and k * 4 <= 144 << 10
+    return 128 if in_lds and (rows > 64 or features * x.element_size() <= 64 << 10) and not (rows <= 128 and features <= 64) else 0
+
+
+def check(x, t, k, layout, tau, smoothing=0.0, reduction="none", upstream=None):
+    rows, group, held = x.shape[0], x.shape[1] // k, held_of(x, k, layout)
+    leaf = (x.to(DEV) if layout == "rows" else x.to(DEV).t().contiguous().t()).requires_grad_(True)
+    loss = C.group_cross_entropy(leaf, t.to(DEV), k, tau=tau, label_smoothing=smoothing, reduction=reduction)
+    up = torch.rand(rows, dtype=loss.dtype, generator=torch.Generator().manual_seed(5)) if reduction == "none" else upstream
+    want, want_grad = K.group_cross_entropy(host(x), t.numpy(), k, tau, smoothing, 1.0, reduction, None if up is None else up.numpy())
+    want, want_grad = np.asarray(want, dtype=np.float64), np.asarray(want_grad, dtype=np.float64)
+    double = x.dtype == torch.float64
+    unit, at = 2.0 ** -53 if double else 2.0 ** -24, np.arange(rows)
+    with np.errstate(all="ignore"):
+        parts = host(x).reshape(rows, k, group)
+        scores = parts.sum(2) / tau
+        top = scores.max(1, keepdims=True)
+        d = (top - scores) * 1.442696
+        off = LN2 * (2 * d + 2 * held) + 8
+        if double:                                                    # (as many roundings as additions, and those of the scale, of two classes)
+            sums = np.abs(parts).sum(2) / tau * (group + 8)
+            off = off + sums + sums[at, scores.argmax(1)][:, None]
+        p = np.exp(scores - top)
+        p = p / p.sum(1, keepdims=True)
+        each = np.where(p > 0, p * off * unit, 0.0) + 2.0 ** -126
+        total = each.sum(1)
+        target = t.numpy()
+        but = total - each[at, target]
+        d_t = d[at, target]
+        margin = np.where(held > 0, LN2 * (2 * held + d_t), 2.0 ** -20 * (1 + d_t)) * unit
+        if double:
+            margin = (LN2 * d_t * 2 + sums[at, target] + sums[at, scores.argmax(1)] + 8) * unit
+        bound = np.where((d_t == 0) & (smoothing == 0), but, total + margin)
+        if smoothing:
+            bound = bound + smoothing * (LN2 * held * unit + LN2 * d.mean(1) * (k + 8) * 2.0 ** -53)
+    half = torch.finfo(loss.dtype).eps / 2
+    if reduction == "mean":
+        bound = bound.mean()
+    error = np.abs(host(loss) - want)
+    assert (error <= bound + 4 * half * np.abs(want)).all(), (host(loss), want, error - bound)
+    got, = torch.autograd.grad(loss, leaf, None if up is None else up.to(DEV))
+    size = np.ones((rows, 1)) / tau / (rows if reduction == "mean" else 1) * (1.0 if up is None else np.abs(up.numpy().reshape(-1, 1)))
+    limit = each + p * total[:, None] + smoothing / k * 8 * unit
+    limit[at, target] = but + (1 - p[at, target]).clip(0) * total + smoothing * 8 * unit
+    eps, tiny = torch.finfo(x.dtype).eps / 2, torch.finfo(x.dtype).smallest_normal * torch.finfo(x.dtype).eps
+    error = np.abs(host(got) - want_grad)
+    limit = np.repeat(size * limit, group, 1) + (eps * 1.001) * np.abs(want_grad) + tiny
+    assert (error <= limit).all(), (error - limit).max()
+
+
+VALUES = [-1e4, -65504.0, -1e9, "lowest"]
+
+
+def cases(dtype):
+    for value in VALUES:
+        if value == "lowest":
+            yield torch.finfo(dtype).min
+        elif value >= torch.finfo(dtype).min:
+            yield value
+
+
+# rows in pieces of their classes; samples in columns, one or several to a lane, classes whole or in slices
+PIECES = [("rows", 40, 2100, 8), ("rows", 3, 40000, 1), ("rows", 7, 5001, 5), ("columns", 33, 10, 4), ("columns", 5, 700, 1), ("columns", 300, 64, 2), ("columns", 1030, 1500, 2),
+          ("columns", 64, 10, 2048), ("columns", 257, 5, 513)]
+
+
+@pytest.mark.parametrize("layout,rows,k,group", PIECES + [("rows", 130, 37000, 2), ("columns", 12, 30000, 1)])
+def test_classes_in_pieces(layout, rows, k, group):
+    for value in cases(torch.float32):
+        x, free = masked(rows, k, group, torch.float32, value)
+        check(x, targets(free), k, layout, 0.3 * group ** 0.5)
+
+
+@pytest.mark.parametrize("dtype,layout,rows,k,group", [(d, *size) for d in (torch.float64, torch.bfloat16, torch.float16) for size in PIECES + [("rows", 40, 4200, 8)]
+                                                       if d == torch.float64 or size[0] == "columns" or size[2] * size[3] > 32768])      # (shorter rows go whole)
+def test_classes_in_pieces_of_other_types(dtype, layout, rows, k, group):
+    for value in cases(dtype):
+        x, free = masked(rows, k, group, dtype, value)
+        check(x, targets(free), k, layout, 0.3 * group ** 0.5)
+
+
+@pytest.mark.parametrize("layout,rows,k,group", PIECES)
+def test_classes_in_pieces_with_smoothing_and_masked_targets(layout, rows, k, group):
+    for value in cases(torch.float32):
+        x, free = masked(rows, k, group, torch.float32, value)
+        t = targets(free)
+        tau = 0.3 * group ** 0.5 + 0.7                                # (losses stay in float32's range: the smoothing's part of the masks is their mean)
+        check(x, t, k, layout, tau * group, smoothing=0.1)
+        check(x, t, k, layout, tau, reduction="mean", upstream=torch.tensor(3.0))
+        if value >= -1e9:
+            check(x, torch.where(torch.arange(rows) % 8 >= 4, t, 0), k, layout, tau)
