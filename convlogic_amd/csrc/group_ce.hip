@@ -344,10 +344,12 @@ struct Classes {
     }
 };
 
-// A workgroup per row.  Its scores, in units, are in LDS as S.  Those of up to 64 features to a class are floats relative to the score of class 0: as exact as a
-// 32-bit exponential can tell, and twice as many.  Bound by memory: 4096 rows of 32768 classes of 4 bfloat16 with their gradient, 2.1 GB, 368 us, 5.8 TB/s (vector
-// units 46 % busy; with the next pieces loaded under the sums of these 392).
+// A workgroup per row.  Its scores, in units, are in LDS as S.  Those of up to 64 features to a class are floats relative to a pivot, twice as many as doubles: the
+// score of class 0, or, where the highest turns out to be more than kFar from it, the highest itself, by two more passes over the features.  Near the
+// highest a score is then off by half a step of a float under kFar, 2^-18, as any argument of that size of an exponential is.  Bound by memory:
+// 4096 rows of 32768 classes of 4 bfloat16 with their gradient, 2.1 GB, 368 us, 5.8 TB/s (vector units 46 % busy; with the next pieces loaded under the sums of these 392).
 constexpr int kNear = 64;
+constexpr float kFar = 128;
 template <typename T, int THREADS, int PACK, typename S>
 __global__ __launch_bounds__(THREADS) void rows_kernel(CeArgs a)
 {
@@ -378,14 +380,26 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(CeArgs a)
             pivot = wave_sum(lane < a.group ? (double)(A)x[lane] : 0.0) * (a.inv_tau * kUnit);
             if (!(__builtin_fabs(pivot) <= __DBL_MAX__)) pivot = 0;
         }
-        S m[1] = {lowest(S(0))};
-        classes.sums(x, 0, a.k, (int64_t)a.k * a.group, [&](int c, double s, bool mine) {
-            const S u = (S)(s * (a.inv_tau * kUnit) - pivot);
-            if (mine) score[c] = u;
-            m[0] = max_of(m[0], u);
-        });
-        __syncthreads();                                              // (also: room is free again)
-        block_reduce<false, THREADS>(m, reinterpret_cast<S *>(room));
+        S m[1];
+        const auto hold = [&] {
+            m[0] = lowest(S(0));
+            classes.sums(x, 0, a.k, (int64_t)a.k * a.group, [&](int c, double s, bool mine) {
+                const S u = (S)(s * (a.inv_tau * kUnit) - pivot);
+                if (mine) score[c] = u;
+                m[0] = max_of(m[0], u);
+            });
+            __syncthreads();                                          // (also: room is free again)
+            block_reduce<false, THREADS>(m, reinterpret_cast<S *>(room));
+        };
+        hold();
+        if (sizeof(S) == 4 && !(__builtin_fabs(m[0]) <= kFar)) {
+            double top[1] = {lowest(0.0)};
+            classes.sums(x, 0, a.k, (int64_t)a.k * a.group, [&](int, double s, bool) { top[0] = max_of(top[0], s); });
+            __syncthreads();
+            block_reduce<false, THREADS>(top, room);
+            pivot = __builtin_isinf(top[0]) ? 0 : top[0] * (a.inv_tau * kUnit);
+            hold();
+        }
         double sums[2] = {0, 0};
         for (int c = threadIdx.x; c < a.k; c += THREADS) {
             const S u = score[c];

@@ -139,3 +139,50 @@ def test_classes_in_pieces_with_smoothing_and_masked_targets(layout, rows, k, gr
         check(x, t, k, layout, tau, reduction="mean", upstream=torch.tensor(3.0))
         if value >= -1e9:
             check(x, torch.where(torch.arange(rows) % 8 >= 4, t, 0), k, layout, tau)
+
+
+# a workgroup for a row: scores in 32 bits of groups up to 64 features, else in 64
+WHOLE = [(129, 10, 1), (200, 1000, 1), (1100, 300, 4), (130, 12, 5), (70, 300, 64), (65, 2000, 16), (150, 9, 100), (130, 30000, 1)]
+
+
+@pytest.mark.parametrize("rows,k,group", WHOLE)
+def test_whole_rows(rows, k, group):
+    for value in cases(torch.float32):
+        x, free = masked(rows, k, group, torch.float32, value)
+        check(x, targets(free), k, "rows", 0.3 * group ** 0.5)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,k,group", WHOLE[:-1] + [(40, 2100, 8), (7, 5001, 5)])
+def test_whole_rows_of_other_types(rows, k, group, dtype):
+    for value in cases(dtype):
+        x, free = masked(rows, k, group, dtype, value)
+        check(x, targets(free), k, "rows", 0.3 * group ** 0.5)
+
+
+@pytest.mark.parametrize("rows,k,group", WHOLE)
+def test_whole_rows_with_masked_targets(rows, k, group):
+    for value in cases(torch.float32):
+        x, free = masked(rows, k, group, torch.float32, value)
+        t = targets(free)
+        check(x, t, k, "rows", group ** 0.5, reduction="mean", upstream=torch.tensor(3.0))
+        if value >= -1e9:
+            check(x, torch.where(torch.arange(rows) % 8 >= 4, t, 0), k, "rows", group ** 0.5)
+
+
+@pytest.mark.parametrize("level", [-1e6, 1e4, 1e9, 1e30])
+@pytest.mark.parametrize("first", [0.0, -math.inf])
+def test_whole_rows_far_from_zero_and_from_their_first_class(first, level):
+    # (steps of 32 bits at these levels: the scores differ by them, and by hundreds)
+    step = abs(level) * 2.0 ** -20 if abs(level) > 1e5 else 0.25
+    x = (level + step * torch.randint(0, 8, (200, 50), generator=torch.Generator().manual_seed(0)).double()).float()
+    x[:, 0] = first if first else x[:, 1]
+    t = torch.randint(1, 50, (200,), generator=torch.Generator().manual_seed(1))
+    leaf = x.to(DEV).requires_grad_(True)
+    tau = step / 0.75
+    loss = C.group_cross_entropy(leaf, t.to(DEV), 50, tau=tau, reduction="none")
+    grad, = torch.autograd.grad(loss.sum(), leaf)
+    want, want_grad = K.group_cross_entropy(host(x), t.numpy(), 50, tau, 0.0, 1.0, "none")
+    # distances up to 8 powers of two from the highest
+    bound = (LN2 * (2 * 8 + 2 * 128) + 8) * 2.0 ** -24
+    assert (np.abs(host(loss) - want) <= bound * 3 * (1 + want)).all() and (np.abs(host(grad) * tau - want_grad * tau) <= 3 * bound).all()
