@@ -13,7 +13,8 @@
 
 namespace {
 
-// Exponentials of scores, as the sums take them: of differences of scores times `unit`, which are 64-bit numbers, rounded to A; 2^x by one instruction for float.
+// Exponentials of scores, as the sums take them: of differences of classes' sums, which are 64-bit numbers, times `unit` over tau, rounded to A; 2^x by one instruction
+// for float.  (Differences before the factor, not after it: the rounding of a product of 10^38 is many powers of two.)
 template <typename A>
 struct Unit;
 template <>
@@ -37,13 +38,13 @@ struct CeArgs {
     double inv_tau, smoothing, scale;                                 // scale: weight, over the rows where their number is known to be all
     int reduction, count;                                             // count: to be counted here (1), or in per_count (2)
     double *per_count, *row_loss;                                     // 1 / rows that count; [rows]
-    double *final;                                                    // [rows][4]: M in units, O, Z
+    double *final;                                                    // [rows][4]: the highest sum, O, Z
     void *out;                                                        // [rows] in A, or NULL
     const void *upstream;                                             // in A, [rows] for CLG_REDUCE_NONE, or NULL for 1
     int if_changed;                                                   // nothing to do for an upstream gradient of 1
     // pieces
     int pieces, per_piece;                                            // of the classes
-    double *stats, *target_score;                                     // [pieces][rows][4], [rows]
+    double *stats, *target_sum;                                       // [pieces][rows][4], [rows]
     double *scores, *partial;                                         // "columns": [k][rows], [slices][k][rows], or NULL
     int slices, lanes_log2;                                           // of a class's features; lanes to a class, or samples side by side
 };
@@ -67,25 +68,25 @@ __device__ __forceinline__ double per_row(const CeArgs &a, double *room)
     return n[0] == 0 ? 0 : 1 / n[0];
 }
 
-// The statistics of a part of a row's classes, of scores in units: the highest so far, O and the sum of (highest - score) relative to it, and the number of
+// The statistics of a part of a row's classes, of their sums: the highest so far, O and the sum of (highest - sum) relative to it, and the number of
 // classes.  Differences are taken in 64 bits before anything is rounded to A: relative to a score that is not the highest -- a masked class's, the first one's --
 // those of all others would lose their digits.
 template <typename A>
 struct Stats {
     double m = lowest(0.0), others = 0, down = 0, n = 0;
-    __device__ __forceinline__ void add(double score, bool is_target, bool smooth)
+    __device__ __forceinline__ void add(double sum, bool is_target, bool smooth, double unit)
     {
-        if (score > m) {
+        if (sum > m) {
             if (m != lowest(0.0)) {
-                others *= (double)Unit<A>::power((A)(m - score));
-                down += n * (score - m);
+                others *= (double)Unit<A>::power((A)((m - sum) * unit));
+                down += n * (sum - m);
             }
-            m = score;
+            m = sum;
         }
-        const A e = score == lowest(0.0) ? A(0) : Unit<A>::power((A)(score - m));
+        const A e = sum == lowest(0.0) ? A(0) : Unit<A>::power((A)((sum - m) * unit));
         others += is_target ? 0.0 : (double)e;
         if (smooth) {
-            down += score == lowest(0.0) ? -lowest(0.0) : m - score;
+            down += sum == lowest(0.0) ? -lowest(0.0) : m - sum;
             n += 1;
         }
     }
@@ -98,19 +99,19 @@ struct Joint {
     __device__ __forceinline__ explicit Joint(const Stats<A> &s) : m(s.m), others(s.others), down(s.down), n(s.n) {}
     __device__ __forceinline__ explicit Joint(const double *p) : m(p[0]), others(p[1]), down(p[2]), n(p[3]) {}
     __device__ __forceinline__ void store(double *p) const { p[0] = m, p[1] = others, p[2] = down, p[3] = n; }
-    __device__ __forceinline__ void raise(double to)
+    __device__ __forceinline__ void raise(double to, double unit)
     {
         if (!(to > m)) return;
         if (m != lowest(0.0)) {
-            others *= (double)Unit<A>::power((A)(m - to));
+            others *= (double)Unit<A>::power((A)((m - to) * unit));
             down += n * (to - m);
         }
         m = to;
     }
-    __device__ __forceinline__ void join(Joint b)
+    __device__ __forceinline__ void join(Joint b, double unit)
     {
-        raise(b.m);
-        b.raise(m);
+        raise(b.m, unit);
+        b.raise(m, unit);
         others += b.others;
         down += b.down;
         n += b.n;
@@ -344,12 +345,13 @@ struct Classes {
     }
 };
 
-// A workgroup per row.  Its scores, in units, are in LDS as S.  Those of up to 64 features to a class are floats relative to a pivot, twice as many as doubles: the
-// score of class 0, or, where the highest turns out to be more than kFar from it, the highest itself, by two more passes over the features.  Near the
-// highest a score is then off by half a step of a float under kFar, 2^-18, as any argument of that size of an exponential is.  Bound by memory:
-// 4096 rows of 32768 classes of 4 bfloat16 with their gradient, 2.1 GB, 368 us, 5.8 TB/s (vector units 46 % busy; with the next pieces loaded under the sums of these 392).
+// A workgroup per row.  Its classes' sums are in LDS as S; those of up to 64 features as floats, twice as many: scores in units relative to a pivot, the sum of class 0,
+// or, where the highest turns out to be more than kFar from it, the highest itself, by two more passes over the features.  Near the highest a score is then off
+// by half a step of a float under kFar, 2^-18, as any argument of that size of an exponential is.  Bound by memory: 4096 rows of 32768 classes of 4 bfloat16 with their
+// gradient, 2.1 GB, 368 us, 5.8 TB/s (vector units 46 % busy; with the next pieces loaded under the sums of these 392).
 constexpr int kNear = 64;
 constexpr float kFar = 128;
+constexpr double kLevel = 1 << 28;                                    // units up to which the product of a sum with its unit is as good as the sum
 template <typename T, int THREADS, int PACK, typename S>
 __global__ __launch_bounds__(THREADS) void rows_kernel(CeArgs a)
 {
@@ -357,7 +359,8 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(CeArgs a)
     extern __shared__ char lds[];
     __shared__ double room[32], shared[2];
     S *score = reinterpret_cast<S *>(lds);
-    constexpr double kUnit = Unit<A>::unit;
+    constexpr bool kFloats = sizeof(S) == 4;
+    const double unit = a.inv_tau * Unit<A>::unit;
     const Classes<T, THREADS, PACK> classes(a.group, a.lanes_log2);
     const double per = per_row<THREADS>(a, room);
     if (a.count == 1 && blockIdx.x == 0 && threadIdx.x == 0) *a.per_count = per;
@@ -375,35 +378,41 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(CeArgs a)
             continue;
         }
         double pivot = 0;
-        if constexpr (sizeof(S) == 4) {                               // (each wavefront adds up class 0 for itself)
+        if constexpr (kFloats) {                                      // (each wavefront adds up class 0 for itself)
             const int lane = threadIdx.x & 63;
-            pivot = wave_sum(lane < a.group ? (double)(A)x[lane] : 0.0) * (a.inv_tau * kUnit);
+            pivot = wave_sum(lane < a.group ? (double)(A)x[lane] : 0.0);
             if (!(__builtin_fabs(pivot) <= __DBL_MAX__)) pivot = 0;
         }
         S m[1];
-        const auto hold = [&] {
+        const auto hold = [&](auto held) {
             m[0] = lowest(S(0));
             classes.sums(x, 0, a.k, (int64_t)a.k * a.group, [&](int c, double s, bool mine) {
-                const S u = (S)(s * (a.inv_tau * kUnit) - pivot);
+                const S u = (S)held(s);
                 if (mine) score[c] = u;
                 m[0] = max_of(m[0], u);
             });
             __syncthreads();                                          // (also: room is free again)
             block_reduce<false, THREADS>(m, reinterpret_cast<S *>(room));
         };
-        hold();
-        if (sizeof(S) == 4 && !(__builtin_fabs(m[0]) <= kFar)) {
-            double top[1] = {lowest(0.0)};
-            classes.sums(x, 0, a.k, (int64_t)a.k * a.group, [&](int, double s, bool) { top[0] = max_of(top[0], s); });
-            __syncthreads();
-            block_reduce<false, THREADS>(top, room);
-            pivot = __builtin_isinf(top[0]) ? 0 : top[0] * (a.inv_tau * kUnit);
-            hold();
+        if constexpr (kFloats) {
+            const double at = pivot * unit;
+            hold([&](double s) { return s * unit - at; });
+            if (!(__builtin_fabs(m[0]) <= kFar && __builtin_fabs(at) <= kLevel)) {
+                double top[1] = {lowest(0.0)};
+                classes.sums(x, 0, a.k, (int64_t)a.k * a.group, [&](int, double s, bool) { top[0] = max_of(top[0], s); });
+                __syncthreads();
+                block_reduce<false, THREADS>(top, room);
+                pivot = __builtin_isinf(top[0]) ? 0 : top[0];
+                hold([&](double s) { return (s - pivot) * unit; });
+            }
+        } else {
+            hold([](double s) { return s; });
         }
+        const double to_unit = kFloats ? 1.0 : unit, to_score = kFloats ? 1 / Unit<A>::unit : a.inv_tau;
         double sums[2] = {0, 0};
         for (int c = threadIdx.x; c < a.k; c += THREADS) {
             const S u = score[c];
-            const A e = Unit<A>::power((A)(u - m[0]));
+            const A e = Unit<A>::power(kFloats ? (A)(u - m[0]) : (A)((u - m[0]) * to_unit));
             if (c == t) {
                 shared[0] = (double)u;
                 shared[1] = (double)e;
@@ -420,11 +429,11 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(CeArgs a)
         const double scale = a.scale * per;
         const Grad g(r, scale * a.inv_tau, a.smoothing, a.k);
         if (threadIdx.x == 0) {
-            const double loss = r.loss(((double)m[0] - shared[0]) / kUnit, sums[1] / kUnit, a.k, a.smoothing) * scale;
+            const double loss = r.loss(((double)m[0] - shared[0]) * to_score, sums[1] * to_score, a.k, a.smoothing) * scale;
             if (a.row_loss) a.row_loss[row] = loss;
             if (a.out) static_cast<A *>(a.out)[row] = (A)loss;
             double *f = a.final + 4 * row;
-            f[0] = (double)m[0] + pivot, f[1] = r.others, f[2] = r.total;
+            f[0] = kFloats ? pivot + (double)m[0] / unit : (double)m[0], f[1] = r.others, f[2] = r.total;
         }
         if (grad) {
             const A factor = (A)g.factor, off = (A)g.off, target = (A)g.target;
@@ -447,6 +456,7 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(CeArgs a, void *out_sum)
     const double per = per_row<1024>(a, room);
     if (a.count == 1 && threadIdx.x == 0) *a.per_count = per;
     const int l = threadIdx.x % 16;
+    const double unit = a.inv_tau * Unit<A>::unit;
     double sum[1] = {0};
     for (int64_t row = threadIdx.x / 16; row < a.rows; row += 64) {
         const T *x = static_cast<const T *>(a.x) + row * a.stride;
@@ -460,7 +470,6 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(CeArgs a, void *out_sum)
             s[i] = 0;
             if (c >= a.k) continue;
             for (int j = 0; j < a.group; ++j) s[i] += (double)(A)x[c * a.group + j];
-            s[i] *= a.inv_tau;
             m = max_of(m, s[i]);
             if (c == t) s_target = s[i];
         }
@@ -470,7 +479,7 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(CeArgs a, void *out_sum)
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const int c = l + 16 * i;
-            e[i] = c < a.k ? Unit<A>::power((A)((s[i] - m) * Unit<A>::unit)) : A(0);
+            e[i] = c < a.k ? Unit<A>::power((A)((s[i] - m) * unit)) : A(0);
             if (c >= a.k) continue;
             if (c == t) of_target = (double)e[i];
             else others += (double)e[i];
@@ -481,8 +490,8 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(CeArgs a, void *out_sum)
         const bool counts = t >= 0 && t < a.k;
         const double scale = a.scale * per, none = t < 0 ? 0.0 : __builtin_nan("");
         const Grad g(r, scale * a.inv_tau, a.smoothing, a.k);
-        const double loss = counts ? r.loss(m - s_target, down, a.k, a.smoothing) * scale : none;
-        if (l < 3) a.final[4 * row + l] = l == 0 ? m * Unit<A>::unit : l == 1 ? r.others : r.total;
+        const double loss = counts ? r.loss((m - s_target) * a.inv_tau, down * a.inv_tau, a.k, a.smoothing) * scale : none;
+        if (l < 3) a.final[4 * row + l] = l == 0 ? m : l == 1 ? r.others : r.total;
         if (l == 0) {
             sum[0] += loss;
             if (a.out) static_cast<A *>(a.out)[row] = (A)loss;
@@ -503,12 +512,12 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(CeArgs a, void *out_sum)
 
 // Statistics over THREADS threads, valid in thread 0.
 template <int THREADS, typename A>
-__device__ __forceinline__ Joint<A> block_stats(const Stats<A> &mine, double *room)
+__device__ __forceinline__ Joint<A> block_stats(const Stats<A> &mine, double unit, double *room)
 {
     Joint<A> s(mine);
     double m[1] = {s.m};
     block_reduce<false, THREADS>(m, room);
-    s.raise(m[0]);
+    s.raise(m[0], unit);
     double sums[3] = {s.others, s.down, s.n};
     __syncthreads();
     block_reduce<true, THREADS>(sums, room);
@@ -527,6 +536,7 @@ __global__ __launch_bounds__(kPart) void row_stats_kernel(CeArgs a)
     __shared__ double room[3 * kPart / kWave];
     const Classes<T, kPart, PACK> classes(a.group, a.lanes_log2);
     const bool smooth = a.smoothing != 0;
+    const double unit = a.inv_tau * Unit<A>::unit;
     for (int64_t task = blockIdx.x; task < a.rows * a.pieces; task += gridDim.x) {
         const int64_t row = task / a.pieces;
         const int piece = (int)(task % a.pieces), first = piece * a.per_piece, end = first + a.per_piece < a.k ? first + a.per_piece : a.k;
@@ -534,28 +544,27 @@ __global__ __launch_bounds__(kPart) void row_stats_kernel(CeArgs a)
         const T *x = static_cast<const T *>(a.x) + row * a.stride;
         Stats<A> s;
         if (t >= 0 && t < a.k) {
-            const double unit = a.inv_tau * Unit<A>::unit;
             classes.sums(x, first, end, (int64_t)a.k * a.group, [&](int c, double sum, bool mine) {
                 if (!mine) return;
-                s.add(sum * unit, c == t, smooth);
-                if (c == t) a.target_score[row] = sum * unit;
+                s.add(sum, c == t, smooth, unit);
+                if (c == t) a.target_sum[row] = sum;
             });
         }
-        const Joint<A> all = block_stats<kPart>(s, room);
+        const Joint<A> all = block_stats<kPart>(s, unit, room);
         if (threadIdx.x == 0) all.store(a.stats + 4 * ((int64_t)piece * a.rows + row));
     }
 }
 
-// A row's loss from its statistics, which become M, O and Z.
+// A row's loss from its statistics, which become the highest sum, O and Z.
 template <typename A>
 __device__ __forceinline__ double row_of(const CeArgs &a, int64_t row, Joint<A> s, double target, double per)
 {
     if (__builtin_isinf(s.m)) s.others = __builtin_nan("");
-    const Row r{s.others, s.others + (double)Unit<A>::power((A)(target - s.m))};
+    const Row r{s.others, s.others + (double)Unit<A>::power((A)((target - s.m) * (a.inv_tau * Unit<A>::unit)))};
     a.final[4 * row] = s.m, a.final[4 * row + 1] = r.others, a.final[4 * row + 2] = r.total;
-    return r.loss((s.m - target) / Unit<A>::unit, s.down / Unit<A>::unit, a.k, a.smoothing) * a.scale * per;
+    return r.loss((s.m - target) * a.inv_tau, s.down * a.inv_tau, a.k, a.smoothing) * a.scale * per;
 }
-// The statistics of a row's pieces into M, O, Z and the loss: LANES to a row.  One workgroup for all rows (`out_sum`) also adds their losses.
+// The statistics of a row's pieces into the highest sum, O, Z and the loss: LANES to a row.  One workgroup for all rows (`out_sum`) also adds their losses.
 template <typename A, int LANES, int THREADS>
 __global__ __launch_bounds__(THREADS) void join_kernel(CeArgs a, void *out_sum)
 {
@@ -564,21 +573,22 @@ __global__ __launch_bounds__(THREADS) void join_kernel(CeArgs a, void *out_sum)
     const double per = per_row<THREADS>(a, room);
     if (a.count == 1 && blockIdx.x == 0 && threadIdx.x == 0) *a.per_count = per;
     const int l = threadIdx.x % LANES;
+    const double unit = a.inv_tau * Unit<A>::unit;
     double sum[1] = {0};
     for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * ROWS) {
         const int64_t t = target_of(a, row);
         double loss = t < 0 ? 0.0 : __builtin_nan("");
         if (t >= 0 && t < a.k) {
             Joint<A> s;
-            for (int p = l; p < a.pieces; p += LANES) s.join(Joint<A>(a.stats + 4 * ((int64_t)p * a.rows + row)));
+            for (int p = l; p < a.pieces; p += LANES) s.join(Joint<A>(a.stats + 4 * ((int64_t)p * a.rows + row)), unit);
             if constexpr (LANES == 16) {
-                s.raise(row16_max(s.m));
+                s.raise(row16_max(s.m), unit);
                 s.others = row16_sum(s.others), s.down = row16_sum(s.down);
             } else {
-                s.raise(wave_max(s.m));
+                s.raise(wave_max(s.m), unit);
                 s.others = wave_sum(s.others), s.down = wave_sum(s.down);
             }
-            if (l == 0) loss = row_of(a, row, s, a.target_score[row], per);
+            if (l == 0) loss = row_of(a, row, s, a.target_sum[row], per);
         }
         if (l != 0) continue;
         sum[0] += loss;
@@ -590,7 +600,7 @@ __global__ __launch_bounds__(THREADS) void join_kernel(CeArgs a, void *out_sum)
     if (threadIdx.x == 0) *static_cast<A *>(out_sum) = (A)sum[0];
 }
 
-// What a gradient is computed from: M and the factors.
+// What a gradient is computed from: the highest sum and the factors.
 template <typename A>
 struct GradOf {
     double m, unit;
@@ -606,7 +616,7 @@ struct GradOf {
     }
     __device__ __forceinline__ A operator()(double sum, bool is_target) const
     {
-        const A e = Unit<A>::power((A)__builtin_fma(sum, unit, -m));
+        const A e = Unit<A>::power((A)((sum - m) * unit));
         return is_target ? target : __builtin_elementwise_fma(e, factor, -off);
     }
 };
@@ -743,7 +753,7 @@ __device__ __forceinline__ void column_stream(const CeArgs &a, const Column<V> &
 }
 // Statistics of the workgroup's wavefronts, V samples a lane: valid in the first wavefront's, after which `finish` is called for each sample.
 template <typename A, int V, int WAVES, typename F>
-__device__ __forceinline__ void column_finish(const Column<V> &col, const Stats<A> (&s)[V], double (&room)[WAVES][V][kWave][4], F finish)
+__device__ __forceinline__ void column_finish(const Column<V> &col, const Stats<A> (&s)[V], double unit, double (&room)[WAVES][V][kWave][4], F finish)
 {
 #pragma unroll
     for (int v = 0; v < V; ++v) Joint<A>(s[v]).store(room[col.wave][v][threadIdx.x & 63]);
@@ -752,7 +762,7 @@ __device__ __forceinline__ void column_finish(const Column<V> &col, const Stats<
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         Joint<A> all(s[v]);
-        for (int w = 1; w < WAVES; ++w) all.join(Joint<A>(room[w][v][threadIdx.x & 63]));
+        for (int w = 1; w < WAVES; ++w) all.join(Joint<A>(room[w][v][threadIdx.x & 63]), unit);
         finish(v, all);
     }
 }
@@ -781,8 +791,8 @@ __global__ __launch_bounds__(kPart) void column_sums_kernel(CeArgs a)
         if (store && a.scores) store_part<V>(a.scores + (int64_t)c * a.rows + col.row, sum);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            s[v].add(sum[v] * unit, c == t[v], smooth);
-            if (store && c == t[v]) a.target_score[col.row + v] = sum[v] * unit;
+            s[v].add(sum[v], c == t[v], smooth, unit);
+            if (store && c == t[v]) a.target_sum[col.row + v] = sum[v];
         }
     };
     const T *x = static_cast<const T *>(a.x);
@@ -799,7 +809,7 @@ __global__ __launch_bounds__(kPart) void column_sums_kernel(CeArgs a)
         column_stream(a, col, x, c0, (int64_t)c0 * a.group, (int64_t)c1 * a.group, a.group, score);
     }
     if (a.slices == 1)
-        column_finish(col, s, room, [&](int v, const Joint<A> &all) { all.store(a.stats + 4 * ((int64_t)blockIdx.y * a.rows + col.row + v)); });
+        column_finish(col, s, unit, room, [&](int v, const Joint<A> &all) { all.store(a.stats + 4 * ((int64_t)blockIdx.y * a.rows + col.row + v)); });
 }
 // The same from the sums of the slices, of all classes by one workgroup, which ends the rows' losses too.
 template <typename T>
@@ -820,12 +830,12 @@ __global__ __launch_bounds__(1024) void column_stats_kernel(CeArgs a)
 #pragma unroll 8
         for (int i = col.sub; i < a.slices; i += col.subs) sum += a.partial[((int64_t)i * a.k + c) * a.rows + col.row];
         for (int by = 1 << a.lanes_log2; by < 64; by <<= 1) sum += __shfl_xor(sum, by);
-        s[0].add(sum * unit, c == t, smooth);
+        s[0].add(sum, c == t, smooth, unit);
         if (store) a.scores[(int64_t)c * a.rows + col.row] = sum;
-        if (store && c == t) a.target_score[col.row] = sum * unit;
+        if (store && c == t) a.target_sum[col.row] = sum;
     }
-    column_finish(col, s, room, [&](int, const Joint<A> &all) {       // (behind a barrier: the target's score is there)
-        const double loss = t < 0 ? 0.0 : t >= a.k ? __builtin_nan("") : row_of(a, col.row, all, a.target_score[col.row], per);
+    column_finish(col, s, unit, room, [&](int, const Joint<A> &all) {       // (behind a barrier: the target's score is there)
+        const double loss = t < 0 ? 0.0 : t >= a.k ? __builtin_nan("") : row_of(a, col.row, all, a.target_sum[col.row], per);
         if (a.row_loss) a.row_loss[col.row] = loss;
         if (a.out) static_cast<A *>(a.out)[col.row] = (A)loss;
     });
@@ -975,7 +985,7 @@ Rooms rooms_of(const Plan &p, CeArgs *a, void *kept, void *scratch)
     r.row_loss = take(scratch, p.n);
     take(scratch, clg_ceil_div(p.n, kSlice));
     if (!p.whole) {
-        r.target_score = take(scratch, p.n);
+        r.target_sum = take(scratch, p.n);
         r.stats = take(scratch, 4 * p.pieces * p.n);
     }
     if (p.scores && !p.kept_scores) r.scores = take(scratch, p.k * p.n);

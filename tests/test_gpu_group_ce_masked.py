@@ -186,3 +186,19 @@ def test_whole_rows_far_from_zero_and_from_their_first_class(first, level):
     # distances up to 8 powers of two from the highest
     bound = (LN2 * (2 * 8 + 2 * 128) + 8) * 2.0 ** -24
     assert (np.abs(host(loss) - want) <= bound * 3 * (1 + want)).all() and (np.abs(host(grad) * tau - want_grad * tau) <= 3 * bound).all()
+
+
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("layout,rows,k", [("rows", 200, 50), ("rows", 20, 50), ("rows", 3, 40000), ("columns", 20, 50), ("columns", 1030, 1500)])
+def test_rows_of_the_lowest_or_highest_value(layout, rows, k, sign):
+    # the classes that are not -inf are alike: each has the same probability
+    x = torch.full((rows, k), sign * torch.finfo(torch.float32).max)
+    x[:, 0] = -math.inf
+    t = torch.full((rows,), k - 1)
+    leaf = (x.to(DEV) if layout == "rows" else x.to(DEV).t().contiguous().t()).requires_grad_(True)
+    loss = C.group_cross_entropy(leaf, t.to(DEV), k, reduction="none")
+    grad, = torch.autograd.grad(loss.sum(), leaf)
+    want = torch.full((rows, k), 1 / (k - 1), dtype=torch.float64)
+    want[:, 0], want[:, -1] = 0, 1 / (k - 1) - 1
+    assert np.abs(host(loss) - math.log(k - 1)).max() <= 4 * 2.0 ** -24 * math.log(k - 1)
+    assert (np.abs(host(grad) - want.numpy()) <= 8 * 2.0 ** -24 * np.abs(want.numpy())).all()
