@@ -345,15 +345,19 @@ struct Classes {
     }
 };
 
-// A workgroup per row.  Its classes' sums are in LDS as S; those of up to 64 features as floats, twice as many: scores in units relative to a pivot, the sum of class 0,
-// or, where the highest turns out to be more than kFar from it, the highest itself, by two more passes over the features.  Near the highest a score is then off
-// by half a step of a float under kFar, 2^-18, as any argument of that size of an exponential is.  Bound by memory: 4096 rows of 32768 classes of 4 bfloat16 with their
-// gradient, 2.1 GB, 368 us, 5.8 TB/s (vector units 46 % busy; with the next pieces loaded under the sums of these 392).
+// A workgroup per row.  Its classes' sums are in LDS as S; those of up to 64 features as floats, twice as many: scores in units relative to the highest of the classes
+// in the row's first 64 features, or, where these do not fill 16-byte pieces, of the first class and the middle one.  Where the row's highest turns out to be more than kFar
+// from that, as where these classes are masked, they are made again relative to the highest.  Near the highest a score is then off by half a step of a float under
+// kFar, 2^-18, as any argument of that size of an exponential is.  (Relative to the target's, which is seldom masked, but whose place has to be read first: loss_tokens
+// 398 us, not 383.)  Bound by memory: 4096 rows of 32768 classes of 4 bfloat16 with their gradient, 2.1 GB, 368 us, 5.8 TB/s (vector units 46 % busy; with the next
+// pieces loaded under the sums of these 392).
 constexpr int kNear = 64;
 constexpr float kFar = 128;
-constexpr double kLevel = 1 << 28;                                    // units up to which the product of a sum with its unit is as good as the sum
+constexpr double kLevel = 1 << 28;                                    // units up to which a multiply-add with the rounded product of another sum is a difference
+// wavefronts that a SIMD shall hold of rows_kernel: 2000 rows of 6000 classes of 5 bfloat16 79 us with five, 82 with the four that 99 registers leave
+constexpr int rows_waves(int threads, int pack, size_t held) { return threads != 256 || held == 8 ? 1 : pack == 0 ? 5 : 4; }
 template <typename T, int THREADS, int PACK, typename S>
-__global__ __launch_bounds__(THREADS) void rows_kernel(CeArgs a)
+__global__ __launch_bounds__(THREADS, rows_waves(THREADS, PACK, sizeof(S))) void rows_kernel(CeArgs a)
 {
     typedef typename Wide<T>::type A;
     extern __shared__ char lds[];
@@ -377,42 +381,56 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(CeArgs a)
             if (grad) classes.store(grad, 0, a.k, [&](int) { return (A)v; });
             continue;
         }
-        double pivot = 0;
-        if constexpr (kFloats) {                                      // (each wavefront adds up class 0 for itself)
+        double at = 0;                                                // what floats are relative to
+        if constexpr (kFloats) {                                      // (each wavefront finds it for itself)
             const int lane = threadIdx.x & 63;
-            pivot = wave_sum(lane < a.group ? (double)(A)x[lane] : 0.0);
-            if (!(__builtin_fabs(pivot) <= __DBL_MAX__)) pivot = 0;
-        }
-        S m[1];
-        const auto hold = [&](auto held) {
-            m[0] = lowest(S(0));
-            classes.sums(x, 0, a.k, (int64_t)a.k * a.group, [&](int c, double s, bool mine) {
-                const S u = (S)held(s);
-                if (mine) score[c] = u;
-                m[0] = max_of(m[0], u);
-            });
-            __syncthreads();                                          // (also: room is free again)
-            block_reduce<false, THREADS>(m, reinterpret_cast<S *>(room));
-        };
-        if constexpr (kFloats) {
-            const double at = pivot * unit;
-            hold([&](double s) { return s * unit - at; });
-            if (!(__builtin_fabs(m[0]) <= kFar && __builtin_fabs(at) <= kLevel)) {
-                double top[1] = {lowest(0.0)};
-                classes.sums(x, 0, a.k, (int64_t)a.k * a.group, [&](int, double s, bool) { top[0] = max_of(top[0], s); });
-                __syncthreads();
-                block_reduce<false, THREADS>(top, room);
-                pivot = __builtin_isinf(top[0]) ? 0 : top[0];
-                hold([&](double s) { return (s - pivot) * unit; });
+            if constexpr (PACK == 0) {
+                const T *other = x + (int64_t)(a.k / 2) * a.group;
+                const double v = lane < a.group ? (double)(A)x[lane] : 0.0, w = lane < a.group ? (double)(A)other[lane] : 0.0;
+                at = max_of(wave_sum(v), wave_sum(w));
+            } else {
+                const bool there = lane < a.k * PACK;
+                double v = there ? (double)(A)x[lane] : 0.0;
+                if constexpr (PACK > 1) v += dpp_zero<0xB1, 0xF>(v);
+                if constexpr (PACK > 2) v += dpp_zero<0x4E, 0xF>(v);
+                if constexpr (PACK > 4) v += dpp_zero<0x141, 0xF>(v);
+                at = wave_max(there ? v : lowest(0.0));
             }
-        } else {
-            hold([](double s) { return s; });
+            at *= unit;
+            if (!(__builtin_fabs(at) <= kLevel)) at = 0;
         }
-        const double to_unit = kFloats ? 1.0 : unit, to_score = kFloats ? 1 / Unit<A>::unit : a.inv_tau;
+        S m[1] = {lowest(S(0))};
+        classes.sums(x, 0, a.k, (int64_t)a.k * a.group, [&](int c, double s, bool mine) {
+            const S u = (S)(kFloats ? s * unit - at : s);
+            if (mine) score[c] = u;
+            m[0] = max_of(m[0], u);
+        });
+        __syncthreads();                                              // (also: room is free again)
+        block_reduce<false, THREADS>(m, reinterpret_cast<S *>(room));
+        double highest = kFloats ? (at + (double)m[0]) / unit : (double)m[0];
+        // (what follows for few rows, by plain loops that take no registers from the others)
+        const auto plain_sum = [&](int c) {
+            double s = 0;
+#pragma unroll 1
+            for (int j = 0; j < a.group; ++j) s += (double)(A)x[c * a.group + j];
+            return s;
+        };
+        if (kFloats && !(__builtin_fabs(m[0]) <= kFar)) {
+            double top[1] = {lowest(0.0)};
+            for (int c = threadIdx.x; c < a.k; c += THREADS) top[0] = max_of(top[0], plain_sum(c));
+            __syncthreads();
+            block_reduce<false, THREADS>(top, room);
+            highest = top[0];
+            const double from = __builtin_isinf(highest) ? 0 : highest;
+            for (int c = threadIdx.x; c < a.k; c += THREADS) score[c] = (S)((plain_sum(c) - from) * unit);
+            m[0] = (S)(highest - from);
+            __syncthreads();
+        }
+        const double to_score = kFloats ? 1 / Unit<A>::unit : a.inv_tau;
         double sums[2] = {0, 0};
         for (int c = threadIdx.x; c < a.k; c += THREADS) {
             const S u = score[c];
-            const A e = Unit<A>::power(kFloats ? (A)(u - m[0]) : (A)((u - m[0]) * to_unit));
+            const A e = Unit<A>::power(kFloats ? (A)(u - m[0]) : (A)((u - m[0]) * unit));
             if (c == t) {
                 shared[0] = (double)u;
                 shared[1] = (double)e;
@@ -433,7 +451,7 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(CeArgs a)
             if (a.row_loss) a.row_loss[row] = loss;
             if (a.out) static_cast<A *>(a.out)[row] = (A)loss;
             double *f = a.final + 4 * row;
-            f[0] = kFloats ? pivot + (double)m[0] / unit : (double)m[0], f[1] = r.others, f[2] = r.total;
+            f[0] = highest, f[1] = r.others, f[2] = r.total;
         }
         if (grad) {
             const A factor = (A)g.factor, off = (A)g.off, target = (A)g.target;
