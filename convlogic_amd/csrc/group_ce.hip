@@ -443,6 +443,19 @@ __global__ __launch_bounds__(THREADS, rows_waves(THREADS, PACK, sizeof(S))) void
         __syncthreads();
         block_reduce<true, THREADS>(sums, room);
         __syncthreads();
+        if (kFloats && (sums[1] == -lowest(0.0) || shared[0] == lowest(0.0))) {
+            // a score further below the highest than floats reach: what the loss takes of it
+            double down[1] = {0};
+            __syncthreads();                                          // (everyone has seen the target's)
+            for (int c = threadIdx.x; c < a.k; c += THREADS) {
+                const double d = (highest - plain_sum(c)) * unit;
+                down[0] += d;
+                if (c == t) shared[0] = (double)m[0] - d;
+            }
+            block_reduce<true, THREADS>(down, room);
+            __syncthreads();
+            sums[1] = down[0];
+        }
         const Row r{sums[0], sums[0] + shared[1]};
         const double scale = a.scale * per;
         const Grad g(r, scale * a.inv_tau, a.smoothing, a.k);

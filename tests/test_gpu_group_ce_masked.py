@@ -202,3 +202,17 @@ def test_rows_of_the_lowest_or_highest_value(layout, rows, k, sign):
     want[:, 0], want[:, -1] = 0, 1 / (k - 1) - 1
     assert np.abs(host(loss) - math.log(k - 1)).max() <= 4 * 2.0 ** -24 * math.log(k - 1)
     assert (np.abs(host(grad) - want.numpy()) <= 8 * 2.0 ** -24 * np.abs(want.numpy())).all()
+
+@pytest.mark.parametrize("rows,k,group", WHOLE)
+def test_whole_rows_with_smoothing(rows, k, group):
+    for value in cases(torch.float32):
+        x, free = masked(rows, k, group, torch.float32, value)
+        check(x, targets(free), k, "rows", (0.3 * group ** 0.5 + 0.7) * group, smoothing=0.1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,k,group", WHOLE)
+def test_whole_rows_with_targets_of_the_lowest_value(rows, k, group, dtype):
+    # the loss of a target at the lowest value, in float32's range after tau; in powers of two its score is beyond it
+    x, free = masked(rows, k, group, dtype, torch.finfo(dtype).min)
+    check(x, torch.where(torch.arange(rows) % 8 >= 4, targets(free), 0), k, "rows", 1.2 * group)
