@@ -53,6 +53,8 @@ __device__ __forceinline__ int64_t target_of(const CeArgs &a, int64_t row)
 {
     return a.targets64 ? static_cast<const int64_t *>(a.targets)[row] : static_cast<const int32_t *>(a.targets)[row];
 }
+// behind the last class of the piece that begins with `first`
+__device__ __forceinline__ int end_of(const CeArgs &a, int first) { return a.k - first > a.per_piece ? first + a.per_piece : a.k; }
 template <typename A>
 __device__ __forceinline__ bool nothing_to_do(const CeArgs &a) { return a.if_changed && *static_cast<const A *>(a.upstream) == A(1); }
 
@@ -140,6 +142,7 @@ struct Grad {
 };
 
 // ---- rows in memory ------------------------------------------------------------------------------------------------------------
+// (Rows have up to 2^31 - 1 features: indexes do not go beyond the last one, or are differences.)
 // The classes of a row by THREADS threads.  PACK != 0: G = PACK features, of which a 16-byte piece holds a whole number of classes; a thread takes
 // pieces.  PACK == 0: teams of 1 to 64 lanes take a class each, by pieces of 16 bytes and what is left behind them.
 template <typename T, int THREADS, int PACK>
@@ -171,7 +174,7 @@ struct Classes {
 #pragma unroll
             for (int j = 0; j < E; ++j) s += (double)(typename Wide<T>::type)v[j];
         }
-        for (i = pieces * E + lane; i < group; i += lanes) s += (double)(typename Wide<T>::type)p[i];
+        for (i = lane; i < group - pieces * E; i += lanes) s += (double)(typename Wide<T>::type)p[pieces * E + i];
         for (int by = lanes >> 1; by > 0; by >>= 1) s += __shfl_xor(s, by);
         return s;
     }
@@ -188,7 +191,7 @@ struct Classes {
     {
         const int pieces = group / E;
         if (pieces > 0) {
-            for (int i = lane; i * E < group; i += lanes) *reinterpret_cast<V *>(p + (i < pieces ? i * E : group - E)) = (V)value;
+            for (int i = lane; i < pieces + (group > pieces * E); i += lanes) *reinterpret_cast<V *>(p + (i < pieces ? i * E : group - E)) = (V)value;
             return;
         }
         if (lane != 0) return;
@@ -265,8 +268,8 @@ struct Classes {
                 for (int u = 0; u < 4; ++u) of(i + u * THREADS, v[u]);
             }
             for (; i < pieces; i += THREADS) of(i, reinterpret_cast<const V *>(p)[i]);
-            const int c = first + pieces * EACH + (int)threadIdx.x;
-            if (c < end) {
+            const int left = pieces * EACH + (int)threadIdx.x, c = first + left;
+            if (left < end - first) {
                 double s = 0;
 #pragma unroll
                 for (int j = 0; j < PACK; ++j) s += (double)(typename Wide<T>::type)row[(int64_t)c * PACK + j];
@@ -305,8 +308,8 @@ struct Classes {
                 for (int u = 0; u < 4; ++u) of(i + u * THREADS, v[u]);
             }
             for (; i < pieces; i += THREADS) of(i, reinterpret_cast<const V *>(p)[i]);
-            const int c = first + pieces * EACH + (int)threadIdx.x;
-            if (c < end) {
+            const int left = pieces * EACH + (int)threadIdx.x, c = first + left;
+            if (left < end - first) {
                 double s = 0;
 #pragma unroll
                 for (int j = 0; j < PACK; ++j) s += (double)(typename Wide<T>::type)row[(int64_t)c * PACK + j];
@@ -335,8 +338,8 @@ struct Classes {
                 }
                 reinterpret_cast<V *>(p)[i] = v;
             }
-            const int c = first + pieces * EACH + (int)threadIdx.x;
-            if (c < end) {
+            const int left = pieces * EACH + (int)threadIdx.x, c = first + left;
+            if (left < end - first) {
                 const T u = (T)value(c);
 #pragma unroll
                 for (int j = 0; j < PACK; ++j) row[(int64_t)c * PACK + j] = u;
@@ -570,7 +573,7 @@ __global__ __launch_bounds__(kPart) void row_stats_kernel(CeArgs a)
     const double unit = a.inv_tau * Unit<A>::unit;
     for (int64_t task = blockIdx.x; task < a.rows * a.pieces; task += gridDim.x) {
         const int64_t row = task / a.pieces;
-        const int piece = (int)(task % a.pieces), first = piece * a.per_piece, end = first + a.per_piece < a.k ? first + a.per_piece : a.k;
+        const int piece = (int)(task % a.pieces), first = piece * a.per_piece, end = end_of(a, first);
         const int64_t t = target_of(a, row);
         const T *x = static_cast<const T *>(a.x) + row * a.stride;
         Stats<A> s;
@@ -660,7 +663,7 @@ __global__ __launch_bounds__(kPart) void row_grad_kernel(CeArgs a)
     const Classes<T, kPart, PACK> classes(a.group, a.lanes_log2);
     for (int64_t task = blockIdx.x; task < a.rows * a.pieces; task += gridDim.x) {
         const int64_t row = task / a.pieces;
-        const int piece = (int)(task % a.pieces), first = piece * a.per_piece, end = first + a.per_piece < a.k ? first + a.per_piece : a.k;
+        const int piece = (int)(task % a.pieces), first = piece * a.per_piece, end = end_of(a, first);
         const int64_t t = target_of(a, row);
         T *grad = static_cast<T *>(a.grad) + row * ((int64_t)a.k * a.group);
         if (t < 0 || t >= a.k) {
@@ -696,6 +699,14 @@ struct Column {
         if (row + V > a.rows) row = a.rows - V;
     }
 };
+// the classes of the wavefront that has a part of a piece's
+__device__ __forceinline__ void wave_classes(int first, int end, int wave, int &c0, int &c1)
+{
+    constexpr int WAVES = kPart / kWave;
+    const int n = end - first, run = n / WAVES + (n % WAVES != 0), from = wave * run < n ? wave * run : n;
+    c0 = first + from;
+    c1 = n - from > run ? c0 + run : end;
+}
 template <typename T>
 __device__ __forceinline__ double column_sum(const CeArgs &a, const Column<1> &col, int64_t from, int64_t to)
 {
@@ -806,7 +817,7 @@ __global__ __launch_bounds__(kPart) void column_sums_kernel(CeArgs a)
     typedef typename Wide<T>::type A;
     __shared__ double room[kPart / kWave][V][kWave][4];
     const Column<V> col(a);
-    const int first = (int)blockIdx.y * a.per_piece, end = first + a.per_piece < a.k ? first + a.per_piece : a.k, slice = blockIdx.z;
+    const int first = (int)blockIdx.y * a.per_piece, end = end_of(a, first), slice = blockIdx.z;
     const int64_t from = (int64_t)a.group * slice / a.slices, to = (int64_t)a.group * (slice + 1) / a.slices;
     int64_t t[V];
 #pragma unroll
@@ -827,7 +838,8 @@ __global__ __launch_bounds__(kPart) void column_sums_kernel(CeArgs a)
         }
     };
     const T *x = static_cast<const T *>(a.x);
-    const int run = (end - first + kPart / kWave - 1) / (kPart / kWave), c0 = first + col.wave * run, c1 = c0 + run < end ? c0 + run : end;
+    int c0, c1;
+    wave_classes(first, end, col.wave, c0, c1);
     if (V == 1 && col.subs > 1) {
         if constexpr (V == 1)
             for (int c = c0; c < c1; ++c) {
@@ -878,7 +890,7 @@ __global__ __launch_bounds__(kPart) void column_grad_kernel(CeArgs a)
     typedef typename Wide<T>::type A;
     if (nothing_to_do<A>(a)) return;
     const Column<V> col(a);
-    const int first = (int)blockIdx.y * a.per_piece, end = first + a.per_piece < a.k ? first + a.per_piece : a.k, slice = blockIdx.z;
+    const int first = (int)blockIdx.y * a.per_piece, end = end_of(a, first), slice = blockIdx.z;
     const int64_t from = (int64_t)a.group * slice / a.slices, to = (int64_t)a.group * (slice + 1) / a.slices;
     int64_t t[V];
     GradOf<A> g[V];
@@ -896,7 +908,8 @@ __global__ __launch_bounds__(kPart) void column_grad_kernel(CeArgs a)
         T *p = grad + ((int64_t)c * a.group + from + col.sub) * a.rows;
         for (int64_t i = from + col.sub; i < to; i += col.subs, p += col.subs * a.rows) store_part<V>(p, value);
     };
-    const int run = (end - first + kPart / kWave - 1) / (kPart / kWave), c0 = first + col.wave * run, c1 = c0 + run < end ? c0 + run : end;
+    int c0, c1;
+    wave_classes(first, end, col.wave, c0, c1);
     if (c0 >= c1) return;
     if (V > 1 || col.subs == 1) {
         if (a.scores) column_stream(a, col, a.scores, c0, c0, c1, 1, store);

@@ -216,3 +216,35 @@ def test_whole_rows_with_targets_of_the_lowest_value(rows, k, group, dtype):
     # the loss of a target at the lowest value, in float32's range after tau; in powers of two its score is beyond it
     x, free = masked(rows, k, group, dtype, torch.finfo(dtype).min)
     check(x, torch.where(torch.arange(rows) % 8 >= 4, targets(free), 0), k, "rows", 1.2 * group)
+
+
+# 2^31 - 1 features, as many as a row may have
+@pytest.mark.parametrize("layout,rows", [("rows", 1), ("columns", 2)])
+def test_as_many_classes_as_there_may_be(layout, rows):
+    k = (1 << 31) - 1
+    x = torch.zeros((rows, k) if layout == "rows" else (k, rows), dtype=torch.bfloat16, device=DEV)
+    leaf = (x if layout == "rows" else x.t())
+    leaf[-1, -1] = 20.0
+    leaf.requires_grad_(True)
+    t = torch.full((rows,), k - 1, device=DEV)
+    loss = C.group_cross_entropy(leaf, t, k, reduction="none")
+    grad, = torch.autograd.grad(loss.sum(), leaf)
+    others = (k - 1) * math.exp(-20.0)
+    step = (LN2 * 2 * 29 + 8) * 2.0 ** -24
+    assert abs(float(loss[-1].detach()) - math.log1p(others)) <= step * (1 + math.log1p(others))
+    assert abs(float(grad[-1, -1]) + others / (1 + others)) <= 2.0 ** -8
+    each = math.exp(-20.0) / (1 + others)
+    assert abs(float(grad[-1, 0]) - each) <= (2.0 ** -8 + 2 * step) * each
+    row = grad[-1]
+    assert int((row != row[0]).sum()) == 1                            # (all are written)
+    if rows > 1:
+        assert abs(float(loss[0].detach()) - math.log(k)) <= step * math.log(k) and int((grad[0] != grad[0, 0]).sum()) == 1
+
+
+def test_a_class_of_as_many_features_as_there_may_be():
+    features = (1 << 31) - 1
+    x = torch.zeros(1, features, dtype=torch.bfloat16, device=DEV).requires_grad_(True)
+    loss = C.group_cross_entropy(x, torch.zeros(1, dtype=torch.int64, device=DEV), 1)
+    assert loss == 0
+    grad, = torch.autograd.grad(loss, x, torch.tensor(3.0, device=DEV))
+    assert int((grad != 0).sum()) == 0
