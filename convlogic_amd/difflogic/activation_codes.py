@@ -110,22 +110,23 @@ def check_bits(bits):
 
 
 class RecomputedFromCodes(torch.autograd.Function):
-    """y = evaluate(x, weights), with the gradients of that at what the codes of x stand for: x is kept in codes, and the backward pass evaluates again."""
+    """y = evaluate(x, weights, *wiring), with the gradients of that at what the codes of x stand for: x is kept in codes, and the backward pass evaluates
+    again, with the wiring of the forward pass (autograd refuses one that was written since)."""
 
     @staticmethod
-    def forward(ctx, x, weights, evaluate):
+    def forward(ctx, x, weights, evaluate, *wiring):
         kept = encode_activations(x)
-        ctx.save_for_backward(kept.codes, kept.scales, weights)
+        ctx.save_for_backward(kept.codes, kept.scales, weights, *wiring)
         ctx.of, ctx.evaluate = (kept.shape, kept.stride, kept.dtype), evaluate
-        return evaluate(x.detach(), weights.detach())
+        return evaluate(x.detach(), weights.detach(), *wiring)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
-        codes, scales, weights = ctx.saved_tensors
+        codes, scales, weights, *wiring = ctx.saved_tensors
         x = ActivationCodes(codes, scales, *ctx.of).decode().requires_grad_(ctx.needs_input_grad[0])
         w = weights.detach().requires_grad_(ctx.needs_input_grad[1])
         wanted = [t for t in (x, w) if t.requires_grad]
         with torch.enable_grad():
-            grads = list(torch.autograd.grad(ctx.evaluate(x, w), wanted, grad_y))
-        return grads.pop(0) if x.requires_grad else None, grads.pop(0) if w.requires_grad else None, None
+            grads = list(torch.autograd.grad(ctx.evaluate(x, w, *wiring), wanted, grad_y))
+        return (grads.pop(0) if x.requires_grad else None, grads.pop(0) if w.requires_grad else None, None) + (None,) * len(wiring)

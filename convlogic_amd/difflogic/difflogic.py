@@ -38,6 +38,15 @@ def _reverse_wiring(idx0, idx1, in_dim):
     return torch.from_numpy(start), torch.from_numpy(neuron[order].copy())
 
 
+# the output of a layer in training, from its weights and its wiring alone: what a layer that keeps codes evaluates again
+def _evaluate_python(x, weights, a, b):
+    return bin_op_s(x[..., a], x[..., b], torch.nn.functional.softmax(weights, dim=-1))
+
+
+def _evaluate_probabilities(x, weights, a, b, start, flat):
+    return LogicLayerCudaFunction.apply(x, a, b, torch.nn.functional.softmax(weights, dim=-1).to(x.dtype), start, flat)
+
+
 class LogicLayer(torch.nn.Module):
     """out_dim two-input logic gate neurons over in_dim features (src/difflogic/difflogic.py:14-90).
 
@@ -100,13 +109,10 @@ class LogicLayer(torch.nn.Module):
     def forward_python(self, x):
         assert x.shape[-1] == self.in_dim, (x.shape[-1], self.in_dim)
         if self._keeps_codes(x):
-            return RecomputedFromCodes.apply(x, self.weights, self._evaluate_python)
+            return RecomputedFromCodes.apply(x, self.weights, _evaluate_python, self.indices_0, self.indices_1)
         a, b = x[..., self.indices_0], x[..., self.indices_1]
         w = self._gate_weights(torch.float32 if not self.training else self.weights.dtype)
         return bin_op_s(a, b, w)
-
-    def _evaluate_python(self, x, weights):
-        return bin_op_s(x[..., self.indices_0], x[..., self.indices_1], torch.nn.functional.softmax(weights, dim=-1))
 
     def _keeps_codes(self, x):
         """True for a call whose backward pass reads the input from codes."""
@@ -152,12 +158,8 @@ class LogicLayer(torch.nn.Module):
             inside = _transposes_with_kernel(x)
             return _lib.nodes().fc_layer(x if inside else _feature_major(x), buffers["indices_0"], buffers["indices_1"], weights,
                                          buffers["given_x_indices_of_y_start"], buffers["given_x_indices_of_y"], self._sole_consumers(key), inside, True)
-        return RecomputedFromCodes.apply(_feature_major(x), weights, self._evaluate_probabilities).transpose(0, 1)
-
-    def _evaluate_probabilities(self, x, weights):
-        buffers = self._buffers
-        return LogicLayerCudaFunction.apply(x, buffers["indices_0"], buffers["indices_1"], torch.nn.functional.softmax(weights, dim=-1).to(x.dtype),
-                                            buffers["given_x_indices_of_y_start"], buffers["given_x_indices_of_y"])
+        return RecomputedFromCodes.apply(_feature_major(x), weights, _evaluate_probabilities, buffers["indices_0"], buffers["indices_1"],
+                                         buffers["given_x_indices_of_y_start"], buffers["given_x_indices_of_y"]).transpose(0, 1)
 
     def prefold_candidate(self):
         """The logits a network may fold for this layer ahead of its forward call (one launch for all its layers,

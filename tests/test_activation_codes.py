@@ -188,3 +188,24 @@ def test_the_oracle_against_autograd():
     gx, gz = torch.autograd.grad(out, (kept, z), up)
     _, want_x, want_z, _, _ = K.layer(x.numpy(), a.numpy(), b.numpy(), z.detach().numpy(), up.numpy())
     assert np.allclose(gx.numpy(), want_x, rtol=1e-11, atol=1e-13) and np.allclose(gz.numpy(), want_z, rtol=1e-9, atol=1e-12)
+
+
+def test_an_updated_wiring_is_refused_by_the_backward_pass():
+    layer = layer_of(6, 9, checkpoint_bits=8)
+    x = activations((20, 6)).requires_grad_(True)
+    y = layer(x)
+    y.sum().backward(retain_graph=True)
+    with torch.no_grad():
+        layer.indices_0.copy_(layer.indices_0.flip(0))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_a_replaced_wiring_leaves_the_backward_pass_its_own():
+    layer = layer_of(6, 9, checkpoint_bits=8)
+    x = activations((20, 6)).requires_grad_(True)
+    y = layer(x)
+    want = torch.autograd.grad(y.sum(), (x, layer.weights), retain_graph=True)
+    layer.indices_0 = layer.indices_0.flip(0)
+    got = torch.autograd.grad(y.sum(), (x, layer.weights))
+    assert all(torch.equal(u, v) for u, v in zip(got, want))

@@ -457,3 +457,15 @@ def test_a_recorded_step_of_a_network():
         assert value == float(loss.detach()) and all(torch.equal(u, v) for u, v in zip(grads, want))
         del loss
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float16])
+def test_an_updated_wiring_of_other_types_is_refused_by_the_backward_pass(dtype):
+    layer = layer_of(30, 20)
+    if dtype == torch.float64:
+        layer = layer.double()
+    y = layer(activations((30, 64), dtype).to(DEV).t().requires_grad_(True))
+    with torch.no_grad():
+        layer.indices_0.copy_(layer.indices_0.flip(0))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
