@@ -1067,8 +1067,8 @@ template <typename T, int THREADS, int PACK, typename S>
 int launch_rows(const char *name, const CeArgs &a, hipStream_t stream)
 {
     const size_t lds = a.k * sizeof(S);
-    if (lds > 48 << 10) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(rows_kernel<T, THREADS, PACK, S>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (lds > 48 << 10) {                                             // (of all calls the same: another thread's may come between this one and the launch)
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(rows_kernel<T, THREADS, PACK, S>), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
         if (e != hipSuccess) {
             clg_set_error("%s: %s", name, hipGetErrorString(e));
             return CLG_ELAUNCH;

@@ -8,6 +8,7 @@ under 2^-126.  A total is off by its classes' parts, a gradient by its class's a
 and the logarithm of the total, or of 1 + the others where the target is the highest.  2^-53 for float64, whose scores are off by the additions of their features too.
 Half a step of the type on top."""
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -248,3 +249,27 @@ def test_a_class_of_as_many_features_as_there_may_be():
     assert loss == 0
     grad, = torch.autograd.grad(loss, x, torch.tensor(3.0, device=DEV))
     assert int((grad != 0).sum()) == 0
+
+
+def test_two_threads_at_once():
+    sizes, t = (36000, 13000), torch.zeros(130, dtype=torch.int64, device=DEV)
+    x = {k: masked(130, k, 1, torch.float32, -1e9)[0].to(DEV) for k in sizes}
+    want = {k: C.group_cross_entropy(x[k], t, k, reduction="none") for k in sizes}
+    torch.cuda.synchronize()
+    failed = []
+
+    def calls(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got = [C.group_cross_entropy(x[k], t, k, reduction="none") for _ in range(50)]
+                torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(v, want[k]) for v in got):
+                failed.append(k)
+        except RuntimeError as e:
+            failed.append(e)
+    threads = [threading.Thread(target=calls, args=(k,)) for k in sizes]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not failed
