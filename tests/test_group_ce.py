@@ -89,3 +89,18 @@ def test_refusals():
             C.group_cross_entropy(**{**dict(x=x, targets=t, k=3), **bad})
     with pytest.raises(RuntimeError, match="columns"):
         C.group_cross_entropy(torch.ones(4, 0), t, 1)
+
+
+@pytest.mark.parametrize("value", [-1e4, -1e9, torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("k,group,smoothing", [(10, 1, 0.0), (7, 5, 0.1)])
+def test_classes_masked_with_finite_values(k, group, smoothing, value):
+    x, t = features(8, k, group), labels(8, k)
+    x[::2, :group] = value
+    t[::2] = t[::2].clamp(min=1)
+    x = x.float().requires_grad_(True)
+    loss = C.group_cross_entropy(x, t, k, tau=float(group), label_smoothing=smoothing, reduction="none")
+    grad, = torch.autograd.grad(loss.sum(), x)
+    want, want_grad = K.group_cross_entropy(x.detach().numpy(), t.numpy(), k, float(group), smoothing, 1.0, "none")
+    # (scores and exponentials in 64 bits: the rounding to float32 is what is left)
+    assert np.allclose(loss.detach().numpy(), np.asarray(want, dtype=np.float64), rtol=2.0 ** -24 * 1.01, atol=1e-12)
+    assert np.allclose(grad.numpy(), np.asarray(want_grad, dtype=np.float64), rtol=2.0 ** -24 * 1.01, atol=1e-12)
