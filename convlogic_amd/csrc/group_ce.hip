@@ -352,8 +352,8 @@ struct Classes {
 // in the row's first 64 features, or, where these do not fill 16-byte pieces, of the first class and the middle one.  Where the row's highest turns out to be more than kFar
 // from that, as where these classes are masked, they are made again relative to the highest.  Near the highest a score is then off by half a step of a float under
 // kFar, 2^-18, as any argument of that size of an exponential is.  (Relative to the target's, which is seldom masked, but whose place has to be read first: loss_tokens
-// 398 us, not 383.)  Bound by memory: 4096 rows of 32768 classes of 4 bfloat16 with their gradient, 2.1 GB, 368 us, 5.8 TB/s (vector units 46 % busy; with the next
-// pieces loaded under the sums of these 392).
+// 398 us, not 385.)  Bound by memory: 4096 rows of 32768 classes of 4 bfloat16 with their gradient, 2.1 GB, 375 us, 5.7 TB/s (with the next pieces loaded under the sums of
+// these 392); of 1 bfloat16 422 us in all, and 490 where the first 64 classes are -10^4.
 constexpr int kNear = 64;
 constexpr float kFar = 128;
 constexpr double kLevel = 1 << 28;                                    // units up to which a multiply-add with the rounded product of another sum is a difference
@@ -402,16 +402,22 @@ __global__ __launch_bounds__(THREADS, rows_waves(THREADS, PACK, sizeof(S))) void
             at *= unit;
             if (!(__builtin_fabs(at) <= kLevel)) at = 0;
         }
-        S m[1] = {lowest(S(0))};
-        classes.sums(x, 0, a.k, (int64_t)a.k * a.group, [&](int c, double s, bool mine) {
-            const S u = (S)(kFloats ? s * unit - at : s);
-            if (mine) score[c] = u;
-            m[0] = max_of(m[0], u);
-        });
-        __syncthreads();                                              // (also: room is free again)
-        block_reduce<false, THREADS>(m, reinterpret_cast<S *>(room));
+        S m[1];
+        for (bool again = false;; again = true) {
+            m[0] = lowest(S(0));
+            classes.sums(x, 0, a.k, (int64_t)a.k * a.group, [&](int c, double s, bool mine) {
+                const S u = (S)(kFloats ? s * unit - at : s);
+                if (mine) score[c] = u;
+                m[0] = max_of(m[0], u);
+            });
+            __syncthreads();                                          // (also: room is free again)
+            block_reduce<false, THREADS>(m, reinterpret_cast<S *>(room));
+            if (!kFloats || again || __builtin_fabs(m[0]) <= kFar || !(__builtin_fabs(at + (double)m[0]) <= kLevel)) break;
+            at += (double)m[0];                                       // the highest but for 2^-24 of its distance, 32 units at most
+            __syncthreads();                                          // (room is read)
+        }
         double highest = kFloats ? (at + (double)m[0]) / unit : (double)m[0];
-        // (what follows for few rows, by plain loops that take no registers from the others)
+        // (for rows that are further off, or whose scores are beyond kLevel, by plain loops that take no registers from the others)
         const auto plain_sum = [&](int c) {
             double s = 0;
 #pragma unroll 1
