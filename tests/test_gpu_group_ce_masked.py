@@ -273,3 +273,25 @@ def test_two_threads_at_once():
     for th in threads:
         th.join()
     assert not failed
+
+
+@pytest.mark.parametrize("smoothing", [0.0, 0.1])
+@pytest.mark.parametrize("layout,rows,k,group", [("rows", 200, 50, 1), ("rows", 200, 50, 6), ("rows", 150, 30, 80), ("rows", 5, 3000, 8), ("columns", 1030, 400, 2)])
+def test_infinite_and_nan_classes_in_every_place(layout, rows, k, group, smoothing):
+    # a class of each row, at another place in each, is not finite; the target is that class, or another one
+    x, _ = masked(rows, k, group, torch.float32, 0.0)
+    row = torch.arange(rows)
+    at, t = 7 * row % k, torch.where(row % 2 == 0, 7 * row % k, (7 * row + 1 + row % (k - 1)) % k)
+    x[row, at * group + row % group] = torch.tensor([-math.inf, math.inf, math.nan])[row // 2 % 3]
+    leaf = (x.to(DEV) if layout == "rows" else x.to(DEV).t().contiguous().t()).requires_grad_(True)
+    loss = C.group_cross_entropy(leaf, t.to(DEV), k, tau=group ** 0.5, label_smoothing=smoothing, reduction="none")
+    grad, = torch.autograd.grad(loss.sum(), leaf)
+    want, want_grad = K.group_cross_entropy(host(x), t.numpy(), k, group ** 0.5, smoothing, 1.0, "none")
+    loss, grad, want, want_grad = host(loss), host(grad), np.asarray(want, dtype=np.float64), np.asarray(want_grad, dtype=np.float64)
+    nan = (row // 2 % 3 != 0).numpy()
+    assert np.isnan(loss[nan]).all() and np.isnan(want[nan]).all()
+    # (the target's gradient alone could be finite: of +inf elsewhere, all are NaN)
+    assert np.isnan(grad[nan]).any(1).all() and (np.isnan(grad) == np.isnan(want_grad)).all()
+    step = (LN2 * (2 * 40 + 2 * 128) + 8) * 2.0 ** -24               # (distances up to 40 powers of two)
+    assert np.allclose(loss[~nan], want[~nan], rtol=step, atol=step)
+    assert np.allclose(grad[~nan] * group ** 0.5, want_grad[~nan] * group ** 0.5, rtol=0, atol=2 * step)
