@@ -207,7 +207,7 @@ class ConvLogicLayer(nn.Module):
 
     checkpoint_bits=8 (no counterpart in the reference; complete float32 blocks on the GPU): a training step keeps the input in 8 bits (encode_activations)
     instead of the input itself.  The output, and which element of a window the pooling takes, are those of the input; both gradients are computed from
-    the values that the codes stand for.  (A block on 0/1 inputs keeps a bit per tap anyway.)"""
+    the values that the codes stand for, which the backward pass writes out for the time of its call.  (A block on 0/1 inputs keeps a bit per tap anyway.)"""
 
     def __init__(self, in_channels: int, out_channels: int, stride=1, padding=1, kernel=3, groups: int = 1,
                  selection=None, residual_init: bool = False, implementation: str = "cuda", grad_factor: float = 1.0,

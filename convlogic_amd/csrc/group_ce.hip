@@ -3,7 +3,7 @@
 //     loss = w [ (1 - e) (M - s_t + log Z) + e (log Z + mean_c (M - s_c)) ]
 //     d loss / d feature of c = w / tau [ exp(s_c - M) / Z - e / k ],  of t  w / tau [ -O / Z + e - e / k ]
 // Where the target is the highest, log Z = log1p(O): with O apart, losses and gradients near 0 keep their digits.  A score is a long sum, and its rounding is a
-// relative error of its exponential: sums over features, and what is taken of a score before its exponential, are in 64 bits.
+// relative error of its exponential: sums over features and the differences of scores that exponentials are taken of are in 64 bits, but for rows_kernel's floats.
 //
 // Rows in memory ("rows", features dense): a workgroup has a row, whose scores stay in LDS from the sums to the gradient, so the features are read once (rows_kernel);
 // rows of more classes than LDS holds, or too few rows to fill the chip, go in pieces of the classes, once for the sums and the highest (row_stats_kernel) and once

@@ -45,8 +45,9 @@ def _check(x):
 
 
 def encode_activations(x):
-    """The ActivationCodes of a float tensor: an element of a group of 128 with lowest value l and highest h is off by at most (h - l) / 510 and the rounding of
-    its type; the lowest and the highest are kept, so 0 and 1 are exact where a group holds both, or one of them alone.  Groups run through the elements as
+    """The ActivationCodes of a float tensor: an element of a group of 128 with lowest value l and highest h is off by at most (h - l) / 510 and the roundings of
+    the step and of its type (by more where the step is no normal number, for ranges under 255 times the smallest one: in the end all are l).  The lowest value is kept, the
+    highest but for these roundings; 0 and 1 are exact where a group holds both, or one of them alone.  Groups run through the elements as
     they lie in memory (those of a tensor with gaps as of its contiguous copy).  All elements of a group with a NaN or an infinity become NaN.  A constant for
     autograd, whatever x is."""
     _check(x)

@@ -51,7 +51,8 @@ class LogicLayer(torch.nn.Module):
     """out_dim two-input logic gate neurons over in_dim features (src/difflogic/difflogic.py:14-90).
 
     checkpoint_bits=8 (no counterpart in the reference): a training step keeps the input in 8 bits (encode_activations) instead of the input itself.  The
-    output is that of the input; both gradients are those at the values that the codes stand for."""
+    output is that of the input; both gradients are those at the values that the codes stand for.  Beside its codes a float32
+    step keeps 96 bytes a neuron, without them 80 beside the input: a layer with more than 0.18 in_dim batch neurons keeps more with codes than without."""
 
     def __init__(self, in_dim: int, out_dim: int, grad_factor: float = 1.0, implementation: str = None,
                  connections: str = "random", residual_init: bool = False, checkpoint_bits: int = None):
