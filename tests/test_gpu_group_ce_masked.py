@@ -76,7 +76,7 @@ def check(x, t, k, layout, tau, smoothing=0.0, reduction="none", upstream=None):
         each = np.where(p > 0, p * off * unit, 0.0) + 2.0 ** -126
         total = each.sum(1)
         target = t.numpy()
-        but = total - each[at, target]
+        but = np.where(np.arange(k) == target[:, None], 0.0, each).sum(1)      # (not total less the target's: a loss near 0 has a bound near 0)
         d_t = d[at, target]
         margin = np.where(held > 0, LN2 * (2 * held + d_t), 2.0 ** -20 * (1 + d_t)) * unit
         if double:
